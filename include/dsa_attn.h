@@ -399,6 +399,36 @@ int dsa_split_bf16_combine_qkv(const void *yq, const void *yk, const void *yv, i
 int dsa_round_bf16_x3(const float *a, const float *b, const float *c, int64_t na, int64_t nb, int64_t nc, void *ya, void *yb,
                       void *yc, void *stream);
 
+/*
+ * Gated delta rule over packed sequences (models/qwen3_5/model.py:178-186), chunked: a state S (Dk x Dv, fp32) per sequence and value head,
+ *   S_t = e^g_t S_{t-1} + beta_t k_t (v_t - e^g_t S_{t-1}^T k_t)^T,   o_t = scale S_t^T q_t,
+ *   g = -exp(a_log) softplus(a + dt_bias), beta = sigmoid(b), q and k divided by sqrt(|.|^2 + 1e-6) first where l2_norm is set.
+ * q, k (T,Hk,Dk), v (T,Hv,Dv) bf16 with any token and head strides that are multiples of 8 elements, rows on 16-byte boundaries; value head h
+ * reads key head h / (Hv/Hk).  a, b (T,Hv) bf16 or fp32 (a_f32, b_f32), head stride 1; a_log, dt_bias (Hv) both bf16 or both fp32 (param_f32).
+ * Dk, Dv multiples of 8 up to 128.  cu_seqlens as everywhere; rows behind cu[N] give zeros.
+ *
+ * dsa_delta_fwd writes out (T,Hv,Dv) bf16 and, where they are not null, reads initial (N,Hv,Dk,Dv) fp32 and writes final, the same.  `ws` holds
+ * dsa_delta_workspace_bytes(args, save) bytes; with `save` it is what dsa_delta_bwd reads.
+ * dsa_delta_bwd: dout (T,Hv,Dv) bf16 contiguous, dfinal (may be null) -> dq, dk (T,Hk,Dk), dv (T,Hv,Dv) bf16, da, db (T,Hv) and da_log, ddt_bias
+ * (Hv) in their inputs' types, all contiguous, dinitial fp32 where it is not null.  `scratch` holds dsa_delta_scratch_bytes(args) bytes.
+ * dsa_delta_step: one token for each of T requests; state (T,Hv,Dk,Dv) fp32, requests state_stride elements apart (a multiple of 4, on a 16-byte
+ * boundary), is read and written in place.  cu and N are not used.
+ */
+typedef struct {
+    const void *q, *k, *v, *a, *b, *a_log, *dt_bias;
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, a_tok, b_tok;
+    const int32_t *cu;
+    int T, N, Hk, Hv, Dk, Dv;
+    float scale;
+    int l2_norm, a_f32, b_f32, param_f32;
+} dsa_delta_args;
+size_t dsa_delta_workspace_bytes(const dsa_delta_args *args, int save);
+size_t dsa_delta_scratch_bytes(const dsa_delta_args *args);
+int dsa_delta_fwd(const dsa_delta_args *args, const float *initial, void *out, float *final, int save, void *ws, size_t ws_bytes, void *stream);
+int dsa_delta_bwd(const dsa_delta_args *args, const void *dout, const float *dfinal, const void *ws, size_t ws_bytes, void *dq, void *dk, void *dv,
+                  void *da, void *db, void *da_log, void *ddt_bias, float *dinitial, void *scratch, size_t scratch_bytes, void *stream);
+int dsa_delta_step(const dsa_delta_args *args, float *state, int64_t state_stride, void *out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

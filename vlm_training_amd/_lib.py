@@ -19,7 +19,22 @@ DSA_DTYPE_SPLIT_BF16 = 2
 DSA_NORM_OFFSET, DSA_NORM_WEIGHT_BF16 = 1, 2                                               # norm_flags of the prologue
 DSA_BWD_DELTA, DSA_BWD_BITMAP, DSA_BWD_DQ, DSA_BWD_DKV, DSA_BWD_ALL = 1, 2, 4, 8, 15      # parts of dsa_attn_bwd_parts
 
+
+class DeltaArgs(ctypes.Structure):
+    """dsa_delta_args of include/dsa_attn.h; its functions take a pointer to one (ctypes.byref)."""
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "a", "b", "a_log", "dt_bias")]
+                + [(n, c_int64) for n in ("q_tok", "q_head", "k_tok", "k_head", "v_tok", "v_head", "a_tok", "b_tok")] + [("cu", c_void_p)]
+                + [(n, c_int) for n in ("T", "N", "Hk", "Hv", "Dk", "Dv")] + [("scale", c_float)]
+                + [(n, c_int) for n in ("l2_norm", "a_f32", "b_f32", "param_f32")])
+
+
 _SIGNATURES = {
+    "dsa_delta_workspace_bytes": (c_size_t, [c_void_p, c_int]),
+    "dsa_delta_scratch_bytes": (c_size_t, [c_void_p]),
+    "dsa_delta_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "dsa_delta_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                              c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "dsa_delta_step": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "dsa_version": (c_char_p, []),
     "dsa_last_error": (c_char_p, []),
     "dsa_indexer_scores": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int,

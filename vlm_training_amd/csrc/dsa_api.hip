@@ -8,9 +8,13 @@
 #include <string.h>
 
 #include "dsa_common.h"
+#include "dsa_delta.h"
 #include "../../include/dsa_attn.h"
 
 extern "C" {
+hipError_t dsa_launch_delta_fwd(const DeltaArgs *a, int save, hipStream_t stream);
+hipError_t dsa_launch_delta_bwd(const DeltaArgs *a, hipStream_t stream);
+hipError_t dsa_launch_delta_step(const dsa_delta_args *in, float *state, int64_t state_req, void *out, hipStream_t stream);
 hipError_t dsa_launch_topk(const float *scores, int64_t ld, int row_begin, int row_end, const int32_t *cu, int N,
                            int K, int32_t *idx, int32_t *n, uint32_t *bitmap, int ldw, float *sel, hipStream_t stream);
 hipError_t dsa_launch_indexer_kl(const float *sel, const float *mass, const int32_t *n, int T, int K, float grad_scale,
@@ -1023,4 +1027,104 @@ extern "C" int dsa_round_bf16_x3(const float *a, const float *b, const float *c,
         return fail(DSA_ERR_ARG, "inputs must be 16-byte aligned, outputs 8-byte aligned");
     hipError_t e = dsa_launch_round_bf16_x3(a, b, c, na, nb, nc, ya, yb, yc, (hipStream_t)stream);
     return e == hipSuccess ? DSA_OK : hip_fail(e, "bf16 rounding launch");
+}
+
+// ---------------------------------------------------------------------------------------------------
+// gated delta rule
+// ---------------------------------------------------------------------------------------------------
+static int check_delta(const dsa_delta_args *a, bool packed) {
+    if (!a) return fail(DSA_ERR_ARG, "null arguments");
+    if (a->T < 0 || a->Hk < 1 || a->Hv < 1 || a->Hv % a->Hk) return fail(DSA_ERR_ARG, "T=%d Hk=%d Hv=%d: value heads must be a multiple of key heads", a->T, a->Hk, a->Hv);
+    if (a->Dk < 8 || a->Dk > 128 || a->Dk % 8 || a->Dv < 8 || a->Dv > 128 || a->Dv % 8)
+        return fail(DSA_ERR_UNSUPPORTED, "head dims %d and %d: need multiples of 8 up to 128", a->Dk, a->Dv);
+    if (packed && (a->N < 1 || !a->cu)) return fail(DSA_ERR_ARG, "cu_seqlens: N=%d", a->N);
+    if (a->Hk > 65535 || (packed ? (int64_t)a->N : a->T) * a->Hv * 4 > 0x7fffffffll) return fail(DSA_ERR_UNSUPPORTED, "N=%d T=%d Hv=%d: too many heads for one launch", a->N, a->T, a->Hv);
+    if (!(a->scale != 0.f)) return fail(DSA_ERR_ARG, "scale=%g", (double)a->scale);
+    if (a->T == 0) return DSA_OK;
+    if (!a->q || !a->k || !a->v || !a->a || !a->b || !a->a_log || !a->dt_bias) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if ((a->q_tok | a->q_head | a->k_tok | a->k_head | a->v_tok | a->v_head) % 8) return fail(DSA_ERR_ARG, "token and head strides must be multiples of 8 elements");
+    if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & 15) return fail(DSA_ERR_ARG, "q, k and v must lie on 16-byte boundaries");
+    return DSA_OK;
+}
+// the parts of the workspace, each on a 256-byte boundary; returns the bytes of all of them
+static size_t delta_layout(const dsa_delta_args *in, int save, char *ws, DeltaArgs *d) {
+    d->in = *in;
+    d->slots = in->T / DELTA_CHUNK + in->N + 2;          // every sequence's last chunk, and the rows behind the last one
+    d->Dkp = in->Dk > 64 ? 128 : 64;
+    d->Dvp = in->Dv > 64 ? 128 : 64;
+    const size_t cells = (size_t)d->slots * in->Hv;
+    size_t at = 0;
+    auto part = [&](size_t bytes) { char *const p = ws + at; at += align_up(bytes, 256); return p; };
+    d->rows = (float *)part(cells * DELTA_ROWS * 64 * 4);
+    d->tmat = (bf16_t *)part(cells * 8192 * 2);
+    d->pmat = (bf16_t *)part(cells * 4096 * 2);
+    d->state = (bf16_t *)part(save ? cells * d->Dkp * d->Dvp * 2 : 0);
+    d->news = (bf16_t *)part(save ? cells * 64 * d->Dvp * 2 : 0);
+    return at;
+}
+static size_t delta_scratch(char *ws, DeltaArgs *d) {
+    const size_t cells = (size_t)d->slots * d->in.Hv;
+    size_t at = 0;
+    auto part = [&](size_t bytes) { char *const p = ws + at; at += align_up(bytes, 256); return p; };
+    d->dstate = (bf16_t *)part(cells * d->Dkp * d->Dvp * 2);
+    d->drs = (bf16_t *)part(cells * 64 * d->Dvp * 2);
+    d->part = (float *)part(cells * 2 * 4);
+    return at;
+}
+
+extern "C" size_t dsa_delta_workspace_bytes(const dsa_delta_args *args, int save) {
+    DeltaArgs d = {};
+    return check_delta(args, true) ? 0 : delta_layout(args, save, nullptr, &d);
+}
+extern "C" size_t dsa_delta_scratch_bytes(const dsa_delta_args *args) {
+    DeltaArgs d = {};
+    if (check_delta(args, true)) return 0;
+    delta_layout(args, 1, nullptr, &d);
+    return delta_scratch(nullptr, &d);
+}
+
+extern "C" int dsa_delta_fwd(const dsa_delta_args *args, const float *initial, void *out, float *final, int save, void *ws, size_t ws_bytes, void *stream) {
+    if (int rc = check_delta(args, true)) return rc;
+    if (args->T > 0 && !out) return fail(DSA_ERR_ARG, "null tensor pointer");
+    DeltaArgs d = {};
+    const size_t need = delta_layout(args, save, (char *)ws, &d);
+    if (!ws || ws_bytes < need) return fail(DSA_ERR_WORKSPACE, "gated delta rule workspace: have %zu bytes, need %zu", ws_bytes, need);
+    d.initial = initial;
+    d.final = final;
+    d.out = (bf16_t *)out;
+    const hipError_t e = dsa_launch_delta_fwd(&d, save, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "gated delta rule forward launch");
+}
+
+extern "C" int dsa_delta_bwd(const dsa_delta_args *args, const void *dout, const float *dfinal, const void *ws, size_t ws_bytes, void *dq, void *dk, void *dv,
+                             void *da, void *db, void *da_log, void *ddt_bias, float *dinitial, void *scratch, size_t scratch_bytes, void *stream) {
+    if (int rc = check_delta(args, true)) return rc;
+    if (!da_log || !ddt_bias || (args->T > 0 && (!dout || !dq || !dk || !dv || !da || !db))) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if ((uintptr_t)dout & 15) return fail(DSA_ERR_ARG, "dout must lie on a 16-byte boundary");
+    DeltaArgs d = {};
+    const size_t need = delta_layout(args, 1, (char *)const_cast<void *>(ws), &d), need2 = delta_scratch((char *)scratch, &d);
+    if (!ws || ws_bytes < need) return fail(DSA_ERR_WORKSPACE, "gated delta rule workspace: have %zu bytes, need %zu", ws_bytes, need);
+    if (!scratch || scratch_bytes < need2) return fail(DSA_ERR_WORKSPACE, "gated delta rule scratch: have %zu bytes, need %zu", scratch_bytes, need2);
+    d.dout = (const bf16_t *)dout;
+    d.dfinal = dfinal;
+    d.dinitial = dinitial;
+    d.dq = (bf16_t *)dq;
+    d.dk = (bf16_t *)dk;
+    d.dv = (bf16_t *)dv;
+    d.da = da;
+    d.db = db;
+    d.da_log = da_log;
+    d.ddt = ddt_bias;
+    const hipError_t e = dsa_launch_delta_bwd(&d, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "gated delta rule backward launch");
+}
+
+extern "C" int dsa_delta_step(const dsa_delta_args *args, float *state, int64_t state_stride, void *out, void *stream) {
+    if (int rc = check_delta(args, false)) return rc;
+    if (args->T == 0) return DSA_OK;
+    if (!state || !out) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if (((uintptr_t)state & 15) || state_stride % 4 || (args->T > 1 && state_stride < (int64_t)args->Hv * args->Dk * args->Dv))
+        return fail(DSA_ERR_ARG, "state: requests must lie on 16-byte boundaries and apart from each other");
+    const hipError_t e = dsa_launch_delta_step(args, state, state_stride, out, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "gated delta rule step launch");
 }

@@ -1,0 +1,156 @@
+// The gated delta rule's kernels share this: arguments, workspace, tiles of 64 rows in LDS and their MFMA fragments.
+//
+// One value head of one sequence carries a state S (Dk x Dv, fp32):
+//     S_t = e^g_t S_{t-1} + beta_t k_t (v_t - e^g_t S_{t-1}^T k_t)^T,   o_t = scale S_t^T q_t
+// with q, k of unit length, g = -e^a_log softplus(a + dt_bias), beta = sigmoid(b).  In chunks of 64 rows, G the running sum of g inside the
+// chunk, E_ij = e^(G_i - G_j) for j <= i:
+//     A_ij = beta_i E_ij k_i.k_j (j < i)      P_ij = scale E_ij q_i.k_j (j <= i)      T = (I + A)^-1
+//     R = beta (V - e^G K S0)     N = T R     O = scale e^G Q S0 + P N     S1 = e^G_63 S0 + K^T e^(G_63 - G) N
+// T and P depend on no state: all chunks at once; S goes from chunk to chunk, its columns independent of each other.  The factors
+// 1/|q|, 1/|k|, e^G, beta multiply rows of fp32 results, so that q, k and v enter the products as the bf16 they are; T, S, R and N go in as two
+// bf16 (hi + lo, 2^-17 of the value is lost), without lo x lo.
+#pragma once
+#include "dsa_tile.h"
+#include "../../include/dsa_attn.h"
+
+#define DELTA_CHUNK 64
+#define DELTA_TS 72                    // row stride of a 64-wide tile: 16-byte rows, four banks on per row
+// per chunk and value head, 64 floats each: e^G, e^(G_63 - G), beta, 1/|k|, scale/|q|, G in two floats (hi + lo)
+enum { DELTA_EG, DELTA_EC, DELTA_BETA, DELTA_RK, DELTA_RQ, DELTA_GH, DELTA_GL, DELTA_ROWS };
+
+struct DeltaArgs {
+    dsa_delta_args in;
+    int slots, Dkp, Dvp;               // chunks at the most; head dims padded to 64 or 128
+    float *rows;                       // (slots, Hv, DELTA_ROWS, 64)
+    bf16_t *tmat, *pmat;               // (slots, Hv, 2, 64, 64) T as hi, lo;  (slots, Hv, 64, 64) P
+    bf16_t *state, *news;              // for the backward: (slots, Hv, Dvp, Dkp) S0 transposed, (slots, Hv, 64, Dvp) N
+    const float *initial;              // (N, Hv, Dk, Dv) or null
+    float *final;
+    bf16_t *out;
+    // backward
+    const bf16_t *dout;
+    const float *dfinal;
+    bf16_t *dstate, *drs;              // (slots, Hv, Dvp, Dkp) dS1 transposed, (slots, Hv, 64, Dvp) dR
+    float *part;                       // (2, Hv, slots) sums of a chunk for da_log and ddt_bias
+    float *dinitial;
+    bf16_t *dq, *dk, *dv;
+    void *da, *db, *da_log, *ddt;
+};
+
+// a chunk of the batch: its segment's first row and the chunk's first row and number of rows.  cu is read as it is, but rows stay within [0, T).
+struct DeltaChunk { int row0, rows, seg, index, of; };
+// slot -> chunk, by a whole wave (slot wave-uniform); false: a spare slot, `index` then counts the spare ones
+__device__ __forceinline__ bool delta_locate(const int32_t *cu, int N, int T, int slot, DeltaChunk &c) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < N; base += 64) {
+        const int seg = min(base + lane, N - 1);
+        const int lo = cu[seg], len = cu[seg + 1] - lo;
+        const int nb = base + lane < N && len > 0 ? (len + DELTA_CHUNK - 1) / DELTA_CHUNK : 0, upto = wave_prefix_i(nb);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > slot);
+        if (past) {
+            const int w = (int)__builtin_ctzll(past);
+            const int s0 = __builtin_amdgcn_readlane(lo, w), L = __builtin_amdgcn_readlane(len, w);
+            c.of = __builtin_amdgcn_readlane(nb, w);
+            c.index = slot - (__builtin_amdgcn_readlane(upto, w) - c.of);
+            c.seg = base + w;
+            c.row0 = max(s0 + c.index * DELTA_CHUNK, 0);
+            c.rows = max(0, min(min(DELTA_CHUNK, L - c.index * DELTA_CHUNK), T - c.row0));
+            return true;
+        }
+        slot -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    c.index = slot;
+    return false;
+}
+// segment -> its first slot, its chunks and first row, by a whole wave
+__device__ __forceinline__ void delta_segment(const int32_t *cu, int N, int seg, int &slot0, int &chunks, int &s0, int &L) {
+    const int lane = threadIdx.x & 63;
+    slot0 = 0;
+    for (int base = 0; base < seg; base += 64) {
+        const int i = min(base + lane, N - 1), len = cu[i + 1] - cu[i];
+        slot0 += wave_sum_i(base + lane < seg && len > 0 ? (len + DELTA_CHUNK - 1) / DELTA_CHUNK : 0);
+    }
+    s0 = cu[seg];
+    L = max(cu[seg + 1] - s0, 0);
+    chunks = (L + DELTA_CHUNK - 1) / DELTA_CHUNK;
+}
+
+// What a wave's lanes wrote to LDS is there for its other lanes: the hardware keeps a wave's LDS operations in order, the compiler has to.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// ---- fragments of mfma16 (16x16x32): lane l of a row-major tile ------------------------------------------------------------------------
+// rows r0 + l%16, columns c0 + 8 (l/16) ..: an operand whose contraction runs along the row
+__device__ __forceinline__ bf16x8 frag_n(const bf16_t *t, int stride, int r0, int c0) {
+    const int l = threadIdx.x & 63;
+    return *reinterpret_cast<const bf16x8 *>(t + (r0 + (l & 15)) * stride + c0 + 8 * (l >> 4));
+}
+// rows k0 + 8 (l/16) .., column m0 + l%16: an operand whose contraction runs down the rows
+__device__ __forceinline__ bf16x8 frag_t(bf16_t *t, int stride, int k0, int m0) {
+    const int l = threadIdx.x & 63, s = l & 15;
+    bf16_t *const p = t + (k0 + 8 * (l >> 4) + (s >> 2)) * stride + m0 + 4 * (s & 3);
+    return tr_pair((lds_u8 *)p, (lds_u8 *)(p + 4 * stride));
+}
+__device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+
+typedef uint32_t __attribute__((may_alias, ext_vector_type(2))) u32x2_any;
+typedef uint32_t __attribute__((may_alias, ext_vector_type(4))) u32x4_any;
+__device__ __forceinline__ u32x2 hi4(f32x4 x) { return u32x2{pack2bf(x[0], x[1]), pack2bf(x[2], x[3])}; }
+// what hi4 left over
+__device__ __forceinline__ u32x2 lo4(f32x4 x, u32x2 h) {
+    return u32x2{pack2bf(x[0] - __uint_as_float(h[0] << 16), x[1] - __uint_as_float(h[0] & 0xffff0000u)),
+                 pack2bf(x[2] - __uint_as_float(h[1] << 16), x[3] - __uint_as_float(h[1] & 0xffff0000u))};
+}
+__device__ __forceinline__ void put4(bf16_t *p, u32x2 x) { *reinterpret_cast<u32x2_any *>(p) = x; }
+__device__ __forceinline__ void put_split4(bf16_t *h, bf16_t *l, f32x4 x) {
+    const u32x2 a = hi4(x);
+    put4(h, a);
+    put4(l, lo4(x, a));
+}
+
+// ---- tiles of 64 rows by 256 threads: global -> registers -> LDS -------------------------------------------------------------------------
+template <int W> struct Tile64 { u32x4 x[W / 32]; };
+// rows of `width` (a multiple of 8, at most W) elements, `tok` elements apart; beyond `rows` and `width` zero
+template <int W>
+__device__ __forceinline__ void tile_load(Tile64<W> &t, const bf16_t *src, int64_t tok, int rows, int width) {
+#pragma unroll
+    for (int u = 0; u < W / 32; ++u) {
+        const int i = threadIdx.x + 256 * u, r = i / (W / 8), c = i % (W / 8) * 8;
+        t.x[u] = r < rows && c < width ? *reinterpret_cast<const u32x4 *>(src + r * tok + c) : u32x4{0u, 0u, 0u, 0u};
+    }
+}
+template <int W>
+__device__ __forceinline__ void tile_put(const Tile64<W> &t, bf16_t *lds, int stride) {
+#pragma unroll
+    for (int u = 0; u < W / 32; ++u) {
+        const int i = threadIdx.x + 256 * u;
+        *reinterpret_cast<u32x4_any *>(lds + i / (W / 8) * stride + i % (W / 8) * 8) = t.x[u];
+    }
+}
+template <int W>
+__device__ __forceinline__ void tile_copy(bf16_t *lds, int stride, const bf16_t *src, int64_t tok, int rows, int width) {
+    Tile64<W> t;
+    tile_load<W>(t, src, tok, rows, width);
+    tile_put<W>(t, lds, stride);
+}
+
+__device__ __forceinline__ float load_any(const void *p, int64_t i, int f32) {
+    return f32 ? reinterpret_cast<const float *>(p)[i] : (float)reinterpret_cast<const bf16_t *>(p)[i];
+}
+__device__ __forceinline__ void store_any(void *p, int64_t i, int f32, float x) {
+    if (f32) reinterpret_cast<float *>(p)[i] = x;
+    else reinterpret_cast<bf16_t *>(p)[i] = (bf16_t)x;
+}
+__device__ __forceinline__ float softplus_f(float x) { return x > 20.f ? x : log1pf(expf(x)); }
+// the log decay of a row.  Held above -1e4, where e^g has long been zero: a decay of -inf would make G_i - G_j of later rows NaN.  (A NaN stays one.)
+__device__ __forceinline__ float delta_gate(const dsa_delta_args &in, int64_t t, int h) {
+    const float x = load_any(in.a, t * in.a_tok + h, in.a_f32) + load_any(in.dt_bias, h, in.param_f32);
+    const float g = -expf(load_any(in.a_log, h, in.param_f32)) * softplus_f(x);
+    return g < -1e4f ? -1e4f : g;
+}
+__device__ __forceinline__ float delta_beta(const dsa_delta_args &in, int64_t t, int h) {
+    return 1.f / (1.f + expf(-load_any(in.b, t * in.b_tok + h, in.b_f32)));
+}

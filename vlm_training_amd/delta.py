@@ -1,0 +1,37 @@
+"""The gated delta rule: the token mixer of the linear-attention layers in the reference's hybrid stack.
+
+``gated_delta_rule``  runs packed sequences in chunks (models/qwen3_5/model.py:178-186: ``q``, ``k`` normalised inside, decay and write strength
+                      from the projections ``a``, ``b`` and the parameters ``a_log``, ``dt_bias``), with gradients for every input, from and to states.
+``gated_delta_step``  one token for each of a batch of requests, the states updated in place (decoding).
+
+Per value head a state ``S`` (Dk, Dv) in fp32, with ``g = -exp(a_log) * softplus(a + dt_bias)`` and ``beta = sigmoid(b)``:
+``S = exp(g) * S + beta * k (v - exp(g) * S^T k)^T``, ``o = scale * S^T q``.  Value head ``h`` reads key head ``h // (Hv // Hk)``.
+Autograd nodes in csrc/dsa_host_layer.cpp over the C ABI; there is no fallback path.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+
+@torch.compiler.disable
+def gated_delta_rule(q, k, v, a, b, a_log, dt_bias, cu_seqlens, *, scale=None, l2_norm: bool = True, initial_state=None,
+                     return_final_state: bool = False):
+    """q, k (T, Hk, Dk), v (T, Hv, Dv) bf16 views, a, b (T, Hv), a_log, dt_bias (Hv,) bf16 or fp32 -> (T, Hv, Dv) bf16.
+
+    Head dims are multiples of 8 up to 128.  ``scale`` defaults to ``Dk ** -0.5``; ``l2_norm=False`` takes q and k as they are.
+    ``cu_seqlens`` (N+1,) are the packed sequences' offsets (empty ones allowed); rows behind the last sequence give zeros.  ``initial_state`` (N, Hv, Dk, Dv)
+    fp32 is where the sequences start (zeros without one); with ``return_final_state`` the states behind them come as a second result, fp32.
+    Both states take part in the backward pass.
+
+    With a graph the call keeps, beside its inputs, about 1.3 KB per row and value head of 128 x 128 for the backward pass."""
+    out = _lib.host().gated_delta_rule(q, k, v, a, b, a_log, dt_bias, cu_seqlens, scale, bool(l2_norm), initial_state, bool(return_final_state))
+    return tuple(out) if return_final_state else out[0]
+
+
+@torch.compiler.disable
+def gated_delta_step(q, k, v, a, b, a_log, dt_bias, state, *, scale=None, l2_norm: bool = True):
+    """The next token of B requests: q, k (B, Hk, Dk), v (B, Hv, Dv), a, b (B, Hv) -> (B, Hv, Dv); ``state`` (B, Hv, Dk, Dv) fp32 is
+    updated in place (a slice of a larger pool of requests will do).  No backward pass."""
+    return _lib.host().gated_delta_step(q, k, v, a, b, a_log, dt_bias, state, scale, bool(l2_norm))
