@@ -429,6 +429,53 @@ int dsa_delta_bwd(const dsa_delta_args *args, const void *dout, const float *dfi
                   void *da, void *db, void *da_log, void *ddt_bias, float *dinitial, void *scratch, size_t scratch_bytes, void *stream);
 int dsa_delta_step(const dsa_delta_args *args, float *state, int64_t state_stride, void *out, void *stream);
 
+/*
+ * Short causal convolution over packed sequences (models/qwen3_5/model.py:173-176), depthwise: z_t = bias + sum_{j<W} w[c][W-1-j] x_{t-j} inside
+ * a sequence, y = z sigmoid(z) with `silu`, else z.  x (T,C) bf16, rows x_tok elements apart; w (C,W), bias (C, may be null) bf16 or fp32
+ * (w_f32, bias_f32); W 2 to 4, C and strides multiples of 8, rows on 16-byte boundaries; y, dx (T,C) bf16 contiguous; rows behind cu[N] give zeros.
+ * initial (N,C,W-1) bf16 holds the inputs before a sequence's first row (null: zeros); final, the same, receives each one's last W-1 inputs.
+ * dsa_conv_bwd: dy (T,C) bf16 rows dy_tok apart -> dx, dw, dbias in their inputs' types (dbias null without a bias).  `ws` holds
+ * dsa_conv_bwd_workspace_bytes(T, C, W) bytes.  dsa_conv_step: one token for each of B requests, state (B,C,W-1) bf16, requests
+ * state_stride elements apart, moves on in place.
+ */
+size_t dsa_conv_bwd_workspace_bytes(int T, int C, int W);
+int dsa_conv_fwd(const void *x, int64_t x_tok, const void *w, int w_f32, const void *bias, int bias_f32, int silu, const int32_t *cu_seqlens, int T,
+                 int N, int C, int W, const void *initial, void *y, void *final, void *stream);
+int dsa_conv_bwd(const void *x, int64_t x_tok, const void *dy, int64_t dy_tok, const void *w, int w_f32, const void *bias, int bias_f32, int silu,
+                 const int32_t *cu_seqlens, int T, int N, int C, int W, const void *initial, void *dx, void *dw, void *dbias, void *ws,
+                 size_t ws_bytes, void *stream);
+int dsa_conv_step(const void *x, int64_t x_tok, const void *w, int w_f32, const void *bias, int bias_f32, int silu, int B, int C, int W, void *state,
+                  int64_t state_stride, void *y, void *stream);
+
+/*
+ * Norm of a block's output fused with its SiLU gate (models/qwen3_5/model.py:38-44): y = x rsqrt(mean x^2 + eps) (w + offset) z sigmoid(z) per row of D.
+ * x, z (T,H,D) bf16 with token and head strides that are multiples of 8, rows on 16-byte boundaries; w (D) bf16 or fp32; D a multiple of 8 up
+ * to 512; y, dx, dz contiguous; rstd (T,H) fp32 (may be null in the forward where no backward follows).  dw in w's type; `ws` holds
+ * dsa_gated_norm_bwd_workspace_bytes(T, H, D) bytes.
+ */
+size_t dsa_gated_norm_bwd_workspace_bytes(int T, int H, int D);
+int dsa_gated_norm_fwd(const void *x, int64_t x_tok, int64_t x_head, const void *z, int64_t z_tok, int64_t z_head, const void *w, int w_f32, float eps,
+                       float offset, int T, int H, int D, void *y, float *rstd, void *stream);
+int dsa_gated_norm_bwd(const void *dy, const void *x, int64_t x_tok, int64_t x_head, const void *z, int64_t z_tok, int64_t z_head, const void *w,
+                       int w_f32, float offset, int T, int H, int D, const float *rstd, void *dx, void *dz, void *dw, void *ws, size_t ws_bytes,
+                       void *stream);
+
+/*
+ * Residual add and the next block's norm (models/qwen3_5/model.py, the decoder layer's two additions): xn = x + scale sigmoid(gate) n, h = norm(xn) (w + offset),
+ * with n = norm(y) (post + offset), or y where post is null; gate and scale may be null.  x, xn (T,C) bf16 or fp32 (x_f32), y, gate, h (T,C) bf16, all
+ * contiguous on 16-byte boundaries; w, post, scale (C) bf16 or fp32; C a multiple of 8 up to 8192.  rstd, rstd_y (T) fp32 may be null where no backward follows.
+ * dsa_residual_norm_bwd: dxn (as xn) and dh, either may be null -> dx (as x), dy, dgate, dw, dpost, dscale (the last three where their inputs are
+ * there).  `ws` holds dsa_residual_norm_bwd_workspace_bytes(T, C) bytes.
+ */
+size_t dsa_residual_norm_bwd_workspace_bytes(int T, int C);
+int dsa_residual_norm_fwd(const void *x, int x_f32, const void *y, const void *gate, const void *w, int w_f32, const void *post, int post_f32,
+                          const void *scale, int scale_f32, float eps, float offset, int T, int C, void *xn, void *h, float *rstd, float *rstd_y,
+                          void *stream);
+int dsa_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x_f32, const void *y, const void *gate, const void *w, int w_f32,
+                          const void *post, int post_f32, const void *scale, int scale_f32, float offset, int T, int C, const float *rstd,
+                          const float *rstd_y, void *dx, void *dy, void *dgate, void *dw, void *dpost, void *dscale, void *ws, size_t ws_bytes,
+                          void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,6 +35,24 @@ _SIGNATURES = {
     "dsa_delta_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                               c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "dsa_delta_step": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "dsa_conv_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "dsa_conv_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int,
+                             c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dsa_conv_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int,
+                             c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "dsa_conv_step": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                              c_int64, c_void_p, c_void_p]),
+    "dsa_gated_norm_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "dsa_gated_norm_fwd": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int, c_float, c_float,
+                                   c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "dsa_gated_norm_bwd": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int, c_float,
+                                   c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "dsa_residual_norm_bwd_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "dsa_residual_norm_fwd": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
+                                      c_float, c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dsa_residual_norm_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                      c_int, c_void_p, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "dsa_version": (c_char_p, []),
     "dsa_last_error": (c_char_p, []),
     "dsa_indexer_scores": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int,

@@ -12,6 +12,16 @@
 #include "../../include/dsa_attn.h"
 
 extern "C" {
+int dsa_conv_blocks(int T, int C);
+hipError_t dsa_launch_conv_fwd(const void *x, int64_t x_tok, const void *w, int w_f32, const void *bias, int b_f32, int silu, const int32_t *cu, int T, int N, int C, int W, const void *state, void *y, void *final, hipStream_t stream);
+hipError_t dsa_launch_conv_bwd(const void *x, int64_t x_tok, const void *dy, int64_t dy_tok, const void *w, int w_f32, const void *bias, int b_f32, int silu, const int32_t *cu, int T, int N, int C, int W, const void *state, void *dx, void *dw, void *dbias, float *part, hipStream_t stream);
+hipError_t dsa_launch_conv_step(const void *x, int64_t x_tok, const void *w, int w_f32, const void *bias, int b_f32, int silu, int B, int C, int W, void *state, int64_t state_req, void *y, hipStream_t stream);
+int dsa_gated_norm_blocks(int64_t rows, int D);
+hipError_t dsa_launch_gated_norm_fwd(const void *x, int64_t x_tok, int64_t x_head, const void *z, int64_t z_tok, int64_t z_head, const void *w, int w_f32, float eps, float offset, int T, int H, int D, void *y, float *rstd, hipStream_t stream);
+hipError_t dsa_launch_gated_norm_bwd(const void *dy, const void *x, int64_t x_tok, int64_t x_head, const void *z, int64_t z_tok, int64_t z_head, const void *w, int w_f32, float offset, int T, int H, int D, const float *rstd, void *dx, void *dz, void *dw, float *part, hipStream_t stream);
+int dsa_residual_norm_blocks(int64_t rows, int C);
+hipError_t dsa_launch_residual_norm_fwd(const void *x, int x_f32, const void *y, const void *gate, const void *w, int w_f32, const void *post, int post_f32, const void *scale, int scale_f32, float eps, float offset, int T, int C, void *xn, void *h, float *rstd, float *rstd_y, hipStream_t stream);
+hipError_t dsa_launch_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x_f32, const void *y, const void *gate, const void *w, int w_f32, const void *post, int post_f32, const void *scale, int scale_f32, float offset, int T, int C, const float *rstd, const float *rstd_y, void *dx, void *dy, void *dgate, void *dw, void *dpost, void *dscale, float *part, hipStream_t stream);
 hipError_t dsa_launch_delta_fwd(const DeltaArgs *a, int save, hipStream_t stream);
 hipError_t dsa_launch_delta_bwd(const DeltaArgs *a, hipStream_t stream);
 hipError_t dsa_launch_delta_step(const dsa_delta_args *in, float *state, int64_t state_req, void *out, hipStream_t stream);
@@ -1127,4 +1137,116 @@ extern "C" int dsa_delta_step(const dsa_delta_args *args, float *state, int64_t 
         return fail(DSA_ERR_ARG, "state: requests must lie on 16-byte boundaries and apart from each other");
     const hipError_t e = dsa_launch_delta_step(args, state, state_stride, out, (hipStream_t)stream);
     return e == hipSuccess ? DSA_OK : hip_fail(e, "gated delta rule step launch");
+}
+
+// ---------------------------------------------------------------------------------------------------
+// short convolution, gated norm, residual norm
+// ---------------------------------------------------------------------------------------------------
+static bool off16(const void *p) { return ((uintptr_t)p & 15) != 0; }
+static int check_conv(const void *x, int64_t x_tok, const void *w, const int32_t *cu, int T, int N, int C, int W) {
+    if (T < 0 || N < 1 || !cu) return fail(DSA_ERR_ARG, "T=%d N=%d", T, N);
+    if (W < 2 || W > 4) return fail(DSA_ERR_UNSUPPORTED, "convolution width %d: need 2 to 4", W);
+    if (C < 8 || C % 8) return fail(DSA_ERR_UNSUPPORTED, "channels=%d: need a multiple of 8", C);
+    if (!w || (T > 0 && !x)) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if (x_tok % 8 || off16(x)) return fail(DSA_ERR_ARG, "rows must lie on 16-byte boundaries");
+    return DSA_OK;
+}
+extern "C" size_t dsa_conv_bwd_workspace_bytes(int T, int C, int W) {
+    if (T <= 0 || C < 8 || W < 2) return 0;
+    return (size_t)dsa_conv_blocks(T, C) * C * (W + 1) * sizeof(float);
+}
+extern "C" int dsa_conv_fwd(const void *x, int64_t x_tok, const void *w, int w_f32, const void *bias, int bias_f32, int silu, const int32_t *cu, int T, int N, int C,
+                            int W, const void *initial, void *y, void *final, void *stream) {
+    if (int rc = check_conv(x, x_tok, w, cu, T, N, C, W)) return rc;
+    if (T > 0 && (!y || off16(y))) return fail(DSA_ERR_ARG, "y: null or not on a 16-byte boundary");
+    const hipError_t e = dsa_launch_conv_fwd(x, x_tok, w, w_f32, bias, bias_f32, silu, cu, T, N, C, W, initial, y, final, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "convolution forward launch");
+}
+extern "C" int dsa_conv_bwd(const void *x, int64_t x_tok, const void *dy, int64_t dy_tok, const void *w, int w_f32, const void *bias, int bias_f32, int silu,
+                            const int32_t *cu, int T, int N, int C, int W, const void *initial, void *dx, void *dw, void *dbias, void *ws, size_t ws_bytes,
+                            void *stream) {
+    if (int rc = check_conv(x, x_tok, w, cu, T, N, C, W)) return rc;
+    if (!dw || (bias && !dbias) || (T > 0 && (!dy || !dx))) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if (dy_tok % 8 || off16(dy) || off16(dx)) return fail(DSA_ERR_ARG, "rows must lie on 16-byte boundaries");
+    const size_t need = dsa_conv_bwd_workspace_bytes(T, C, W);
+    if (need && (!ws || ws_bytes < need)) return fail(DSA_ERR_WORKSPACE, "convolution backward workspace: have %zu bytes, need %zu", ws_bytes, need);
+    const hipError_t e = dsa_launch_conv_bwd(x, x_tok, dy, dy_tok, w, w_f32, bias, bias_f32, silu, cu, T, N, C, W, initial, dx, dw, bias ? dbias : nullptr, (float *)ws,
+                                             (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "convolution backward launch");
+}
+extern "C" int dsa_conv_step(const void *x, int64_t x_tok, const void *w, int w_f32, const void *bias, int bias_f32, int silu, int B, int C, int W, void *state,
+                             int64_t state_stride, void *y, void *stream) {
+    const int32_t none = 0;                              // (no offsets here)
+    if (int rc = check_conv(x, x_tok, w, &none, B, 1, C, W)) return rc;
+    if (B == 0) return DSA_OK;
+    if (!state || !y || off16(y)) return fail(DSA_ERR_ARG, "state or y: null or not on a 16-byte boundary");
+    if (off16(state) || state_stride % 8 || (B > 1 && state_stride < (int64_t)C * (W - 1)))
+        return fail(DSA_ERR_ARG, "state: requests must lie on 16-byte boundaries and apart from each other");
+    const hipError_t e = dsa_launch_conv_step(x, x_tok, w, w_f32, bias, bias_f32, silu, B, C, W, state, state_stride, y, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "convolution step launch");
+}
+
+static int check_gated_norm(const void *x, int64_t x_tok, int64_t x_head, const void *z, int64_t z_tok, int64_t z_head, const void *w, int T, int H, int D) {
+    if (T < 0 || H < 1) return fail(DSA_ERR_ARG, "T=%d H=%d", T, H);
+    if (D < 8 || D > 512 || D % 8) return fail(DSA_ERR_UNSUPPORTED, "row length %d: need a multiple of 8 up to 512", D);
+    if (!w || (T > 0 && (!x || !z))) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if ((x_tok | x_head | z_tok | z_head) % 8 || off16(x) || off16(z)) return fail(DSA_ERR_ARG, "rows must lie on 16-byte boundaries");
+    return DSA_OK;
+}
+extern "C" size_t dsa_gated_norm_bwd_workspace_bytes(int T, int H, int D) {
+    if (T <= 0 || H < 1 || D < 8) return 0;
+    return (size_t)dsa_gated_norm_blocks((int64_t)T * H, D) * D * sizeof(float);
+}
+extern "C" int dsa_gated_norm_fwd(const void *x, int64_t x_tok, int64_t x_head, const void *z, int64_t z_tok, int64_t z_head, const void *w, int w_f32, float eps,
+                                  float offset, int T, int H, int D, void *y, float *rstd, void *stream) {
+    if (int rc = check_gated_norm(x, x_tok, x_head, z, z_tok, z_head, w, T, H, D)) return rc;
+    if (T > 0 && (!y || off16(y))) return fail(DSA_ERR_ARG, "y: null or not on a 16-byte boundary");
+    const hipError_t e = dsa_launch_gated_norm_fwd(x, x_tok, x_head, z, z_tok, z_head, w, w_f32, eps, offset, T, H, D, y, rstd, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "gated norm forward launch");
+}
+extern "C" int dsa_gated_norm_bwd(const void *dy, const void *x, int64_t x_tok, int64_t x_head, const void *z, int64_t z_tok, int64_t z_head, const void *w, int w_f32,
+                                  float offset, int T, int H, int D, const float *rstd, void *dx, void *dz, void *dw, void *ws, size_t ws_bytes, void *stream) {
+    if (int rc = check_gated_norm(x, x_tok, x_head, z, z_tok, z_head, w, T, H, D)) return rc;
+    if (!dw || (T > 0 && (!dy || !rstd || !dx || !dz))) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if (off16(dy) || off16(dx) || off16(dz)) return fail(DSA_ERR_ARG, "rows must lie on 16-byte boundaries");
+    const size_t need = dsa_gated_norm_bwd_workspace_bytes(T, H, D);
+    if (need && (!ws || ws_bytes < need)) return fail(DSA_ERR_WORKSPACE, "gated norm backward workspace: have %zu bytes, need %zu", ws_bytes, need);
+    const hipError_t e = dsa_launch_gated_norm_bwd(dy, x, x_tok, x_head, z, z_tok, z_head, w, w_f32, offset, T, H, D, rstd, dx, dz, dw, (float *)ws, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "gated norm backward launch");
+}
+
+static int check_residual_norm(const void *w, int T, int C) {
+    if (T < 0) return fail(DSA_ERR_ARG, "T=%d", T);
+    if (C < 8 || C > 8192 || C % 8) return fail(DSA_ERR_UNSUPPORTED, "row length %d: need a multiple of 8 up to 8192", C);
+    if (!w) return fail(DSA_ERR_ARG, "null tensor pointer");
+    return DSA_OK;
+}
+extern "C" size_t dsa_residual_norm_bwd_workspace_bytes(int T, int C) {
+    if (T <= 0 || C < 8) return 0;
+    return (size_t)dsa_residual_norm_blocks(T, C) * 3 * C * sizeof(float);
+}
+extern "C" int dsa_residual_norm_fwd(const void *x, int x_f32, const void *y, const void *gate, const void *w, int w_f32, const void *post, int post_f32,
+                                     const void *scale, int scale_f32, float eps, float offset, int T, int C, void *xn, void *h, float *rstd, float *rstd_y,
+                                     void *stream) {
+    if (int rc = check_residual_norm(w, T, C)) return rc;
+    if (T > 0 && (!x || !y || !xn || !h)) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if (off16(x) || off16(y) || off16(gate) || off16(xn) || off16(h)) return fail(DSA_ERR_ARG, "rows must lie on 16-byte boundaries");
+    const hipError_t e = dsa_launch_residual_norm_fwd(x, x_f32, y, gate, w, w_f32, post, post_f32, scale, scale_f32, eps, offset, T, C, xn, h, rstd, rstd_y,
+                                                      (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "residual norm forward launch");
+}
+extern "C" int dsa_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x_f32, const void *y, const void *gate, const void *w, int w_f32,
+                                     const void *post, int post_f32, const void *scale, int scale_f32, float offset, int T, int C, const float *rstd,
+                                     const float *rstd_y, void *dx, void *dy, void *dgate, void *dw, void *dpost, void *dscale, void *ws, size_t ws_bytes,
+                                     void *stream) {
+    if (int rc = check_residual_norm(w, T, C)) return rc;
+    if (!dw || (post && !dpost) || (scale && !dscale)) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if (T > 0 && (!xn || !rstd || !dx || !dy || (gate && !dgate) || ((post || gate || scale) && !y) || (post && !rstd_y))) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if (off16(dxn) || off16(dh) || off16(xn) || off16(y) || off16(gate) || off16(dx) || off16(dy) || off16(dgate))
+        return fail(DSA_ERR_ARG, "rows must lie on 16-byte boundaries");
+    const size_t need = dsa_residual_norm_bwd_workspace_bytes(T, C);
+    if (need && (!ws || ws_bytes < need)) return fail(DSA_ERR_WORKSPACE, "residual norm backward workspace: have %zu bytes, need %zu", ws_bytes, need);
+    const hipError_t e = dsa_launch_residual_norm_bwd(dxn, dh, xn, x_f32, y, gate, w, w_f32, post, post_f32, scale, scale_f32, offset, T, C, rstd, rstd_y, dx, dy, dgate, dw,
+                                                      dpost, dscale, (float *)ws, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "residual norm backward launch");
 }

@@ -156,10 +156,234 @@ Tensor gated_delta_step(const Tensor &q, const Tensor &k, const Tensor &v, const
     return out;
 }
 
+// ---- short convolution ------------------------------------------------------------------------------------------------------
+struct ConvInputs { Tensor x, w, bias; int64_t T, C, W; int f32, bias_f32; };
+ConvInputs conv_inputs(const Tensor &x, const Tensor &w, const OptTensor &bias) {
+    need_gpu(x);
+    need_gpu(w);
+    same_device(x, w, "weight");
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.scalar_type() == at::kBFloat16 && x.size(0) <= INT32_MAX, "x must be a bf16 (T, channels) tensor");
+    TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) == x.size(1) && half_or_float(w), "weight must be (", x.size(1), ", width) bf16 or fp32");
+    ConvInputs in{x, w.contiguous(), Tensor(), x.size(0), x.size(1), w.size(1), w.scalar_type() == at::kFloat, 0};
+    if (!(x.numel() == 0 || (x.stride(1) == 1 && (in.T == 1 || x.stride(0) % 8 == 0) && aligned16(x)))) {
+        in.x = x.contiguous();
+        if (!aligned16(in.x)) in.x = in.x.clone();
+    }
+    if (bias) {
+        need_gpu(*bias);
+        same_device(x, *bias, "bias");
+        TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == in.C && half_or_float(*bias), "bias must be (", in.C, ") bf16 or fp32");
+        in.bias = bias->contiguous();
+        in.bias_f32 = bias->scalar_type() == at::kFloat;
+    }
+    return in;
+}
+void check_conv_state(const Tensor &s, const Tensor &x, at::IntArrayRef sizes) {
+    need_gpu(s);
+    same_device(x, s, "the state");
+    TORCH_CHECK_VALUE(s.sizes() == sizes && s.scalar_type() == at::kBFloat16, "the state must be a ", sizes, " bf16 tensor, not ", s.sizes(), " ", s.scalar_type());
+}
+
+class ConvNode : public torch::autograd::Function<ConvNode> {
+public:
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &bias, const Tensor &cu, const OptTensor &initial_, bool silu,
+                                 bool want_final) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const ConvInputs in = conv_inputs(x, w, bias);
+        const int64_t N = cu.numel() - 1;
+        Tensor initial;
+        if (initial_) {
+            check_conv_state(*initial_, x, {N, in.C, in.W - 1});
+            initial = initial_->contiguous();
+        }
+        const Tensor y = empty({in.T, in.C}, at::kBFloat16, x), last = want_final ? empty({N, in.C, in.W - 1}, at::kBFloat16, x) : Tensor();
+        check(dsa_conv_fwd(ptr(in.x), in.T > 1 ? in.x.stride(0) : 0, ptr(in.w), in.f32, ptr(in.bias), in.bias_f32, silu, iptr(cu), (int)in.T, (int)N, (int)in.C, (int)in.W,
+                           ptr(initial), ptr(y), ptr(last), stream_of(x)), "dsa_conv_fwd");
+        ctx->save_for_backward({in.x, in.w, in.bias, cu, initial});
+        ctx->saved_data["s"] = silu;
+        ctx->set_materialize_grads(false);
+        if (!want_final) return {y};
+        ctx->mark_non_differentiable({last});
+        return {y, last};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        if (!grads[0].defined()) return variable_list(7);
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor &x = s[0], &w = s[1], &bias = s[2], &cu = s[3], &initial = s[4];
+        const c10::OptionalDeviceGuard guard(x.device());
+        const int64_t T = x.size(0), C = x.size(1), W = w.size(1);
+        const Tensor dy = as_bf16(grads[0]), dx = empty({T, C}, at::kBFloat16, x), dw = empty(w.sizes(), w.scalar_type(), x);
+        const Tensor dbias = bias.defined() ? empty({C}, bias.scalar_type(), x) : Tensor();
+        const size_t bytes = dsa_conv_bwd_workspace_bytes((int)T, (int)C, (int)W);
+        const Tensor ws = empty_bytes(bytes, x);
+        check(dsa_conv_bwd(ptr(x), T > 1 ? x.stride(0) : 0, ptr(dy), C, ptr(w), w.scalar_type() == at::kFloat, ptr(bias), bias.defined() && bias.scalar_type() == at::kFloat,
+                           ctx->saved_data["s"].toBool(), iptr(cu), (int)T, (int)cu.numel() - 1, (int)C, (int)W, ptr(initial), ptr(dx), ptr(dw), ptr(dbias), ptr(ws), bytes,
+                           stream_of(x)), "dsa_conv_bwd");
+        return {dx, dw, dbias, Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+variable_list short_conv(const Tensor &x, const Tensor &w, const OptTensor &bias, const Tensor &cu, bool silu, const OptTensor &initial, bool want_final) {
+    const Tensor none;
+    no_forward_mode({&x, &w, bias ? &*bias : &none, initial ? &*initial : &none}, "short_conv");
+    need_gpu(x);
+    need_gpu(cu);
+    same_device(x, cu, "cu_seqlens");
+    TORCH_CHECK_VALUE(!initial || !initial->requires_grad(), "initial_state takes no part in the backward pass: detach it");
+    const c10::OptionalDeviceGuard guard(x.device());
+    return ConvNode::apply(x, w, bias, checked_cu(cu), initial, silu, want_final);
+}
+
+Tensor short_conv_step(const Tensor &x, const Tensor &state, const Tensor &w, const OptTensor &bias, bool silu) {
+    const Tensor none;
+    no_forward_mode({&x, &w, bias ? &*bias : &none, &state}, "short_conv_step");
+    no_graph({&x, &state, &w, bias ? &*bias : &none}, "short_conv_step");
+    need_gpu(x);
+    const c10::OptionalDeviceGuard guard(x.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    const ConvInputs in = conv_inputs(x, w, bias);
+    const int64_t B = in.T, per = in.C * (in.W - 1);
+    check_conv_state(state, x, {B, in.C, in.W - 1});
+    TORCH_CHECK_VALUE(B == 0 || (state.select(0, 0).is_contiguous() && aligned16(state) && (B == 1 || (state.stride(0) % 8 == 0 && state.stride(0) >= per))),
+                      "the state is updated in place: each request's part must be contiguous, on a 16-byte boundary and apart from the others");
+    const Tensor y = empty({B, in.C}, at::kBFloat16, x);
+    check(dsa_conv_step(ptr(in.x), B > 1 ? in.x.stride(0) : 0, ptr(in.w), in.f32, ptr(in.bias), in.bias_f32, silu, (int)B, (int)in.C, (int)in.W, ptr(state),
+                        B > 1 ? state.stride(0) : 0, ptr(y), stream_of(x)), "dsa_conv_step");
+    torch::autograd::impl::bump_version(state);
+    return y;
+}
+
+// ---- norms behind and between blocks -------------------------------------------------------------------------------------------
+class GatedNormNode : public torch::autograd::Function<GatedNormNode> {
+public:
+    static Tensor forward(AutogradContext *ctx, const Tensor &x_, const Tensor &gate, const Tensor &weight, double eps, bool offset) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        for (const Tensor *t : {&x_, &gate, &weight}) {
+            need_gpu(*t);
+            same_device(x_, *t, "a tensor");
+        }
+        check_bf16_thd(x_, "x");
+        check_bf16_thd(gate, "gate");
+        TORCH_CHECK_VALUE(gate.sizes() == x_.sizes(), "gate must have the shape of x");
+        const int64_t T = x_.size(0), H = x_.size(1), D = x_.size(2);
+        TORCH_CHECK_VALUE(weight.dim() == 1 && weight.size(0) == D && half_or_float(weight), "weight must be (", D, ") bf16 or fp32");
+        TORCH_CHECK_VALUE(T <= INT32_MAX, "too many rows: ", T);
+        const Tensor x = rows16(x_), z = rows16(gate), w = weight.contiguous();
+        const Tensor y = empty(x.sizes(), at::kBFloat16, x), rstd = empty({T, H}, at::kFloat, x);
+        check(dsa_gated_norm_fwd(ptr(x), tok_of(x), head_of(x), ptr(z), tok_of(z), head_of(z), ptr(w), w.scalar_type() == at::kFloat, (float)eps, offset ? 1.f : 0.f, (int)T,
+                                 (int)H, (int)D, ptr(y), fptr(rstd), stream_of(x)), "dsa_gated_norm_fwd");
+        ctx->save_for_backward({x, z, w, rstd});
+        ctx->saved_data["o"] = offset;
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor &x = s[0], &z = s[1], &w = s[2], &rstd = s[3];
+        const c10::OptionalDeviceGuard guard(x.device());
+        const int64_t T = x.size(0), H = x.size(1), D = x.size(2);
+        const Tensor dy = as_bf16(grads[0]), dx = empty(x.sizes(), at::kBFloat16, x), dz = empty(x.sizes(), at::kBFloat16, x), dw = empty({D}, w.scalar_type(), x);
+        const size_t bytes = dsa_gated_norm_bwd_workspace_bytes((int)T, (int)H, (int)D);
+        const Tensor ws = empty_bytes(bytes, x);
+        check(dsa_gated_norm_bwd(ptr(dy), ptr(x), tok_of(x), head_of(x), ptr(z), tok_of(z), head_of(z), ptr(w), w.scalar_type() == at::kFloat,
+                                 ctx->saved_data["o"].toBool() ? 1.f : 0.f, (int)T, (int)H, (int)D, fptr(rstd), ptr(dx), ptr(dz), ptr(dw), ptr(ws), bytes, stream_of(x)),
+              "dsa_gated_norm_bwd");
+        return {dx, dz, dw, Tensor(), Tensor()};
+    }
+};
+
+Tensor gated_rms_norm(const Tensor &x, const Tensor &gate, const Tensor &weight, double eps, bool offset) {
+    no_forward_mode({&x, &gate, &weight}, "gated_rms_norm");
+    need_gpu(x);
+    const c10::OptionalDeviceGuard guard(x.device());
+    return GatedNormNode::apply(x, gate, weight, eps, offset);
+}
+
+Tensor packed_rows(const Tensor &x) {
+    const Tensor c = x.contiguous();
+    return aligned16(c) ? c : c.clone();
+}
+
+class ResidualNormNode : public torch::autograd::Function<ResidualNormNode> {
+public:
+    // everything (T, C) and (C)
+    static variable_list forward(AutogradContext *ctx, const Tensor &x_, const Tensor &y_, const Tensor &weight, const OptTensor &post_, const OptTensor &gate_,
+                                 const OptTensor &scale_, double eps, bool offset) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const int64_t T = x_.size(0), C = x_.size(1);
+        auto parameter = [&](const OptTensor &t, const char *name) {
+            if (!t) return Tensor();
+            need_gpu(*t);
+            same_device(x_, *t, name);
+            TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == C && half_or_float(*t), name, " must be (", C, ") bf16 or fp32");
+            return t->contiguous();
+        };
+        const Tensor w = parameter(weight, "weight"), post = parameter(post_, "post_weight"), scale = parameter(scale_, "scale");
+        const Tensor x = packed_rows(x_), y = packed_rows(y_), gate = gate_ ? packed_rows(*gate_) : Tensor();
+        auto f32 = [](const Tensor &t) { return t.defined() && t.scalar_type() == at::kFloat; };
+        const Tensor xn = empty({T, C}, x.scalar_type(), x), h = empty({T, C}, at::kBFloat16, x), rstd = empty({T}, at::kFloat, x);
+        const Tensor rstd_y = post.defined() ? empty({T}, at::kFloat, x) : Tensor();
+        check(dsa_residual_norm_fwd(ptr(x), f32(x), ptr(y), ptr(gate), ptr(w), f32(w), ptr(post), f32(post), ptr(scale), f32(scale), (float)eps, offset ? 1.f : 0.f, (int)T,
+                                    (int)C, ptr(xn), ptr(h), fptr(rstd), fptr(rstd_y), stream_of(x)), "dsa_residual_norm_fwd");
+        const bool through = post.defined() || gate.defined() || scale.defined();          // (y is not read otherwise)
+        ctx->save_for_backward({xn, through ? y : Tensor(), gate, w, post, scale, rstd, rstd_y});
+        ctx->saved_data["o"] = offset;
+        ctx->set_materialize_grads(false);
+        return {xn, h};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor &xn = s[0], &y = s[1], &gate = s[2], &w = s[3], &post = s[4], &scale = s[5], &rstd = s[6], &rstd_y = s[7];
+        const c10::OptionalDeviceGuard guard(xn.device());
+        const int64_t T = xn.size(0), C = xn.size(1);
+        auto f32 = [](const Tensor &t) { return t.defined() && t.scalar_type() == at::kFloat; };
+        auto like = [&](const Tensor &t) { return t.defined() ? empty(t.sizes(), t.scalar_type(), xn) : Tensor(); };
+        const Tensor dxn = grads[0].defined() ? packed_rows(grads[0].to(xn.scalar_type())) : Tensor(), dh = grads[1].defined() ? as_bf16(grads[1]) : Tensor();
+        const Tensor dx = like(xn), dy = empty({T, C}, at::kBFloat16, xn), dgate = like(gate), dw = like(w), dpost = like(post), dscale = like(scale);
+        const size_t bytes = dsa_residual_norm_bwd_workspace_bytes((int)T, (int)C);
+        const Tensor ws = empty_bytes(bytes, xn);
+        check(dsa_residual_norm_bwd(ptr(dxn), ptr(dh), ptr(xn), f32(xn), ptr(y), ptr(gate), ptr(w), f32(w), ptr(post), f32(post), ptr(scale), f32(scale),
+                                    ctx->saved_data["o"].toBool() ? 1.f : 0.f, (int)T, (int)C, fptr(rstd), fptr(rstd_y), ptr(dx), ptr(dy), ptr(dgate), ptr(dw), ptr(dpost),
+                                    ptr(dscale), ptr(ws), bytes, stream_of(xn)), "dsa_residual_norm_bwd");
+        return {dx, dy, dw, dpost, dgate, dscale, Tensor(), Tensor()};
+    }
+};
+
+variable_list residual_rms_norm(const Tensor &x, const Tensor &y, const Tensor &weight, const OptTensor &post, const OptTensor &gate, const OptTensor &scale, double eps,
+                                bool offset) {
+    const Tensor none;
+    no_forward_mode({&x, &y, &weight, post ? &*post : &none, gate ? &*gate : &none, scale ? &*scale : &none}, "residual_rms_norm");
+    need_gpu(x);
+    need_gpu(y);
+    same_device(x, y, "y");
+    TORCH_CHECK_VALUE(x.dim() >= 1 && half_or_float(x), "x must be bf16 or fp32");
+    TORCH_CHECK_VALUE(y.sizes() == x.sizes() && y.scalar_type() == at::kBFloat16, "y must be bf16 and have the shape of x");
+    const int64_t C = x.size(-1), T = C ? x.numel() / C : 0;
+    TORCH_CHECK_VALUE(T <= INT32_MAX, "too many rows: ", T);
+    OptTensor rows_of_gate;
+    if (gate) {
+        need_gpu(*gate);
+        same_device(x, *gate, "gate");
+        TORCH_CHECK_VALUE(gate->sizes() == x.sizes() && gate->scalar_type() == at::kBFloat16, "gate must be bf16 and have the shape of x");
+        rows_of_gate = gate->reshape({T, C});
+    }
+    const c10::OptionalDeviceGuard guard(x.device());
+    variable_list out = ResidualNormNode::apply(x.reshape({T, C}), y.reshape({T, C}), weight, post, rows_of_gate, scale, eps, offset);
+    if (x.dim() != 2)
+        for (Tensor &t : out) t = t.view(x.sizes());
+    return out;
+}
+
 }  // namespace
 
 void bind_layer(py::module_ &m) {
     const auto nogil = py::call_guard<py::gil_scoped_release>();
     m.def("gated_delta_rule", &gated_delta_rule, nogil);
     m.def("gated_delta_step", &gated_delta_step, nogil);
+    m.def("short_conv", &short_conv, nogil);
+    m.def("short_conv_step", &short_conv_step, nogil);
+    m.def("gated_rms_norm", &gated_rms_norm, nogil);
+    m.def("residual_rms_norm", &residual_rms_norm, nogil);
 }

@@ -16,22 +16,8 @@
 // with backward 372 -> 332 us (5.5 TB/s over all); a layer whose next kernel reads the result (8192 tokens) is not slower for it.
 // The backward pass returns the gradients of the projections' outputs and per-workgroup partial sums of
 // the two norm weights' gradients (reduced by a second kernel in a fixed order: no atomics).
-#include "dsa_common.h"
+#include "dsa_rows.h"
 
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ f32x8 bf8_to_f32(u32x4 w) {
-    f32x8 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        r[2 * i] = __uint_as_float(w[i] << 16);
-        r[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-    return r;
-}
-__device__ __forceinline__ u32x4 f32_to_bf8(f32x8 x) {
-    return u32x4{pack2bf(x[0], x[1]), pack2bf(x[2], x[3]), pack2bf(x[4], x[5]), pack2bf(x[6], x[7])};
-}
 // the eight bf16 of another lane
 __device__ __forceinline__ u32x4 shfl4(u32x4 x, int lane) {
     return u32x4{(uint32_t)__shfl((int)x[0], lane, 64), (uint32_t)__shfl((int)x[1], lane, 64), (uint32_t)__shfl((int)x[2], lane, 64), (uint32_t)__shfl((int)x[3], lane, 64)};

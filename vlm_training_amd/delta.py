@@ -1,5 +1,7 @@
-"""The gated delta rule: the token mixer of the linear-attention layers in the reference's hybrid stack.
+"""The token mixer of the linear-attention layers in the reference's hybrid stack: a short convolution and the gated delta rule.
 
+``short_conv``        depthwise causal convolution with SiLU over packed sequences (models/qwen3_5/model.py:173-176), ``short_conv_step`` for one
+                      token of each request.
 ``gated_delta_rule``  runs packed sequences in chunks (models/qwen3_5/model.py:178-186: ``q``, ``k`` normalised inside, decay and write strength
                       from the projections ``a``, ``b`` and the parameters ``a_log``, ``dt_bias``), with gradients for every input, from and to states.
 ``gated_delta_step``  one token for each of a batch of requests, the states updated in place (decoding).
@@ -35,3 +37,30 @@ def gated_delta_step(q, k, v, a, b, a_log, dt_bias, state, *, scale=None, l2_nor
     """The next token of B requests: q, k (B, Hk, Dk), v (B, Hv, Dv), a, b (B, Hv) -> (B, Hv, Dv); ``state`` (B, Hv, Dk, Dv) fp32 is
     updated in place (a slice of a larger pool of requests will do).  No backward pass."""
     return _lib.host().gated_delta_step(q, k, v, a, b, a_log, dt_bias, state, scale, bool(l2_norm))
+
+
+def _taps(weight):
+    return weight.squeeze(1) if weight.dim() == 3 and weight.shape[1] == 1 else weight
+
+
+def _silu(activation):
+    if activation not in ("silu", "swish", None):
+        raise ValueError(f"activation must be 'silu' or None, not {activation!r}")
+    return activation is not None
+
+
+@torch.compiler.disable
+def short_conv(x, weight, bias, cu_seqlens, *, activation="silu", initial_state=None, return_final_state: bool = False):
+    """x (T, channels) bf16 view, weight (channels, width) or (channels, 1, width), width 2 to 4, bias (channels,) or None -> (T, channels).
+
+    Row t of a sequence sees the ``width - 1`` rows before it in the same sequence; before its first row lie ``initial_state`` (N, channels, width - 1) bf16, or
+    zeros.  ``return_final_state`` adds each sequence's last ``width - 1`` inputs.  The states take no part in the backward pass.  Rows behind the last
+    sequence give zeros."""
+    out = _lib.host().short_conv(x, _taps(weight), bias, cu_seqlens, _silu(activation), initial_state, bool(return_final_state))
+    return tuple(out) if return_final_state else out[0]
+
+
+@torch.compiler.disable
+def short_conv_step(x, state, weight, bias=None, *, activation="silu"):
+    """The next token of B requests: x (B, channels) -> (B, channels); ``state`` (B, channels, width - 1) bf16 moves on in place.  No backward pass."""
+    return _lib.host().short_conv_step(x, state, _taps(weight), bias, _silu(activation))
