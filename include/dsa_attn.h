@@ -405,7 +405,7 @@ int dsa_round_bf16_x3(const float *a, const float *b, const float *c, int64_t na
  *   g = -exp(a_log) softplus(a + dt_bias), beta = sigmoid(b), q and k divided by sqrt(|.|^2 + 1e-6) first where l2_norm is set.
  * q, k (T,Hk,Dk), v (T,Hv,Dv) bf16 with any token and head strides that are multiples of 8 elements, rows on 16-byte boundaries; value head h
  * reads key head h / (Hv/Hk).  a, b (T,Hv) bf16 or fp32 (a_f32, b_f32), head stride 1; a_log, dt_bias (Hv) both bf16 or both fp32 (param_f32).
- * Dk, Dv multiples of 8 up to 128.  cu_seqlens as everywhere; rows behind cu[N] give zeros.
+ * Dk, Dv multiples of 8 up to 128; rows up to DSA_DELTA_MAX_ROW elements apart.  cu_seqlens as everywhere; rows behind cu[N] give zeros.
  *
  * dsa_delta_fwd writes out (T,Hv,Dv) bf16 and, where they are not null, reads initial (N,Hv,Dk,Dv) fp32 and writes final, the same.  `ws` holds
  * dsa_delta_workspace_bytes(args, save) bytes; with `save` it is what dsa_delta_bwd reads.
@@ -414,6 +414,7 @@ int dsa_round_bf16_x3(const float *a, const float *b, const float *c, int64_t na
  * dsa_delta_step: one token for each of T requests; state (T,Hv,Dk,Dv) fp32, requests state_stride elements apart (a multiple of 4, on a 16-byte
  * boundary), is read and written in place.  cu and N are not used.
  */
+#define DSA_DELTA_MAX_ROW (1 << 23)
 typedef struct {
     const void *q, *k, *v, *a, *b, *a_log, *dt_bias;
     int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, a_tok, b_tok;

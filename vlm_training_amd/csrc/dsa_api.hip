@@ -1049,37 +1049,36 @@ static int check_delta(const dsa_delta_args *a, bool packed) {
         return fail(DSA_ERR_UNSUPPORTED, "head dims %d and %d: need multiples of 8 up to 128", a->Dk, a->Dv);
     if (packed && (a->N < 1 || !a->cu)) return fail(DSA_ERR_ARG, "cu_seqlens: N=%d", a->N);
     if (a->Hk > 65535 || (packed ? (int64_t)a->N : a->T) * a->Hv * 4 > 0x7fffffffll) return fail(DSA_ERR_UNSUPPORTED, "N=%d T=%d Hv=%d: too many heads for one launch", a->N, a->T, a->Hv);
-    if (!(a->scale != 0.f)) return fail(DSA_ERR_ARG, "scale=%g", (double)a->scale);
+    if (!(fabsf(a->scale) > 0.f && fabsf(a->scale) < 3.4e38f)) return fail(DSA_ERR_ARG, "scale=%g", (double)a->scale);
     if (a->T == 0) return DSA_OK;
     if (!a->q || !a->k || !a->v || !a->a || !a->b || !a->a_log || !a->dt_bias) return fail(DSA_ERR_ARG, "null tensor pointer");
     if ((a->q_tok | a->q_head | a->k_tok | a->k_head | a->v_tok | a->v_head) % 8) return fail(DSA_ERR_ARG, "token and head strides must be multiples of 8 elements");
     if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & 15) return fail(DSA_ERR_ARG, "q, k and v must lie on 16-byte boundaries");
+    // a chunk's 64 rows are addressed by 32-bit offsets
+    for (const int64_t tok : {a->q_tok, a->k_tok, a->v_tok, (int64_t)a->Hv * a->Dv, (int64_t)a->Hk * a->Dk})
+        if (tok < 0 || tok > DSA_DELTA_MAX_ROW) return fail(DSA_ERR_UNSUPPORTED, "rows %lld elements apart: up to %d are supported", (long long)tok, DSA_DELTA_MAX_ROW);
     return DSA_OK;
 }
-// the parts of the workspace, each on a 256-byte boundary; returns the bytes of all of them
+// the parts of the workspace; returns the bytes of all of them
 static size_t delta_layout(const dsa_delta_args *in, int save, char *ws, DeltaArgs *d) {
     d->in = *in;
     d->slots = in->T / DELTA_CHUNK + in->N + 2;          // every sequence's last chunk, and the rows behind the last one
     d->Dkp = in->Dk > 64 ? 128 : 64;
     d->Dvp = in->Dv > 64 ? 128 : 64;
     const size_t cells = (size_t)d->slots * in->Hv;
-    size_t at = 0;
-    auto part = [&](size_t bytes) { char *const p = ws + at; at += align_up(bytes, 256); return p; };
-    d->rows = (float *)part(cells * DELTA_ROWS * 64 * 4);
-    d->tmat = (bf16_t *)part(cells * 8192 * 2);
-    d->pmat = (bf16_t *)part(cells * 4096 * 2);
-    d->state = (bf16_t *)part(save ? cells * d->Dkp * d->Dvp * 2 : 0);
-    d->news = (bf16_t *)part(save ? cells * 64 * d->Dvp * 2 : 0);
-    return at;
+    d->planes = save ? 4 : 2;
+    d->mats_bytes = DELTA_T + 2 * d->planes * DELTA_PLANE;
+    d->saved_bytes = save ? d->Dkp * d->Dvp * 2 + 256 * d->Dvp : 0;
+    d->back_bytes = d->Dkp * d->Dvp * 2 + 128 * d->Dvp;
+    d->mats = ws;
+    d->saved = ws + cells * d->mats_bytes;               // (blocks are multiples of 1024 bytes)
+    return cells * ((size_t)d->mats_bytes + d->saved_bytes);
 }
 static size_t delta_scratch(char *ws, DeltaArgs *d) {
     const size_t cells = (size_t)d->slots * d->in.Hv;
-    size_t at = 0;
-    auto part = [&](size_t bytes) { char *const p = ws + at; at += align_up(bytes, 256); return p; };
-    d->dstate = (bf16_t *)part(cells * d->Dkp * d->Dvp * 2);
-    d->drs = (bf16_t *)part(cells * 64 * d->Dvp * 2);
-    d->part = (float *)part(cells * 2 * 4);
-    return at;
+    d->back = ws;
+    d->part = (float *)(ws + cells * d->back_bytes);
+    return cells * ((size_t)d->back_bytes + 2 * sizeof(float));
 }
 
 extern "C" size_t dsa_delta_workspace_bytes(const dsa_delta_args *args, int save) {

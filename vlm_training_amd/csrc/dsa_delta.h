@@ -7,35 +7,39 @@
 //     A_ij = beta_i E_ij k_i.k_j (j < i)      P_ij = scale E_ij q_i.k_j (j <= i)      T = (I + A)^-1
 //     R = beta (V - e^G K S0)     N = T R     O = scale e^G Q S0 + P N     S1 = e^G_63 S0 + K^T e^(G_63 - G) N
 // T and P depend on no state: all chunks at once; S goes from chunk to chunk, its columns independent of each other.  The factors
-// 1/|q|, 1/|k|, e^G, beta multiply rows of fp32 results, so that q, k and v enter the products as the bf16 they are; T, S, R and N go in as two
-// bf16 (hi + lo, 2^-17 of the value is lost), without lo x lo.
+// 1/|q|, 1/|k|, e^G, beta multiply rows of fp32 results, so that q, k and v enter the products as the bf16 they are; T, P, S, R and N go in as two
+// bf16 (hi + lo, 2^-17 of the value is lost), without lo x lo: where keys repeat, rows of P N are sums of 64 terms that cancel to the size of one.
 #pragma once
 #include "dsa_tile.h"
 #include "../../include/dsa_attn.h"
 
 #define DELTA_CHUNK 64
 #define DELTA_TS 72                    // row stride of a 64-wide tile: 16-byte rows, four banks on per row
-// per chunk and value head, 64 floats each: e^G, e^(G_63 - G), beta, 1/|k|, scale/|q|, G in two floats (hi + lo)
+#define DELTA_RS 36                    // of a 32-wide one
+// factors of a chunk's rows, 64 floats each: e^G, e^(G_63 - G), beta, 1/|k|, scale/|q|, G in two floats (hi + lo)
 enum { DELTA_EG, DELTA_EC, DELTA_BETA, DELTA_RK, DELTA_RQ, DELTA_GH, DELTA_GL, DELTA_ROWS };
 
 struct DeltaArgs {
     dsa_delta_args in;
     int slots, Dkp, Dvp;               // chunks at the most; head dims padded to 64 or 128
-    float *rows;                       // (slots, Hv, DELTA_ROWS, 64)
-    bf16_t *tmat, *pmat;               // (slots, Hv, 2, 64, 64) T as hi, lo;  (slots, Hv, 64, 64) P
-    bf16_t *state, *news;              // for the backward: (slots, Hv, Dvp, Dkp) S0 transposed, (slots, Hv, 64, Dvp) N
+    // A chunk of a value head ("cell", slots x Hv of them) has a block of each of three arrays.
+    // mats: the rows' factors (DELTA_ROWS x 64 floats), then planes of 64 x 64 bf16: T as hi, lo and, where a backward follows, transposed hi, lo; P the same
+    // saved, for the backward: S0 transposed (Dvp x Dkp), N as hi, lo (2 x 64 x Dvp);  back, the backward's own: dS1 transposed, dR (64 x Dvp)
+    char *mats, *saved, *back;
+    int planes, mats_bytes, saved_bytes, back_bytes;
     const float *initial;              // (N, Hv, Dk, Dv) or null
     float *final;
     bf16_t *out;
     // backward
     const bf16_t *dout;
     const float *dfinal;
-    bf16_t *dstate, *drs;              // (slots, Hv, Dvp, Dkp) dS1 transposed, (slots, Hv, 64, Dvp) dR
     float *part;                       // (2, Hv, slots) sums of a chunk for da_log and ddt_bias
     float *dinitial;
     bf16_t *dq, *dk, *dv;
     void *da, *db, *da_log, *ddt;
 };
+#define DELTA_T 2048                   // byte of a cell's block in mats where the planes begin
+#define DELTA_PLANE 8192
 
 // a chunk of the batch: its segment's first row and the chunk's first row and number of rows.  cu is read as it is, but rows stay within [0, T).
 struct DeltaChunk { int row0, rows, seg, index, of; };
@@ -135,6 +139,42 @@ __device__ __forceinline__ void tile_copy(bf16_t *lds, int stride, const bf16_t 
     Tile64<W> t;
     tile_load<W>(t, src, tok, rows, width);
     tile_put<W>(t, lds, stride);
+}
+
+// ---- memory through buffers: a wave-uniform start, an offset per lane that stays the same from chunk to chunk, zeros past the end (and nothing
+// written there).  A lane that has nothing to read or write gets the offset NOWHERE once, in front of the loop; no address is formed inside it.
+// (With 64-bit addresses and masks formed per chunk a walk of 512 chunks took 1.74 ms, most of it their arithmetic.)
+#define NOWHERE 0x7fffff00
+typedef __amdgpu_buffer_rsrc_t buffer_t;
+__device__ __forceinline__ buffer_t buffer_of(const void *p, int bytes) {
+    const int64_t a = reinterpret_cast<int64_t>(p);
+    const int64_t u = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)a) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32);
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(u), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+// rows of a strided tensor: from the first row's first element, `rows` rows `tok` elements apart of `width` elements
+__device__ __forceinline__ buffer_t rows_buffer(const char *p, int tok, int rows, int width) { return buffer_of(p, rows > 0 ? ((rows - 1) * tok + width) * 2 : 0); }
+// `at`: a constant that the end is not checked for
+__device__ __forceinline__ bf16x8 buf16(buffer_t b, int off, int at = 0) { return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(b, off, at, 0)); }
+__device__ __forceinline__ u32x2 buf8(buffer_t b, int off) { return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0)); }
+__device__ __forceinline__ float buf4(buffer_t b, int off) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, off, 0, 0)); }
+__device__ __forceinline__ void buf_put8(buffer_t b, int off, u32x2 x, int at = 0) { __builtin_amdgcn_raw_buffer_store_b64(x, b, off, at, 0); }
+// every load so far has arrived: in front of a loop whose loads are waited for by count (what is in flight there from before would be counted in with them)
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// 16 bytes of a row from column c on, zero where there is none
+__device__ __forceinline__ bf16x8 row_frag(const bf16_t *row, int c, bool in) {
+    return in ? *reinterpret_cast<const bf16x8 *>(row + c) : zero_bf16x8();
+}
+__device__ __forceinline__ f32x4 up4(u32x2 x) {
+    return f32x4{__uint_as_float(x[0] << 16), __uint_as_float(x[0] & 0xffff0000u), __uint_as_float(x[1] << 16), __uint_as_float(x[1] & 0xffff0000u)};
+}
+
+// Which walk a workgroup takes: the column blocks of one head on one of the chip's eight dies (consecutive workgroups go round them), where they find the
+// rows that they share in its L2.  False: a spare workgroup.
+__device__ __forceinline__ bool delta_walk_unit(int id, int blocks, int64_t units, int64_t &unit, int &block) {
+    const int die = id & 7, j = id >> 3;
+    unit = (int64_t)(j / blocks) * 8 + die;
+    block = j % blocks;
+    return unit < units;
 }
 
 __device__ __forceinline__ float load_any(const void *p, int64_t i, int f32) {

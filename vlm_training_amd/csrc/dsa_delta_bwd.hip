@@ -10,173 +10,240 @@
 #include "dsa_delta.h"
 
 // ---- the walk: as the forward's, from the last chunk to the first ------------------------------------------------------------------------
-template <int DK>
-__global__ __launch_bounds__(256) void dsa_delta_back_kernel(DeltaArgs a) {
-    constexpr int KS = DK + 8, TS = DELTA_TS, NS = 20, SS = 16 * KS > 64 * NS ? 16 * KS : 64 * NS;     // dR takes the place of dS in the wave's LDS
-    __shared__ bf16_t ks[64 * KS], qs[64 * KS], th[64 * TS], tl[64 * TS], ps[64 * TS], ds[64 * TS];
-    __shared__ bf16_t wsh[4][SS], wsl[4][SS], wrh[4][16 * TS], wrl[4][16 * TS], wo[4][2][64 * NS];
-    __shared__ float rows[5 * 64];
+// Wave w has rows 16 w .. of the chunk; P and T come transposed.  dR takes the place of dS in LDS once the first product has read that.
+template <int DK, int NC>
+__global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
+    constexpr int KS = DK + 8, RS = DELTA_RS, NT = DK / 64, SS = 16 * NC * KS > 64 * RS ? 16 * NC * KS : 64 * RS;
+    __shared__ bf16_t ks[64 * KS], qs[64 * KS], sh[SS], sl[SS], os[64 * RS], oh[64 * RS], ol[64 * RS], nh[64 * RS], nl[64 * RS];
     const dsa_delta_args &in = a.in;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, l16 = lane & 15, g4 = lane >> 4;
-    const int blocks = a.Dvp / 64, h = blockIdx.x / blocks % in.Hv, seg = blockIdx.x / blocks / in.Hv, dv0 = blockIdx.x % blocks * 64;
-    const int hk = h / (in.Hv / in.Hk), dv = dv0 + 16 * wv + l16;
-    int slot0, chunks, s0, L;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g4 = lane >> 4, row = 16 * wv + l16;
+    int64_t unit;
+    int block, slot0, chunks, s0, L;
+    if (!delta_walk_unit(blockIdx.x, a.Dvp / (16 * NC), (int64_t)in.N * in.Hv, unit, block)) return;
+    const int h = (int)(unit % in.Hv), seg = (int)(unit / in.Hv), hk = h / (in.Hv / in.Hk), dv0 = 16 * NC * block;
     delta_segment(in.cu, in.N, seg, slot0, chunks, s0, L);
     chunks = min(chunks, a.slots - slot0);
     s0 = max(s0, 0);
-    bf16_t *const sh = wsh[wv], *const sl = wsl[wv], *const rh = wrh[wv], *const rl = wrl[wv], *const oh = wo[wv][0], *const ol = wo[wv][1];
-    f32x4 st[DK / 16];                                   // dS[dk = 16 t + 4 g4 + v][dv]
-    const int64_t cell = ((int64_t)seg * in.Hv + h) * in.Dk * in.Dv + dv;
+    f32x4 st[NT][NC];                                    // dS[dk = 16 (NT wv + t) + 4 g4 + v][dv0 + 16 c + l16]
+    const int64_t cell = ((int64_t)seg * in.Hv + h) * in.Dk * in.Dv + dv0 + l16;
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int k = 16 * t + 4 * g4 + v;
-            st[t][v] = a.dfinal && k < in.Dk && dv < in.Dv ? a.dfinal[cell + (int64_t)k * in.Dv] : 0.f;
-        }
-    Tile64<DK> tk, tq;
-    Tile64<64> tth, ttl, tp, td;
-    float tr[2];
-    auto fetch = [&](int c) __attribute__((always_inline)) {
-        const int row0 = s0 + 64 * c, n = min(min(64, L - 64 * c), in.T - row0);
-        const int64_t p = (int64_t)(slot0 + c) * in.Hv + h;
-        tile_load<DK>(tk, (const bf16_t *)in.k + row0 * in.k_tok + hk * in.k_head, in.k_tok, n, in.Dk);
-        tile_load<DK>(tq, (const bf16_t *)in.q + row0 * in.q_tok + hk * in.q_head, in.q_tok, n, in.Dk);
-        tile_load<64>(tth, a.tmat + p * 8192, 64, 64, 64);
-        tile_load<64>(ttl, a.tmat + p * 8192 + 4096, 64, 64, 64);
-        tile_load<64>(tp, a.pmat + p * 4096, 64, 64, 64);
-        tile_load<64>(td, a.dout + ((int64_t)row0 * in.Hv + h) * in.Dv + dv0, (int64_t)in.Hv * in.Dv, n, in.Dv - dv0);
-        tr[0] = a.rows[p * DELTA_ROWS * 64 + tid];
-        tr[1] = tid < 64 ? a.rows[p * DELTA_ROWS * 64 + 256 + tid] : 0.f;
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const int k = 16 * (NT * wv + t) + 4 * g4 + v;
+                st[t][c][v] = a.dfinal && k < in.Dk && dv0 + 16 * c + l16 < in.Dv ? a.dfinal[cell + (int64_t)k * in.Dv + 16 * c] : 0.f;
+            }
+    loads_done();
+    int at_k[DK / 32], at_q[DK / 32], at_o[NC];          // offsets of this lane, in bytes
+#pragma unroll
+    for (int s = 0; s < DK / 32; ++s) {
+        const int d = 32 * s + 8 * g4;
+        at_k[s] = d < in.Dk ? (row * (int)in.k_tok + d) * 2 : NOWHERE;
+        at_q[s] = d < in.Dk ? (row * (int)in.q_tok + d) * 2 : NOWHERE;
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = dv0 + 16 * c + 4 * g4;
+        at_o[c] = d < in.Dv ? (row * in.Hv * in.Dv + d) * 2 : NOWHERE;
+    }
+    const int at_t = wv < 2 ? row * 128 + 16 * g4 : NOWHERE, at_t1 = row * 128 + 16 * g4 + 64;       // (transposed rows begin at the diagonal)
+    const int at_s = ((dv0 + l16) * DK + 16 * NT * wv + 4 * g4) * 2, at_n = (row * a.Dvp + dv0 + 4 * g4) * 2;
+    struct BackRows {
+        bf16x8 k[DK / 32], q[DK / 32], th[2], tl[2], ph[2], pl[2];
+        u32x2 o[NC];
+        float eg, ec, beta, rk, rq, end;
     };
-    if (chunks > 0) fetch(chunks - 1);
-    for (int c = chunks - 1; c >= 0; --c) {
-        const int row0 = s0 + 64 * c, n = min(min(64, L - 64 * c), in.T - row0);
-        const int64_t p = (int64_t)(slot0 + c) * in.Hv + h;
-        tile_put<DK>(tk, ks, KS);
-        tile_put<DK>(tq, qs, KS);
-        tile_put<64>(tth, th, TS);
-        tile_put<64>(ttl, tl, TS);
-        tile_put<64>(tp, ps, TS);
-        tile_put<64>(td, ds, TS);
-        rows[tid] = tr[0];
-        if (tid < 64) rows[256 + tid] = tr[1];
-        __syncthreads();
-        if (c > 0) fetch(c - 1);
-        const float *const eg = rows + DELTA_EG * 64, *const ec = rows + DELTA_EC * 64, *const beta = rows + DELTA_BETA * 64, *const rk = rows + DELTA_RK * 64,
-                    *const rq = rows + DELTA_RQ * 64;
-        // dS1 as [dv][dk], and e^G scale/|q| dO as [row][dv] (lane: its row)
+    // where the next chunk to be fetched, and the one at hand, lie; a chunk further they are a fixed number of bytes back
+    const int64_t last = (int64_t)(slot0 + chunks - 1) * in.Hv + h, t_last = s0 + 64 * (int64_t)(chunks - 1);
+    const char *pk = (const char *)in.k + (t_last * in.k_tok + hk * in.k_head) * 2, *pq = (const char *)in.q + (t_last * in.q_tok + hk * in.q_head) * 2;
+    const char *po = (const char *)(a.dout + (t_last * in.Hv + h) * in.Dv), *pm = a.mats + last * a.mats_bytes;
+    char *pb = a.back + last * a.back_bytes, *pv = (char *)(a.dv + (t_last * in.Hv + h) * in.Dv);
+    const int64_t step_m = (int64_t)in.Hv * a.mats_bytes, step_b = (int64_t)in.Hv * a.back_bytes;
+    const int step_k = (int)in.k_tok * 128, step_q = (int)in.q_tok * 128, step_o = in.Hv * in.Dv * 128;
+    const int rows_all = min(L, in.T - s0);
+    auto fetch_q = [&](int i, BackRows &w) __attribute__((always_inline)) {
+        const int n = min(64, rows_all - 64 * i);
+        const buffer_t q = rows_buffer(pq, (int)in.q_tok, n, in.Dk), o = rows_buffer(po, in.Hv * in.Dv, n, in.Dv);
 #pragma unroll
-        for (int t = 0; t < DK / 16; ++t) {
-            const u32x2 x = hi4(st[t]);
-            put4(sh + l16 * KS + 16 * t + 4 * g4, x);
-            put4(sl + l16 * KS + 16 * t + 4 * g4, lo4(st[t], x));
-            put4(a.dstate + (p * a.Dvp + dv) * DK + 16 * t + 4 * g4, x);
-        }
-        const float fo = eg[lane] * rq[lane];
+        for (int s = 0; s < DK / 32; ++s) w.q[s] = buf16(q, at_q[s]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            f32x4 x;
+        for (int c = 0; c < NC; ++c) w.o[c] = buf8(o, at_o[c]);
+        pq -= i > 0 ? step_q : 0;                        // (the first one is fetched again: behind a branch, waits would be for every load in flight)
+        po -= i > 0 ? step_o : 0;
+    };
+    auto fetch_k = [&](int i, BackRows &w) __attribute__((always_inline)) {
+        const buffer_t k = rows_buffer(pk, (int)in.k_tok, min(64, rows_all - 64 * i), in.Dk), m = buffer_of(pm, a.mats_bytes);
+        const int p = DELTA_T + (a.planes + 2) * DELTA_PLANE;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) x[v] = (float)ds[lane * TS + 16 * wv + 4 * u + v] * fo;
-            put_split4(oh + lane * NS + 4 * u, ol + lane * NS + 4 * u, x);
-        }
-        wave_sync();
-        f32x4 r[4];                                      // [row 16 m + 4 g4 + v][dv = l16]
+        for (int s = 0; s < DK / 32; ++s) w.k[s] = buf16(k, at_k[s]);
+        w.ph[0] = buf16(m, at_t, p);
+        w.pl[0] = buf16(m, at_t, p + DELTA_PLANE);
+        w.ph[1] = buf16(m, at_t1, p);
+        w.pl[1] = buf16(m, at_t1, p + DELTA_PLANE);
+        pk -= i > 0 ? step_k : 0;
+    };
+    auto fetch_t = [&](int i, BackRows &w) __attribute__((always_inline)) {
+        const buffer_t m = buffer_of(pm, a.mats_bytes);
+        w.th[0] = buf16(m, at_t, DELTA_T + 2 * DELTA_PLANE);
+        w.tl[0] = buf16(m, at_t, DELTA_T + 3 * DELTA_PLANE);
+        w.th[1] = buf16(m, at_t1, DELTA_T + 2 * DELTA_PLANE);
+        w.tl[1] = buf16(m, at_t1, DELTA_T + 3 * DELTA_PLANE);
+        w.eg = buf4(m, DELTA_EG * 256 + row * 4);
+        w.ec = buf4(m, DELTA_EC * 256 + row * 4);
+        w.beta = buf4(m, DELTA_BETA * 256 + row * 4);
+        w.rk = buf4(m, DELTA_RK * 256 + row * 4);
+        w.rq = buf4(m, DELTA_RQ * 256 + row * 4);
+        w.end = buf4(m, DELTA_EG * 256 + 252);
+        pm -= i > 0 ? step_m : 0;
+    };
+    auto chunk = [&](int i, BackRows &x) __attribute__((always_inline)) {
+        const int ahead = max(i - 2, 0);
+        // dS1 as [dv][dk]; K, Q and dO as they are, and scale/|q| e^G dO
+        const buffer_t back = buffer_of(pb, a.back_bytes);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) r[m] = zero4();
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int at = (16 * c + l16) * KS + 16 * (NT * wv + t) + 4 * g4;
+                const u32x2 y = hi4(st[t][c]);
+                put4(sh + at, y);
+                put4(sl + at, lo4(st[t][c], y));
+                buf_put8(back, at_s + c * 32 * DK + 32 * t, y);
+            }
 #pragma unroll
         for (int s = 0; s < DK / 32; ++s) {
-            const bf16x8 bh = frag_n(sh, KS, 0, 32 * s), bl = frag_n(sl, KS, 0, 32 * s);
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const bf16x8 ka = frag_n(ks, KS, 16 * m, 32 * s);
-                r[m] = mfma16(ka, bl, r[m]);
-                r[m] = mfma16(ka, bh, r[m]);
-            }
-        }
-        bf16x8 db[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) db[s] = frag_t(ds, TS, 32 * s, 16 * wv);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) r[m][v] *= ec[16 * m + 4 * g4 + v] * rk[16 * m + 4 * g4 + v];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-                if (32 * s + 31 >= 16 * m) r[m] = mfma16(frag_t(ps, TS, 32 * s, 16 * m), db[s], r[m]);
-            put_split4(rh + l16 * TS + 16 * m + 4 * g4, rl + l16 * TS + 16 * m + 4 * g4, r[m]);
-        }
-        wave_sync();
-        // dR^T = dN^T T: [dv = 4 g4 + v][row 16 m + l16]; columns of T begin at the diagonal
-        bf16x8 ah[2], al[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            ah[s] = frag_n(rh, TS, 0, 32 * s);
-            al[s] = frag_n(rl, TS, 0, 32 * s);
+            *reinterpret_cast<bf16x8 *>(ks + row * KS + 32 * s + 8 * g4) = x.k[s];
+            *reinterpret_cast<bf16x8 *>(qs + row * KS + 32 * s + 8 * g4) = x.q[s];
         }
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            f32x4 x = zero4();
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (32 * s + 31 < 16 * m) continue;
-                const bf16x8 bh = frag_t(th, TS, 32 * s, 16 * m), bl = frag_t(tl, TS, 32 * s, 16 * m);
-                x = mfma16(al[s], bh, x);
-                x = mfma16(ah[s], bl, x);
-                x = mfma16(ah[s], bh, x);
-            }
-            const int i = 16 * m + l16, d = dv0 + 16 * wv + 4 * g4;
-            put4(a.drs + (p * 64 + i) * a.Dvp + d, hi4(x));
-            if (i < n && d < in.Dv) put4(a.dv + ((int64_t)(row0 + i) * in.Hv + h) * in.Dv + d, hi4(x * beta[i]));
-            put_split4(sh + i * NS + 4 * g4, sl + i * NS + 4 * g4, x * (-beta[i] * eg[i] * rk[i]));
+        for (int c = 0; c < NC; ++c) {
+            const int at = row * RS + 16 * c + 4 * g4;
+            put4(os + at, x.o[c]);
+            put_split4(oh + at, ol + at, up4(x.o[c]) * (x.eg * x.rq));
         }
-        wave_sync();
-        // dS0 = e^G_63 dS1 + Q^T (..) + K^T (..)
-        const float e = eg[63];
-        bf16x8 bh[2], bl[2], qh[2], ql[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            bh[s] = frag_t(sh, NS, 32 * s, 0);
-            bl[s] = frag_t(sl, NS, 32 * s, 0);
-            qh[s] = frag_t(oh, NS, 32 * s, 0);
-            ql[s] = frag_t(ol, NS, 32 * s, 0);
-        }
-#pragma unroll
-        for (int t = 0; t < DK / 16; ++t) {
-            st[t] *= e;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const bf16x8 ka = frag_t(ks, KS, 32 * s, 16 * t), qa = frag_t(qs, KS, 32 * s, 16 * t);
-                st[t] = mfma16(ka, bl[s], st[t]);
-                st[t] = mfma16(ka, bh[s], st[t]);
-                st[t] = mfma16(qa, ql[s], st[t]);
-                st[t] = mfma16(qa, qh[s], st[t]);
-            }
-        }
+        fetch_q(ahead, x);
         __syncthreads();
+        // dN^T = e^(G_63 - G) dS1^T K^T + dO^T P
+        f32x4 r[NC];                                     // [dv = 16 c + 4 g4 + v][row]
+#pragma unroll
+        for (int c = 0; c < NC; ++c) r[c] = zero4();
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                r[c] = mfma16(frag_n(sl, KS, 16 * c, 32 * s), x.k[s], r[c]);
+                r[c] = mfma16(frag_n(sh, KS, 16 * c, 32 * s), x.k[s], r[c]);
+            }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            r[c] *= x.ec * x.rk;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s == 0 && wv >= 2) continue;
+                const bf16x8 o = frag_t(os, RS, 32 * s, 16 * c);
+                r[c] = mfma16(o, x.pl[s], r[c]);
+                r[c] = mfma16(o, x.ph[s], r[c]);
+            }
+            put_split4(nh + row * RS + 16 * c + 4 * g4, nl + row * RS + 16 * c + 4 * g4, r[c]);
+        }
+        fetch_k(ahead, x);
+        __syncthreads();
+        // dR^T = dN^T T
+        const buffer_t dvs = rows_buffer(pv, in.Hv * in.Dv, min(64, rows_all - 64 * i), in.Dv);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            f32x4 y = zero4();
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s == 0 && wv >= 2) continue;
+                const bf16x8 ah = frag_t(nh, RS, 32 * s, 16 * c), al = frag_t(nl, RS, 32 * s, 16 * c);
+                y = mfma16(al, x.th[s], y);
+                y = mfma16(ah, x.tl[s], y);
+                y = mfma16(ah, x.th[s], y);
+            }
+            const int at = row * RS + 16 * c + 4 * g4;
+            buf_put8(back, at_n + 32 * c, hi4(y), a.Dvp * DK * 2);
+            buf_put8(dvs, at_o[c], hi4(y * x.beta));
+            put_split4(sh + at, sl + at, y * (-x.beta * x.eg * x.rk));
+        }
+        const float end = x.end;
+        fetch_t(ahead, x);
+        __syncthreads();
+        // dS0 = e^G_63 dS1 + Q^T (..) + K^T (..)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) st[t][c] *= end;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            bf16x8 bh[NC], bl[NC], ch[NC], cl[NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                bh[c] = frag_t(sh, RS, 32 * s, 16 * c);
+                bl[c] = frag_t(sl, RS, 32 * s, 16 * c);
+                ch[c] = frag_t(oh, RS, 32 * s, 16 * c);
+                cl[c] = frag_t(ol, RS, 32 * s, 16 * c);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const bf16x8 ka = frag_t(ks, KS, 32 * s, 16 * (NT * wv + t)), qa = frag_t(qs, KS, 32 * s, 16 * (NT * wv + t));
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    st[t][c] = mfma16(ka, bl[c], st[t][c]);
+                    st[t][c] = mfma16(qa, cl[c], st[t][c]);
+                    st[t][c] = mfma16(ka, bh[c], st[t][c]);
+                    st[t][c] = mfma16(qa, ch[c], st[t][c]);
+                }
+            }
+        }
+        pb -= step_b;
+        pv -= step_o;
+        __syncthreads();
+    };
+    BackRows x, y;
+    if (chunks > 0) {
+        int i = chunks - 1;
+        fetch_q(i, x);
+        fetch_k(i, x);
+        fetch_t(i, x);
+        fetch_q(max(i - 1, 0), y);
+        fetch_k(max(i - 1, 0), y);
+        fetch_t(max(i - 1, 0), y);
+        for (; i > 0; i -= 2) {
+            chunk(i, x);
+            chunk(i - 1, y);
+        }
+        if (i == 0) chunk(0, x);
     }
     if (a.dinitial) {
 #pragma unroll
-        for (int t = 0; t < DK / 16; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int k = 16 * t + 4 * g4 + v;
-                if (k < in.Dk && dv < in.Dv) a.dinitial[cell + (int64_t)k * in.Dv] = st[t][v];
-            }
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const int k = 16 * (NT * wv + t) + 4 * g4 + v;
+                    if (k < in.Dk && dv0 + 16 * c + l16 < in.Dv) a.dinitial[cell + (int64_t)k * in.Dv + 16 * c] = st[t][c][v];
+                }
     }
 }
 
 // ---- everything that needs one chunk alone: one workgroup per chunk and key head, its value heads in turn --------------------------------
-// dq and dk of the key head are summed over its value heads in registers (wave w: rows 16 w ..), in that order.  The matrices of 64 x 64 are formed
-// transposed (lane: one row i, four neighbours j), so that they go to LDS in row order.
+// Wave w has rows 16 w ..; N, X and Z go into their products as hi + lo (where keys repeat, a row of X K is a sum that cancels).  Everything is formed transposed (lane: its row, four neighbouring columns), so that a row's factor is one register and its
+// sums stay in four lanes.  dq and dk of the key head are summed over its value heads in registers, in that order.  The columns of the values are taken 64 at
+// a time, so that two workgroups share a compute unit's LDS and one's loads pass under the other's products; dO and dR are read by their own rows' wave alone.
 template <int DK, int DV>
-__global__ __launch_bounds__(256) void dsa_delta_grad_kernel(DeltaArgs a) {
-    constexpr int KS = DK + 8, VS = DV + 8, TS = DELTA_TS, NT = DK / 16;
-    __shared__ bf16_t ks[64 * KS], qs[64 * KS], os[64 * VS], rs[64 * VS], ns[64 * VS], ss[DV * KS], xs[64 * TS], zs[64 * TS];
-    __shared__ float rows[DELTA_ROWS * 64], dg_row[64], dg_col[4][64], dg_q[64], dg_k[64], dg_s[64], dbeta[64], dots[4];
+__global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
+    constexpr int KS = DK + 8, TS = DELTA_TS, NT = DK / 16;
+    __shared__ bf16_t ks[64 * KS], qs[64 * KS], pool[4 * 64 * TS];
+    __shared__ float rows[DELTA_ROWS * 64], dg_row[64], dg_col[4][64], dg_s[64], dots[4];
+    bf16_t *const ns = pool, *const ss = pool + 2 * 64 * TS;                                              // N as hi, lo; S0, then dS1: 64 columns of the values
+    bf16_t *const xs = pool, *const zs = pool + 2 * 64 * TS;                                              // in their place X and Z as hi, lo
+    static_assert(64 * KS <= 2 * 64 * TS, "64 rows of the state lie in two tiles");
     const dsa_delta_args &in = a.in;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, l16 = lane & 15, g4 = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g4 = lane >> 4, row = 16 * wv + l16;
     const int slot = blockIdx.x, hk = blockIdx.y, rep = in.Hv / in.Hk;
     DeltaChunk c;
     if (!delta_locate(in.cu, in.N, in.T, slot, c)) {
@@ -196,7 +263,7 @@ __global__ __launch_bounds__(256) void dsa_delta_grad_kernel(DeltaArgs a) {
     tile_copy<DK>(ks, KS, (const bf16_t *)in.k + c.row0 * in.k_tok + hk * in.k_head, in.k_tok, c.rows, in.Dk);
     tile_copy<DK>(qs, KS, (const bf16_t *)in.q + c.row0 * in.q_tok + hk * in.q_head, in.q_tok, c.rows, in.Dk);
     __syncthreads();
-    f32x4 kk[4], qk[4];                                  // [j = 16 t + 4 g4 + v], row i = 16 wv + l16
+    f32x4 kk[4], qk[4];                                  // [j = 16 t + 4 g4 + v][row]
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         kk[t] = qk[t] = zero4();
@@ -209,186 +276,198 @@ __global__ __launch_bounds__(256) void dsa_delta_grad_kernel(DeltaArgs a) {
             }
         }
     }
-    f32x4 dq[NT], dk[NT];                                // [row 16 wv + 4 g4 + v][16 t + l16], times scale/|q| and 1/|k|
+    f32x4 dq[NT], dk[NT];                                // [16 t + 4 g4 + v][row], times scale/|q| and 1/|k|
 #pragma unroll
     for (int t = 0; t < NT; ++t) dq[t] = dk[t] = zero4();
-    const float *const eg = rows + DELTA_EG * 64, *const ec = rows + DELTA_EC * 64, *const beta = rows + DELTA_BETA * 64, *const rk = rows + DELTA_RK * 64,
-                *const rq = rows + DELTA_RQ * 64, *const gh = rows + DELTA_GH * 64, *const gl = rows + DELTA_GL * 64;
-    const int i = 16 * wv + l16;
+    const bool live = row < c.rows;
+    const bf16_t *const krow = ks + row * KS + 4 * g4, *const qrow = qs + row * KS + 4 * g4;
+    auto four = [](const bf16_t *p) __attribute__((always_inline)) { return up4(*reinterpret_cast<const u32x2_any *>(p)); };
+    auto dot4 = [](f32x4 x, f32x4 y, float s) __attribute__((always_inline)) { return s + ((x[0] * y[0] + x[1] * y[1]) + (x[2] * y[2] + x[3] * y[3])); };
+    auto over_row = [](float x) __attribute__((always_inline)) { x += __shfl_xor(x, 16, 64); return x + __shfl_xor(x, 32, 64); };
+#pragma unroll 1
     for (int u = 0; u < rep; ++u) {
         const int h = hk * rep + u;
         const int64_t p = (int64_t)slot * in.Hv + h;
+        const bf16_t *const state = (const bf16_t *)(a.saved + p * a.saved_bytes), *const news = state + DV * DK;
+        const bf16_t *const dstate = (const bf16_t *)(a.back + p * a.back_bytes), *const drs = dstate + DV * DK;
+        f32x4 x[4], z[4];
+        float dotq = 0.f, dotk = 0.f, dots_ = 0.f, dot = 0.f, db = 0.f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = z[t] = zero4();
         __syncthreads();                                 // (the previous head's LDS has been read)
-        tile_copy<DV>(os, VS, a.dout + ((int64_t)c.row0 * in.Hv + h) * in.Dv, (int64_t)in.Hv * in.Dv, c.rows, in.Dv);
-        tile_copy<DV>(rs, VS, a.drs + p * 64 * DV, DV, 64, DV);
-        tile_copy<DV>(ns, VS, a.news + p * 64 * DV, DV, 64, DV);
-#pragma unroll
-        for (int b = 0; b < DV / 64; ++b) tile_copy<DK>(ss + 64 * b * KS, KS, a.state + (p * DV + 64 * b) * DK, DK, 64, DK);
-        for (int e = tid; e < DELTA_ROWS * 64; e += 256) rows[e] = a.rows[p * DELTA_ROWS * 64 + e];
-        __syncthreads();
-        // X and Z, their products with QK and KK summed over rows and columns
-        float row = 0.f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            f32x4 x = zero4(), z = zero4(), both = zero4();
-            if (t <= wv) {
-#pragma unroll
-                for (int s = 0; s < DV / 32; ++s) {
-                    const bf16x8 nj = frag_n(ns, VS, 16 * t, 32 * s);
-                    x = mfma16(nj, frag_n(os, VS, 16 * wv, 32 * s), x);
-                    z = mfma16(nj, frag_n(rs, VS, 16 * wv, 32 * s), z);
-                }
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const int j = 16 * t + 4 * g4 + v;
-                    const float e = j <= i ? expf((gh[i] - gh[j]) + (gl[i] - gl[j])) * rk[j] : 0.f;
-                    x[v] = j <= i ? x[v] * e * rq[i] : 0.f;
-                    z[v] = j < i ? -z[v] * e * beta[i] * rk[i] : 0.f;
-                    both[v] = x[v] * qk[t][v] + z[v] * kk[t][v];
-                    row += both[v];
-                }
-            }
-            put4(xs + i * TS + 16 * t + 4 * g4, hi4(x));
-            put4(zs + i * TS + 16 * t + 4 * g4, hi4(z));
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                float s = both[v];
-#pragma unroll
-                for (int m = 1; m < 16; m <<= 1) s += __shfl_xor(s, m, 64);
-                if (l16 == 0) dg_col[wv][16 * t + 4 * g4 + v] = s;
-            }
-        }
-        row += __shfl_xor(row, 16, 64);
-        row += __shfl_xor(row, 32, 64);
-        if (g4 == 0) dg_row[i] = row;
-        {   // dR.N: four threads per row
-            const int r = tid >> 2, c0 = (tid & 3) * (DV / 4);
-            float s = 0.f;
-            for (int e = 0; e < DV / 4; ++e) s += (float)rs[r * VS + c0 + e] * (float)ns[r * VS + c0 + e];
-            s += __shfl_xor(s, 1, 64);
-            s += __shfl_xor(s, 2, 64);
-            if ((tid & 3) == 0) dbeta[r] = s;
-        }
-        // through S0: scale e^G dO S0^T into dQ, -beta e^G dR S0^T into dK
-        f32x4 fq, fk, dotq = zero4(), dotk = zero4();
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int r = 16 * wv + 4 * g4 + v;
-            fq[v] = eg[r] * rq[r];
-            fk[v] = -beta[r] * eg[r] * rk[r];
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            f32x4 x = zero4(), y = zero4();
-#pragma unroll
-            for (int s = 0; s < DV / 32; ++s) {
-                const bf16x8 b = frag_t(ss, KS, 32 * s, 16 * t);
-                x = mfma16(frag_n(os, VS, 16 * wv, 32 * s), b, x);
-                y = mfma16(frag_n(rs, VS, 16 * wv, 32 * s), b, y);
-            }
-            x *= fq;
-            y *= fk;
-            dq[t] += x;
-            dk[t] += y;
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int r = 16 * wv + 4 * g4 + v;
-                dotq[v] += x[v] * (float)qs[r * KS + 16 * t + l16];
-                dotk[v] += y[v] * (float)ks[r * KS + 16 * t + l16];
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-#pragma unroll
-            for (int m = 1; m < 16; m <<= 1) {
-                dotq[v] += __shfl_xor(dotq[v], m, 64);
-                dotk[v] += __shfl_xor(dotk[v], m, 64);
-            }
-            if (l16 == 0) {
-                dg_q[16 * wv + 4 * g4 + v] = dotq[v];
-                dg_k[16 * wv + 4 * g4 + v] = dotk[v];
-            }
-        }
-        __syncthreads();
-        // dS1 in the place of S0, their product summed on the way
-        float dot = 0.f;
-#pragma unroll
+        for (int e = tid; e < DELTA_ROWS * 64; e += 256) rows[e] = ((const float *)(a.mats + p * a.mats_bytes))[e];
+#pragma unroll 1
         for (int b = 0; b < DV / 64; ++b) {
-            Tile64<DK> t1;
-            tile_load<DK>(t1, a.dstate + (p * DV + 64 * b) * DK, DK, 64, DK);
+            const bf16_t *const orow = a.dout + ((int64_t)(c.row0 + row) * in.Hv + h) * in.Dv + 64 * b, *const rrow = drs + row * DV + 64 * b;
+            bf16x8 of[2], rf[2];
+            Tile64<64> th, tl;
+            Tile64<DK> ts;
+            tile_load<64>(th, news + 64 * b, DV, 64, 64);
+            tile_load<64>(tl, news + 64 * DV + 64 * b, DV, 64, 64);
+            tile_load<DK>(ts, state + 64 * b * DK, DK, 64, DK);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                of[s] = row_frag(orow, 32 * s + 8 * g4, live && 64 * b + 32 * s + 8 * g4 < in.Dv);
+                rf[s] = row_frag(rrow, 32 * s + 8 * g4, true);
+            }
+            if (b) __syncthreads();                      // (the columns before have been read)
+            tile_put<64>(th, ns, TS);
+            tile_put<64>(tl, ns + 64 * TS, TS);
+            tile_put<DK>(ts, ss, KS);
+            __syncthreads();
+            tile_load<DK>(ts, dstate + 64 * b * DK, DK, 64, DK);
+            // dO N^T and dR N^T
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (t > wv) continue;
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const bf16x8 nj = frag_n(ns, TS, 16 * t, 32 * s), lj = frag_n(ns + 64 * TS, TS, 16 * t, 32 * s);
+                    x[t] = mfma16(lj, of[s], x[t]);
+                    z[t] = mfma16(lj, rf[s], z[t]);
+                    x[t] = mfma16(nj, of[s], x[t]);
+                    z[t] = mfma16(nj, rf[s], z[t]);
+                }
+            }
+            const float rk = rows[DELTA_RK * 64 + row], eg = rows[DELTA_EG * 64 + row];
+            const float fq = eg * rows[DELTA_RQ * 64 + row], fk = -rows[DELTA_BETA * 64 + row] * eg * rk, fs = rows[DELTA_EC * 64 + row] * rk;
+            bf16x8 nf[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                nf[s] = frag_n(ns, TS, 16 * wv, 32 * s);
+                db = dot8_chain(rf[s], nf[s], dot8_chain(rf[s], frag_n(ns + 64 * TS, TS, 16 * wv, 32 * s), db));
+            }
+            // through S0: scale e^G dO S0^T into dQ, -beta e^G dR S0^T into dK
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                f32x4 y = zero4(), w = zero4();
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const bf16x8 m = frag_t(ss, KS, 32 * s, 16 * t);
+                    y = mfma16(m, of[s], y);
+                    w = mfma16(m, rf[s], w);
+                }
+                y *= fq;
+                w *= fk;
+                dq[t] += y;
+                dk[t] += w;
+                dotq = dot4(y, four(qrow + 16 * t), dotq);
+                dotk = dot4(w, four(krow + 16 * t), dotk);
+            }
+            __syncthreads();
+            // dS1 in the place of S0, their product summed on the way
 #pragma unroll
             for (int e = 0; e < DK / 32; ++e) {
                 const int at = tid + 256 * e;
-                bf16_t *const q = ss + (64 * b + at / (DK / 8)) * KS + at % (DK / 8) * 8;
-                dot = dot8_chain(__builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_any *>(q)), __builtin_bit_cast(bf16x8, t1.x[e]), dot);
-                *reinterpret_cast<u32x4_any *>(q) = t1.x[e];
+                bf16_t *const q = ss + at / (DK / 8) * KS + at % (DK / 8) * 8;
+                dot = dot8_chain(__builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_any *>(q)), __builtin_bit_cast(bf16x8, ts.x[e]), dot);
+                *reinterpret_cast<u32x4_any *>(q) = ts.x[e];
             }
+            __syncthreads();
+            // through dS1: e^(G_63 - G) N dS1^T into dK
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                f32x4 y = zero4();
+#pragma unroll
+                for (int s = 0; s < 2; ++s) y = mfma16(frag_t(ss, KS, 32 * s, 16 * t), nf[s], y);
+                y *= fs;
+                dk[t] += y;
+                dots_ = dot4(y, four(krow + 16 * t), dots_);
+            }
+        }
+        __syncthreads();
+        // X and Z, their products with QK and KK summed over rows and columns
+        const float rk = rows[DELTA_RK * 64 + row], fx = rows[DELTA_RQ * 64 + row], fz = -rows[DELTA_BETA * 64 + row] * rk;
+        const float gi = rows[DELTA_GH * 64 + row], gi_lo = rows[DELTA_GL * 64 + row];
+        float sum = 0.f, col[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            f32x4 xv = zero4(), zv = zero4();
+            if (t <= wv) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const int j = 16 * t + 4 * g4 + v;
+                    const float e = j <= row ? expf((gi - rows[DELTA_GH * 64 + j]) + (gi_lo - rows[DELTA_GL * 64 + j])) * rows[DELTA_RK * 64 + j] : 0.f;
+                    xv[v] = j <= row ? x[t][v] * e * fx : 0.f;
+                    zv[v] = j < row ? z[t][v] * e * fz : 0.f;
+                }
+            }
+            const int at = row * TS + 16 * t + 4 * g4;
+            put_split4(xs + at, xs + 64 * TS + at, xv);
+            put_split4(zs + at, zs + 64 * TS + at, zv);
+            const f32x4 both = xv * qk[t] + zv * kk[t];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                sum += both[v];
+                col[4 * t + v] = both[v];
+            }
+        }
+        // sixteen columns' sums over sixteen lanes: each step, a lane keeps one half of its columns and hands the other over; lane l ends with column l
+#pragma unroll
+        for (int m = 8; m > 0; m >>= 1) {
+            const bool up = l16 & m;
+#pragma unroll
+            for (int e = 0; e < m; ++e) {
+                const float keep = up ? col[e + m] : col[e], send = up ? col[e] : col[e + m];
+                col[e] = keep + __shfl_xor(send, m, 64);
+            }
+        }
+        dg_col[wv][16 * (l16 >> 2) + 4 * g4 + (l16 & 3)] = col[0];
+        dots_ = over_row(dots_);
+        sum = over_row(sum) + over_row(dotq) + over_row(dotk) - dots_;
+        db = over_row(db);
+        if (g4 == 0) {
+            dg_row[row] = sum;
+            dg_s[row] = dots_;
+            if (live) store_any(a.db, (int64_t)(c.row0 + row) * in.Hv + h, in.b_f32, (1.f - rows[DELTA_BETA * 64 + row]) * db);
         }
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) dot += __shfl_xor(dot, m, 64);
         if (lane == 0) dots[wv] = dot;
+        __syncthreads();
         // X K, X^T Q, (Z + Z^T) K
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const bool low = 32 * s <= 16 * wv + 15, up = 32 * s + 31 >= 16 * wv;      // columns up to the row; rows from it on
-            const bf16x8 x = frag_n(xs, TS, 16 * wv, 32 * s), z = frag_n(zs, TS, 16 * wv, 32 * s);
-            const bf16x8 xt = frag_t(xs, TS, 32 * s, 16 * wv), zt = frag_t(zs, TS, 32 * s, 16 * wv);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const bf16x8 kb = frag_t(ks, KS, 32 * s, 16 * t);
-                if (low) {
-                    dq[t] = mfma16(x, kb, dq[t]);
-                    dk[t] = mfma16(z, kb, dk[t]);
-                }
-                if (up) {
-                    dk[t] = mfma16(zt, kb, dk[t]);
-                    dk[t] = mfma16(xt, frag_t(qs, KS, 32 * s, 16 * t), dk[t]);
+            for (int half = 1; half >= 0; --half) {      // lo, then hi
+                bf16_t *const xh = xs + half * 64 * TS, *const zh = zs + half * 64 * TS;
+                const bf16x8 xa = frag_n(xh, TS, 16 * wv, 32 * s), za = frag_n(zh, TS, 16 * wv, 32 * s);
+                const bf16x8 xt = frag_t(xh, TS, 32 * s, 16 * wv), zt = frag_t(zh, TS, 32 * s, 16 * wv);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const bf16x8 kb = frag_t(ks, KS, 32 * s, 16 * t);
+                    if (low) {
+                        dq[t] = mfma16(kb, xa, dq[t]);
+                        dk[t] = mfma16(kb, za, dk[t]);
+                    }
+                    if (up) {
+                        dk[t] = mfma16(kb, zt, dk[t]);
+                        dk[t] = mfma16(frag_t(qs, KS, 32 * s, 16 * t), xt, dk[t]);
+                    }
                 }
             }
         }
-        __syncthreads();
-        // through dS1: e^(G_63 - G) N dS1^T into dK
-        f32x4 fs, dots_ = zero4();
-#pragma unroll
-        for (int v = 0; v < 4; ++v) fs[v] = ec[16 * wv + 4 * g4 + v] * rk[16 * wv + 4 * g4 + v];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            f32x4 x = zero4();
-#pragma unroll
-            for (int s = 0; s < DV / 32; ++s) x = mfma16(frag_n(ns, VS, 16 * wv, 32 * s), frag_t(ss, KS, 32 * s, 16 * t), x);
-            x *= fs;
-            dk[t] += x;
-#pragma unroll
-            for (int v = 0; v < 4; ++v) dots_[v] += x[v] * (float)ks[(16 * wv + 4 * g4 + v) * KS + 16 * t + l16];
-        }
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-#pragma unroll
-            for (int m = 1; m < 16; m <<= 1) dots_[v] += __shfl_xor(dots_[v], m, 64);
-            if (l16 == 0) dg_s[16 * wv + 4 * g4 + v] = dots_[v];
-        }
-        __syncthreads();
         if (wv == 0) {                                   // lane: its row
             float ends = dg_s[lane];
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) ends += __shfl_xor(ends, m, 64);
-            ends += eg[63] * ((dots[0] + dots[1]) + (dots[2] + dots[3]));
-            float dg = dg_row[lane] - ((dg_col[0][lane] + dg_col[1][lane]) + (dg_col[2][lane] + dg_col[3][lane])) + dg_q[lane] + dg_k[lane] - dg_s[lane];
+            ends += rows[DELTA_EG * 64 + 63] * ((dots[0] + dots[1]) + (dots[2] + dots[3]));
+            float dg = dg_row[lane] - ((dg_col[0][lane] + dg_col[1][lane]) + (dg_col[2][lane] + dg_col[3][lane]));
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) {
-                const float x = __shfl_down(dg, m, 64);
-                if (lane + m < 64) dg += x;
+                const float y = __shfl_down(dg, m, 64);
+                if (lane + m < 64) dg += y;
             }
             dg += ends;
             float da = 0.f, dlog = 0.f;
             if (lane < c.rows) {
                 const int64_t t = c.row0 + lane;
-                const float g = delta_gate(in, t, h), x = load_any(in.a, t * in.a_tok + h, in.a_f32) + load_any(in.dt_bias, h, in.param_f32);
-                da = -expf(load_any(in.a_log, h, in.param_f32)) / (1.f + expf(-x)) * dg;
+                const float g = delta_gate(in, t, h), y = load_any(in.a, t * in.a_tok + h, in.a_f32) + load_any(in.dt_bias, h, in.param_f32);
+                da = -expf(load_any(in.a_log, h, in.param_f32)) / (1.f + expf(-y)) * dg;
                 dlog = g * dg;
                 if (g == -1e4f) da = dlog = 0.f;
                 store_any(a.da, t * in.Hv + h, in.a_f32, da);
-                store_any(a.db, t * in.Hv + h, in.b_f32, (1.f - beta[lane]) * dbeta[lane]);
             }
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) {
@@ -402,43 +481,22 @@ __global__ __launch_bounds__(256) void dsa_delta_grad_kernel(DeltaArgs a) {
         }
     }
     // back through the unit length: with x = r q (r = 1/|q|), dq = r dx - q r^2 (q . r dx); the accumulators hold r dx
-    __syncthreads();
-    f32x4 pq = zero4(), pk = zero4();
+    float pq = 0.f, pk = 0.f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int r = 16 * wv + 4 * g4 + v;
-            pq[v] += dq[t][v] * (float)qs[r * KS + 16 * t + l16];
-            pk[v] += dk[t][v] * (float)ks[r * KS + 16 * t + l16];
-        }
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        const int r = 16 * wv + 4 * g4 + v;
-#pragma unroll
-        for (int m = 1; m < 16; m <<= 1) {
-            pq[v] += __shfl_xor(pq[v], m, 64);
-            pk[v] += __shfl_xor(pk[v], m, 64);
-        }
-        const float x = rq[r] / in.scale;
-        pq[v] *= in.l2_norm ? x * x : 0.f;
-        pk[v] *= in.l2_norm ? rk[r] * rk[r] : 0.f;
+    for (int t = 0; t < NT; ++t) {
+        pq = dot4(dq[t], four(qrow + 16 * t), pq);
+        pk = dot4(dk[t], four(krow + 16 * t), pk);
     }
+    const float rq = rows[DELTA_RQ * 64 + row] / in.scale, rk = rows[DELTA_RK * 64 + row];
+    pq = in.l2_norm ? over_row(pq) * rq * rq : 0.f;
+    pk = in.l2_norm ? over_row(pk) * rk * rk : 0.f;
+    bf16_t *const dq_row = a.dq + ((int64_t)(c.row0 + row) * in.Hk + hk) * in.Dk, *const dk_row = a.dk + ((int64_t)(c.row0 + row) * in.Hk + hk) * in.Dk;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {                    // (a lane's own places)
-            const int at = (16 * wv + 4 * g4 + v) * KS + 16 * t + l16;
-            qs[at] = (bf16_t)(dq[t][v] - pq[v] * (float)qs[at]);
-            ks[at] = (bf16_t)(dk[t][v] - pk[v] * (float)ks[at]);
-        }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < DK / 32; ++e) {
-        const int at = tid + 256 * e, r = at / (DK / 8), d = at % (DK / 8) * 8;
-        if (r < c.rows && d < in.Dk) {
-            *reinterpret_cast<u32x4_any *>(a.dq + ((int64_t)(c.row0 + r) * in.Hk + hk) * in.Dk + d) = *reinterpret_cast<const u32x4_any *>(qs + r * KS + d);
-            *reinterpret_cast<u32x4_any *>(a.dk + ((int64_t)(c.row0 + r) * in.Hk + hk) * in.Dk + d) = *reinterpret_cast<const u32x4_any *>(ks + r * KS + d);
+    for (int t = 0; t < NT; ++t) {
+        const int d = 16 * t + 4 * g4;
+        if (live && d < in.Dk) {
+            put4(dq_row + d, hi4(dq[t] - four(qrow + 16 * t) * pq));
+            put4(dk_row + d, hi4(dk[t] - four(krow + 16 * t) * pk));
         }
     }
 }
@@ -456,10 +514,14 @@ __global__ __launch_bounds__(256) void dsa_delta_param_kernel(DeltaArgs a) {
     if (threadIdx.x == 0) store_any(which ? a.ddt : a.da_log, h, a.in.param_f32, (red[0] + red[1]) + (red[2] + red[3]));
 }
 
+extern "C" int dsa_delta_columns(const DeltaArgs *a);
 extern "C" hipError_t dsa_launch_delta_bwd(const DeltaArgs *a, hipStream_t stream) {
-    const dim3 walks((unsigned)((int64_t)a->in.N * a->in.Hv * (a->Dvp / 64))), grid(a->slots, a->in.Hk);
-    if (a->Dkp == 64) hipLaunchKernelGGL((dsa_delta_back_kernel<64>), walks, dim3(256), 0, stream, *a);
-    else hipLaunchKernelGGL((dsa_delta_back_kernel<128>), walks, dim3(256), 0, stream, *a);
+    const int nc = dsa_delta_columns(a);
+    const dim3 walks((unsigned)(((int64_t)a->in.N * a->in.Hv + 7) / 8 * 8 * (a->Dvp / (16 * nc)))), grid(a->slots, a->in.Hk);
+    if (a->Dkp == 64 && nc == 1) hipLaunchKernelGGL((dsa_delta_back_kernel<64, 1>), walks, dim3(256), 0, stream, *a);
+    else if (a->Dkp == 64) hipLaunchKernelGGL((dsa_delta_back_kernel<64, 2>), walks, dim3(256), 0, stream, *a);
+    else if (nc == 1) hipLaunchKernelGGL((dsa_delta_back_kernel<128, 1>), walks, dim3(256), 0, stream, *a);
+    else hipLaunchKernelGGL((dsa_delta_back_kernel<128, 2>), walks, dim3(256), 0, stream, *a);
     if (a->Dkp == 64 && a->Dvp == 64) hipLaunchKernelGGL((dsa_delta_grad_kernel<64, 64>), grid, dim3(256), 0, stream, *a);
     else if (a->Dkp == 64) hipLaunchKernelGGL((dsa_delta_grad_kernel<64, 128>), grid, dim3(256), 0, stream, *a);
     else if (a->Dvp == 64) hipLaunchKernelGGL((dsa_delta_grad_kernel<128, 64>), grid, dim3(256), 0, stream, *a);

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
         const int h = hk * rep + u;
         const int64_t p = (int64_t)slot * in.Hv + h;
         __syncthreads();                                 // (the previous head's LDS has been read)
-        float *const rows = a.rows + p * DELTA_ROWS * 64;
+        float *const rows = (float *)(a.mats + p * a.mats_bytes);
         if (wv == 0) {
             const bool live = lane < c.rows;
             const int64_t t = c.row0 + (live ? lane : 0);
@@ -83,7 +83,8 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
             rows[DELTA_GL * 64 + lane] = gl[lane];
         }
         __syncthreads();
-        bf16_t *const pm = a.pmat + p * 4096;
+        bf16_t *const tg = (bf16_t *)(a.mats + p * a.mats_bytes + DELTA_T), *const pm = tg + a.planes * 4096;
+        f32x4 px[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             f32x4 x = zero4(), y = zero4();
@@ -94,7 +95,8 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
                 x[v] = j <= i ? e * rq[i] * rk[j] * qk[t][v] : 0.f;
                 y[v] = j < i ? e * bt[i] * rk[i] * rk[j] * kk[t][v] : 0.f;
             }
-            put4(pm + i * 64 + 16 * t + 4 * g4, hi4(x));
+            put_split4(pm + i * 64 + 16 * t + 4 * g4, pm + 4096 + i * 64 + 16 * t + 4 * g4, x);
+            px[t] = x;
             *reinterpret_cast<f32x4 *>(am + i * FS + 16 * t + 4 * g4) = y;
             if (t > wv) *reinterpret_cast<f32x4 *>(tm + i * FS + 16 * t + 4 * g4) = zero4();
         }
@@ -134,170 +136,253 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
             }
         }
         __syncthreads();
-        {
-            bf16_t *const th = a.tmat + p * 8192 + (tid >> 2) * 64 + (tid & 3) * 16, *const tl = th + 4096;
+        const int r = tid >> 2, c0 = (tid & 3) * 16;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) put_split4(th + 4 * e, tl + 4 * e, *reinterpret_cast<const f32x4 *>(tm + (tid >> 2) * FS + (tid & 3) * 16 + 4 * e));
+        for (int e = 0; e < 4; ++e) put_split4(tg + r * 64 + c0 + 4 * e, tg + 4096 + r * 64 + c0 + 4 * e, *reinterpret_cast<const f32x4 *>(tm + r * FS + c0 + 4 * e));
+        if (a.planes > 2) {                              // transposed, P through A's place
+#pragma unroll
+            for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4 *>(am + i * FS + 16 * t + 4 * g4) = px[t];
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f32x4 x, y;
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    x[v] = tm[(c0 + 4 * e + v) * FS + r];
+                    y[v] = am[(c0 + 4 * e + v) * FS + r];
+                }
+                put_split4(tg + 2 * 4096 + r * 64 + c0 + 4 * e, tg + 3 * 4096 + r * 64 + c0 + 4 * e, x);
+                put_split4(pm + 2 * 4096 + r * 64 + c0 + 4 * e, pm + 3 * 4096 + r * 64 + c0 + 4 * e, y);
+            }
         }
     }
 }
 
-// ---- the walk: one workgroup per sequence, value head and 64 columns of the state, a wave per 16 of them ----------------------------------
-// A wave's 16 columns (Dk x 16 fp32) stay in its registers from the first chunk to the last; what it multiplies with is shared by the four
-// waves in LDS, the next chunk's on its way into registers meanwhile.  Bound by the chain of a chunk's three products, each of which has to be laid out
-// anew for the next one (through the wave's own LDS, no barrier).
-template <int DK, bool SAVE>
-__global__ __launch_bounds__(256) void dsa_delta_walk_kernel(DeltaArgs a) {
-    constexpr int KS = DK + 8, TS = DELTA_TS, NS = 20;
-    __shared__ bf16_t ks[64 * KS], qs[64 * KS], th[64 * TS], tl[64 * TS], ps[64 * TS], vs[64 * TS];
-    __shared__ bf16_t wsh[4][16 * KS], wsl[4][16 * KS], wrh[4][16 * TS], wrl[4][16 * TS], wn[4][3][64 * NS];
-    __shared__ float rows[5 * 64];
+// ---- the walk: one workgroup per sequence, value head and 16 NC columns of the state -------------------------------------------------------
+// Wave w has rows 16 w .. of the chunk and rows Dk/4 w .. of the state, which stay in registers (fp32) from the first chunk to the last.  A chunk is a chain
+// of three products over the same columns - K S0 (and Q S0), T R, K^T N (and P N) - so their results go through LDS to the other waves, a barrier each; they are
+// formed transposed (lane: its row, four neighbouring columns), which makes every factor of a row one register and every access 8 or 16 bytes.
+// Rows of K, Q, T and P are needed by their own wave alone, as fragments that come from memory straight into registers; K also goes to LDS, for K^T.
+// Two sets of them take turns, and a set's loads for the chunk after next go out as soon as a product has read it: a chunk takes about as
+// long as memory takes to answer.  (With waves side by side over the columns instead, each of them read all of K, Q, T, P from LDS: 5.3 us per chunk.)
+template <int DK, int NC> struct WalkRows {
+    bf16x8 k[DK / 32], q[DK / 32], th[2], tl[2], ph[2], pl[2];
+    u32x2 v[NC];
+    float eg, ec, beta, rk, rq, end;
+};
+template <int DK, int NC, bool SAVE>
+__global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
+    constexpr int KS = DK + 8, RS = DELTA_RS, NT = DK / 64;
+    __shared__ bf16_t ks[2][64 * KS], sh[16 * NC * KS], sl[16 * NC * KS], rh[64 * RS], rl[64 * RS], nh[64 * RS], nl[64 * RS], mh[64 * RS], ml[64 * RS];
     const dsa_delta_args &in = a.in;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, l16 = lane & 15, g4 = lane >> 4;
-    const int blocks = a.Dvp / 64, h = blockIdx.x / blocks % in.Hv, seg = blockIdx.x / blocks / in.Hv, dv0 = blockIdx.x % blocks * 64;
-    const int hk = h / (in.Hv / in.Hk), dv = dv0 + 16 * wv + l16;
-    int slot0, chunks, s0, L;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g4 = lane >> 4, row = 16 * wv + l16;
+    int64_t unit;
+    int block, slot0, chunks, s0, L;
+    if (!delta_walk_unit(blockIdx.x, a.Dvp / (16 * NC), (int64_t)in.N * in.Hv, unit, block)) return;
+    const int h = (int)(unit % in.Hv), seg = (int)(unit / in.Hv), hk = h / (in.Hv / in.Hk), dv0 = 16 * NC * block;
     delta_segment(in.cu, in.N, seg, slot0, chunks, s0, L);
     chunks = min(chunks, a.slots - slot0);
     s0 = max(s0, 0);
-    bf16_t *const sh = wsh[wv], *const sl = wsl[wv], *const rh = wrh[wv], *const rl = wrl[wv], *const nh = wn[wv][0], *const nl = wn[wv][1], *const np = wn[wv][2];
-    f32x4 st[DK / 16];                                   // S[dk = 16 t + 4 g4 + v][dv]
-    const int64_t cell = ((int64_t)seg * in.Hv + h) * in.Dk * in.Dv + dv;
+    f32x4 st[NT][NC];                                    // S[dk = 16 (NT wv + t) + 4 g4 + v][dv0 + 16 c + l16]
+    const int64_t cell = ((int64_t)seg * in.Hv + h) * in.Dk * in.Dv + dv0 + l16;
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int k = 16 * t + 4 * g4 + v;
-            st[t][v] = a.initial && k < in.Dk && dv < in.Dv ? a.initial[cell + (int64_t)k * in.Dv] : 0.f;
-        }
-    Tile64<DK> tk, tq;
-    Tile64<64> tth, ttl, tp, tv;
-    float tr[2];
-    auto fetch = [&](int c) __attribute__((always_inline)) {
-        const int row0 = s0 + 64 * c, n = min(min(64, L - 64 * c), in.T - row0);
-        const int64_t p = (int64_t)(slot0 + c) * in.Hv + h;
-        tile_load<DK>(tk, (const bf16_t *)in.k + row0 * in.k_tok + hk * in.k_head, in.k_tok, n, in.Dk);
-        tile_load<DK>(tq, (const bf16_t *)in.q + row0 * in.q_tok + hk * in.q_head, in.q_tok, n, in.Dk);
-        tile_load<64>(tth, a.tmat + p * 8192, 64, 64, 64);
-        tile_load<64>(ttl, a.tmat + p * 8192 + 4096, 64, 64, 64);
-        tile_load<64>(tp, a.pmat + p * 4096, 64, 64, 64);
-        tile_load<64>(tv, (const bf16_t *)in.v + row0 * in.v_tok + h * in.v_head + dv0, in.v_tok, n, in.Dv - dv0);
-        tr[0] = a.rows[p * DELTA_ROWS * 64 + tid];
-        tr[1] = tid < 64 ? a.rows[p * DELTA_ROWS * 64 + 256 + tid] : 0.f;
-    };
-    if (chunks > 0) fetch(0);
-    for (int c = 0; c < chunks; ++c) {
-        const int row0 = s0 + 64 * c, n = min(min(64, L - 64 * c), in.T - row0);
-        const int64_t p = (int64_t)(slot0 + c) * in.Hv + h;
-        tile_put<DK>(tk, ks, KS);
-        tile_put<DK>(tq, qs, KS);
-        tile_put<64>(tth, th, TS);
-        tile_put<64>(ttl, tl, TS);
-        tile_put<64>(tp, ps, TS);
-        tile_put<64>(tv, vs, TS);
-        rows[tid] = tr[0];
-        if (tid < 64) rows[256 + tid] = tr[1];
-        __syncthreads();
-        if (c + 1 < chunks) fetch(c + 1);
-        const float *const eg = rows + DELTA_EG * 64, *const ec = rows + DELTA_EC * 64, *const beta = rows + DELTA_BETA * 64, *const rk = rows + DELTA_RK * 64,
-                    *const rq = rows + DELTA_RQ * 64;
-        // S0 as [dv][dk]
-#pragma unroll
-        for (int t = 0; t < DK / 16; ++t) {
-            const u32x2 x = hi4(st[t]);
-            put4(sh + l16 * KS + 16 * t + 4 * g4, x);
-            put4(sl + l16 * KS + 16 * t + 4 * g4, lo4(st[t], x));
-            if (SAVE) put4(a.state + (p * a.Dvp + dv) * DK + 16 * t + 4 * g4, x);
-        }
-        wave_sync();
-        f32x4 o[4], r[4];                                // o: [dv = 4 g4 + v][row 16 m + l16];  r: [row 16 m + 4 g4 + v][dv = l16]
-#pragma unroll
-        for (int m = 0; m < 4; ++m) o[m] = r[m] = zero4();
-#pragma unroll
-        for (int s = 0; s < DK / 32; ++s) {
-            const bf16x8 bh = frag_n(sh, KS, 0, 32 * s), bl = frag_n(sl, KS, 0, 32 * s);
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const bf16x8 ka = frag_n(ks, KS, 16 * m, 32 * s);
-                r[m] = mfma16(ka, bl, r[m]);
-                r[m] = mfma16(ka, bh, r[m]);
-                o[m] = mfma16(bh, frag_n(qs, KS, 16 * m, 32 * s), o[m]);
-            }
-        }
-        // R = beta (V - e^G K S0), as [dv][row]
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            f32x4 x;
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                const int i = 16 * m + 4 * g4 + v;
-                x[v] = beta[i] * ((float)vs[i * TS + 16 * wv + l16] - eg[i] * rk[i] * r[m][v]);
+                const int k = 16 * (NT * wv + t) + 4 * g4 + v;
+                st[t][c][v] = a.initial && k < in.Dk && dv0 + 16 * c + l16 < in.Dv ? a.initial[cell + (int64_t)k * in.Dv + 16 * c] : 0.f;
             }
-            put_split4(rh + l16 * TS + 16 * m + 4 * g4, rl + l16 * TS + 16 * m + 4 * g4, x);
-        }
-        wave_sync();
-        // N^T = R^T T^T: [dv = 4 g4 + v][row 16 m + l16]; rows of T end at the diagonal
+    loads_done();
+    // offsets of this lane, in bytes
+    int at_k[DK / 32], at_q[DK / 32], at_v[NC], at_o[NC];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            f32x4 x = zero4();
+    for (int s = 0; s < DK / 32; ++s) {
+        const int d = 32 * s + 8 * g4;
+        at_k[s] = d < in.Dk ? (row * (int)in.k_tok + d) * 2 : NOWHERE;
+        at_q[s] = d < in.Dk ? (row * (int)in.q_tok + d) * 2 : NOWHERE;
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = dv0 + 16 * c + 4 * g4;
+        at_v[c] = d < in.Dv ? (row * (int)in.v_tok + d) * 2 : NOWHERE;
+        at_o[c] = d < in.Dv ? (row * in.Hv * in.Dv + d) * 2 : NOWHERE;
+    }
+    const int at_t = row * 128 + 16 * g4, at_t1 = wv >= 2 ? at_t + 64 : NOWHERE;          // (rows of T and P end at the diagonal)
+    const int at_s = ((dv0 + l16) * DK + 16 * NT * wv + 4 * g4) * 2, at_n = (row * a.Dvp + dv0 + 4 * g4) * 2;
+    // where the next chunk to be fetched, and the one at hand, lie; a chunk further they are a fixed number of bytes on
+    const int64_t first = (int64_t)slot0 * in.Hv + h;
+    const char *pk = (const char *)in.k + (s0 * in.k_tok + hk * in.k_head) * 2, *pq = (const char *)in.q + (s0 * in.q_tok + hk * in.q_head) * 2;
+    const char *pv = (const char *)in.v + (s0 * in.v_tok + h * in.v_head) * 2, *pm = a.mats + first * a.mats_bytes;
+    char *ps = a.saved + first * a.saved_bytes, *po = (char *)(a.out + ((int64_t)s0 * in.Hv + h) * in.Dv);
+    const int64_t step_m = (int64_t)in.Hv * a.mats_bytes, step_s = (int64_t)in.Hv * a.saved_bytes;
+    const int step_k = (int)in.k_tok * 128, step_q = (int)in.q_tok * 128, step_v = (int)in.v_tok * 128, step_o = in.Hv * in.Dv * 128;
+    const int rows_all = min(L, in.T - s0);              // (one chunk after the other takes its 64 of them)
+    typedef WalkRows<DK, NC> Rows;
+    auto fetch_rows = [&](int i, Rows &w) __attribute__((always_inline)) {
+        const int n = min(64, rows_all - 64 * i);
+        const buffer_t k = rows_buffer(pk, (int)in.k_tok, n, in.Dk), q = rows_buffer(pq, (int)in.q_tok, n, in.Dk), v = rows_buffer(pv, (int)in.v_tok, n, in.Dv);
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) {
+            w.k[s] = buf16(k, at_k[s]);
+            w.q[s] = buf16(q, at_q[s]);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) w.v[c] = buf8(v, at_v[c]);
+        const bool on = i + 1 < chunks;                  // (the last one is fetched again: behind a branch, waits would be for every load in flight)
+        pk += on ? step_k : 0;
+        pq += on ? step_q : 0;
+        pv += on ? step_v : 0;
+    };
+    auto fetch_t = [&](Rows &w) __attribute__((always_inline)) {
+        const buffer_t m = buffer_of(pm, a.mats_bytes);
+        w.th[0] = buf16(m, at_t, DELTA_T);
+        w.tl[0] = buf16(m, at_t, DELTA_T + DELTA_PLANE);
+        w.th[1] = buf16(m, at_t1, DELTA_T);
+        w.tl[1] = buf16(m, at_t1, DELTA_T + DELTA_PLANE);
+    };
+    auto fetch_p = [&](int i, Rows &w) __attribute__((always_inline)) {
+        const buffer_t m = buffer_of(pm, a.mats_bytes);
+        const int p = DELTA_T + a.planes * DELTA_PLANE;
+        w.ph[0] = buf16(m, at_t, p);
+        w.pl[0] = buf16(m, at_t, p + DELTA_PLANE);
+        w.ph[1] = buf16(m, at_t1, p);
+        w.pl[1] = buf16(m, at_t1, p + DELTA_PLANE);
+        w.eg = buf4(m, DELTA_EG * 256 + row * 4);
+        w.ec = buf4(m, DELTA_EC * 256 + row * 4);
+        w.beta = buf4(m, DELTA_BETA * 256 + row * 4);
+        w.rk = buf4(m, DELTA_RK * 256 + row * 4);
+        w.rq = buf4(m, DELTA_RQ * 256 + row * 4);
+        w.end = buf4(m, DELTA_EG * 256 + 252);
+        pm += i + 1 < chunks ? step_m : 0;
+    };
+    auto chunk = [&](int i, Rows &x, bf16_t *kt) __attribute__((always_inline)) {
+        const int ahead = min(i + 2, chunks - 1);
+        // S0 as [dv][dk], K as it is
+        const buffer_t save = buffer_of(ps, a.saved_bytes);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int at = (16 * c + l16) * KS + 16 * (NT * wv + t) + 4 * g4;
+                const u32x2 y = hi4(st[t][c]);
+                put4(sh + at, y);
+                put4(sl + at, lo4(st[t][c], y));
+                if (SAVE) buf_put8(save, at_s + c * 32 * DK + 32 * t, y);
+            }
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) *reinterpret_cast<bf16x8 *>(kt + row * KS + 32 * s + 8 * g4) = x.k[s];
+        __syncthreads();
+        f32x4 o[NC], r[NC];                              // [dv = 16 c + 4 g4 + v][row]
+#pragma unroll
+        for (int c = 0; c < NC; ++c) o[c] = r[c] = zero4();
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const bf16x8 ah = frag_n(sh, KS, 16 * c, 32 * s), al = frag_n(sl, KS, 16 * c, 32 * s);
+                r[c] = mfma16(al, x.k[s], r[c]);
+                o[c] = mfma16(al, x.q[s], o[c]);
+                r[c] = mfma16(ah, x.k[s], r[c]);
+                o[c] = mfma16(ah, x.q[s], o[c]);
+            }
+        const float f = x.eg * x.rk;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) put_split4(rh + row * RS + 16 * c + 4 * g4, rl + row * RS + 16 * c + 4 * g4, (up4(x.v[c]) - r[c] * f) * x.beta);
+        fetch_rows(ahead, x);
+        __syncthreads();
+        // N^T = R^T T^T
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            f32x4 y = zero4();
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                if (32 * s > 16 * m + 15) continue;
-                const bf16x8 ah = frag_n(rh, TS, 0, 32 * s), al = frag_n(rl, TS, 0, 32 * s), bh = frag_n(th, TS, 16 * m, 32 * s), bl = frag_n(tl, TS, 16 * m, 32 * s);
-                x = mfma16(al, bh, x);
-                x = mfma16(ah, bl, x);
-                x = mfma16(ah, bh, x);
+                if (s == 1 && wv < 2) continue;
+                const bf16x8 ah = frag_t(rh, RS, 32 * s, 16 * c), al = frag_t(rl, RS, 32 * s, 16 * c);
+                y = mfma16(al, x.th[s], y);
+                y = mfma16(ah, x.tl[s], y);
+                y = mfma16(ah, x.th[s], y);
             }
-            const int i = 16 * m + l16;
-            const u32x2 y = hi4(x);
-            put4(np + i * NS + 4 * g4, y);
-            if (SAVE) put4(a.news + (p * 64 + i) * a.Dvp + dv0 + 16 * wv + 4 * g4, y);
-            const float f = ec[i] * rk[i];
-            put_split4(nh + i * NS + 4 * g4, nl + i * NS + 4 * g4, x * f);
+            const int at = row * RS + 16 * c + 4 * g4;
+            const u32x2 yh = hi4(y), yl = lo4(y, yh);
+            put4(nh + at, yh);
+            put4(nl + at, yl);
+            put_split4(mh + at, ml + at, y * (x.ec * x.rk));
+            if (SAVE) {
+                buf_put8(save, at_n + 32 * c, yh, a.Dvp * DK * 2);
+                buf_put8(save, at_n + 32 * c, yl, a.Dvp * (DK * 2 + 128));
+            }
         }
-        wave_sync();
-        // O^T = scale e^G S0^T Q^T + N^T P^T
-        bf16x8 na[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) na[s] = frag_t(np, NS, 32 * s, 0);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const int i = 16 * m + l16;
-            o[m] *= eg[i] * rq[i];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-                if (32 * s <= 16 * m + 15) o[m] = mfma16(na[s], frag_n(ps, TS, 16 * m, 32 * s), o[m]);
-            const int d = dv0 + 16 * wv + 4 * g4;
-            if (i < n && d < in.Dv) put4(a.out + ((int64_t)(row0 + i) * in.Hv + h) * in.Dv + d, hi4(o[m]));
-        }
+        fetch_t(x);
+        __syncthreads();
         // S1 = e^G_63 S0 + K^T e^(G_63 - G) N
-        const float e = eg[63];
-        bf16x8 bh[2], bl[2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) st[t][c] *= x.end;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            bh[s] = frag_t(nh, NS, 32 * s, 0);
-            bl[s] = frag_t(nl, NS, 32 * s, 0);
-        }
+            bf16x8 bh[NC], bl[NC];
 #pragma unroll
-        for (int t = 0; t < DK / 16; ++t) {
-            st[t] *= e;
+            for (int c = 0; c < NC; ++c) {
+                bh[c] = frag_t(mh, RS, 32 * s, 16 * c);
+                bl[c] = frag_t(ml, RS, 32 * s, 16 * c);
+            }
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const bf16x8 ka = frag_t(ks, KS, 32 * s, 16 * t);
-                st[t] = mfma16(ka, bl[s], st[t]);
-                st[t] = mfma16(ka, bh[s], st[t]);
+            for (int t = 0; t < NT; ++t) {
+                const bf16x8 ka = frag_t(kt, KS, 32 * s, 16 * (NT * wv + t));
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    st[t][c] = mfma16(ka, bl[c], st[t][c]);
+                    st[t][c] = mfma16(ka, bh[c], st[t][c]);
+                }
             }
         }
-        __syncthreads();
+        // O^T = scale e^G S0^T Q^T + N^T P^T
+        const buffer_t out = rows_buffer(po, in.Hv * in.Dv, min(64, rows_all - 64 * i), in.Dv);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            o[c] *= x.eg * x.rq;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s == 1 && wv < 2) continue;
+                const bf16x8 ah = frag_t(nh, RS, 32 * s, 16 * c), al = frag_t(nl, RS, 32 * s, 16 * c);
+                o[c] = mfma16(al, x.ph[s], o[c]);
+                o[c] = mfma16(ah, x.pl[s], o[c]);
+                o[c] = mfma16(ah, x.ph[s], o[c]);
+            }
+            buf_put8(out, at_o[c], hi4(o[c]));
+        }
+        fetch_p(ahead, x);
+        po += step_o;
+        if (SAVE) ps += step_s;
+    };
+    Rows x, y;
+    if (chunks > 0) {
+        fetch_rows(0, x);
+        fetch_t(x);
+        fetch_p(0, x);
+        fetch_rows(min(1, chunks - 1), y);
+        fetch_t(y);
+        fetch_p(min(1, chunks - 1), y);
+        int i = 0;
+        for (; i + 1 < chunks; i += 2) {
+            chunk(i, x, ks[0]);
+            chunk(i + 1, y, ks[1]);
+        }
+        if (i < chunks) chunk(i, x, ks[0]);
     }
     if (a.final) {
 #pragma unroll
-        for (int t = 0; t < DK / 16; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int k = 16 * t + 4 * g4 + v;
-                if (k < in.Dk && dv < in.Dv) a.final[cell + (int64_t)k * in.Dv] = st[t][v];
-            }
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const int k = 16 * (NT * wv + t) + 4 * g4 + v;
+                    if (k < in.Dk && dv0 + 16 * c + l16 < in.Dv) a.final[cell + (int64_t)k * in.Dv + 16 * c] = st[t][c][v];
+                }
     }
 }
 
@@ -393,21 +478,24 @@ __global__ __launch_bounds__(256) void dsa_delta_step_kernel(dsa_delta_args in, 
     }
 }
 
+// Groups of 16 columns per walk: one where the launch leaves compute units without a walk of two
+extern "C" int dsa_delta_columns(const DeltaArgs *a) { return (int64_t)a->in.N * a->in.Hv * (a->Dvp / 32) < 256 ? 1 : 2; }
 extern "C" hipError_t dsa_launch_delta_fwd(const DeltaArgs *a, int save, hipStream_t stream) {
     if (a->in.T > 0) {
         const dim3 grid(a->slots, a->in.Hk);
         if (a->Dkp == 64) hipLaunchKernelGGL((dsa_delta_prep_kernel<64>), grid, dim3(256), 0, stream, *a);
         else hipLaunchKernelGGL((dsa_delta_prep_kernel<128>), grid, dim3(256), 0, stream, *a);
     }
-    const dim3 walks((unsigned)((int64_t)a->in.N * a->in.Hv * (a->Dvp / 64)));
     if (a->in.T > 0 || a->final) {
-        if (a->Dkp == 64) {
-            if (save) hipLaunchKernelGGL((dsa_delta_walk_kernel<64, true>), walks, dim3(256), 0, stream, *a);
-            else hipLaunchKernelGGL((dsa_delta_walk_kernel<64, false>), walks, dim3(256), 0, stream, *a);
-        } else {
-            if (save) hipLaunchKernelGGL((dsa_delta_walk_kernel<128, true>), walks, dim3(256), 0, stream, *a);
-            else hipLaunchKernelGGL((dsa_delta_walk_kernel<128, false>), walks, dim3(256), 0, stream, *a);
-        }
+        const int nc = dsa_delta_columns(a);
+        const dim3 walks((unsigned)(((int64_t)a->in.N * a->in.Hv + 7) / 8 * 8 * (a->Dvp / (16 * nc))));
+#define DELTA_WALK(DK, NC)                                                                                                    \
+    if (save) hipLaunchKernelGGL((dsa_delta_walk_kernel<DK, NC, true>), walks, dim3(256), 0, stream, *a);                      \
+    else hipLaunchKernelGGL((dsa_delta_walk_kernel<DK, NC, false>), walks, dim3(256), 0, stream, *a);
+        if (a->Dkp == 64 && nc == 1) { DELTA_WALK(64, 1) }
+        else if (a->Dkp == 64) { DELTA_WALK(64, 2) }
+        else if (nc == 1) { DELTA_WALK(128, 1) }
+        else { DELTA_WALK(128, 2) }
     }
     return hipGetLastError();
 }

@@ -14,7 +14,8 @@ void same_device(const Tensor &a, const Tensor &b, const char *name) {
 }
 // The tensor itself where its rows can be read 16 bytes at a time in place, a contiguous copy otherwise
 Tensor rows16(const Tensor &x) {
-    const bool ok = x.numel() == 0 || (x.stride(2) == 1 && (x.size(1) == 1 || x.stride(1) % 8 == 0) && (x.size(0) == 1 || x.stride(0) % 8 == 0) && aligned16(x));
+    const bool ok = x.numel() == 0 || (x.stride(2) == 1 && (x.size(1) == 1 || x.stride(1) % 8 == 0) && (x.size(0) == 1 || (x.stride(0) % 8 == 0 && x.stride(0) <= DSA_DELTA_MAX_ROW)) &&
+                    aligned16(x));
     if (ok) return x;
     const Tensor c = x.contiguous();
     return aligned16(c) ? c : c.clone();

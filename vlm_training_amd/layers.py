@@ -5,6 +5,8 @@
 * ``SelfAttention``         - models/qwen3_5/model.py:76-136: the same with ``q_proj`` emitting ``[q | gate]`` per
   head, OffsetRMSNorm (``1 + weight``), a rotary width that may be smaller than head_dim, the output multiplied by
   ``sigmoid(gate)``, and DTensor unwrap / rewrap around the kernels (models/qwen3_5/model.py:124,132).
+* ``GatedDeltaNet``         - models/qwen3_5/model.py:138-228: the linear-attention layers of the same stack: projections -> short convolution with
+  SiLU -> gated delta rule -> gated norm -> ``out_proj``;  ``forward(x, cu_seqlens)``, and ``step(x, state)`` for one token per request.
 * ``DsaIndexer``            - the lightning indexer's projections as module parameters (the reference holds no
   indexer): hidden -> Hi*Di index queries, hidden -> Di index key (one per token), hidden -> Hi head weights.
 
@@ -24,10 +26,11 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .delta import gated_delta_rule, gated_delta_step, short_conv, short_conv_step
 from .dtensor_utils import _dtensor_rewrap, _dtensor_unwrap, _local
 from .model_attention import run_varlen_attn
 from .ops import dsa_varlen_attn, indexer_kl_loss
-from .prologue import qk_norm_rope, sigmoid_gate
+from .prologue import gated_rms_norm, qk_norm_rope, sigmoid_gate
 
 
 @dataclass
@@ -249,3 +252,75 @@ class SelfAttention(nn.Module):
         out = attention_core(self, qg[..., :D], k, v, cos, sin, cu_seqlens, max_seqlen, x=x, gate=qg[..., D:], offset=True)
         out = _dtensor_rewrap(out, wrap)
         return self.o_proj(out.reshape(1, total, -1).to(x.dtype))
+
+
+@dataclass
+class DeltaState:
+    """What a ``GatedDeltaNet`` layer carries from token to token for B requests: the convolution's last inputs (B, channels, width - 1) bf16 and
+    the rule's states (B, value heads, Dk, Dv) fp32, both updated in place by ``step``."""
+    conv: torch.Tensor
+    delta: torch.Tensor
+
+
+class GatedDeltaNet(nn.Module):
+    """models/qwen3_5/model.py:138-228 (the linear-attention layers of the hybrid stack) with the parameter names of its checkpoints; ``cfg`` holds hidden_size,
+    linear_num_key_heads, linear_num_value_heads, linear_key_head_dim, linear_value_head_dim, linear_conv_kernel_dim and
+    rms_norm_eps.  Head counts come from the projections' outputs, so a head-sharded layer sees its own."""
+
+    def __init__(self, cfg):
+        super().__init__()
+        self.key_dim, self.value_dim = cfg.linear_key_head_dim, cfg.linear_value_head_dim
+        hk, hv = cfg.linear_num_key_heads, cfg.linear_num_value_heads
+        keys, values = hk * self.key_dim, hv * self.value_dim
+        self.in_proj_qkv = nn.Linear(cfg.hidden_size, 2 * keys + values, bias=False)
+        self.in_proj_z = nn.Linear(cfg.hidden_size, values, bias=False)
+        self.in_proj_b = nn.Linear(cfg.hidden_size, hv, bias=False)
+        self.in_proj_a = nn.Linear(cfg.hidden_size, hv, bias=False)
+        self.conv1d = nn.Conv1d(2 * keys + values, 2 * keys + values, cfg.linear_conv_kernel_dim, groups=2 * keys + values, bias=False)
+        self.dt_bias = nn.Parameter(torch.ones(hv))
+        self.A_log = nn.Parameter(torch.empty(hv).uniform_(1, 16).log())
+        self.norm = RMSNorm(self.value_dim, eps=cfg.rms_norm_eps)
+        self.out_proj = nn.Linear(values, cfg.hidden_size, bias=False)
+
+    def _project(self, x):
+        lin = _projections(x, (self.in_proj_qkv, self.in_proj_z, self.in_proj_b, self.in_proj_a), None)
+        if lin is not None:
+            return lin, None
+        h = x.reshape(-1, x.shape[-1])
+        return _dtensor_unwrap(*(_bf16(m(h)) for m in (self.in_proj_qkv, self.in_proj_z, self.in_proj_b, self.in_proj_a)))
+
+    def _heads(self, mixed, z):
+        """q, k, v and z as (rows, heads, dim) views."""
+        values = z.shape[1]
+        keys = (mixed.shape[1] - values) // 2
+        q, k, v = mixed.split((keys, keys, values), dim=1)
+        return (q.unflatten(1, (-1, self.key_dim)), k.unflatten(1, (-1, self.key_dim)), v.unflatten(1, (-1, self.value_dim)),
+                z.unflatten(1, (-1, self.value_dim)))
+
+    def _out(self, out, z, wrap, like):
+        out = gated_rms_norm(out, z, _local(self.norm.weight), eps=self.norm.eps)
+        out = _dtensor_rewrap(out.flatten(1), wrap)
+        return self.out_proj(out.to(like.dtype)).reshape(like.shape)
+
+    def forward(self, x, cu_seqlens, state: Optional[DeltaState] = None, return_state: bool = False):
+        """x (1, T, hidden) packed -> (1, T, hidden); ``state`` is where the N sequences start, ``return_state`` adds the ``DeltaState`` behind them
+        (to go on with ``step``)."""
+        (mixed, z, b, a), wrap = self._project(x)
+        conv = short_conv(mixed, _local(self.conv1d.weight), _local(self.conv1d.bias), cu_seqlens, initial_state=None if state is None else state.conv,
+                          return_final_state=return_state)
+        mixed, conv_state = conv if return_state else (conv, None)
+        q, k, v, z = self._heads(mixed, z)
+        out = gated_delta_rule(q, k, v, a, b, _local(self.A_log), _local(self.dt_bias), cu_seqlens, initial_state=None if state is None else state.delta,
+                               return_final_state=return_state)
+        out, delta_state = out if return_state else (out, None)
+        out = self._out(out, z, wrap, x)
+        return (out, DeltaState(conv_state, delta_state)) if return_state else out
+
+    @torch.no_grad()
+    def step(self, x, state: DeltaState):
+        """The next token of B requests: x (B, hidden) -> (B, hidden), ``state`` moves on in place."""
+        (mixed, z, b, a), wrap = self._project(x)
+        mixed = short_conv_step(mixed, state.conv, _local(self.conv1d.weight), _local(self.conv1d.bias))
+        q, k, v, z = self._heads(mixed, z)
+        out = gated_delta_step(q, k, v, a, b, _local(self.A_log), _local(self.dt_bias), state.delta)
+        return self._out(out, z, wrap, x)
