@@ -23,8 +23,12 @@ struct DeltaArgs {
     dsa_delta_args in;
     int slots, Dkp, Dvp;               // chunks at the most; head dims padded to 64 or 128
     // A chunk of a value head ("cell", slots x Hv of them) has a block of each of three arrays.
-    // mats: the rows' factors (DELTA_ROWS x 64 floats), then planes of 64 x 64 bf16: T as hi, lo and, where a backward follows, transposed hi, lo; P the same
-    // saved, for the backward: S0 transposed (Dvp x Dkp), N as hi, lo (2 x 64 x Dvp);  back, the backward's own: dS1 transposed, dR (64 x Dvp)
+    // mats: the rows' factors (DELTA_ROWS x 64 floats), then planes of 64 x 64 bf16: T as hi, lo and, where a backward follows, transposed hi, lo; P the same.
+    //       A plane lies in the order of its fragments: wave, half of the columns, lane, eight elements.
+    // saved, for the backward: S0 (Dvp x Dkp), N as hi, lo (Dvp x 64 x 2);  back, the backward's own: dS1, dR (Dvp x 64).  They lie as the walks' lanes
+    //       hold them: 16 columns of the values, wave, lane, its elements (state: DK/16 of them, N: four as hi, four as lo, dR: four).
+    // (A quad of lanes that reads or writes four rows takes four times as long as one that stays in one: with rows of T, P, S and N in row order, K and
+    // Q as fragments straight from their rows and 8-byte stores, the walk of 16 384 tokens took 0.62 ms.)
     char *mats, *saved, *back;
     int planes, mats_bytes, saved_bytes, back_bytes;
     const float *initial;              // (N, Hv, Dk, Dv) or null
@@ -145,6 +149,7 @@ __device__ __forceinline__ void tile_copy(bf16_t *lds, int stride, const bf16_t 
 // written there).  A lane that has nothing to read or write gets the offset NOWHERE once, in front of the loop; no address is formed inside it.
 // (With 64-bit addresses and masks formed per chunk a walk of 512 chunks took 1.74 ms, most of it their arithmetic.)
 #define NOWHERE 0x7fffff00
+__device__ __forceinline__ int further(int off, int by) { return (int)((uint32_t)off + (uint32_t)by); }       // (from NOWHERE on still past any end)
 typedef __amdgpu_buffer_rsrc_t buffer_t;
 __device__ __forceinline__ buffer_t buffer_of(const void *p, int bytes) {
     const int64_t a = reinterpret_cast<int64_t>(p);
@@ -160,6 +165,32 @@ __device__ __forceinline__ float buf4(buffer_t b, int off) { return __uint_as_fl
 __device__ __forceinline__ void buf_put8(buffer_t b, int off, u32x2 x, int at = 0) { __builtin_amdgcn_raw_buffer_store_b64(x, b, off, at, 0); }
 // every load so far has arrived: in front of a loop whose loads are waited for by count (what is in flight there from before would be counted in with them)
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+__device__ __forceinline__ void buf_put16(buffer_t b, int off, u32x4 x, int at = 0) { __builtin_amdgcn_raw_buffer_store_b128(x, b, off, at, 0); }
+// four or eight elements at a time
+template <int N> struct Piece { uint32_t x[N / 2]; };
+template <int N> __device__ __forceinline__ Piece<N> buf_piece(buffer_t b, int off) {
+    if constexpr (N == 8) return __builtin_bit_cast(Piece<8>, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+    else return __builtin_bit_cast(Piece<4>, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0));
+}
+template <int N> __device__ __forceinline__ void buf_put_piece(buffer_t b, int off, Piece<N> p, int at = 0) {
+    if constexpr (N == 8) buf_put16(b, off, __builtin_bit_cast(u32x4, p), at);
+    else buf_put8(b, off, __builtin_bit_cast(u32x2, p), at);
+}
+// LDS, on 8-byte boundaries
+template <int N> __device__ __forceinline__ void put_piece(bf16_t *t, Piece<N> p) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) *reinterpret_cast<u32x2_any *>(t + 4 * i) = u32x2{p.x[2 * i], p.x[2 * i + 1]};
+}
+template <int N> __device__ __forceinline__ Piece<N> get_piece(const bf16_t *t) {
+    Piece<N> p;
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        const u32x2 x = *reinterpret_cast<const u32x2_any *>(t + 4 * i);
+        p.x[2 * i] = x[0];
+        p.x[2 * i + 1] = x[1];
+    }
+    return p;
+}
 // 16 bytes of a row from column c on, zero where there is none
 __device__ __forceinline__ bf16x8 row_frag(const bf16_t *row, int c, bool in) {
     return in ? *reinterpret_cast<const bf16x8 *>(row + c) : zero_bf16x8();

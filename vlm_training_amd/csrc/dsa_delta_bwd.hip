@@ -36,23 +36,16 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
                 st[t][c][v] = a.dfinal && k < in.Dk && dv0 + 16 * c + l16 < in.Dv ? a.dfinal[cell + (int64_t)k * in.Dv + 16 * c] : 0.f;
             }
     loads_done();
-    int at_k[DK / 32], at_q[DK / 32], at_o[NC];          // offsets of this lane, in bytes
-#pragma unroll
-    for (int s = 0; s < DK / 32; ++s) {
-        const int d = 32 * s + 8 * g4;
-        at_k[s] = d < in.Dk ? (row * (int)in.k_tok + d) * 2 : NOWHERE;
-        at_q[s] = d < in.Dk ? (row * (int)in.q_tok + d) * 2 : NOWHERE;
-    }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int d = dv0 + 16 * c + 4 * g4;
-        at_o[c] = d < in.Dv ? (row * in.Hv * in.Dv + d) * 2 : NOWHERE;
-    }
-    const int at_t = wv < 2 ? row * 128 + 16 * g4 : NOWHERE, at_t1 = row * 128 + 16 * g4 + 64;       // (transposed rows begin at the diagonal)
-    const int at_s = ((dv0 + l16) * DK + 16 * NT * wv + 4 * g4) * 2, at_n = (row * a.Dvp + dv0 + 4 * g4) * 2;
+    // offsets of this lane, in bytes
+    constexpr int LPR = DK / 8, RPI = 64 / LPR;          // lanes to a row of K or Q, rows to a load
+    const int rrow = 16 * wv + lane / LPR, rcol = lane % LPR * 8, vrow = 16 * wv + lane / 4, vcol = lane % 4 * 4 * NC;
+    const int at_k = rcol < in.Dk ? (rrow * (int)in.k_tok + rcol) * 2 : NOWHERE, at_q = rcol < in.Dk ? (rrow * (int)in.q_tok + rcol) * 2 : NOWHERE;
+    const int at_o = dv0 + vcol < in.Dv ? (vrow * in.Hv * in.Dv + dv0 + vcol) * 2 : NOWHERE;
+    const int at_t = wv < 2 ? wv * 2048 + lane * 16 : NOWHERE, at_t1 = wv * 2048 + lane * 16 + 1024;                 // (transposed rows begin at the diagonal)
+    const int at_s = (dv0 * DK + (wv * 64 + lane) * 4 * NT) * 2, at_n = (dv0 / 16 * 256 + wv * 64 + lane) * 8;
     struct BackRows {
         bf16x8 k[DK / 32], q[DK / 32], th[2], tl[2], ph[2], pl[2];
-        u32x2 o[NC];
+        Piece<4 * NC> o;
         float eg, ec, beta, rk, rq, end;
     };
     // where the next chunk to be fetched, and the one at hand, lie; a chunk further they are a fixed number of bytes back
@@ -67,22 +60,24 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
         const int n = min(64, rows_all - 64 * i);
         const buffer_t q = rows_buffer(pq, (int)in.q_tok, n, in.Dk), o = rows_buffer(po, in.Hv * in.Dv, n, in.Dv);
 #pragma unroll
-        for (int s = 0; s < DK / 32; ++s) w.q[s] = buf16(q, at_q[s]);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) w.o[c] = buf8(o, at_o[c]);
+        for (int s = 0; s < DK / 32; ++s) w.q[s] = buf16(q, further(at_q, s * RPI * (int)in.q_tok * 2));
+        w.o = buf_piece<4 * NC>(o, at_o);
         pq -= i > 0 ? step_q : 0;                        // (the first one is fetched again: behind a branch, waits would be for every load in flight)
         po -= i > 0 ? step_o : 0;
     };
     auto fetch_k = [&](int i, BackRows &w) __attribute__((always_inline)) {
-        const buffer_t k = rows_buffer(pk, (int)in.k_tok, min(64, rows_all - 64 * i), in.Dk), m = buffer_of(pm, a.mats_bytes);
-        const int p = DELTA_T + (a.planes + 2) * DELTA_PLANE;
+        const buffer_t k = rows_buffer(pk, (int)in.k_tok, min(64, rows_all - 64 * i), in.Dk);
 #pragma unroll
-        for (int s = 0; s < DK / 32; ++s) w.k[s] = buf16(k, at_k[s]);
+        for (int s = 0; s < DK / 32; ++s) w.k[s] = buf16(k, further(at_k, s * RPI * (int)in.k_tok * 2));
+        pk -= i > 0 ? step_k : 0;
+    };
+    auto fetch_p = [&](BackRows &w) __attribute__((always_inline)) {
+        const buffer_t m = buffer_of(pm, a.mats_bytes);
+        const int p = DELTA_T + (a.planes + 2) * DELTA_PLANE;
         w.ph[0] = buf16(m, at_t, p);
         w.pl[0] = buf16(m, at_t, p + DELTA_PLANE);
         w.ph[1] = buf16(m, at_t1, p);
         w.pl[1] = buf16(m, at_t1, p + DELTA_PLANE);
-        pk -= i > 0 ? step_k : 0;
     };
     auto fetch_t = [&](int i, BackRows &w) __attribute__((always_inline)) {
         const buffer_t m = buffer_of(pm, a.mats_bytes);
@@ -103,39 +98,47 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
         // dS1 as [dv][dk]; K, Q and dO as they are, and scale/|q| e^G dO
         const buffer_t back = buffer_of(pb, a.back_bytes);
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int c = 0; c < NC; ++c) {
+            Piece<4 * NT> all;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
+            for (int t = 0; t < NT; ++t) {
                 const int at = (16 * c + l16) * KS + 16 * (NT * wv + t) + 4 * g4;
                 const u32x2 y = hi4(st[t][c]);
                 put4(sh + at, y);
                 put4(sl + at, lo4(st[t][c], y));
-                buf_put8(back, at_s + c * 32 * DK + 32 * t, y);
+                all.x[2 * t] = y[0];
+                all.x[2 * t + 1] = y[1];
             }
+            buf_put_piece<4 * NT>(back, at_s + c * 32 * DK, all);
+        }
 #pragma unroll
         for (int s = 0; s < DK / 32; ++s) {
-            *reinterpret_cast<bf16x8 *>(ks + row * KS + 32 * s + 8 * g4) = x.k[s];
-            *reinterpret_cast<bf16x8 *>(qs + row * KS + 32 * s + 8 * g4) = x.q[s];
+            *reinterpret_cast<bf16x8 *>(ks + (rrow + s * RPI) * KS + rcol) = x.k[s];
+            *reinterpret_cast<bf16x8 *>(qs + (rrow + s * RPI) * KS + rcol) = x.q[s];
         }
+        put_piece<4 * NC>(os + vrow * RS + vcol, x.o);
+        fetch_q(ahead, x);
+        fetch_k(ahead, x);
+        wave_sync();
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int at = row * RS + 16 * c + 4 * g4;
-            put4(os + at, x.o[c]);
-            put_split4(oh + at, ol + at, up4(x.o[c]) * (x.eg * x.rq));
+            put_split4(oh + at, ol + at, up4(*reinterpret_cast<const u32x2_any *>(os + at)) * (x.eg * x.rq));
         }
-        fetch_q(ahead, x);
         __syncthreads();
         // dN^T = e^(G_63 - G) dS1^T K^T + dO^T P
         f32x4 r[NC];                                     // [dv = 16 c + 4 g4 + v][row]
 #pragma unroll
         for (int c = 0; c < NC; ++c) r[c] = zero4();
 #pragma unroll
-        for (int s = 0; s < DK / 32; ++s)
+        for (int s = 0; s < DK / 32; ++s) {
+            const bf16x8 kb = frag_n(ks, KS, 16 * wv, 32 * s);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                r[c] = mfma16(frag_n(sl, KS, 16 * c, 32 * s), x.k[s], r[c]);
-                r[c] = mfma16(frag_n(sh, KS, 16 * c, 32 * s), x.k[s], r[c]);
+                r[c] = mfma16(frag_n(sl, KS, 16 * c, 32 * s), kb, r[c]);
+                r[c] = mfma16(frag_n(sh, KS, 16 * c, 32 * s), kb, r[c]);
             }
+        }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             r[c] *= x.ec * x.rk;
@@ -148,7 +151,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
             }
             put_split4(nh + row * RS + 16 * c + 4 * g4, nl + row * RS + 16 * c + 4 * g4, r[c]);
         }
-        fetch_k(ahead, x);
+        fetch_p(x);
         __syncthreads();
         // dR^T = dN^T T
         const buffer_t dvs = rows_buffer(pv, in.Hv * in.Dv, min(64, rows_all - 64 * i), in.Dv);
@@ -164,10 +167,12 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
                 y = mfma16(ah, x.th[s], y);
             }
             const int at = row * RS + 16 * c + 4 * g4;
-            buf_put8(back, at_n + 32 * c, hi4(y), a.Dvp * DK * 2);
-            buf_put8(dvs, at_o[c], hi4(y * x.beta));
+            buf_put8(back, at_n + c * 2048, hi4(y), a.Dvp * DK * 2);
+            put4(os + at, hi4(y * x.beta));
             put_split4(sh + at, sl + at, y * (-x.beta * x.eg * x.rk));
         }
+        wave_sync();
+        buf_put_piece<4 * NC>(dvs, at_o, get_piece<4 * NC>(os + vrow * RS + vcol));
         const float end = x.end;
         fetch_t(ahead, x);
         __syncthreads();
@@ -207,9 +212,11 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
         int i = chunks - 1;
         fetch_q(i, x);
         fetch_k(i, x);
+        fetch_p(x);
         fetch_t(i, x);
         fetch_q(max(i - 1, 0), y);
         fetch_k(max(i - 1, 0), y);
+        fetch_p(y);
         fetch_t(max(i - 1, 0), y);
         for (; i > 0; i -= 2) {
             chunk(i, x);
@@ -298,24 +305,42 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         for (int e = tid; e < DELTA_ROWS * 64; e += 256) rows[e] = ((const float *)(a.mats + p * a.mats_bytes))[e];
 #pragma unroll 1
         for (int b = 0; b < DV / 64; ++b) {
-            const bf16_t *const orow = a.dout + ((int64_t)(c.row0 + row) * in.Hv + h) * in.Dv + 64 * b, *const rrow = drs + row * DV + 64 * b;
+            const bf16_t *const orow = a.dout + ((int64_t)(c.row0 + row) * in.Hv + h) * in.Dv + 64 * b;
             bf16x8 of[2], rf[2];
-            Tile64<64> th, tl;
-            Tile64<DK> ts;
-            tile_load<64>(th, news + 64 * b, DV, 64, 64);
-            tile_load<64>(tl, news + 64 * DV + 64 * b, DV, 64, 64);
-            tile_load<DK>(ts, state + 64 * b * DK, DK, 64, DK);
+            u32x4 tn[4], ts[DK / 32];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tn[e] = *reinterpret_cast<const u32x4_any *>(news + (64 * b * 16 + tid + 256 * e) * 8);
+#pragma unroll
+            for (int e = 0; e < DK / 32; ++e) ts[e] = *reinterpret_cast<const u32x4_any *>(state + 64 * b * DK + (tid + 256 * e) * 8);
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 of[s] = row_frag(orow, 32 * s + 8 * g4, live && 64 * b + 32 * s + 8 * g4 < in.Dv);
-                rf[s] = row_frag(rrow, 32 * s + 8 * g4, true);
+                // eight columns of dR: two lanes' four
+                const bf16_t *const r4 = drs + ((4 * b + 2 * s + (g4 >> 1)) * 256 + wv * 64 + (g4 & 1) * 32 + l16) * 4;
+                const u32x2 lo = *reinterpret_cast<const u32x2_any *>(r4), hi = *reinterpret_cast<const u32x2_any *>(r4 + 64);
+                rf[s] = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
             }
             if (b) __syncthreads();                      // (the columns before have been read)
-            tile_put<64>(th, ns, TS);
-            tile_put<64>(tl, ns + 64 * TS, TS);
-            tile_put<DK>(ts, ss, KS);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {                // N: 16 columns e, wave wv, this lane
+                bf16_t *const to = ns + row * TS + 16 * e + 4 * g4;
+                put4(to, u32x2{tn[e][0], tn[e][1]});
+                put4(to + 64 * TS, u32x2{tn[e][2], tn[e][3]});
+            }
+            // the state's pieces of four: 16 columns, wave, lane, NS of them
+            constexpr int NS = DK / 64;
+            auto place = [&](int e, int half) __attribute__((always_inline)) {
+                const int piece = (tid + 256 * e) * 2 + half, l = piece / NS % 64;
+                return ss + (piece / (NS * 256) * 16 + l % 16) * KS + (piece / (NS * 64) % 4 * NS + piece % NS) * 16 + l / 16 * 4;
+            };
+#pragma unroll
+            for (int e = 0; e < DK / 32; ++e) {
+                put4(place(e, 0), u32x2{ts[e][0], ts[e][1]});
+                put4(place(e, 1), u32x2{ts[e][2], ts[e][3]});
+            }
             __syncthreads();
-            tile_load<DK>(ts, dstate + 64 * b * DK, DK, 64, DK);
+#pragma unroll
+            for (int e = 0; e < DK / 32; ++e) ts[e] = *reinterpret_cast<const u32x4_any *>(dstate + 64 * b * DK + (tid + 256 * e) * 8);
             // dO N^T and dR N^T
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -358,10 +383,11 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             // dS1 in the place of S0, their product summed on the way
 #pragma unroll
             for (int e = 0; e < DK / 32; ++e) {
-                const int at = tid + 256 * e;
-                bf16_t *const q = ss + at / (DK / 8) * KS + at % (DK / 8) * 8;
-                dot = dot8_chain(__builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_any *>(q)), __builtin_bit_cast(bf16x8, ts.x[e]), dot);
-                *reinterpret_cast<u32x4_any *>(q) = ts.x[e];
+                bf16_t *const q0 = place(e, 0), *const q1 = place(e, 1);
+                const u32x2 lo = *reinterpret_cast<const u32x2_any *>(q0), hi = *reinterpret_cast<const u32x2_any *>(q1);
+                dot = dot8_chain(__builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]}), __builtin_bit_cast(bf16x8, ts[e]), dot);
+                put4(q0, u32x2{ts[e][0], ts[e][1]});
+                put4(q1, u32x2{ts[e][2], ts[e][3]});
             }
             __syncthreads();
             // through dS1: e^(G_63 - G) N dS1^T into dK

@@ -95,7 +95,6 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
                 x[v] = j <= i ? e * rq[i] * rk[j] * qk[t][v] : 0.f;
                 y[v] = j < i ? e * bt[i] * rk[i] * rk[j] * kk[t][v] : 0.f;
             }
-            put_split4(pm + i * 64 + 16 * t + 4 * g4, pm + 4096 + i * 64 + 16 * t + 4 * g4, x);
             px[t] = x;
             *reinterpret_cast<f32x4 *>(am + i * FS + 16 * t + 4 * g4) = y;
             if (t > wv) *reinterpret_cast<f32x4 *>(tm + i * FS + 16 * t + 4 * g4) = zero4();
@@ -136,23 +135,29 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
             }
         }
         __syncthreads();
-        const int r = tid >> 2, c0 = (tid & 3) * 16;
+        // P through A's place, then the planes in the order of their fragments
 #pragma unroll
-        for (int e = 0; e < 4; ++e) put_split4(tg + r * 64 + c0 + 4 * e, tg + 4096 + r * 64 + c0 + 4 * e, *reinterpret_cast<const f32x4 *>(tm + r * FS + c0 + 4 * e));
-        if (a.planes > 2) {                              // transposed, P through A's place
+        for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4 *>(am + i * FS + 16 * t + 4 * g4) = px[t];
+        __syncthreads();
+        auto plane = [&](bf16_t *to, int at, f32x4 x, f32x4 y) __attribute__((always_inline)) {
+            const u32x2 xh = hi4(x), yh = hi4(y), xl = lo4(x, xh), yl = lo4(y, yh);
+            *reinterpret_cast<u32x4_any *>(to + at) = u32x4{xh[0], xh[1], yh[0], yh[1]};
+            *reinterpret_cast<u32x4_any *>(to + 4096 + at) = u32x4{xl[0], xl[1], yl[0], yl[1]};
+        };
 #pragma unroll
-            for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4 *>(am + i * FS + 16 * t + 4 * g4) = px[t];
-            __syncthreads();
+        for (int e = 0; e < 2; ++e) {
+            const int at = tid + 256 * e, r = at / 128 * 16 + l16, c0 = at / 64 % 2 * 32 + 8 * g4;
+            plane(tg, at * 8, *reinterpret_cast<const f32x4 *>(tm + r * FS + c0), *reinterpret_cast<const f32x4 *>(tm + r * FS + c0 + 4));
+            plane(pm, at * 8, *reinterpret_cast<const f32x4 *>(am + r * FS + c0), *reinterpret_cast<const f32x4 *>(am + r * FS + c0 + 4));
+            if (a.planes > 2) {                          // transposed
+                f32x4 x[2], y[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                f32x4 x, y;
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    x[v] = tm[(c0 + 4 * e + v) * FS + r];
-                    y[v] = am[(c0 + 4 * e + v) * FS + r];
+                for (int v = 0; v < 8; ++v) {
+                    x[v / 4][v % 4] = tm[(c0 + v) * FS + r];
+                    y[v / 4][v % 4] = am[(c0 + v) * FS + r];
                 }
-                put_split4(tg + 2 * 4096 + r * 64 + c0 + 4 * e, tg + 3 * 4096 + r * 64 + c0 + 4 * e, x);
-                put_split4(pm + 2 * 4096 + r * 64 + c0 + 4 * e, pm + 3 * 4096 + r * 64 + c0 + 4 * e, y);
+                plane(tg + 2 * 4096, at * 8, x[0], x[1]);
+                plane(pm + 2 * 4096, at * 8, y[0], y[1]);
             }
         }
     }
@@ -162,18 +167,21 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
 // Wave w has rows 16 w .. of the chunk and rows Dk/4 w .. of the state, which stay in registers (fp32) from the first chunk to the last.  A chunk is a chain
 // of three products over the same columns - K S0 (and Q S0), T R, K^T N (and P N) - so their results go through LDS to the other waves, a barrier each; they are
 // formed transposed (lane: its row, four neighbouring columns), which makes every factor of a row one register and every access 8 or 16 bytes.
-// Rows of K, Q, T and P are needed by their own wave alone, as fragments that come from memory straight into registers; K also goes to LDS, for K^T.
-// Two sets of them take turns, and a set's loads for the chunk after next go out as soon as a product has read it: a chunk takes about as
-// long as memory takes to answer.  (With waves side by side over the columns instead, each of them read all of K, Q, T, P from LDS: 5.3 us per chunk.)
+// Rows of K, Q, T and P are needed by their own wave alone (K by all of them as K^T): T and P come as fragments straight into registers, rows of K, Q and V
+// 16 bytes a lane through the wave's own part of LDS.  Two sets of registers take turns, and a set's loads for the chunk after next go out as soon as it has
+// been read: a chunk takes about as long as memory takes to answer.  (With waves side by side over the columns instead, each of them read all of K, Q, T, P from LDS: 5.3 us per chunk.)
 template <int DK, int NC> struct WalkRows {
     bf16x8 k[DK / 32], q[DK / 32], th[2], tl[2], ph[2], pl[2];
-    u32x2 v[NC];
+    Piece<4 * NC> v;
     float eg, ec, beta, rk, rq, end;
 };
 template <int DK, int NC, bool SAVE>
 __global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
     constexpr int KS = DK + 8, RS = DELTA_RS, NT = DK / 64;
-    __shared__ bf16_t ks[2][64 * KS], sh[16 * NC * KS], sl[16 * NC * KS], rh[64 * RS], rl[64 * RS], nh[64 * RS], nl[64 * RS], mh[64 * RS], ml[64 * RS];
+    __shared__ bf16_t ks[2][64 * KS], sh[16 * NC * KS], sl[16 * NC * KS], rh[64 * RS], rl[64 * RS], pool[4 * 64 * RS];
+    // N and e^(G_63 - G)/|k| N as hi, lo; Q before they are there
+    bf16_t *const nh = pool, *const nl = pool + 64 * RS, *const mh = pool + 128 * RS, *const ml = pool + 192 * RS, *const qt = pool;
+    static_assert(KS <= 4 * RS, "Q lies in N's place");
     const dsa_delta_args &in = a.in;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g4 = lane >> 4, row = 16 * wv + l16;
     int64_t unit;
@@ -196,21 +204,12 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
             }
     loads_done();
     // offsets of this lane, in bytes
-    int at_k[DK / 32], at_q[DK / 32], at_v[NC], at_o[NC];
-#pragma unroll
-    for (int s = 0; s < DK / 32; ++s) {
-        const int d = 32 * s + 8 * g4;
-        at_k[s] = d < in.Dk ? (row * (int)in.k_tok + d) * 2 : NOWHERE;
-        at_q[s] = d < in.Dk ? (row * (int)in.q_tok + d) * 2 : NOWHERE;
-    }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int d = dv0 + 16 * c + 4 * g4;
-        at_v[c] = d < in.Dv ? (row * (int)in.v_tok + d) * 2 : NOWHERE;
-        at_o[c] = d < in.Dv ? (row * in.Hv * in.Dv + d) * 2 : NOWHERE;
-    }
-    const int at_t = row * 128 + 16 * g4, at_t1 = wv >= 2 ? at_t + 64 : NOWHERE;          // (rows of T and P end at the diagonal)
-    const int at_s = ((dv0 + l16) * DK + 16 * NT * wv + 4 * g4) * 2, at_n = (row * a.Dvp + dv0 + 4 * g4) * 2;
+    constexpr int LPR = DK / 8, RPI = 64 / LPR;          // lanes to a row of K or Q, rows to a load
+    const int rrow = 16 * wv + lane / LPR, rcol = lane % LPR * 8, vrow = 16 * wv + lane / 4, vcol = lane % 4 * 4 * NC;
+    const int at_k = rcol < in.Dk ? (rrow * (int)in.k_tok + rcol) * 2 : NOWHERE, at_q = rcol < in.Dk ? (rrow * (int)in.q_tok + rcol) * 2 : NOWHERE;
+    const int at_v = dv0 + vcol < in.Dv ? (vrow * (int)in.v_tok + dv0 + vcol) * 2 : NOWHERE, at_o = dv0 + vcol < in.Dv ? (vrow * in.Hv * in.Dv + dv0 + vcol) * 2 : NOWHERE;
+    const int at_t = wv * 2048 + lane * 16, at_t1 = wv >= 2 ? at_t + 1024 : NOWHERE;       // (rows of T and P end at the diagonal)
+    const int at_s = (dv0 * DK + (wv * 64 + lane) * 4 * NT) * 2, at_n = (dv0 / 16 * 256 + wv * 64 + lane) * 16;
     // where the next chunk to be fetched, and the one at hand, lie; a chunk further they are a fixed number of bytes on
     const int64_t first = (int64_t)slot0 * in.Hv + h;
     const char *pk = (const char *)in.k + (s0 * in.k_tok + hk * in.k_head) * 2, *pq = (const char *)in.q + (s0 * in.q_tok + hk * in.q_head) * 2;
@@ -224,12 +223,11 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
         const int n = min(64, rows_all - 64 * i);
         const buffer_t k = rows_buffer(pk, (int)in.k_tok, n, in.Dk), q = rows_buffer(pq, (int)in.q_tok, n, in.Dk), v = rows_buffer(pv, (int)in.v_tok, n, in.Dv);
 #pragma unroll
-        for (int s = 0; s < DK / 32; ++s) {
-            w.k[s] = buf16(k, at_k[s]);
-            w.q[s] = buf16(q, at_q[s]);
+        for (int s = 0; s < DK / 32; ++s) {              
+            w.k[s] = buf16(k, further(at_k, s * RPI * (int)in.k_tok * 2));
+            w.q[s] = buf16(q, further(at_q, s * RPI * (int)in.q_tok * 2));
         }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) w.v[c] = buf8(v, at_v[c]);
+        w.v = buf_piece<4 * NC>(v, at_v);
         const bool on = i + 1 < chunks;                  // (the last one is fetched again: behind a branch, waits would be for every load in flight)
         pk += on ? step_k : 0;
         pq += on ? step_q : 0;
@@ -262,35 +260,49 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
         // S0 as [dv][dk], K as it is
         const buffer_t save = buffer_of(ps, a.saved_bytes);
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int c = 0; c < NC; ++c) {
+            Piece<4 * NT> all;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
+            for (int t = 0; t < NT; ++t) {
                 const int at = (16 * c + l16) * KS + 16 * (NT * wv + t) + 4 * g4;
                 const u32x2 y = hi4(st[t][c]);
                 put4(sh + at, y);
                 put4(sl + at, lo4(st[t][c], y));
-                if (SAVE) buf_put8(save, at_s + c * 32 * DK + 32 * t, y);
+                all.x[2 * t] = y[0];
+                all.x[2 * t + 1] = y[1];
             }
+            if (SAVE) buf_put_piece<4 * NT>(save, at_s + c * 32 * DK, all);
+        }
 #pragma unroll
-        for (int s = 0; s < DK / 32; ++s) *reinterpret_cast<bf16x8 *>(kt + row * KS + 32 * s + 8 * g4) = x.k[s];
+        for (int s = 0; s < DK / 32; ++s) *reinterpret_cast<bf16x8 *>(kt + (rrow + s * RPI) * KS + rcol) = x.k[s];
         __syncthreads();
+        // Q and V: the wave's own rows
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) *reinterpret_cast<bf16x8 *>(qt + (rrow + s * RPI) * KS + rcol) = x.q[s];
+        put_piece<4 * NC>(rh + vrow * RS + vcol, x.v);
+        fetch_rows(ahead, x);
+        wave_sync();
         f32x4 o[NC], r[NC];                              // [dv = 16 c + 4 g4 + v][row]
 #pragma unroll
         for (int c = 0; c < NC; ++c) o[c] = r[c] = zero4();
 #pragma unroll
-        for (int s = 0; s < DK / 32; ++s)
+        for (int s = 0; s < DK / 32; ++s) {
+            const bf16x8 kb = frag_n(kt, KS, 16 * wv, 32 * s), qb = frag_n(qt, KS, 16 * wv, 32 * s);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const bf16x8 ah = frag_n(sh, KS, 16 * c, 32 * s), al = frag_n(sl, KS, 16 * c, 32 * s);
-                r[c] = mfma16(al, x.k[s], r[c]);
-                o[c] = mfma16(al, x.q[s], o[c]);
-                r[c] = mfma16(ah, x.k[s], r[c]);
-                o[c] = mfma16(ah, x.q[s], o[c]);
+                r[c] = mfma16(al, kb, r[c]);
+                o[c] = mfma16(al, qb, o[c]);
+                r[c] = mfma16(ah, kb, r[c]);
+                o[c] = mfma16(ah, qb, o[c]);
             }
+        }
         const float f = x.eg * x.rk;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) put_split4(rh + row * RS + 16 * c + 4 * g4, rl + row * RS + 16 * c + 4 * g4, (up4(x.v[c]) - r[c] * f) * x.beta);
-        fetch_rows(ahead, x);
+        for (int c = 0; c < NC; ++c) {
+            const int at = row * RS + 16 * c + 4 * g4;
+            put_split4(rh + at, rl + at, (up4(*reinterpret_cast<const u32x2_any *>(rh + at)) - r[c] * f) * x.beta);
+        }
         __syncthreads();
         // N^T = R^T T^T
 #pragma unroll
@@ -309,10 +321,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
             put4(nh + at, yh);
             put4(nl + at, yl);
             put_split4(mh + at, ml + at, y * (x.ec * x.rk));
-            if (SAVE) {
-                buf_put8(save, at_n + 32 * c, yh, a.Dvp * DK * 2);
-                buf_put8(save, at_n + 32 * c, yl, a.Dvp * (DK * 2 + 128));
-            }
+            if (SAVE) buf_put16(save, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]}, a.Dvp * DK * 2);
         }
         fetch_t(x);
         __syncthreads();
@@ -352,8 +361,10 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
                 o[c] = mfma16(ah, x.pl[s], o[c]);
                 o[c] = mfma16(ah, x.ph[s], o[c]);
             }
-            buf_put8(out, at_o[c], hi4(o[c]));
+            put4(rh + row * RS + 16 * c + 4 * g4, hi4(o[c]));
         }
+        wave_sync();
+        buf_put_piece<4 * NC>(out, at_o, get_piece<4 * NC>(rh + vrow * RS + vcol));
         fetch_p(ahead, x);
         po += step_o;
         if (SAVE) ps += step_s;
