@@ -4,9 +4,9 @@
 //     dP = dO N^T   dA = -dR N^T   X = scale E dP   Z = beta E dA (below the diagonal)
 //     dQ = X K + scale e^G dO S0^T          dK = X^T Q + (Z + Z^T) K + e^(G_63 - G) N dS1^T - beta e^G dR S0^T
 //     db = (1 - beta) dR.N                  (dR.N = beta dbeta: both of beta's places, in R and in A, at once)
-//     dG_i = rows of (X QK + Z KK) - columns of it + q.(scale e^G S0 dO) - k.(beta e^G S0 dR) - k.(e^(G_63 - G) dS1 N)
+//     dG_i = q.(X K + scale e^G S0 dO) + k.(Z K - beta e^G S0 dR) - k.(X^T Q + Z^T K + e^(G_63 - G) dS1 N)
 //     dG_63 also + all k.(e^(G_63 - G) dS1 N) + e^G_63 <dS1, S0>
-// dg is the sum of dG from its row on.  Rows and columns of X QK come from one rounding, so that a pair of rows behind t leaves nothing in dg_t.
+// dg is the sum of dG from its row on.  What a pair of rows behind t adds comes in twice with opposite signs, from one X and Z: it leaves 2^-17 of itself.
 #include "dsa_delta.h"
 
 // ---- the walk: as the forward's, from the last chunk to the first ------------------------------------------------------------------------
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
         pm -= i > 0 ? step_m : 0;
     };
     auto chunk = [&](int i, BackRows &x) __attribute__((always_inline)) {
-        const int ahead = max(i - 2, 0);
+        const int ahead = max(i - 1, 0);
         // dS1 as [dv][dk]; K, Q and dO as they are, and scale/|q| e^G dO
         const buffer_t back = buffer_of(pb, a.back_bytes);
 #pragma unroll
@@ -207,22 +207,13 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
         pv -= step_o;
         __syncthreads();
     };
-    BackRows x, y;
+    BackRows x;
     if (chunks > 0) {
-        int i = chunks - 1;
-        fetch_q(i, x);
-        fetch_k(i, x);
+        fetch_q(chunks - 1, x);
+        fetch_k(chunks - 1, x);
         fetch_p(x);
-        fetch_t(i, x);
-        fetch_q(max(i - 1, 0), y);
-        fetch_k(max(i - 1, 0), y);
-        fetch_p(y);
-        fetch_t(max(i - 1, 0), y);
-        for (; i > 0; i -= 2) {
-            chunk(i, x);
-            chunk(i - 1, y);
-        }
-        if (i == 0) chunk(0, x);
+        fetch_t(chunks - 1, x);
+        for (int i = chunks - 1; i >= 0; --i) chunk(i, x);
     }
     if (a.dinitial) {
 #pragma unroll
@@ -245,7 +236,7 @@ template <int DK, int DV>
 __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
     constexpr int KS = DK + 8, TS = DELTA_TS, NT = DK / 16;
     __shared__ bf16_t ks[64 * KS], qs[64 * KS], pool[4 * 64 * TS];
-    __shared__ float rows[DELTA_ROWS * 64], dg_row[64], dg_col[4][64], dg_s[64], dots[4];
+    __shared__ float rows[DELTA_ROWS * 64], dg_row[64], dg_s[64], dots[4];
     bf16_t *const ns = pool, *const ss = pool + 2 * 64 * TS;                                              // N as hi, lo; S0, then dS1: 64 columns of the values
     bf16_t *const xs = pool, *const zs = pool + 2 * 64 * TS;                                              // in their place X and Z as hi, lo
     static_assert(64 * KS <= 2 * 64 * TS, "64 rows of the state lie in two tiles");
@@ -269,20 +260,6 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
     }
     tile_copy<DK>(ks, KS, (const bf16_t *)in.k + c.row0 * in.k_tok + hk * in.k_head, in.k_tok, c.rows, in.Dk);
     tile_copy<DK>(qs, KS, (const bf16_t *)in.q + c.row0 * in.q_tok + hk * in.q_head, in.q_tok, c.rows, in.Dk);
-    __syncthreads();
-    f32x4 kk[4], qk[4];                                  // [j = 16 t + 4 g4 + v][row]
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        kk[t] = qk[t] = zero4();
-        if (t <= wv) {
-#pragma unroll
-            for (int s = 0; s < DK / 32; ++s) {
-                const bf16x8 kj = frag_n(ks, KS, 16 * t, 32 * s);
-                kk[t] = mfma16(kj, frag_n(ks, KS, 16 * wv, 32 * s), kk[t]);
-                qk[t] = mfma16(kj, frag_n(qs, KS, 16 * wv, 32 * s), qk[t]);
-            }
-        }
-    }
     f32x4 dq[NT], dk[NT];                                // [16 t + 4 g4 + v][row], times scale/|q| and 1/|k|
 #pragma unroll
     for (int t = 0; t < NT; ++t) dq[t] = dk[t] = zero4();
@@ -298,7 +275,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         const bf16_t *const state = (const bf16_t *)(a.saved + p * a.saved_bytes), *const news = state + DV * DK;
         const bf16_t *const dstate = (const bf16_t *)(a.back + p * a.back_bytes), *const drs = dstate + DV * DK;
         f32x4 x[4], z[4];
-        float dotq = 0.f, dotk = 0.f, dots_ = 0.f, dot = 0.f, db = 0.f;
+        float sum = 0.f, dots_ = 0.f, dot = 0.f, db = 0.f;      // sum: what the row adds to dG
 #pragma unroll
         for (int t = 0; t < 4; ++t) x[t] = z[t] = zero4();
         __syncthreads();                                 // (the previous head's LDS has been read)
@@ -376,8 +353,8 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 w *= fk;
                 dq[t] += y;
                 dk[t] += w;
-                dotq = dot4(y, four(qrow + 16 * t), dotq);
-                dotk = dot4(w, four(krow + 16 * t), dotk);
+                sum = dot4(y, four(qrow + 16 * t), sum);
+                sum = dot4(w, four(krow + 16 * t), sum);
             }
             __syncthreads();
             // dS1 in the place of S0, their product summed on the way
@@ -402,10 +379,9 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             }
         }
         __syncthreads();
-        // X and Z, their products with QK and KK summed over rows and columns
+        // X and Z
         const float rk = rows[DELTA_RK * 64 + row], fx = rows[DELTA_RQ * 64 + row], fz = -rows[DELTA_BETA * 64 + row] * rk;
         const float gi = rows[DELTA_GH * 64 + row], gi_lo = rows[DELTA_GL * 64 + row];
-        float sum = 0.f, col[16];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             f32x4 xv = zero4(), zv = zero4();
@@ -421,65 +397,61 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             const int at = row * TS + 16 * t + 4 * g4;
             put_split4(xs + at, xs + 64 * TS + at, xv);
             put_split4(zs + at, zs + 64 * TS + at, zv);
-            const f32x4 both = xv * qk[t] + zv * kk[t];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                sum += both[v];
-                col[4 * t + v] = both[v];
-            }
         }
-        // sixteen columns' sums over sixteen lanes: each step, a lane keeps one half of its columns and hands the other over; lane l ends with column l
 #pragma unroll
-        for (int m = 8; m > 0; m >>= 1) {
-            const bool up = l16 & m;
+        for (int m = 1; m < 64; m <<= 1) dot += __shfl_xor(dot, m, 64);
+        if (lane == 0) dots[wv] = dot;
+        __syncthreads();
+        // X K, X^T Q, (Z + Z^T) K.  X and Z keep to columns up to the row; transposed, to rows from it on
+        bf16x8 xa[2][2], za[2][2], xt[2][2], zt[2][2];   // [hi, lo][32 columns or rows]
 #pragma unroll
-            for (int e = 0; e < m; ++e) {
-                const float keep = up ? col[e + m] : col[e], send = up ? col[e] : col[e + m];
-                col[e] = keep + __shfl_xor(send, m, 64);
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                bf16_t *const xh = xs + half * 64 * TS, *const zh = zs + half * 64 * TS;
+                xa[half][s] = frag_n(xh, TS, 16 * wv, 32 * s);
+                za[half][s] = frag_n(zh, TS, 16 * wv, 32 * s);
+                xt[half][s] = frag_t(xh, TS, 32 * s, 16 * wv);
+                zt[half][s] = frag_t(zh, TS, 32 * s, 16 * wv);
             }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            f32x4 y = zero4(), w = zero4(), u1 = zero4();
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const bf16x8 kb = frag_t(ks, KS, 32 * s, 16 * t);
+#pragma unroll
+                for (int half = 1; half >= 0; --half) {
+                    if (s == 0 || wv >= 2) {
+                        y = mfma16(kb, xa[half][s], y);
+                        w = mfma16(kb, za[half][s], w);
+                    }
+                    if (s == 1 || wv < 2) {
+                        u1 = mfma16(kb, zt[half][s], u1);
+                        u1 = mfma16(frag_t(qs, KS, 32 * s, 16 * t), xt[half][s], u1);
+                    }
+                }
+            }
+            sum = dot4(y, four(qrow + 16 * t), sum);
+            sum = dot4(w - u1, four(krow + 16 * t), sum);
+            dq[t] += y;
+            dk[t] += w + u1;
         }
-        dg_col[wv][16 * (l16 >> 2) + 4 * g4 + (l16 & 3)] = col[0];
         dots_ = over_row(dots_);
-        sum = over_row(sum) + over_row(dotq) + over_row(dotk) - dots_;
+        sum = over_row(sum) - dots_;
         db = over_row(db);
         if (g4 == 0) {
             dg_row[row] = sum;
             dg_s[row] = dots_;
             if (live) store_any(a.db, (int64_t)(c.row0 + row) * in.Hv + h, in.b_f32, (1.f - rows[DELTA_BETA * 64 + row]) * db);
         }
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) dot += __shfl_xor(dot, m, 64);
-        if (lane == 0) dots[wv] = dot;
         __syncthreads();
-        // X K, X^T Q, (Z + Z^T) K
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const bool low = 32 * s <= 16 * wv + 15, up = 32 * s + 31 >= 16 * wv;      // columns up to the row; rows from it on
-#pragma unroll
-            for (int half = 1; half >= 0; --half) {      // lo, then hi
-                bf16_t *const xh = xs + half * 64 * TS, *const zh = zs + half * 64 * TS;
-                const bf16x8 xa = frag_n(xh, TS, 16 * wv, 32 * s), za = frag_n(zh, TS, 16 * wv, 32 * s);
-                const bf16x8 xt = frag_t(xh, TS, 32 * s, 16 * wv), zt = frag_t(zh, TS, 32 * s, 16 * wv);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const bf16x8 kb = frag_t(ks, KS, 32 * s, 16 * t);
-                    if (low) {
-                        dq[t] = mfma16(kb, xa, dq[t]);
-                        dk[t] = mfma16(kb, za, dk[t]);
-                    }
-                    if (up) {
-                        dk[t] = mfma16(kb, zt, dk[t]);
-                        dk[t] = mfma16(frag_t(qs, KS, 32 * s, 16 * t), xt, dk[t]);
-                    }
-                }
-            }
-        }
         if (wv == 0) {                                   // lane: its row
             float ends = dg_s[lane];
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) ends += __shfl_xor(ends, m, 64);
             ends += rows[DELTA_EG * 64 + 63] * ((dots[0] + dots[1]) + (dots[2] + dots[3]));
-            float dg = dg_row[lane] - ((dg_col[0][lane] + dg_col[1][lane]) + (dg_col[2][lane] + dg_col[3][lane]));
+            float dg = dg_row[lane];
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) {
                 const float y = __shfl_down(dg, m, 64);

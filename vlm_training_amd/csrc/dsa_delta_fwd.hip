@@ -168,8 +168,7 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
 // of three products over the same columns - K S0 (and Q S0), T R, K^T N (and P N) - so their results go through LDS to the other waves, a barrier each; they are
 // formed transposed (lane: its row, four neighbouring columns), which makes every factor of a row one register and every access 8 or 16 bytes.
 // Rows of K, Q, T and P are needed by their own wave alone (K by all of them as K^T): T and P come as fragments straight into registers, rows of K, Q and V
-// 16 bytes a lane through the wave's own part of LDS.  Two sets of registers take turns, and a set's loads for the chunk after next go out as soon as it has
-// been read: a chunk takes about as long as memory takes to answer.  (With waves side by side over the columns instead, each of them read all of K, Q, T, P from LDS: 5.3 us per chunk.)
+// 16 bytes a lane through the wave's own part of LDS.  The next chunk's loads go out as soon as a register has been read.  (With waves side by side over the columns instead, each of them read all of K, Q, T, P from LDS: 5.3 us per chunk.)
 template <int DK, int NC> struct WalkRows {
     bf16x8 k[DK / 32], q[DK / 32], th[2], tl[2], ph[2], pl[2];
     Piece<4 * NC> v;
@@ -256,7 +255,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
         pm += i + 1 < chunks ? step_m : 0;
     };
     auto chunk = [&](int i, Rows &x, bf16_t *kt) __attribute__((always_inline)) {
-        const int ahead = min(i + 2, chunks - 1);
+        const int ahead = min(i + 1, chunks - 1);
         // S0 as [dv][dk], K as it is
         const buffer_t save = buffer_of(ps, a.saved_bytes);
 #pragma unroll
@@ -369,20 +368,12 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
         po += step_o;
         if (SAVE) ps += step_s;
     };
-    Rows x, y;
+    Rows x;
     if (chunks > 0) {
         fetch_rows(0, x);
         fetch_t(x);
         fetch_p(0, x);
-        fetch_rows(min(1, chunks - 1), y);
-        fetch_t(y);
-        fetch_p(min(1, chunks - 1), y);
-        int i = 0;
-        for (; i + 1 < chunks; i += 2) {
-            chunk(i, x, ks[0]);
-            chunk(i + 1, y, ks[1]);
-        }
-        if (i < chunks) chunk(i, x, ks[0]);
+        for (int i = 0; i < chunks; ++i) chunk(i, x, ks[i & 1]);
     }
     if (a.final) {
 #pragma unroll
