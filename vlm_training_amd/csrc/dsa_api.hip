@@ -1069,7 +1069,7 @@ static size_t delta_layout(const dsa_delta_args *in, int save, char *ws, DeltaAr
     d->planes = save ? 4 : 2;
     d->mats_bytes = DELTA_T + 2 * d->planes * DELTA_PLANE;
     d->saved_bytes = save ? d->Dkp * d->Dvp * 2 + 256 * d->Dvp : 0;
-    d->back_bytes = d->Dkp * d->Dvp * 2 + 128 * d->Dvp;
+    d->back_bytes = d->Dkp * d->Dvp * 2 + 256 * d->Dvp;
     d->mats = ws;
     d->saved = ws + cells * d->mats_bytes;               // (blocks are multiples of 1024 bytes)
     return cells * ((size_t)d->mats_bytes + d->saved_bytes);

@@ -25,8 +25,8 @@ struct DeltaArgs {
     // A chunk of a value head ("cell", slots x Hv of them) has a block of each of three arrays.
     // mats: the rows' factors (DELTA_ROWS x 64 floats), then planes of 64 x 64 bf16: T as hi, lo and, where a backward follows, transposed hi, lo; P the same.
     //       A plane lies in the order of its fragments: wave, half of the columns, lane, eight elements.
-    // saved, for the backward: S0 (Dvp x Dkp), N as hi, lo (Dvp x 64 x 2);  back, the backward's own: dS1, dR (Dvp x 64).  They lie as the walks' lanes
-    //       hold them: 16 columns of the values, wave, lane, its elements (state: DK/16 of them, N: four as hi, four as lo, dR: four).
+    // saved, for the backward: S0 (Dvp x Dkp), N as hi, lo (Dvp x 64 x 2);  back, the backward's own: dS1, dR as hi, lo.  They lie as the walks' lanes
+    //       hold them: 16 columns of the values, wave, lane, its elements (state: Dkp/16 of them, N and dR: four as hi, four as lo).
     // (A quad of lanes that reads or writes four rows takes four times as long as one that stays in one: with rows of T, P, S and N in row order, K and
     // Q as fragments straight from their rows and 8-byte stores, the walk of 16 384 tokens took 0.62 ms.)
     char *mats, *saved, *back;
@@ -162,19 +162,21 @@ __device__ __forceinline__ buffer_t rows_buffer(const char *p, int tok, int rows
 __device__ __forceinline__ bf16x8 buf16(buffer_t b, int off, int at = 0) { return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(b, off, at, 0)); }
 __device__ __forceinline__ u32x2 buf8(buffer_t b, int off) { return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0)); }
 __device__ __forceinline__ float buf4(buffer_t b, int off) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, off, 0, 0)); }
-__device__ __forceinline__ void buf_put8(buffer_t b, int off, u32x2 x, int at = 0) { __builtin_amdgcn_raw_buffer_store_b64(x, b, off, at, 0); }
+__device__ __forceinline__ void buf_put8(buffer_t b, int off, u32x2 x) { __builtin_amdgcn_raw_buffer_store_b64(x, b, off, 0, 0); }
 // every load so far has arrived: in front of a loop whose loads are waited for by count (what is in flight there from before would be counted in with them)
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
-__device__ __forceinline__ void buf_put16(buffer_t b, int off, u32x4 x, int at = 0) { __builtin_amdgcn_raw_buffer_store_b128(x, b, off, at, 0); }
+// (Never with a scalar offset: the compiler then leaves out the wait state between a 16-byte store and an instruction that overwrites what it stores, and
+// stored values came out wrong here and there.)
+__device__ __forceinline__ void buf_put16(buffer_t b, int off, u32x4 x) { __builtin_amdgcn_raw_buffer_store_b128(x, b, off, 0, 0); }
 // four or eight elements at a time
 template <int N> struct Piece { uint32_t x[N / 2]; };
 template <int N> __device__ __forceinline__ Piece<N> buf_piece(buffer_t b, int off) {
     if constexpr (N == 8) return __builtin_bit_cast(Piece<8>, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
     else return __builtin_bit_cast(Piece<4>, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0));
 }
-template <int N> __device__ __forceinline__ void buf_put_piece(buffer_t b, int off, Piece<N> p, int at = 0) {
-    if constexpr (N == 8) buf_put16(b, off, __builtin_bit_cast(u32x4, p), at);
-    else buf_put8(b, off, __builtin_bit_cast(u32x2, p), at);
+template <int N> __device__ __forceinline__ void buf_put_piece(buffer_t b, int off, Piece<N> p) {
+    if constexpr (N == 8) buf_put16(b, off, __builtin_bit_cast(u32x4, p));
+    else buf_put8(b, off, __builtin_bit_cast(u32x2, p));
 }
 // LDS, on 8-byte boundaries
 template <int N> __device__ __forceinline__ void put_piece(bf16_t *t, Piece<N> p) {

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
     const int at_k = rcol < in.Dk ? (rrow * (int)in.k_tok + rcol) * 2 : NOWHERE, at_q = rcol < in.Dk ? (rrow * (int)in.q_tok + rcol) * 2 : NOWHERE;
     const int at_o = dv0 + vcol < in.Dv ? (vrow * in.Hv * in.Dv + dv0 + vcol) * 2 : NOWHERE;
     const int at_t = wv < 2 ? wv * 2048 + lane * 16 : NOWHERE, at_t1 = wv * 2048 + lane * 16 + 1024;                 // (transposed rows begin at the diagonal)
-    const int at_s = (dv0 * DK + (wv * 64 + lane) * 4 * NT) * 2, at_n = (dv0 / 16 * 256 + wv * 64 + lane) * 8;
+    const int at_s = (dv0 * DK + (wv * 64 + lane) * 4 * NT) * 2, at_n = a.Dvp * DK * 2 + (dv0 / 16 * 256 + wv * 64 + lane) * 16;
     struct BackRows {
         bf16x8 k[DK / 32], q[DK / 32], th[2], tl[2], ph[2], pl[2];
         Piece<4 * NC> o;
@@ -167,7 +167,8 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
                 y = mfma16(ah, x.th[s], y);
             }
             const int at = row * RS + 16 * c + 4 * g4;
-            buf_put8(back, at_n + c * 2048, hi4(y), a.Dvp * DK * 2);
+            const u32x2 yh = hi4(y), yl = lo4(y, yh);
+            buf_put16(back, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]});
             put4(os + at, hi4(y * x.beta));
             put_split4(sh + at, sl + at, y * (-x.beta * x.eg * x.rk));
         }
@@ -280,10 +281,11 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         for (int t = 0; t < 4; ++t) x[t] = z[t] = zero4();
         __syncthreads();                                 // (the previous head's LDS has been read)
         for (int e = tid; e < DELTA_ROWS * 64; e += 256) rows[e] = ((const float *)(a.mats + p * a.mats_bytes))[e];
+        const int halves = __builtin_amdgcn_readfirstlane(a.Dvp) / 64;       // (DV / 64, unknown to the compiler: a single turn drawn into what is around it spills)
 #pragma unroll 1
-        for (int b = 0; b < DV / 64; ++b) {
+        for (int b = 0; b < halves; ++b) {
             const bf16_t *const orow = a.dout + ((int64_t)(c.row0 + row) * in.Hv + h) * in.Dv + 64 * b;
-            bf16x8 of[2], rf[2];
+            bf16x8 of[2], rf[2], rl[2];                  // the wave's rows of dO, and of dR as hi, lo
             u32x4 tn[4], ts[DK / 32];
 #pragma unroll
             for (int e = 0; e < 4; ++e) tn[e] = *reinterpret_cast<const u32x4_any *>(news + (64 * b * 16 + tid + 256 * e) * 8);
@@ -293,9 +295,10 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             for (int s = 0; s < 2; ++s) {
                 of[s] = row_frag(orow, 32 * s + 8 * g4, live && 64 * b + 32 * s + 8 * g4 < in.Dv);
                 // eight columns of dR: two lanes' four
-                const bf16_t *const r4 = drs + ((4 * b + 2 * s + (g4 >> 1)) * 256 + wv * 64 + (g4 & 1) * 32 + l16) * 4;
-                const u32x2 lo = *reinterpret_cast<const u32x2_any *>(r4), hi = *reinterpret_cast<const u32x2_any *>(r4 + 64);
-                rf[s] = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+                const bf16_t *const r4 = drs + ((4 * b + 2 * s + (g4 >> 1)) * 256 + wv * 64 + (g4 & 1) * 32 + l16) * 8;
+                const u32x4 r0 = *reinterpret_cast<const u32x4_any *>(r4), r1 = *reinterpret_cast<const u32x4_any *>(r4 + 128);
+                rf[s] = __builtin_bit_cast(bf16x8, u32x4{r0[0], r0[1], r1[0], r1[1]});
+                rl[s] = __builtin_bit_cast(bf16x8, u32x4{r0[2], r0[3], r1[2], r1[3]});
             }
             if (b) __syncthreads();                      // (the columns before have been read)
 #pragma unroll
@@ -327,6 +330,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                     const bf16x8 nj = frag_n(ns, TS, 16 * t, 32 * s), lj = frag_n(ns + 64 * TS, TS, 16 * t, 32 * s);
                     x[t] = mfma16(lj, of[s], x[t]);
                     z[t] = mfma16(lj, rf[s], z[t]);
+                    z[t] = mfma16(nj, rl[s], z[t]);
                     x[t] = mfma16(nj, of[s], x[t]);
                     z[t] = mfma16(nj, rf[s], z[t]);
                 }
@@ -337,7 +341,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 nf[s] = frag_n(ns, TS, 16 * wv, 32 * s);
-                db = dot8_chain(rf[s], nf[s], dot8_chain(rf[s], frag_n(ns + 64 * TS, TS, 16 * wv, 32 * s), db));
+                db = dot8_chain(rf[s], nf[s], dot8_chain(rl[s], nf[s], dot8_chain(rf[s], frag_n(ns + 64 * TS, TS, 16 * wv, 32 * s), db)));
             }
             // through S0: scale e^G dO S0^T into dQ, -beta e^G dR S0^T into dK
 #pragma unroll
@@ -355,6 +359,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 dk[t] += w;
                 sum = dot4(y, four(qrow + 16 * t), sum);
                 sum = dot4(w, four(krow + 16 * t), sum);
+                if (t % 2) __builtin_amdgcn_sched_barrier(0);        // (the products' operands of all t at once are more than the registers hold)
             }
             __syncthreads();
             // dS1 in the place of S0, their product summed on the way
@@ -376,6 +381,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 y *= fs;
                 dk[t] += y;
                 dots_ = dot4(y, four(krow + 16 * t), dots_);
+                if (t % 2) __builtin_amdgcn_sched_barrier(0);
             }
         }
         __syncthreads();
@@ -389,7 +395,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
                     const int j = 16 * t + 4 * g4 + v;
-                    const float e = j <= row ? expf((gi - rows[DELTA_GH * 64 + j]) + (gi_lo - rows[DELTA_GL * 64 + j])) * rows[DELTA_RK * 64 + j] : 0.f;
+                    const float e = expf(fminf((gi - rows[DELTA_GH * 64 + j]) + (gi_lo - rows[DELTA_GL * 64 + j]), 0.f)) * rows[DELTA_RK * 64 + j];
                     xv[v] = j <= row ? x[t][v] * e * fx : 0.f;
                     zv[v] = j < row ? z[t][v] * e * fz : 0.f;
                 }
@@ -402,7 +408,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         for (int m = 1; m < 64; m <<= 1) dot += __shfl_xor(dot, m, 64);
         if (lane == 0) dots[wv] = dot;
         __syncthreads();
-        // X K, X^T Q, (Z + Z^T) K.  X and Z keep to columns up to the row; transposed, to rows from it on
+        // X K, X^T Q, (Z + Z^T) K: zeros and all (left out by wave, their branches cost more)
         bf16x8 xa[2][2], za[2][2], xt[2][2], zt[2][2];   // [hi, lo][32 columns or rows]
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -419,23 +425,20 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             f32x4 y = zero4(), w = zero4(), u1 = zero4();
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const bf16x8 kb = frag_t(ks, KS, 32 * s, 16 * t);
+                const bf16x8 kb = frag_t(ks, KS, 32 * s, 16 * t), qb = frag_t(qs, KS, 32 * s, 16 * t);
 #pragma unroll
                 for (int half = 1; half >= 0; --half) {
-                    if (s == 0 || wv >= 2) {
-                        y = mfma16(kb, xa[half][s], y);
-                        w = mfma16(kb, za[half][s], w);
-                    }
-                    if (s == 1 || wv < 2) {
-                        u1 = mfma16(kb, zt[half][s], u1);
-                        u1 = mfma16(frag_t(qs, KS, 32 * s, 16 * t), xt[half][s], u1);
-                    }
+                    y = mfma16(kb, xa[half][s], y);
+                    w = mfma16(kb, za[half][s], w);
+                    u1 = mfma16(kb, zt[half][s], u1);
+                    u1 = mfma16(qb, xt[half][s], u1);
                 }
             }
             sum = dot4(y, four(qrow + 16 * t), sum);
             sum = dot4(w - u1, four(krow + 16 * t), sum);
             dq[t] += y;
             dk[t] += w + u1;
+            if (t % 2) __builtin_amdgcn_sched_barrier(0);
         }
         dots_ = over_row(dots_);
         sum = over_row(sum) - dots_;

@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
                 const int j = 16 * t + 4 * g4 + v;
-                const float e = j <= i ? expf((gh[i] - gh[j]) + (gl[i] - gl[j])) : 0.f;
+                const float e = expf(fminf((gh[i] - gh[j]) + (gl[i] - gl[j]), 0.f));
                 x[v] = j <= i ? e * rq[i] * rk[j] * qk[t][v] : 0.f;
                 y[v] = j < i ? e * bt[i] * rk[i] * rk[j] * kk[t][v] : 0.f;
             }
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
     const int at_k = rcol < in.Dk ? (rrow * (int)in.k_tok + rcol) * 2 : NOWHERE, at_q = rcol < in.Dk ? (rrow * (int)in.q_tok + rcol) * 2 : NOWHERE;
     const int at_v = dv0 + vcol < in.Dv ? (vrow * (int)in.v_tok + dv0 + vcol) * 2 : NOWHERE, at_o = dv0 + vcol < in.Dv ? (vrow * in.Hv * in.Dv + dv0 + vcol) * 2 : NOWHERE;
     const int at_t = wv * 2048 + lane * 16, at_t1 = wv >= 2 ? at_t + 1024 : NOWHERE;       // (rows of T and P end at the diagonal)
-    const int at_s = (dv0 * DK + (wv * 64 + lane) * 4 * NT) * 2, at_n = (dv0 / 16 * 256 + wv * 64 + lane) * 16;
+    const int at_s = (dv0 * DK + (wv * 64 + lane) * 4 * NT) * 2, at_n = a.Dvp * DK * 2 + (dv0 / 16 * 256 + wv * 64 + lane) * 16;
     // where the next chunk to be fetched, and the one at hand, lie; a chunk further they are a fixed number of bytes on
     const int64_t first = (int64_t)slot0 * in.Hv + h;
     const char *pk = (const char *)in.k + (s0 * in.k_tok + hk * in.k_head) * 2, *pq = (const char *)in.q + (s0 * in.q_tok + hk * in.q_head) * 2;
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_walk_kernel(DeltaArgs a) {
             put4(nh + at, yh);
             put4(nl + at, yl);
             put_split4(mh + at, ml + at, y * (x.ec * x.rk));
-            if (SAVE) buf_put16(save, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]}, a.Dvp * DK * 2);
+            if (SAVE) buf_put16(save, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]});
         }
         fetch_t(x);
         __syncthreads();
