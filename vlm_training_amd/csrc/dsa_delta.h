@@ -92,15 +92,22 @@ __device__ __forceinline__ void wave_sync() {
 
 // ---- fragments of mfma16 (16x16x32): lane l of a row-major tile ------------------------------------------------------------------------
 // rows r0 + l%16, columns c0 + 8 (l/16) ..: an operand whose contraction runs along the row
-__device__ __forceinline__ bf16x8 frag_n(const bf16_t *t, int stride, int r0, int c0) {
-    const int l = threadIdx.x & 63;
+__device__ __forceinline__ bf16x8 frag_n(const bf16_t *t, int stride, int r0, int c0, int l) {
     return *reinterpret_cast<const bf16x8 *>(t + (r0 + (l & 15)) * stride + c0 + 8 * (l >> 4));
 }
 // rows k0 + 8 (l/16) .., column m0 + l%16: an operand whose contraction runs down the rows
-__device__ __forceinline__ bf16x8 frag_t(bf16_t *t, int stride, int k0, int m0) {
-    const int l = threadIdx.x & 63, s = l & 15;
+__device__ __forceinline__ bf16x8 frag_t(bf16_t *t, int stride, int k0, int m0, int l) {
+    const int s = l & 15;
     bf16_t *const p = t + (k0 + 8 * (l >> 4) + (s >> 2)) * stride + m0 + 4 * (s & 3);
     return tr_pair((lds_u8 *)p, (lds_u8 *)(p + 4 * stride));
+}
+__device__ __forceinline__ bf16x8 frag_n(const bf16_t *t, int stride, int r0, int c0) { return frag_n(t, stride, r0, c0, threadIdx.x & 63); }
+__device__ __forceinline__ bf16x8 frag_t(bf16_t *t, int stride, int k0, int m0) { return frag_t(t, stride, k0, m0, threadIdx.x & 63); }
+// the lane as a value that the compiler knows nothing about: addresses made from it inside a loop are not carried into it in registers
+__device__ __forceinline__ int fresh_lane() {
+    int l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    return l;
 }
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 

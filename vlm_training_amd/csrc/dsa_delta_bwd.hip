@@ -284,6 +284,8 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         const int halves = __builtin_amdgcn_readfirstlane(a.Dvp) / 64;       // (DV / 64, unknown to the compiler: a single turn drawn into what is around it spills)
 #pragma unroll 1
         for (int b = 0; b < halves; ++b) {
+            const int ln = fresh_lane(), l16 = ln & 15, g4 = ln >> 4, row = 16 * wv + l16, tid = 64 * wv + ln;
+            const bf16_t *const krow = ks + row * KS + 4 * g4, *const qrow = qs + row * KS + 4 * g4;
             const bf16_t *const orow = a.dout + ((int64_t)(c.row0 + row) * in.Hv + h) * in.Dv + 64 * b;
             bf16x8 of[2], rf[2], rl[2];                  // the wave's rows of dO, and of dR as hi, lo
             u32x4 tn[4], ts[DK / 32];
@@ -293,7 +295,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             for (int e = 0; e < DK / 32; ++e) ts[e] = *reinterpret_cast<const u32x4_any *>(state + 64 * b * DK + (tid + 256 * e) * 8);
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                of[s] = row_frag(orow, 32 * s + 8 * g4, live && 64 * b + 32 * s + 8 * g4 < in.Dv);
+                of[s] = row_frag(orow, 32 * s + 8 * g4, row < c.rows && 64 * b + 32 * s + 8 * g4 < in.Dv);
                 // eight columns of dR: two lanes' four
                 const bf16_t *const r4 = drs + ((4 * b + 2 * s + (g4 >> 1)) * 256 + wv * 64 + (g4 & 1) * 32 + l16) * 8;
                 const u32x4 r0 = *reinterpret_cast<const u32x4_any *>(r4), r1 = *reinterpret_cast<const u32x4_any *>(r4 + 128);
@@ -327,7 +329,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 if (t > wv) continue;
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const bf16x8 nj = frag_n(ns, TS, 16 * t, 32 * s), lj = frag_n(ns + 64 * TS, TS, 16 * t, 32 * s);
+                    const bf16x8 nj = frag_n(ns, TS, 16 * t, 32 * s, ln), lj = frag_n(ns + 64 * TS, TS, 16 * t, 32 * s, ln);
                     x[t] = mfma16(lj, of[s], x[t]);
                     z[t] = mfma16(lj, rf[s], z[t]);
                     z[t] = mfma16(nj, rl[s], z[t]);
@@ -340,8 +342,8 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             bf16x8 nf[2];
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                nf[s] = frag_n(ns, TS, 16 * wv, 32 * s);
-                db = dot8_chain(rf[s], nf[s], dot8_chain(rl[s], nf[s], dot8_chain(rf[s], frag_n(ns + 64 * TS, TS, 16 * wv, 32 * s), db)));
+                nf[s] = frag_n(ns, TS, 16 * wv, 32 * s, ln);
+                db = dot8_chain(rf[s], nf[s], dot8_chain(rl[s], nf[s], dot8_chain(rf[s], frag_n(ns + 64 * TS, TS, 16 * wv, 32 * s, ln), db)));
             }
             // through S0: scale e^G dO S0^T into dQ, -beta e^G dR S0^T into dK
 #pragma unroll
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 f32x4 y = zero4(), w = zero4();
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const bf16x8 m = frag_t(ss, KS, 32 * s, 16 * t);
+                    const bf16x8 m = frag_t(ss, KS, 32 * s, 16 * t, ln);
                     y = mfma16(m, of[s], y);
                     w = mfma16(m, rf[s], w);
                 }
@@ -377,7 +379,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             for (int t = 0; t < NT; ++t) {
                 f32x4 y = zero4();
 #pragma unroll
-                for (int s = 0; s < 2; ++s) y = mfma16(frag_t(ss, KS, 32 * s, 16 * t), nf[s], y);
+                for (int s = 0; s < 2; ++s) y = mfma16(frag_t(ss, KS, 32 * s, 16 * t, ln), nf[s], y);
                 y *= fs;
                 dk[t] += y;
                 dots_ = dot4(y, four(krow + 16 * t), dots_);
@@ -386,6 +388,8 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         }
         __syncthreads();
         // X and Z
+        const int ln = fresh_lane(), l16 = ln & 15, g4 = ln >> 4, row = 16 * wv + l16;
+        const bf16_t *const krow = ks + row * KS + 4 * g4, *const qrow = qs + row * KS + 4 * g4;
         const float rk = rows[DELTA_RK * 64 + row], fx = rows[DELTA_RQ * 64 + row], fz = -rows[DELTA_BETA * 64 + row] * rk;
         const float gi = rows[DELTA_GH * 64 + row], gi_lo = rows[DELTA_GL * 64 + row];
 #pragma unroll
@@ -415,17 +419,17 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 bf16_t *const xh = xs + half * 64 * TS, *const zh = zs + half * 64 * TS;
-                xa[half][s] = frag_n(xh, TS, 16 * wv, 32 * s);
-                za[half][s] = frag_n(zh, TS, 16 * wv, 32 * s);
-                xt[half][s] = frag_t(xh, TS, 32 * s, 16 * wv);
-                zt[half][s] = frag_t(zh, TS, 32 * s, 16 * wv);
+                xa[half][s] = frag_n(xh, TS, 16 * wv, 32 * s, ln);
+                za[half][s] = frag_n(zh, TS, 16 * wv, 32 * s, ln);
+                xt[half][s] = frag_t(xh, TS, 32 * s, 16 * wv, ln);
+                zt[half][s] = frag_t(zh, TS, 32 * s, 16 * wv, ln);
             }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             f32x4 y = zero4(), w = zero4(), u1 = zero4();
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const bf16x8 kb = frag_t(ks, KS, 32 * s, 16 * t), qb = frag_t(qs, KS, 32 * s, 16 * t);
+                const bf16x8 kb = frag_t(ks, KS, 32 * s, 16 * t, ln), qb = frag_t(qs, KS, 32 * s, 16 * t, ln);
 #pragma unroll
                 for (int half = 1; half >= 0; --half) {
                     y = mfma16(kb, xa[half][s], y);
@@ -446,7 +450,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         if (g4 == 0) {
             dg_row[row] = sum;
             dg_s[row] = dots_;
-            if (live) store_any(a.db, (int64_t)(c.row0 + row) * in.Hv + h, in.b_f32, (1.f - rows[DELTA_BETA * 64 + row]) * db);
+            if (row < c.rows) store_any(a.db, (int64_t)(c.row0 + row) * in.Hv + h, in.b_f32, (1.f - rows[DELTA_BETA * 64 + row]) * db);
         }
         __syncthreads();
         if (wv == 0) {                                   // lane: its row
