@@ -32,6 +32,14 @@ __device__ __forceinline__ void store8(void *p, int64_t i, f32x8 x) {
         __builtin_nontemporal_store(f32_to_bf8(x), reinterpret_cast<u32x4 *>((bf16_t *)p + i));
     }
 }
+// Squares are summed at 2^-14 of their size: 8192 of them overflow only where their mean does.
+#define SQUARE_SCALE 0x1p-14f
+__device__ __forceinline__ float squares8(f32x8 x) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += x[i] * SQUARE_SCALE * x[i];
+    return s;
+}
 __device__ __forceinline__ float load1(const void *p, int64_t i, int f32) { return f32 ? ((const float *)p)[i] : (float)((const bf16_t *)p)[i]; }
 __device__ __forceinline__ f32x8 load8_any(const void *p, int64_t i, int f32) {          // a parameter: any alignment
     f32x8 r;
@@ -44,31 +52,62 @@ __device__ __forceinline__ void store1(void *p, int64_t i, int f32, float x) {
     else ((bf16_t *)p)[i] = (bf16_t)x;
 }
 
-// Column sums: out[e] = sum over b < blocks of part[b * stride + e], a thread per column and 1/16 of the blocks, then the sixteen
-__global__ __launch_bounds__(256) void dsa_column_sum_kernel(const float *__restrict__ part, int blocks, int64_t stride, int n, void *__restrict__ out, int f32) {
-    __shared__ float red[16][17];
-    const int x = threadIdx.x & 15, y = threadIdx.x >> 4, e = blockIdx.x * 16 + x;
-    float s = 0.f;
-    if (e < n) {
-#pragma unroll 4
-        for (int b = y; b < blocks; b += 16) s += part[b * stride + e];
+// Column sums: out[i][e] = sum over b < blocks of part[b * stride + at[i] + e], up to three outputs in one launch.  A workgroup has sixteen columns, four to a
+// thread, and 64 threads to a column: each adds every 64th block's, then the 64 are added in order (sixteen of four) - the same order on every run.  (With a column
+// to a thread and sixteen threads to a column, 1024 blocks of 4096: 7.6 us; this form 4.)
+struct SumArgs {
+    const float *part;
+    int blocks;
+    int64_t stride;
+    int at[3], n[3], f32[3];
+    void *out[3];
+};
+__global__ __launch_bounds__(256) void dsa_column_sum_kernel(SumArgs a) {
+    __shared__ f32x4 red[64][4], red2[16][4];
+    const int x = threadIdx.x & 3, y = threadIdx.x >> 2, i = blockIdx.y, e = blockIdx.x * 16 + 4 * x;
+    const bool live = e < a.n[i];                        // (every n is a multiple of 4)
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+        const float *const p = a.part + a.at[i] + e;
+#pragma unroll 8
+        for (int b = y; b < a.blocks; b += 64) s += *reinterpret_cast<const f32x4 *>(p + b * a.stride);
     }
     red[y][x] = s;
     __syncthreads();
-    if (y == 0 && e < n) {
+    if (y < 16) {
+        s = red[4 * y][x];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) s += red[i][x];
-        store1(out, e, f32, s);
+        for (int k = 1; k < 4; ++k) s += red[4 * y + k][x];
+        red2[y][x] = s;
+    }
+    __syncthreads();
+    if (y == 0 && live) {
+        s = red2[0][x];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) s += red2[k][x];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) store1(a.out[i], e + v, a.f32[i], s[v]);
     }
 }
-static void column_sum(const float *part, int blocks, int64_t stride, int n, void *out, int f32, hipStream_t stream) {
-    hipLaunchKernelGGL(dsa_column_sum_kernel, dim3((n + 15) / 16), dim3(256), 0, stream, part, blocks, stride, n, out, f32);
+static void column_sums(const float *part, int blocks, int64_t stride, int count, const int *at, const int *n, void *const *out, const int *f32, hipStream_t stream) {
+    SumArgs a = {part, blocks, stride};
+    int most = 0, m = 0;
+    for (int i = 0; i < count; ++i)
+        if (out[i]) {
+            a.at[m] = at[i];
+            a.n[m] = n[i];
+            a.out[m] = out[i];
+            a.f32[m++] = f32[i];
+            most = n[i] > most ? n[i] : most;
+        }
+    hipLaunchKernelGGL(dsa_column_sum_kernel, dim3((most + 15) / 16, m), dim3(256), 0, stream, a);
 }
 
 // ---- short convolution -------------------------------------------------------------------------------------------------------------------
-// A thread keeps eight channels over a run of consecutive rows: the last W-1 inputs stay in registers, so a row is read once (and W-1 rows once
-// more per run); BATCH rows' loads are in flight together.  lanes_c threads of a workgroup lie side by side over the channels, the others take further runs.
-#define CONV_BATCH 4
+// A thread keeps four channels over a run of consecutive rows: the last W-1 inputs stay in registers, so a row is read once (and W-1 rows once
+// more per run); CONV_BATCH rows' loads are in flight together.  lanes_c threads of a workgroup lie side by side over the channels, the others take further runs.
+// (Eight channels took 256 registers in the backward, two waves per SIMD: 330 us for 16 384 rows of 8192, 2.4 TB/s.)
+#define CONV_BATCH 8
 struct ConvArgs {
     const bf16_t *x, *dy, *state;                        // (T, C) rows x_tok, dy_tok apart;  (N, C, W-1)
     int64_t x_tok, dy_tok;
@@ -79,6 +118,30 @@ struct ConvArgs {
     bf16_t *y;                                           // y or dx, contiguous
     float *part;                                         // (runs of workgroups, C, W + 1)
 };
+__device__ __forceinline__ f32x4 bf4_to_f32(u32x2 w) {
+    return f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
+}
+__device__ __forceinline__ u32x2 f32_to_bf4(f32x4 x) { return u32x2{pack2bf(x[0], x[1]), pack2bf(x[2], x[3])}; }
+__device__ __forceinline__ f32x4 zero4f() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+// the W weights of channels c0 .. c0 + N - 1, which lie one after the other
+template <int W, int N>
+__device__ __forceinline__ void conv_weights(const void *w, int f32, int c0, float (&out)[N][W]) {
+    if (f32) {
+#pragma unroll
+        for (int i = 0; i < N * W; ++i) out[i / W][i % W] = ((const float *)w)[(int64_t)c0 * W + i];
+    } else if (((uintptr_t)w & 7) == 0) {
+        const u32x2 *const p = reinterpret_cast<const u32x2 *>((const bf16_t *)w + (int64_t)c0 * W);           // (N is a multiple of 4)
+#pragma unroll
+        for (int i = 0; i < N * W / 4; ++i) {
+            const f32x4 x = bf4_to_f32(p[i]);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) out[(4 * i + v) / W][(4 * i + v) % W] = x[v];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N * W; ++i) out[i / W][i % W] = (float)((const bf16_t *)w)[(int64_t)c0 * W + i];
+    }
+}
 // where a run stands: the sequence of row t, its first row and the row behind its last
 struct ConvPlace {
     int seg, start, end;
@@ -96,30 +159,36 @@ struct ConvPlace {
         }
     }
 };
-// input j rows before row t, j <= W-1, where that lies before the sequence's first row: the state's column, or zero
+// the input `back` rows before a sequence's first row: the state's column, or zero
 template <int W>
-__device__ __forceinline__ f32x8 conv_before(const ConvArgs &a, const ConvPlace &p, int back, int c0) {      // back = 1: the row before the first
-    if (!a.state || back > W - 1) return zero8();
-    f32x8 r;
+__device__ __forceinline__ f32x4 conv_before(const ConvArgs &a, const ConvPlace &p, int back, int c0) {
+    if (!a.state || back > W - 1) return zero4f();
+    f32x4 r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = (float)a.state[((int64_t)p.seg * a.C + c0 + i) * (W - 1) + W - 1 - back];
+    for (int i = 0; i < 4; ++i) r[i] = (float)a.state[((int64_t)p.seg * a.C + c0 + i) * (W - 1) + W - 1 - back];
     return r;
 }
 template <int W, bool BWD>
 __global__ __launch_bounds__(256) void dsa_conv_kernel(ConvArgs a) {
     const int lx = threadIdx.x % a.lanes_c, ly = threadIdx.x / a.lanes_c, runs_y = 256 / a.lanes_c;
-    const int c0 = (blockIdx.x * a.lanes_c + lx) * 8;
+    const int c0 = (blockIdx.x * a.lanes_c + lx) * 4;
     const bool live = c0 < a.C;
     const int64_t first = ((int64_t)blockIdx.y * runs_y + ly) * a.run;
     const int t0 = (int)(first < a.T ? first : a.T), t1 = min(a.T, t0 + a.run), last = min(max(a.cu[a.N], 0), a.T);
-    f32x8 w[W], b = zero8(), h[W - 1], acc[W], dw[W], db = zero8();
+    f32x4 w[W], b = zero4f(), h[W - 1], acc[W], dw[W], db = zero4f();
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-        acc[j] = dw[j] = zero8();
+    for (int j = 0; j < W; ++j) w[j] = acc[j] = dw[j] = zero4f();
+    if (live) {
+        float all[4][W];
+        conv_weights<W, 4>(a.w, a.w_f32, c0, all);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[j][i] = live ? load1(a.w, (int64_t)(c0 + i) * W + j, a.w_f32) : 0.f;
+        for (int j = 0; j < W; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[j][i] = all[i][j];
+        if (a.bias)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = load1(a.bias, c0 + i, a.b_f32);
     }
-    if (a.bias && live) b = load8_any(a.bias, c0, a.b_f32);
     if (live && t0 < t1) {
         ConvPlace p;
         const bf16_t *const x = a.x + c0, *const g = BWD ? a.dy + c0 : nullptr;
@@ -128,18 +197,18 @@ __global__ __launch_bounds__(256) void dsa_conv_kernel(ConvArgs a) {
 #pragma unroll
             for (int j = 1; j < W; ++j) {
                 const int t = t0 - j;
-                h[j - 1] = t >= p.start ? bf8_to_f32(*reinterpret_cast<const u32x4 *>(x + t * a.x_tok)) : conv_before<W>(a, p, p.start - t, c0);
+                h[j - 1] = t >= p.start ? bf4_to_f32(*reinterpret_cast<const u32x2 *>(x + t * a.x_tok)) : conv_before<W>(a, p, p.start - t, c0);
             }
         }
         // the backward goes on for W-1 rows: they have a share in the run's last gradients
         const int stop = min(BWD ? t1 + W - 1 : t1, last);
         for (int tb = t0; tb < stop; tb += CONV_BATCH) {
-            u32x4 xr[CONV_BATCH], gr[CONV_BATCH];
+            u32x2 xr[CONV_BATCH], gr[CONV_BATCH];
 #pragma unroll
             for (int u = 0; u < CONV_BATCH; ++u) {
                 const int64_t t = min(tb + u, stop - 1);
-                xr[u] = *reinterpret_cast<const u32x4 *>(x + t * a.x_tok);
-                if (BWD) gr[u] = *reinterpret_cast<const u32x4 *>(g + t * a.dy_tok);
+                xr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(x + t * a.x_tok));
+                if (BWD) gr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(g + t * a.dy_tok));
             }
 #pragma unroll
             for (int u = 0; u < CONV_BATCH; ++u) {
@@ -150,21 +219,21 @@ __global__ __launch_bounds__(256) void dsa_conv_kernel(ConvArgs a) {
 #pragma unroll
                     for (int j = 1; j < W; ++j) h[j - 1] = conv_before<W>(a, p, j, c0);
                 }
-                const f32x8 xt = bf8_to_f32(xr[u]);
-                f32x8 z = b + w[W - 1] * xt;
+                const f32x4 xt = bf4_to_f32(xr[u]);
+                f32x4 z = b + w[W - 1] * xt;
 #pragma unroll
                 for (int j = 1; j < W; ++j) z += w[W - 1 - j] * h[j - 1];
                 if (!BWD) {
                     if (a.silu) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) z[i] *= sigmoid_f(z[i]);
+                        for (int i = 0; i < 4; ++i) z[i] *= sigmoid_f(z[i]);
                     }
-                    __builtin_nontemporal_store(f32_to_bf8(z), reinterpret_cast<u32x4 *>(a.y + (int64_t)t * a.C + c0));
+                    __builtin_nontemporal_store(f32_to_bf4(z), reinterpret_cast<u32x2 *>(a.y + (int64_t)t * a.C + c0));
                 } else {
-                    f32x8 dz = bf8_to_f32(gr[u]);
+                    f32x4 dz = bf4_to_f32(gr[u]);
                     if (a.silu) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
+                        for (int i = 0; i < 4; ++i) {
                             const float s = sigmoid_f(z[i]);
                             dz[i] *= s * (1.f + z[i] * (1.f - s));
                         }
@@ -181,7 +250,7 @@ __global__ __launch_bounds__(256) void dsa_conv_kernel(ConvArgs a) {
                     for (int j = 1; j < W; ++j)
                         if (t - j >= p.start) acc[j] += w[W - 1 - j] * dz;
                     const int done = t - (W - 1);
-                    if (done >= t0 && done < t1) __builtin_nontemporal_store(f32_to_bf8(acc[W - 1]), reinterpret_cast<u32x4 *>(a.y + (int64_t)done * a.C + c0));
+                    if (done >= t0 && done < t1) __builtin_nontemporal_store(f32_to_bf4(acc[W - 1]), reinterpret_cast<u32x2 *>(a.y + (int64_t)done * a.C + c0));
 #pragma unroll
                     for (int j = W - 1; j > 0; --j) acc[j] = acc[j - 1];
                 }
@@ -195,33 +264,30 @@ __global__ __launch_bounds__(256) void dsa_conv_kernel(ConvArgs a) {
 #pragma unroll
             for (int j = W - 1; j > 0; --j) {
                 const int t = stop - j;
-                if (t >= t0 && t < t1 && t < last) __builtin_nontemporal_store(f32_to_bf8(acc[j]), reinterpret_cast<u32x4 *>(a.y + (int64_t)t * a.C + c0));
+                if (t >= t0 && t < t1 && t < last) __builtin_nontemporal_store(f32_to_bf4(acc[j]), reinterpret_cast<u32x2 *>(a.y + (int64_t)t * a.C + c0));
             }
         }
         // rows behind the last sequence: zeros
-        for (int t = max(t0, last); t < t1; ++t) *reinterpret_cast<u32x4 *>(a.y + (int64_t)t * a.C + c0) = u32x4{0u, 0u, 0u, 0u};
+        for (int t = max(t0, last); t < t1; ++t) *reinterpret_cast<u32x2 *>(a.y + (int64_t)t * a.C + c0) = u32x2{0u, 0u};
     }
     if (BWD) {
         // the workgroup's sums, its runs in order
-        __shared__ float red[256][8];
+        __shared__ f32x4 red[256];
         const int64_t base = (int64_t)blockIdx.y * (W + 1) * a.C;
+#pragma unroll
         for (int j = 0; j <= W; ++j) {
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float v = db[i];
-#pragma unroll
-                for (int k = 0; k < W; ++k) v = j == k ? dw[k][i] : v;
-                red[threadIdx.x][i] = v;
+            f32x4 s = j < W ? dw[j < W ? j : 0] : db;
+            if (runs_y > 1) {
+                __syncthreads();
+                red[threadIdx.x] = s;
+                __syncthreads();
+                for (int r = 1; r < runs_y && ly == 0; ++r) s += red[r * a.lanes_c + lx];
             }
-            __syncthreads();
             if (ly == 0 && live) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float s = 0.f;
-                    for (int r = 0; r < runs_y; ++r) s += red[r * a.lanes_c + lx][i];
-                    if (j < W) a.part[base + (int64_t)(c0 + i) * W + j] = s;
-                    else a.part[base + (int64_t)W * a.C + c0 + i] = s;
+                for (int i = 0; i < 4; ++i) {
+                    if (j < W) a.part[base + (int64_t)(c0 + i) * W + j] = s[i];
+                    else a.part[base + (int64_t)W * a.C + c0 + i] = s[i];
                 }
             }
         }
@@ -254,16 +320,18 @@ __global__ __launch_bounds__(256) void dsa_conv_step_kernel(ConvArgs a, bf16_t *
 #pragma unroll
     for (int i = 0; i < W - 1; ++i) reinterpret_cast<bf16x8 *>(old)[i] = reinterpret_cast<const bf16x8 *>(s)[i];
     const bf16x8 x = *reinterpret_cast<const bf16x8 *>(a.x + req * a.x_tok + c0);
+    float w[8][W];
+    conv_weights<W, 8>(a.w, a.w_f32, c0, w);
     f32x8 z;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         z[i] = a.bias ? load1(a.bias, c0 + i, a.b_f32) : 0.f;
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) {
-            z[i] += load1(a.w, (int64_t)(c0 + i) * W + j, a.w_f32) * (float)old[i * (W - 1) + j];
+            z[i] += w[i][j] * (float)old[i * (W - 1) + j];
             now[i * (W - 1) + j] = j + 1 < W - 1 ? old[i * (W - 1) + j + 1] : x[i];
         }
-        z[i] += load1(a.w, (int64_t)(c0 + i) * W + W - 1, a.w_f32) * (float)x[i];
+        z[i] += w[i][W - 1] * (float)x[i];
         if (a.silu) z[i] *= sigmoid_f(z[i]);
     }
 #pragma unroll
@@ -274,8 +342,8 @@ __global__ __launch_bounds__(256) void dsa_conv_step_kernel(ConvArgs a, bf16_t *
 // threads side by side over the channels, and the rows of a run: enough runs for the chip's waves, none shorter than 16 rows (W-1 of them come on top)
 static void conv_shape(ConvArgs &a, int &cols, int &rows) {
     a.lanes_c = 1;
-    while (a.lanes_c < 256 && a.lanes_c * 8 < a.C) a.lanes_c *= 2;
-    cols = (a.C / 8 + a.lanes_c - 1) / a.lanes_c;
+    while (a.lanes_c < 256 && a.lanes_c * 4 < a.C) a.lanes_c *= 2;
+    cols = (a.C / 4 + a.lanes_c - 1) / a.lanes_c;
     const int runs_y = 256 / a.lanes_c;
     const int64_t want = (2048 + cols - 1) / cols * (int64_t)runs_y;        // runs
     const int64_t run = (a.T + want - 1) / want;
@@ -319,8 +387,9 @@ extern "C" hipError_t dsa_launch_conv_bwd(const void *x, int64_t x_tok, const vo
 #define CONV_BWD(WW) hipLaunchKernelGGL((dsa_conv_kernel<WW, true>), dim3(cols, rows), dim3(256), 0, stream, a)
     if (T > 0) CONV_SWITCH(W, CONV_BWD)
     const int64_t stride = (int64_t)(W + 1) * C;
-    column_sum(part, T > 0 ? rows : 0, stride, C * W, dw, w_f32, stream);
-    if (dbias) column_sum(part + (int64_t)W * C, T > 0 ? rows : 0, stride, C, dbias, b_f32, stream);
+    const int at[2] = {0, W * C}, n[2] = {W * C, C}, f32[2] = {w_f32, b_f32};
+    void *const out[2] = {dw, dbias};
+    column_sums(part, T > 0 ? rows : 0, stride, 2, at, n, out, f32, stream);
     return hipGetLastError();
 }
 extern "C" hipError_t dsa_launch_conv_step(const void *x, int64_t x_tok, const void *w, int w_f32, const void *bias, int b_f32, int silu, int B, int C, int W, void *state,
@@ -368,12 +437,10 @@ __global__ __launch_bounds__(256) void dsa_gated_norm_kernel(GatedNormArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[i] = sigmoid_f(z[i]);
         if (!BWD) {
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+            float ss = squares8(x);
 #pragma unroll
             for (int m = 1; m < LPR; m <<= 1) ss += __shfl_xor(ss, m, 64);
-            const float rs = rsqrtf(ss * inv + a.eps);
+            const float rs = rsqrtf(ss * (inv / SQUARE_SCALE) + a.eps);
             if (live) {
                 store8<false>(a.y, r * a.D + d0, x * rs * w * z * s);
                 if (d0 == 0 && a.rstd) a.rstd[r] = rs;
@@ -436,7 +503,8 @@ extern "C" hipError_t dsa_launch_gated_norm_bwd(const void *dy, const void *x, i
                        (bf16_t *)dx, (bf16_t *)dz, const_cast<float *>(rstd), part};
     const int grid = gated_norm_grid(a.rows, D, 1024);
     if (grid) GNORM_SWITCH(true, grid)
-    column_sum(part, grid, D, D, dw, w_f32, stream);
+    const int at[1] = {0};
+    column_sums(part, grid, D, 1, at, &D, &dw, &w_f32, stream);
     return hipGetLastError();
 }
 
@@ -501,10 +569,7 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_fwd_k
             if (a.gate) g = load8<false>(a.gate, at);
         }
         if (a.post) {
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
-            const float rs = rsqrtf(row_total<TPR>(ss, red) * inv + a.eps);
+            const float rs = rsqrtf(row_total<TPR>(squares8(v), red) * (inv / SQUARE_SCALE) + a.eps);
             if (live && c == 0 && a.rstd_y) a.rstd_y[r] = rs;
             v = v * rs * post;
         }
@@ -513,10 +578,7 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_fwd_k
             for (int i = 0; i < 8; ++i) v[i] *= sigmoid_f(g[i]);
         }
         x += v * scale;
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-        const float rs = rsqrtf(row_total<TPR>(ss, red) * inv + a.eps);
+        const float rs = rsqrtf(row_total<TPR>(squares8(x), red) * (inv / SQUARE_SCALE) + a.eps);
         if (live) {
             store8<X32>(a.xn, at, x);
             store8<false>(a.h, at, x * rs * w);
@@ -641,8 +703,8 @@ extern "C" hipError_t dsa_launch_residual_norm_bwd(const void *dxn, const void *
         if (x_f32) { RNORM_SWITCH(dsa_residual_norm_bwd_kernel, true, grid) }
         else { RNORM_SWITCH(dsa_residual_norm_bwd_kernel, false, grid) }
     }
-    column_sum(part, grid, 3 * (int64_t)C, C, dw, w_f32, stream);
-    if (post) column_sum(part + C, grid, 3 * (int64_t)C, C, dpost, post_f32, stream);
-    if (scale) column_sum(part + 2 * (int64_t)C, grid, 3 * (int64_t)C, C, dscale, scale_f32, stream);
+    const int at[3] = {0, C, 2 * C}, n[3] = {C, C, C}, f32[3] = {w_f32, post_f32, scale_f32};
+    void *const out[3] = {dw, post ? dpost : nullptr, scale ? dscale : nullptr};
+    column_sums(part, grid, 3 * (int64_t)C, 3, at, n, out, f32, stream);
     return hipGetLastError();
 }
