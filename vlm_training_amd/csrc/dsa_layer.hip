@@ -41,7 +41,8 @@ __device__ __forceinline__ float squares8(f32x8 x) {
     return s;
 }
 __device__ __forceinline__ float load1(const void *p, int64_t i, int f32) { return f32 ? ((const float *)p)[i] : (float)((const bf16_t *)p)[i]; }
-__device__ __forceinline__ f32x8 load8_any(const void *p, int64_t i, int f32) {          // a parameter: any alignment
+__device__ __forceinline__ f32x8 load8_any(const void *p, int64_t i, int f32) {          // a parameter: any alignment; i a multiple of 8
+    if (((uintptr_t)p & 15) == 0) return f32 ? load8<true>(p, i) : load8<false>(p, i);
     f32x8 r;
 #pragma unroll
     for (int e = 0; e < 8; ++e) r[e] = load1(p, i + e, f32);
@@ -546,36 +547,78 @@ __device__ __forceinline__ float row_total(float s, float *red) {
     return s;
 }
 constexpr int residual_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
-template <int TPR, bool X32>
+// eight elements of a row as they lie in memory
+template <bool F32>
+struct Raw8 {
+    u32x4 v[F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void *p, int64_t i) {
+        const u32x4 *const q = reinterpret_cast<const u32x4 *>((const char *)p + i * (F32 ? 4 : 2));
+#pragma unroll
+        for (int k = 0; k < (F32 ? 2 : 1); ++k) v[k] = __builtin_nontemporal_load(q + k);
+    }
+    __device__ __forceinline__ f32x8 get() const {
+        if (!F32) return bf8_to_f32(v[0]);
+        f32x8 r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = __uint_as_float(v[F32 ? i / 4 : 0][i % 4]);
+        return r;
+    }
+};
+// the elements of a row that a thread has, or zeros
+__device__ __forceinline__ f32x8 or_zero(f32x8 x, bool keep) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = keep ? x[i] : 0.f;
+    return x;
+}
+// THROUGH: the block's output passes a norm, a gate or a scale
+template <int TPR, bool X32, bool THROUGH>
 __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_fwd_kernel(ResidualArgs a) {
     __shared__ float red[16];
     constexpr int RPB = residual_threads(TPR) / TPR;
     const int c = threadIdx.x % TPR * 8, ly = threadIdx.x / TPR;
     const bool in_c = c < a.C;
+    const int cc = in_c ? c : 0;                         // (a thread past C reads the row's first elements, and drops them)
     const float inv = 1.f / (float)a.C;
     f32x8 w = zero8(), post = zero8(), scale = zero8() + 1.f;
     if (in_c) {
         w = load8_any(a.w, c, a.w_f32) + a.offset;
-        if (a.post) post = load8_any(a.post, c, a.post_f32) + a.offset;
-        if (a.scale) scale = load8_any(a.scale, c, a.scale_f32);
+        if (THROUGH && a.post) post = load8_any(a.post, c, a.post_f32) + a.offset;
+        if (THROUGH && a.scale) scale = load8_any(a.scale, c, a.scale_f32);
     }
-    for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < a.rows; rb += (int64_t)gridDim.x * RPB) {
-        const int64_t r = rb + ly, at = r * a.C + c;
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t r = (int64_t)blockIdx.x * RPB + ly;
+    Raw8<X32> xr;
+    Raw8<false> yr, gr;
+    auto fetch = [&](int64_t row) {
+        const int64_t at = (row < a.rows ? row : a.rows - 1) * a.C + cc;
+        yr.load(a.y, at);
+        xr.load(a.x, at);
+        if (THROUGH && a.gate) gr.load(a.gate, at);
+    };
+    fetch(r);
+    for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < a.rows; rb += step, r += step) {
+        const int64_t at = r * a.C + c;
         const bool live = in_c && r < a.rows;
-        f32x8 v = zero8(), x = zero8(), g = zero8();
-        if (live) {
-            v = load8<false>(a.y, at);
-            x = load8<X32>(a.x, at);
-            if (a.gate) g = load8<false>(a.gate, at);
-        }
-        if (a.post) {
-            const float rs = rsqrtf(row_total<TPR>(squares8(v), red) * (inv / SQUARE_SCALE) + a.eps);
-            if (live && c == 0 && a.rstd_y) a.rstd_y[r] = rs;
-            v = v * rs * post;
-        }
-        if (a.gate) {
+        f32x8 v = or_zero(yr.get(), in_c), x = or_zero(xr.get(), in_c);
+        if (THROUGH && a.gate) {
+            const f32x8 g = gr.get();
+            f32x8 s;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= sigmoid_f(g[i]);
+            for (int i = 0; i < 8; ++i) s[i] = sigmoid_f(g[i]);
+            fetch(r + step);
+            if (a.post) {
+                const float rs = rsqrtf(row_total<TPR>(squares8(v), red) * (inv / SQUARE_SCALE) + a.eps);
+                if (live && c == 0 && a.rstd_y) a.rstd_y[r] = rs;
+                v = v * rs * post;
+            }
+            v *= s;
+        } else {
+            fetch(r + step);
+            if (THROUGH && a.post) {
+                const float rs = rsqrtf(row_total<TPR>(squares8(v), red) * (inv / SQUARE_SCALE) + a.eps);
+                if (live && c == 0 && a.rstd_y) a.rstd_y[r] = rs;
+                v = v * rs * post;
+            }
         }
         x += v * scale;
         const float rs = rsqrtf(row_total<TPR>(squares8(x), red) * (inv / SQUARE_SCALE) + a.eps);
@@ -586,33 +629,65 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_fwd_k
         }
     }
 }
-template <int TPR, bool X32>
+template <int TPR, bool X32, bool THROUGH>
 __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_bwd_kernel(ResidualArgs a) {
     constexpr int RPB = residual_threads(TPR) / TPR;
+    // AHEAD: the next row's loads before this row's sums, the parameters in registers.  1024 threads have 128 registers each, which the sums of three parameters
+    // leave no room for: there every row reads the parameters again.
+    constexpr bool AHEAD = !(THROUGH && TPR == 1024);
     __shared__ float red[16], sums[RPB > 1 ? 256 : 1][8];
     const int c = threadIdx.x % TPR * 8, ly = threadIdx.x / TPR;
-    const bool in_c = c < a.C, through = a.post || a.gate || a.scale;        // through: y's gradient is not x's
+    const bool in_c = c < a.C;
+    const int cc = in_c ? c : 0;
     const float inv = 1.f / (float)a.C;
     f32x8 w = zero8(), post = zero8() + 1.f, scale = zero8() + 1.f, dw = zero8(), dpost = zero8(), dscale = zero8();
-    if (in_c) {
-        w = load8_any(a.w, c, a.w_f32) + a.offset;
-        if (a.post) post = load8_any(a.post, c, a.post_f32) + a.offset;
-        if (a.scale) scale = load8_any(a.scale, c, a.scale_f32);
-    }
-    for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < a.rows; rb += (int64_t)gridDim.x * RPB) {
-        const int64_t r = rb + ly, at = r * a.C + c;
-        const bool live = in_c && r < a.rows;
-        const float rs = live ? a.rstd[r] : 0.f, ry = live && a.post ? a.rstd_y[r] : 1.f;
-        f32x8 d = zero8(), xh = zero8(), y = zero8(), g = zero8(), dh = zero8();
-        if (live) {
-            if (a.dxn) d = load8<X32>(a.dxn, at);
-            if (a.dh) {
-                dh = load8<false>(a.dh, at);
-                xh = load8<X32>(a.xn, at) * rs;
-            }
-            if (through) y = load8<false>(a.y, at) * ry;
-            if (a.gate) g = load8<false>(a.gate, at);
+    auto parameters = [&](int e) {
+        w = load8_any(a.w, e, a.w_f32) + a.offset;
+        if (THROUGH && a.post) post = load8_any(a.post, e, a.post_f32) + a.offset;
+        if (THROUGH && a.scale) scale = load8_any(a.scale, e, a.scale_f32);
+    };
+    if (AHEAD) parameters(cc);
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t r = (int64_t)blockIdx.x * RPB + ly;
+    Raw8<X32> dr, xr;
+    Raw8<false> hr, yr, gr;
+    float rs_next = 0.f, ry_next = 1.f;
+    auto fetch = [&](int64_t row) {
+        const int64_t clamped = row < a.rows ? row : a.rows - 1, at = clamped * a.C + cc;
+        if (a.dxn) dr.load(a.dxn, at);
+        if (a.dh) {
+            hr.load(a.dh, at);
+            xr.load(a.xn, at);
+            rs_next = a.rstd[clamped];
         }
+        if (THROUGH) {
+            yr.load(a.y, at);
+            if (a.gate) gr.load(a.gate, at);
+            if (a.post) ry_next = a.rstd_y[clamped];
+        }
+    };
+    if (AHEAD) fetch(r);
+    for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < a.rows; rb += step, r += step) {
+        const int64_t at = r * a.C + c;
+        const bool live = in_c && r < a.rows;
+        if (!AHEAD) {
+            int e = cc;
+            asm volatile("" : "+v"(e));                  // (so that they are not kept after all)
+            parameters(e);
+            fetch(r);
+        }
+        const float rs = rs_next, ry = ry_next;
+        f32x8 d = zero8(), xh = zero8(), y = zero8(), g = zero8(), dh = zero8();
+        if (a.dxn) d = or_zero(dr.get(), live);
+        if (a.dh) {
+            dh = or_zero(hr.get(), live);
+            xh = or_zero(xr.get(), live) * rs;
+        }
+        if (THROUGH) {
+            y = or_zero(yr.get(), live) * ry;
+            if (a.gate) g = gr.get();
+        }
+        if (AHEAD) fetch(r + step);
         if (a.dh) {
             dw += dh * xh;
             dh *= w;
@@ -622,7 +697,7 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_bwd_k
             d += (dh - xh * (row_total<TPR>(dot, red) * inv)) * rs;
         }
         if (live) store8<X32>(a.dx, at, d);
-        if (through) {
+        if (THROUGH) {
             f32x8 sg = zero8() + 1.f;
             const f32x8 p = y * post;                    // what gate and scale multiply
             if (a.gate) {
@@ -630,10 +705,10 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_bwd_k
                 for (int i = 0; i < 8; ++i) sg[i] = sigmoid_f(g[i]);
                 if (live) store8<false>(a.dgate, at, d * p * scale * sg * (1.f - sg));
             }
-            dscale += d * p * sg;
+            dscale += or_zero(d * p * sg, live);         // (a row past the last one has its gate's copy)
             d *= scale * sg;
             if (a.post) {
-                dpost += d * y;
+                dpost += or_zero(d * y, live);
                 d *= post;
                 float dot = 0.f;
 #pragma unroll
@@ -645,7 +720,7 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_bwd_k
     }
     float *const part = a.part + (int64_t)blockIdx.x * 3 * a.C;
 #pragma unroll
-    for (int which = 0; which < 3; ++which) {
+    for (int which = 0; which < (THROUGH ? 3 : 1); ++which) {
         if ((which == 1 && !a.post) || (which == 2 && !a.scale)) continue;
         f32x8 s = which == 0 ? dw : which == 1 ? dpost : dscale;
         if (RPB > 1) {                                   // the workgroup's rows, in order
@@ -658,8 +733,8 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_bwd_k
                 for (int i = 0; i < 8; ++i) s[i] += sums[RPB > 1 ? k * TPR + threadIdx.x % TPR : 0][i];
         }
         if (in_c && ly == 0) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) part[(int64_t)which * a.C + c + i] = s[i];
+            *reinterpret_cast<f32x4 *>(part + (int64_t)which * a.C + c) = f32x4{s[0], s[1], s[2], s[3]};
+            *reinterpret_cast<f32x4 *>(part + (int64_t)which * a.C + c + 4) = f32x4{s[4], s[5], s[6], s[7]};
         }
     }
 }
@@ -673,23 +748,31 @@ static int residual_grid(int64_t rows, int C, int most) {
     const int64_t want = (rows + rpb - 1) / rpb;
     return (int)(want < most ? want : most);
 }
-extern "C" int dsa_residual_norm_blocks(int64_t rows, int C) { return residual_grid(rows, C, 1024); }
-#define RNORM_SWITCH(K, X, GRID)                                                                                \
-    switch (residual_tpr(a.C)) {                                                                                 \
-        case 64: hipLaunchKernelGGL((K<64, X>), dim3(GRID), dim3(256), 0, stream, a); break;                     \
-        case 128: hipLaunchKernelGGL((K<128, X>), dim3(GRID), dim3(256), 0, stream, a); break;                   \
-        case 256: hipLaunchKernelGGL((K<256, X>), dim3(GRID), dim3(256), 0, stream, a); break;                   \
-        case 512: hipLaunchKernelGGL((K<512, X>), dim3(GRID), dim3(512), 0, stream, a); break;                   \
-        default: hipLaunchKernelGGL((K<1024, X>), dim3(GRID), dim3(1024), 0, stream, a); break;                  \
+// The backward's workgroups: one or two to every compute unit, so that they all run at once (260 for 1037 rows of 2560: 41 us, 256: 27), and so that
+// their sums, 12 C bytes each, stay a small part of what is written.
+extern "C" int dsa_residual_norm_blocks(int64_t rows, int C) { return residual_grid(rows, C, rows < 2048 ? 256 : 512); }
+#define RNORM_SWITCH(K, X, P, GRID)                                                                               \
+    switch (residual_tpr(a.C)) {                                                                                   \
+        case 64: hipLaunchKernelGGL((K<64, X, P>), dim3(GRID), dim3(256), 0, stream, a); break;                    \
+        case 128: hipLaunchKernelGGL((K<128, X, P>), dim3(GRID), dim3(256), 0, stream, a); break;                  \
+        case 256: hipLaunchKernelGGL((K<256, X, P>), dim3(GRID), dim3(256), 0, stream, a); break;                  \
+        case 512: hipLaunchKernelGGL((K<512, X, P>), dim3(GRID), dim3(512), 0, stream, a); break;                  \
+        default: hipLaunchKernelGGL((K<1024, X, P>), dim3(GRID), dim3(1024), 0, stream, a); break;                 \
+    }
+#define RNORM_LAUNCH(K, GRID)                                                  \
+    {                                                                          \
+        const bool through = a.post || a.gate || a.scale;                      \
+        if (x_f32 && through) RNORM_SWITCH(K, true, true, GRID)                \
+        else if (x_f32) RNORM_SWITCH(K, true, false, GRID)                     \
+        else if (through) RNORM_SWITCH(K, false, true, GRID)                   \
+        else RNORM_SWITCH(K, false, false, GRID)                               \
     }
 extern "C" hipError_t dsa_launch_residual_norm_fwd(const void *x, int x_f32, const void *y, const void *gate, const void *w, int w_f32, const void *post, int post_f32,
                                                    const void *scale, int scale_f32, float eps, float offset, int T, int C, void *xn, void *h, float *rstd, float *rstd_y,
                                                    hipStream_t stream) {
     ResidualArgs a = {x, (const bf16_t *)y, (const bf16_t *)gate, w, post, scale, w_f32, post_f32, scale_f32, C, eps, offset, T, xn, (bf16_t *)h, rstd, rstd_y};
-    const int grid = residual_grid(T, C, 8192);
-    if (!grid) return hipSuccess;
-    if (x_f32) { RNORM_SWITCH(dsa_residual_norm_fwd_kernel, true, grid) }
-    else { RNORM_SWITCH(dsa_residual_norm_fwd_kernel, false, grid) }
+    const int grid = residual_grid(T, C, 1024);
+    if (grid) RNORM_LAUNCH(dsa_residual_norm_fwd_kernel, grid)
     return hipGetLastError();
 }
 extern "C" hipError_t dsa_launch_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x_f32, const void *y, const void *gate, const void *w, int w_f32,
@@ -699,10 +782,7 @@ extern "C" hipError_t dsa_launch_residual_norm_bwd(const void *dxn, const void *
     ResidualArgs a = {nullptr, (const bf16_t *)y, (const bf16_t *)gate, w, post, scale, w_f32, post_f32, scale_f32, C, 0.f, offset, T, const_cast<void *>(xn), nullptr,
                       const_cast<float *>(rstd), const_cast<float *>(rstd_y), dxn, (const bf16_t *)dh, dx, (bf16_t *)dy, (bf16_t *)dgate, part};
     const int grid = dsa_residual_norm_blocks(T, C);
-    if (grid) {
-        if (x_f32) { RNORM_SWITCH(dsa_residual_norm_bwd_kernel, true, grid) }
-        else { RNORM_SWITCH(dsa_residual_norm_bwd_kernel, false, grid) }
-    }
+    if (grid) RNORM_LAUNCH(dsa_residual_norm_bwd_kernel, grid)
     const int at[3] = {0, C, 2 * C}, n[3] = {C, C, C}, f32[3] = {w_f32, post_f32, scale_f32};
     void *const out[3] = {dw, post ? dpost : nullptr, scale ? dscale : nullptr};
     column_sums(part, grid, 3 * (int64_t)C, 3, at, n, out, f32, stream);
