@@ -6,6 +6,8 @@
 // partial sums that a second kernel adds in a fixed order (no atomics).
 #include "dsa_rows.h"
 
+#include <type_traits>
+
 __device__ __forceinline__ f32x8 zero8() {
     f32x8 z;
 #pragma unroll
@@ -106,9 +108,10 @@ static void column_sums(const float *part, int blocks, int64_t stride, int count
 
 // ---- short convolution -------------------------------------------------------------------------------------------------------------------
 // A thread keeps four channels over a run of consecutive rows: the last W-1 inputs stay in registers, so a row is read once (and W-1 rows once
-// more per run); CONV_BATCH rows' loads are in flight together.  lanes_c threads of a workgroup lie side by side over the channels, the others take further runs.
+// more per run); the next CONV_BATCH rows' loads are in flight while these are worked on.  lanes_c threads of a workgroup, whole waves, lie side by side over the channels, the others take
+// further runs: a wave's rows and their addresses are scalars.
 // (Eight channels took 256 registers in the backward, two waves per SIMD: 330 us for 16 384 rows of 8192, 2.4 TB/s.)
-#define CONV_BATCH 8
+#define CONV_BATCH 4
 struct ConvArgs {
     const bf16_t *x, *dy, *state;                        // (T, C) rows x_tok, dy_tok apart;  (N, C, W-1)
     int64_t x_tok, dy_tok;
@@ -170,8 +173,8 @@ __device__ __forceinline__ f32x4 conv_before(const ConvArgs &a, const ConvPlace 
     return r;
 }
 template <int W, bool BWD>
-__global__ __launch_bounds__(256) void dsa_conv_kernel(ConvArgs a) {
-    const int lx = threadIdx.x % a.lanes_c, ly = threadIdx.x / a.lanes_c, runs_y = 256 / a.lanes_c;
+__global__ __launch_bounds__(256, BWD ? 3 : 6) void dsa_conv_kernel(ConvArgs a) {
+    const int lx = threadIdx.x % a.lanes_c, ly = __builtin_amdgcn_readfirstlane(threadIdx.x / a.lanes_c), runs_y = 256 / a.lanes_c;
     const int c0 = (blockIdx.x * a.lanes_c + lx) * 4;
     const bool live = c0 < a.C;
     const int64_t first = ((int64_t)blockIdx.y * runs_y + ly) * a.run;
@@ -192,72 +195,88 @@ __global__ __launch_bounds__(256) void dsa_conv_kernel(ConvArgs a) {
     }
     if (live && t0 < t1) {
         ConvPlace p;
-        const bf16_t *const x = a.x + c0, *const g = BWD ? a.dy + c0 : nullptr;
         if (t0 < last) {
             p.find(a.cu, a.N, t0);
 #pragma unroll
             for (int j = 1; j < W; ++j) {
                 const int t = t0 - j;
-                h[j - 1] = t >= p.start ? bf4_to_f32(*reinterpret_cast<const u32x2 *>(x + t * a.x_tok)) : conv_before<W>(a, p, p.start - t, c0);
+                h[j - 1] = t >= p.start ? bf4_to_f32(*reinterpret_cast<const u32x2 *>(a.x + t * a.x_tok + c0)) : conv_before<W>(a, p, p.start - t, c0);
             }
         }
         // the backward goes on for W-1 rows: they have a share in the run's last gradients
         const int stop = min(BWD ? t1 + W - 1 : t1, last);
-        for (int tb = t0; tb < stop; tb += CONV_BATCH) {
-            u32x2 xr[CONV_BATCH], gr[CONV_BATCH];
+        // one row; INNER: t and the W-1 rows before it lie in the same sequence and in the run
+        auto row = [&](int t, u32x2 xw, u32x2 gw, auto inner) {
+            constexpr bool INNER = decltype(inner)::value;
+            if (!INNER && t >= p.end) {
+                p.next(a.cu, a.N, t);
 #pragma unroll
-            for (int u = 0; u < CONV_BATCH; ++u) {
-                const int64_t t = min(tb + u, stop - 1);
-                xr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(x + t * a.x_tok));
-                if (BWD) gr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(g + t * a.dy_tok));
+                for (int j = 1; j < W; ++j) h[j - 1] = conv_before<W>(a, p, j, c0);
+            }
+            const f32x4 xt = bf4_to_f32(xw);
+            f32x4 z = b + w[W - 1] * xt;
+#pragma unroll
+            for (int j = 1; j < W; ++j) z += w[W - 1 - j] * h[j - 1];
+            if (!BWD) {
+                if (a.silu) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[i] *= sigmoid_f(z[i]);
+                }
+                __builtin_nontemporal_store(f32_to_bf4(z), reinterpret_cast<u32x2 *>(a.y + (int64_t)t * a.C + c0));
+            } else {
+                f32x4 dz = bf4_to_f32(gw);
+                if (a.silu) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float s = sigmoid_f(z[i]), zs = z[i] * s;
+                        dz[i] *= s + zs - zs * s;
+                    }
+                }
+                if (INNER || t < t1) {
+                    db += dz;
+                    dw[W - 1] += dz * xt;
+#pragma unroll
+                    for (int j = 1; j < W; ++j) dw[W - 1 - j] += dz * h[j - 1];
+                }
+                // acc[j]: the gradient of row t - j so far
+                acc[0] = w[W - 1] * dz;
+#pragma unroll
+                for (int j = 1; j < W; ++j)
+                    if (INNER || t - j >= p.start) acc[j] += w[W - 1 - j] * dz;
+                const int done = t - (W - 1);
+                if (INNER || (done >= t0 && done < t1)) __builtin_nontemporal_store(f32_to_bf4(acc[W - 1]), reinterpret_cast<u32x2 *>(a.y + (int64_t)done * a.C + c0));
+#pragma unroll
+                for (int j = W - 1; j > 0; --j) acc[j] = acc[j - 1];
             }
 #pragma unroll
+            for (int j = W - 2; j > 0; --j) h[j] = h[j - 1];
+            h[0] = xt;
+        };
+        u32x2 xr[CONV_BATCH], gr[CONV_BATCH];
+        auto fetch = [&](int tb) {
+#pragma unroll
             for (int u = 0; u < CONV_BATCH; ++u) {
-                const int t = tb + u;
-                if (t >= stop) break;
-                if (t >= p.end) {
-                    p.next(a.cu, a.N, t);
+                const int64_t t = min(tb + u, a.T - 1);
+                xr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(a.x + t * a.x_tok + c0));
+                if (BWD) gr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(a.dy + t * a.dy_tok + c0));
+            }
+        };
+        fetch(t0);
+        for (int tb = t0; tb < stop; tb += CONV_BATCH) {
+            u32x2 xn[CONV_BATCH], gn[CONV_BATCH];
 #pragma unroll
-                    for (int j = 1; j < W; ++j) h[j - 1] = conv_before<W>(a, p, j, c0);
-                }
-                const f32x4 xt = bf4_to_f32(xr[u]);
-                f32x4 z = b + w[W - 1] * xt;
+            for (int u = 0; u < CONV_BATCH; ++u) {
+                xn[u] = xr[u];
+                gn[u] = gr[u];
+            }
+            fetch(tb + CONV_BATCH);
+            if (tb + CONV_BATCH <= min(p.end, BWD ? t1 : stop) && (!BWD || tb - (W - 1) >= max(t0, p.start))) {
 #pragma unroll
-                for (int j = 1; j < W; ++j) z += w[W - 1 - j] * h[j - 1];
-                if (!BWD) {
-                    if (a.silu) {
+                for (int u = 0; u < CONV_BATCH; ++u) row(tb + u, xn[u], gn[u], std::true_type{});
+            } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) z[i] *= sigmoid_f(z[i]);
-                    }
-                    __builtin_nontemporal_store(f32_to_bf4(z), reinterpret_cast<u32x2 *>(a.y + (int64_t)t * a.C + c0));
-                } else {
-                    f32x4 dz = bf4_to_f32(gr[u]);
-                    if (a.silu) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float s = sigmoid_f(z[i]);
-                            dz[i] *= s * (1.f + z[i] * (1.f - s));
-                        }
-                    }
-                    if (t < t1) {
-                        db += dz;
-                        dw[W - 1] += dz * xt;
-#pragma unroll
-                        for (int j = 1; j < W; ++j) dw[W - 1 - j] += dz * h[j - 1];
-                    }
-                    // acc[j]: the gradient of row t - j so far
-                    acc[0] = w[W - 1] * dz;
-#pragma unroll
-                    for (int j = 1; j < W; ++j)
-                        if (t - j >= p.start) acc[j] += w[W - 1 - j] * dz;
-                    const int done = t - (W - 1);
-                    if (done >= t0 && done < t1) __builtin_nontemporal_store(f32_to_bf4(acc[W - 1]), reinterpret_cast<u32x2 *>(a.y + (int64_t)done * a.C + c0));
-#pragma unroll
-                    for (int j = W - 1; j > 0; --j) acc[j] = acc[j - 1];
-                }
-#pragma unroll
-                for (int j = W - 2; j > 0; --j) h[j] = h[j - 1];
-                h[0] = xt;
+                for (int u = 0; u < CONV_BATCH; ++u)
+                    if (tb + u < stop) row(tb + u, xn[u], gn[u], std::false_type{});
             }
         }
         if (BWD) {
@@ -340,13 +359,14 @@ __global__ __launch_bounds__(256) void dsa_conv_step_kernel(ConvArgs a, bf16_t *
     *reinterpret_cast<u32x4 *>(a.y + req * a.C + c0) = f32_to_bf8(z);
 }
 
-// threads side by side over the channels, and the rows of a run: enough runs for the chip's waves, none shorter than 16 rows (W-1 of them come on top)
-static void conv_shape(ConvArgs &a, int &cols, int &rows) {
-    a.lanes_c = 1;
+// Threads side by side over the channels, and the rows of a run, none shorter than 16 (W-1 of them come on top).  As many workgroups as run at once, six to a
+// compute unit forwards and three backwards; 16 384 rows of 8192: forwards 112 us (three: 117), backwards 185 and 6 for the sums (six: 190 and 10).
+static void conv_shape(ConvArgs &a, int &cols, int &rows, int groups) {
+    a.lanes_c = 64;
     while (a.lanes_c < 256 && a.lanes_c * 4 < a.C) a.lanes_c *= 2;
     cols = (a.C / 4 + a.lanes_c - 1) / a.lanes_c;
     const int runs_y = 256 / a.lanes_c;
-    const int64_t want = (2048 + cols - 1) / cols * (int64_t)runs_y;        // runs
+    const int64_t want = (groups + cols - 1) / cols * (int64_t)runs_y;      // runs
     const int64_t run = (a.T + want - 1) / want;
     a.run = (int)(run < 16 ? 16 : run);
     const int64_t per = (int64_t)a.run * runs_y;
@@ -357,7 +377,7 @@ extern "C" int dsa_conv_blocks(int T, int C) {
     a.T = T;
     a.C = C;
     int cols, rows;
-    conv_shape(a, cols, rows);
+    conv_shape(a, cols, rows, 768);
     return rows;
 }
 #define CONV_SWITCH(W, CALL)                  \
@@ -370,7 +390,7 @@ extern "C" hipError_t dsa_launch_conv_fwd(const void *x, int64_t x_tok, const vo
                                           int C, int W, const void *state, void *y, void *final, hipStream_t stream) {
     ConvArgs a = {(const bf16_t *)x, nullptr, (const bf16_t *)state, x_tok, 0, w, bias, w_f32, b_f32, silu, cu, T, N, C, 0, 0, (bf16_t *)y, nullptr};
     int cols, rows;
-    conv_shape(a, cols, rows);
+    conv_shape(a, cols, rows, 1536);
 #define CONV_FWD(WW) hipLaunchKernelGGL((dsa_conv_kernel<WW, false>), dim3(cols, rows), dim3(256), 0, stream, a)
     if (T > 0) CONV_SWITCH(W, CONV_FWD)
     if (final) {
@@ -384,7 +404,7 @@ extern "C" hipError_t dsa_launch_conv_bwd(const void *x, int64_t x_tok, const vo
                                           hipStream_t stream) {
     ConvArgs a = {(const bf16_t *)x, (const bf16_t *)dy, (const bf16_t *)state, x_tok, dy_tok, w, bias, w_f32, b_f32, silu, cu, T, N, C, 0, 0, (bf16_t *)dx, part};
     int cols, rows;
-    conv_shape(a, cols, rows);
+    conv_shape(a, cols, rows, 768);
 #define CONV_BWD(WW) hipLaunchKernelGGL((dsa_conv_kernel<WW, true>), dim3(cols, rows), dim3(256), 0, stream, a)
     if (T > 0) CONV_SWITCH(W, CONV_BWD)
     const int64_t stride = (int64_t)(W + 1) * C;
