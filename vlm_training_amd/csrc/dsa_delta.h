@@ -225,6 +225,8 @@ __device__ __forceinline__ void store_any(void *p, int64_t i, int f32, float x) 
     else reinterpret_cast<bf16_t *>(p)[i] = (bf16_t)x;
 }
 __device__ __forceinline__ float softplus_f(float x) { return x > 20.f ? x : log1pf(expf(x)); }
+// e^x for x <= 0 between rows of a chunk: off by |x| 2^-24 of its value, next to the 2^-17 that E loses in the products
+__device__ __forceinline__ float delta_decay(float x) { return __builtin_amdgcn_exp2f(fminf(x, 0.f) * 1.442695041f); }
 // the log decay of a row.  Held above -1e4, where e^g has long been zero: a decay of -inf would make G_i - G_j of later rows NaN.  (A NaN stays one.)
 __device__ __forceinline__ float delta_gate(const dsa_delta_args &in, int64_t t, int h) {
     const float x = load_any(in.a, t * in.a_tok + h, in.a_f32) + load_any(in.dt_bias, h, in.param_f32);

@@ -237,7 +237,7 @@ template <int DK, int DV>
 __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
     constexpr int KS = DK + 8, TS = DELTA_TS, NT = DK / 16;
     __shared__ bf16_t ks[64 * KS], qs[64 * KS], pool[4 * 64 * TS];
-    __shared__ float rows[DELTA_ROWS * 64], dg_row[64], dg_s[64], dots[4];
+    __shared__ __align__(16) float rows[DELTA_ROWS * 64], dg_row[64], dg_s[64], dots[4];
     bf16_t *const ns = pool, *const ss = pool + 2 * 64 * TS;                                              // N as hi, lo; S0, then dS1: 64 columns of the values
     bf16_t *const xs = pool, *const zs = pool + 2 * 64 * TS;                                              // in their place X and Z as hi, lo
     static_assert(64 * KS <= 2 * 64 * TS, "64 rows of the state lie in two tiles");
@@ -396,12 +396,14 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         for (int t = 0; t < 4; ++t) {
             f32x4 xv = zero4(), zv = zero4();
             if (t <= wv) {
+                const int j0 = 16 * t + 4 * g4;
+                const f32x4 dh = gi - *reinterpret_cast<const f32x4 *>(rows + DELTA_GH * 64 + j0), dl = gi_lo - *reinterpret_cast<const f32x4 *>(rows + DELTA_GL * 64 + j0);
+                const f32x4 rj = *reinterpret_cast<const f32x4 *>(rows + DELTA_RK * 64 + j0);
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
-                    const int j = 16 * t + 4 * g4 + v;
-                    const float e = expf(fminf((gi - rows[DELTA_GH * 64 + j]) + (gi_lo - rows[DELTA_GL * 64 + j]), 0.f)) * rows[DELTA_RK * 64 + j];
-                    xv[v] = j <= row ? x[t][v] * e * fx : 0.f;
-                    zv[v] = j < row ? z[t][v] * e * fz : 0.f;
+                    const float e = delta_decay(dh[v] + dl[v]) * rj[v];
+                    xv[v] = j0 + v <= row ? x[t][v] * e * fx : 0.f;
+                    zv[v] = j0 + v < row ? z[t][v] * e * fz : 0.f;
                 }
             }
             const int at = row * TS + 16 * t + 4 * g4;

@@ -7,12 +7,13 @@
 // each, then T_ij = -T_ii sum_k A_ik T_kj from the diagonal outwards, in fp32 (mfma of 16x16x4): a run of equal keys, whose A is a full triangle of
 // ones, has a T of ones and minus ones that powers of A would lose in cancellation.
 template <int DK>
-__global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(256, 4) void dsa_delta_prep_kernel(DeltaArgs a) {
     constexpr int KS = DK + 8, FS = 68;
-    __shared__ bf16_t ks[64 * KS], qs[64 * KS];
-    __shared__ float am[64 * FS], tm[64 * FS], ms[4][16 * 17], rk[64], rq[64], gh[64], gl[64], bt[64];
+    __shared__ __align__(16) float am[64 * FS], tm[64 * FS], ms[4][16 * 17], rk[64], rq[64], gh[64], gl[64], bt[64];
+    bf16_t *const ks = (bf16_t *)am, *const qs = (bf16_t *)tm;               // K and Q, before their products are there
+    static_assert(64 * KS * 2 <= 64 * FS * 4, "a tile of K lies in A's place");
     const dsa_delta_args &in = a.in;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, l16 = lane & 15, g4 = lane >> 4;
+    const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = tid & 15, g4 = (tid & 63) >> 4;
     const int slot = blockIdx.x, hk = blockIdx.y, rep = in.Hv / in.Hk;
     DeltaChunk c;
     if (!delta_locate(in.cu, in.N, in.T, slot, c)) {
@@ -53,8 +54,8 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
             }
         }
     }
-    const int i = 16 * wv + l16;
     for (int u = 0; u < rep; ++u) {
+        const int lane = fresh_lane(), l16 = lane & 15, g4 = lane >> 4, tid = 64 * wv + lane, i = 16 * wv + l16;
         const int h = hk * rep + u;
         const int64_t p = (int64_t)slot * in.Hv + h;
         __syncthreads();                                 // (the previous head's LDS has been read)
@@ -85,15 +86,19 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
         __syncthreads();
         bf16_t *const tg = (bf16_t *)(a.mats + p * a.mats_bytes + DELTA_T), *const pm = tg + a.planes * 4096;
         f32x4 px[4];
+        const float gi = gh[i], gi_lo = gl[i], fx = rq[i], fy = bt[i] * rk[i];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             f32x4 x = zero4(), y = zero4();
+            if (t <= wv) {
+                const int j0 = 16 * t + 4 * g4;
+                const f32x4 dh = gi - *reinterpret_cast<const f32x4 *>(gh + j0), dl = gi_lo - *reinterpret_cast<const f32x4 *>(gl + j0), r = *reinterpret_cast<const f32x4 *>(rk + j0);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int j = 16 * t + 4 * g4 + v;
-                const float e = expf(fminf((gh[i] - gh[j]) + (gl[i] - gl[j]), 0.f));
-                x[v] = j <= i ? e * rq[i] * rk[j] * qk[t][v] : 0.f;
-                y[v] = j < i ? e * bt[i] * rk[i] * rk[j] * kk[t][v] : 0.f;
+                for (int v = 0; v < 4; ++v) {
+                    const float e = delta_decay(dh[v] + dl[v]) * r[v];
+                    x[v] = j0 + v <= i ? e * fx * qk[t][v] : 0.f;
+                    y[v] = j0 + v < i ? e * fy * kk[t][v] : 0.f;
+                }
             }
             px[t] = x;
             *reinterpret_cast<f32x4 *>(am + i * FS + 16 * t + 4 * g4) = y;
@@ -106,7 +111,12 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
             for (int r = 0; r < 16; ++r) {
                 float s = r == l16 ? 1.f : 0.f;
 #pragma unroll
-                for (int k = 0; k < r; ++k) s -= am[(16 * wv + r) * FS + 16 * wv + k] * x[k];
+                for (int k = 0; k < r; k += 4) {
+                    const f32x4 y = *reinterpret_cast<const f32x4 *>(am + (16 * wv + r) * FS + 16 * wv + k);
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        if (k + v < r) s -= y[v] * x[k + v];
+                }
                 x[r] = s;
             }
             if (g4 == 0) {
@@ -147,9 +157,13 @@ __global__ __launch_bounds__(256) void dsa_delta_prep_kernel(DeltaArgs a) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int at = tid + 256 * e, r = at / 128 * 16 + l16, c0 = at / 64 % 2 * 32 + 8 * g4;
-            plane(tg, at * 8, *reinterpret_cast<const f32x4 *>(tm + r * FS + c0), *reinterpret_cast<const f32x4 *>(tm + r * FS + c0 + 4));
-            plane(pm, at * 8, *reinterpret_cast<const f32x4 *>(am + r * FS + c0), *reinterpret_cast<const f32x4 *>(am + r * FS + c0 + 4));
-            if (a.planes > 2) {                          // transposed
+            // (the quarter that is all zeros is neither written nor read)
+            if (r < 32 && c0 >= 32) {}
+            else {
+                plane(tg, at * 8, *reinterpret_cast<const f32x4 *>(tm + r * FS + c0), *reinterpret_cast<const f32x4 *>(tm + r * FS + c0 + 4));
+                plane(pm, at * 8, *reinterpret_cast<const f32x4 *>(am + r * FS + c0), *reinterpret_cast<const f32x4 *>(am + r * FS + c0 + 4));
+            }
+            if (a.planes > 2 && !(r >= 32 && c0 < 32)) { // transposed
                 f32x4 x[2], y[2];
 #pragma unroll
                 for (int v = 0; v < 8; ++v) {
