@@ -264,10 +264,19 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
     f32x4 dq[NT], dk[NT];                                // [16 t + 4 g4 + v][row], times scale/|q| and 1/|k|
 #pragma unroll
     for (int t = 0; t < NT; ++t) dq[t] = dk[t] = zero4();
+    float sum_q = 0.f, sum_k = 0.f;                      // q.dQ and k.dK of the heads so far, this lane's columns
     const bool live = row < c.rows;
     const bf16_t *const krow = ks + row * KS + 4 * g4, *const qrow = qs + row * KS + 4 * g4;
     auto four = [](const bf16_t *p) __attribute__((always_inline)) { return up4(*reinterpret_cast<const u32x2_any *>(p)); };
     auto dot4 = [](f32x4 x, f32x4 y, float s) __attribute__((always_inline)) { return s + ((x[0] * y[0] + x[1] * y[1]) + (x[2] * y[2] + x[3] * y[3])); };
+    auto dot8 = [](u32x4 x, u32x4 y, float s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t xi = x[i], yi = y[i];         // (a bit cast of a vector's element itself is compiled as one of element 0)
+            s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, xi), __builtin_bit_cast(bf16x2, yi), s, false);
+        }
+        return s;
+    };
     auto over_row = [](float x) __attribute__((always_inline)) { x += __shfl_xor(x, 16, 64); return x + __shfl_xor(x, 32, 64); };
 #pragma unroll 1
     for (int u = 0; u < rep; ++u) {
@@ -276,7 +285,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         const bf16_t *const state = (const bf16_t *)(a.saved + p * a.saved_bytes), *const news = state + DV * DK;
         const bf16_t *const dstate = (const bf16_t *)(a.back + p * a.back_bytes), *const drs = dstate + DV * DK;
         f32x4 x[4], z[4];
-        float sum = 0.f, dots_ = 0.f, dot = 0.f, db = 0.f;      // sum: what the row adds to dG
+        float dots_ = 0.f, kx = 0.f, dot = 0.f, db = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) x[t] = z[t] = zero4();
         __syncthreads();                                 // (the previous head's LDS has been read)
@@ -343,7 +352,6 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 nf[s] = frag_n(ns, TS, 16 * wv, 32 * s, ln);
-                db = dot8_chain(rf[s], nf[s], dot8_chain(rl[s], nf[s], dot8_chain(rf[s], frag_n(ns + 64 * TS, TS, 16 * wv, 32 * s, ln), db)));
             }
             // through S0: scale e^G dO S0^T into dQ, -beta e^G dR S0^T into dK
 #pragma unroll
@@ -355,12 +363,8 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                     y = mfma16(m, of[s], y);
                     w = mfma16(m, rf[s], w);
                 }
-                y *= fq;
-                w *= fk;
-                dq[t] += y;
-                dk[t] += w;
-                sum = dot4(y, four(qrow + 16 * t), sum);
-                sum = dot4(w, four(krow + 16 * t), sum);
+                dq[t] += y * fq;
+                dk[t] += w * fk;
                 if (t % 2) __builtin_amdgcn_sched_barrier(0);        // (the products' operands of all t at once are more than the registers hold)
             }
             __syncthreads();
@@ -369,27 +373,29 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             for (int e = 0; e < DK / 32; ++e) {
                 bf16_t *const q0 = place(e, 0), *const q1 = place(e, 1);
                 const u32x2 lo = *reinterpret_cast<const u32x2_any *>(q0), hi = *reinterpret_cast<const u32x2_any *>(q1);
-                dot = dot8_chain(__builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]}), __builtin_bit_cast(bf16x8, ts[e]), dot);
+                dot = dot8(u32x4{lo[0], lo[1], hi[0], hi[1]}, ts[e], dot);
                 put4(q0, u32x2{ts[e][0], ts[e][1]});
                 put4(q1, u32x2{ts[e][2], ts[e][3]});
             }
             __syncthreads();
             // through dS1: e^(G_63 - G) N dS1^T into dK
+            float part = 0.f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 f32x4 y = zero4();
 #pragma unroll
                 for (int s = 0; s < 2; ++s) y = mfma16(frag_t(ss, KS, 32 * s, 16 * t, ln), nf[s], y);
-                y *= fs;
-                dk[t] += y;
-                dots_ = dot4(y, four(krow + 16 * t), dots_);
+                dk[t] += y * fs;
+                part = dot4(y, four(krow + 16 * t), part);
                 if (t % 2) __builtin_amdgcn_sched_barrier(0);
             }
+            dots_ += part * fs;
         }
         __syncthreads();
         // X and Z
         const int ln = fresh_lane(), l16 = ln & 15, g4 = ln >> 4, row = 16 * wv + l16;
         const bf16_t *const krow = ks + row * KS + 4 * g4, *const qrow = qs + row * KS + 4 * g4;
+        const int diagonal = l16 - 4 * g4;               // (the lane that has the row's own element, and which)
         const float rk = rows[DELTA_RK * 64 + row], fx = rows[DELTA_RQ * 64 + row], fz = -rows[DELTA_BETA * 64 + row] * rk;
         const float gi = rows[DELTA_GH * 64 + row], gi_lo = rows[DELTA_GL * 64 + row];
 #pragma unroll
@@ -404,6 +410,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                     const float e = delta_decay(dh[v] + dl[v]) * rj[v];
                     xv[v] = j0 + v <= row ? x[t][v] * e * fx : 0.f;
                     zv[v] = j0 + v < row ? z[t][v] * e * fz : 0.f;
+                    if (t == wv && v == diagonal) db = z[t][v];      // dR.N
                 }
             }
             const int at = row * TS + 16 * t + 4 * g4;
@@ -426,9 +433,10 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 xt[half][s] = frag_t(xh, TS, 32 * s, 16 * wv, ln);
                 zt[half][s] = frag_t(zh, TS, 32 * s, 16 * wv, ln);
             }
+        float now_q = 0.f, now_k = 0.f;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            f32x4 y = zero4(), w = zero4(), u1 = zero4();
+            f32x4 y = dq[t], w = dk[t], u1 = zero4();
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const bf16x8 kb = frag_t(ks, KS, 32 * s, 16 * t, ln), qb = frag_t(qs, KS, 32 * s, 16 * t, ln);
@@ -440,14 +448,19 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                     u1 = mfma16(qb, xt[half][s], u1);
                 }
             }
-            sum = dot4(y, four(qrow + 16 * t), sum);
-            sum = dot4(w - u1, four(krow + 16 * t), sum);
-            dq[t] += y;
-            dk[t] += w + u1;
+            const f32x4 kr = four(krow + 16 * t);
+            dq[t] = y;
+            dk[t] = w + u1;
+            kx = dot4(u1, kr, kx);
+            now_q = dot4(y, four(qrow + 16 * t), now_q);
+            now_k = dot4(dk[t], kr, now_k);
             if (t % 2) __builtin_amdgcn_sched_barrier(0);
         }
+        // what the head added to q.dQ and k.dK, less twice the part of k.dK that counts the other way
+        const float sum = over_row((now_q - sum_q) + (now_k - sum_k) - 2.f * (kx + dots_));
+        sum_q = now_q;
+        sum_k = now_k;
         dots_ = over_row(dots_);
-        sum = over_row(sum) - dots_;
         db = over_row(db);
         if (g4 == 0) {
             dg_row[row] = sum;
@@ -488,15 +501,9 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         }
     }
     // back through the unit length: with x = r q (r = 1/|q|), dq = r dx - q r^2 (q . r dx); the accumulators hold r dx
-    float pq = 0.f, pk = 0.f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        pq = dot4(dq[t], four(qrow + 16 * t), pq);
-        pk = dot4(dk[t], four(krow + 16 * t), pk);
-    }
     const float rq = rows[DELTA_RQ * 64 + row] / in.scale, rk = rows[DELTA_RK * 64 + row];
-    pq = in.l2_norm ? over_row(pq) * rq * rq : 0.f;
-    pk = in.l2_norm ? over_row(pk) * rk * rk : 0.f;
+    const float pq = in.l2_norm ? over_row(sum_q) * rq * rq : 0.f;
+    const float pk = in.l2_norm ? over_row(sum_k) * rk * rk : 0.f;
     bf16_t *const dq_row = a.dq + ((int64_t)(c.row0 + row) * in.Hk + hk) * in.Dk, *const dk_row = a.dk + ((int64_t)(c.row0 + row) * in.Hk + hk) * in.Dk;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
