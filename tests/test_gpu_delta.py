@@ -131,6 +131,35 @@ def test_corners_of_the_chunk_algebra(kind):
     against(x, [T], check=tuple(n for n in NAMES if n not in dead))
 
 
+# How the state's walk is split over workgroups goes by the number of sequences and heads (empty sequences count): two blocks of columns to a workgroup, a whole head to one
+MANY = [("columns", 64, 2, 64, 96), ("columns", 64, 2, 128, 128), ("head", 64, 8, 128, 128), ("head", 256, 2, 72, 104)]
+
+
+@pytest.mark.parametrize("split,n,hv,dk,dv", MANY)
+def test_many_sequences(split, n, hv, dk, dv):
+    _log(f"{split} {n} sequences, heads of {dk}/{dv}")
+    lens = [0] * n
+    for i, L in zip((0, 1, 7, n // 2, n - 3, n - 1), (64, 1, 130, 65, 200, 63)):
+        lens[i] = L
+    g = torch.Generator().manual_seed(n + dk)
+    x = inputs(sum(lens), hv // 2, hv, dk, dv, seed=n + dv)
+    against(x, lens, 0.5 * torch.randn(n, hv, dk, dv, generator=g), 0.1 * torch.randn(n, hv, dk, dv, generator=g))
+    x = inputs(sum(lens) + 70, hv // 2, hv, dk, dv, seed=n)
+    go, gs = V.gated_delta_rule(*(x[m].to(DEV) for m in NAMES), cu_of(lens), return_final_state=True)             # nothing is kept for a backward
+    o, s = R.gated_delta_rule(*(x[m].double()[:sum(lens)] if m in "qkvab" else x[m].double() for m in NAMES), lens, None)
+    assert off(go[:sum(lens)], o) <= OUT and off(gs, s) <= STATE and not go[sum(lens):].any()
+
+
+@pytest.mark.parametrize("kind", ["same_key", "full_decay", "one_reset"])
+@pytest.mark.parametrize("split,n,hv,dk,dv", MANY[1:3])
+def test_corners_in_many_sequences(split, n, hv, dk, dv, kind):
+    T, big = 200, 3e4
+    change = {"same_key": dict(k=lambda t: t[:1].expand_as(t).contiguous(), a=lambda t: t * 0 - 20, b=lambda t: t * 0 + 8), "full_decay": dict(a=lambda t: t * 0 + big),
+              "one_reset": dict(a=lambda t: torch.where((torch.arange(T) % 50 == 20)[:, None], torch.full_like(t, big), t))}[kind]
+    x = inputs(T, 1, hv, dk, dv, seed=9, **change)
+    against(x, [0] * (n - 1) + [T], check=("q", "k", "v", "b"))
+
+
 def test_decay_of_minus_infinity_starts_anew():
     x = inputs(140, 1, 2, 64, 64, seed=10)
     x["a"][70] = float("inf")

@@ -11,7 +11,7 @@ HIPCC = "/opt/rocm/bin/hipcc"
 
 
 @pytest.mark.skipif(not os.path.exists(HIPCC), reason="needs hipcc")
-@pytest.mark.parametrize("name", ["dsa_delta_fwd", "dsa_delta_bwd"])
+@pytest.mark.parametrize("name", ["dsa_delta_walk", "dsa_delta_chain"])
 def test_wide_buffer_stores_have_no_scalar_offset(name, tmp_path):
     out = tmp_path / "k.s"
     subprocess.run([HIPCC, "-O3", "-std=c++17", "--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-w", "--cuda-device-only", "-S",

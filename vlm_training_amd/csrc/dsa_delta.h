@@ -103,6 +103,12 @@ __device__ __forceinline__ bf16x8 frag_t(bf16_t *t, int stride, int k0, int m0, 
 }
 __device__ __forceinline__ bf16x8 frag_n(const bf16_t *t, int stride, int r0, int c0) { return frag_n(t, stride, r0, c0, threadIdx.x & 63); }
 __device__ __forceinline__ bf16x8 frag_t(bf16_t *t, int stride, int k0, int m0) { return frag_t(t, stride, k0, m0, threadIdx.x & 63); }
+// column c0 + l%16, rows r0 + 4 (l/16) + 0..3 and 16 further
+__device__ __forceinline__ bf16x8 frag_column(bf16_t *t, int stride, int r0, int c0) {
+    const int l = threadIdx.x & 63, s = l & 15;
+    bf16_t *const p = t + (r0 + 4 * (l >> 4) + (s >> 2)) * stride + c0 + 4 * (s & 3);
+    return tr_pair((lds_u8 *)p, (lds_u8 *)(p + 16 * stride));
+}
 // the lane as a value that the compiler knows nothing about: addresses made from it inside a loop are not carried into it in registers
 __device__ __forceinline__ int fresh_lane() {
     int l = threadIdx.x & 63;
@@ -206,6 +212,18 @@ __device__ __forceinline__ bf16x8 row_frag(const bf16_t *row, int c, bool in) {
 }
 __device__ __forceinline__ f32x4 up4(u32x2 x) {
     return f32x4{__uint_as_float(x[0] << 16), __uint_as_float(x[0] & 0xffff0000u), __uint_as_float(x[1] << 16), __uint_as_float(x[1] & 0xffff0000u)};
+}
+
+// The r-th longest segment, so that no long walk begins when the others end (64 segments at most: more even out by themselves)
+__device__ __forceinline__ int delta_longest(const int32_t *cu, int N, int r) {
+    if (N > 64) return r;
+    const int lane = threadIdx.x & 63, i = min(lane, N - 1), n = lane < N ? max(cu[i + 1] - cu[i], 0) : -1;
+    int rank = 0;
+    for (int j = 0; j < N; ++j) {
+        const int o = __builtin_amdgcn_readlane(n, j);
+        rank += o > n || (o == n && j < lane);
+    }
+    return (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < N && rank == r));
 }
 
 // Which walk a workgroup takes: the column blocks of one head on one of the chip's eight dies (consecutive workgroups go round them), where they find the

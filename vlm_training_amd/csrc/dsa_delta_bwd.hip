@@ -9,226 +9,6 @@
 // dg is the sum of dG from its row on.  What a pair of rows behind t adds comes in twice with opposite signs, from one X and Z: it leaves 2^-17 of itself.
 #include "dsa_delta.h"
 
-// ---- the walk: as the forward's, from the last chunk to the first ------------------------------------------------------------------------
-// Wave w has rows 16 w .. of the chunk; P and T come transposed.  dR takes the place of dS in LDS once the first product has read that.
-template <int DK, int NC>
-__global__ __launch_bounds__(256, 2) void dsa_delta_back_kernel(DeltaArgs a) {
-    constexpr int KS = DK + 8, RS = DELTA_RS, NT = DK / 64, SS = 16 * NC * KS > 64 * RS ? 16 * NC * KS : 64 * RS;
-    __shared__ bf16_t ks[64 * KS], qs[64 * KS], sh[SS], sl[SS], os[64 * RS], oh[64 * RS], ol[64 * RS], nh[64 * RS], nl[64 * RS];
-    const dsa_delta_args &in = a.in;
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g4 = lane >> 4, row = 16 * wv + l16;
-    int64_t unit;
-    int block, slot0, chunks, s0, L;
-    if (!delta_walk_unit(blockIdx.x, a.Dvp / (16 * NC), (int64_t)in.N * in.Hv, unit, block)) return;
-    const int h = (int)(unit % in.Hv), seg = (int)(unit / in.Hv), hk = h / (in.Hv / in.Hk), dv0 = 16 * NC * block;
-    delta_segment(in.cu, in.N, seg, slot0, chunks, s0, L);
-    chunks = min(chunks, a.slots - slot0);
-    s0 = max(s0, 0);
-    f32x4 st[NT][NC];                                    // dS[dk = 16 (NT wv + t) + 4 g4 + v][dv0 + 16 c + l16]
-    const int64_t cell = ((int64_t)seg * in.Hv + h) * in.Dk * in.Dv + dv0 + l16;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int k = 16 * (NT * wv + t) + 4 * g4 + v;
-                st[t][c][v] = a.dfinal && k < in.Dk && dv0 + 16 * c + l16 < in.Dv ? a.dfinal[cell + (int64_t)k * in.Dv + 16 * c] : 0.f;
-            }
-    loads_done();
-    // offsets of this lane, in bytes
-    constexpr int LPR = DK / 8, RPI = 64 / LPR;          // lanes to a row of K or Q, rows to a load
-    const int rrow = 16 * wv + lane / LPR, rcol = lane % LPR * 8, vrow = 16 * wv + lane / 4, vcol = lane % 4 * 4 * NC;
-    const int at_k = rcol < in.Dk ? (rrow * (int)in.k_tok + rcol) * 2 : NOWHERE, at_q = rcol < in.Dk ? (rrow * (int)in.q_tok + rcol) * 2 : NOWHERE;
-    const int at_o = dv0 + vcol < in.Dv ? (vrow * in.Hv * in.Dv + dv0 + vcol) * 2 : NOWHERE;
-    const int at_t = wv < 2 ? wv * 2048 + lane * 16 : NOWHERE, at_t1 = wv * 2048 + lane * 16 + 1024;                 // (transposed rows begin at the diagonal)
-    const int at_s = (dv0 * DK + (wv * 64 + lane) * 4 * NT) * 2, at_n = a.Dvp * DK * 2 + (dv0 / 16 * 256 + wv * 64 + lane) * 16;
-    struct BackRows {
-        bf16x8 k[DK / 32], q[DK / 32], th[2], tl[2], ph[2], pl[2];
-        Piece<4 * NC> o;
-        float eg, ec, beta, rk, rq, end;
-    };
-    // where the next chunk to be fetched, and the one at hand, lie; a chunk further they are a fixed number of bytes back
-    const int64_t last = (int64_t)(slot0 + chunks - 1) * in.Hv + h, t_last = s0 + 64 * (int64_t)(chunks - 1);
-    const char *pk = (const char *)in.k + (t_last * in.k_tok + hk * in.k_head) * 2, *pq = (const char *)in.q + (t_last * in.q_tok + hk * in.q_head) * 2;
-    const char *po = (const char *)(a.dout + (t_last * in.Hv + h) * in.Dv), *pm = a.mats + last * a.mats_bytes;
-    char *pb = a.back + last * a.back_bytes, *pv = (char *)(a.dv + (t_last * in.Hv + h) * in.Dv);
-    const int64_t step_m = (int64_t)in.Hv * a.mats_bytes, step_b = (int64_t)in.Hv * a.back_bytes;
-    const int step_k = (int)in.k_tok * 128, step_q = (int)in.q_tok * 128, step_o = in.Hv * in.Dv * 128;
-    const int rows_all = min(L, in.T - s0);
-    auto fetch_q = [&](int i, BackRows &w) __attribute__((always_inline)) {
-        const int n = min(64, rows_all - 64 * i);
-        const buffer_t q = rows_buffer(pq, (int)in.q_tok, n, in.Dk), o = rows_buffer(po, in.Hv * in.Dv, n, in.Dv);
-#pragma unroll
-        for (int s = 0; s < DK / 32; ++s) w.q[s] = buf16(q, further(at_q, s * RPI * (int)in.q_tok * 2));
-        w.o = buf_piece<4 * NC>(o, at_o);
-        pq -= i > 0 ? step_q : 0;                        // (the first one is fetched again: behind a branch, waits would be for every load in flight)
-        po -= i > 0 ? step_o : 0;
-    };
-    auto fetch_k = [&](int i, BackRows &w) __attribute__((always_inline)) {
-        const buffer_t k = rows_buffer(pk, (int)in.k_tok, min(64, rows_all - 64 * i), in.Dk);
-#pragma unroll
-        for (int s = 0; s < DK / 32; ++s) w.k[s] = buf16(k, further(at_k, s * RPI * (int)in.k_tok * 2));
-        pk -= i > 0 ? step_k : 0;
-    };
-    auto fetch_p = [&](BackRows &w) __attribute__((always_inline)) {
-        const buffer_t m = buffer_of(pm, a.mats_bytes);
-        const int p = DELTA_T + (a.planes + 2) * DELTA_PLANE;
-        w.ph[0] = buf16(m, at_t, p);
-        w.pl[0] = buf16(m, at_t, p + DELTA_PLANE);
-        w.ph[1] = buf16(m, at_t1, p);
-        w.pl[1] = buf16(m, at_t1, p + DELTA_PLANE);
-    };
-    auto fetch_t = [&](int i, BackRows &w) __attribute__((always_inline)) {
-        const buffer_t m = buffer_of(pm, a.mats_bytes);
-        w.th[0] = buf16(m, at_t, DELTA_T + 2 * DELTA_PLANE);
-        w.tl[0] = buf16(m, at_t, DELTA_T + 3 * DELTA_PLANE);
-        w.th[1] = buf16(m, at_t1, DELTA_T + 2 * DELTA_PLANE);
-        w.tl[1] = buf16(m, at_t1, DELTA_T + 3 * DELTA_PLANE);
-        w.eg = buf4(m, DELTA_EG * 256 + row * 4);
-        w.ec = buf4(m, DELTA_EC * 256 + row * 4);
-        w.beta = buf4(m, DELTA_BETA * 256 + row * 4);
-        w.rk = buf4(m, DELTA_RK * 256 + row * 4);
-        w.rq = buf4(m, DELTA_RQ * 256 + row * 4);
-        w.end = buf4(m, DELTA_EG * 256 + 252);
-        pm -= i > 0 ? step_m : 0;
-    };
-    auto chunk = [&](int i, BackRows &x) __attribute__((always_inline)) {
-        const int ahead = max(i - 1, 0);
-        // dS1 as [dv][dk]; K, Q and dO as they are, and scale/|q| e^G dO
-        const buffer_t back = buffer_of(pb, a.back_bytes);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            Piece<4 * NT> all;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int at = (16 * c + l16) * KS + 16 * (NT * wv + t) + 4 * g4;
-                const u32x2 y = hi4(st[t][c]);
-                put4(sh + at, y);
-                put4(sl + at, lo4(st[t][c], y));
-                all.x[2 * t] = y[0];
-                all.x[2 * t + 1] = y[1];
-            }
-            buf_put_piece<4 * NT>(back, at_s + c * 32 * DK, all);
-        }
-#pragma unroll
-        for (int s = 0; s < DK / 32; ++s) {
-            *reinterpret_cast<bf16x8 *>(ks + (rrow + s * RPI) * KS + rcol) = x.k[s];
-            *reinterpret_cast<bf16x8 *>(qs + (rrow + s * RPI) * KS + rcol) = x.q[s];
-        }
-        put_piece<4 * NC>(os + vrow * RS + vcol, x.o);
-        fetch_q(ahead, x);
-        fetch_k(ahead, x);
-        wave_sync();
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int at = row * RS + 16 * c + 4 * g4;
-            put_split4(oh + at, ol + at, up4(*reinterpret_cast<const u32x2_any *>(os + at)) * (x.eg * x.rq));
-        }
-        __syncthreads();
-        // dN^T = e^(G_63 - G) dS1^T K^T + dO^T P
-        f32x4 r[NC];                                     // [dv = 16 c + 4 g4 + v][row]
-#pragma unroll
-        for (int c = 0; c < NC; ++c) r[c] = zero4();
-#pragma unroll
-        for (int s = 0; s < DK / 32; ++s) {
-            const bf16x8 kb = frag_n(ks, KS, 16 * wv, 32 * s);
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                r[c] = mfma16(frag_n(sl, KS, 16 * c, 32 * s), kb, r[c]);
-                r[c] = mfma16(frag_n(sh, KS, 16 * c, 32 * s), kb, r[c]);
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            r[c] *= x.ec * x.rk;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (s == 0 && wv >= 2) continue;
-                const bf16x8 o = frag_t(os, RS, 32 * s, 16 * c);
-                r[c] = mfma16(o, x.pl[s], r[c]);
-                r[c] = mfma16(o, x.ph[s], r[c]);
-            }
-            put_split4(nh + row * RS + 16 * c + 4 * g4, nl + row * RS + 16 * c + 4 * g4, r[c]);
-        }
-        fetch_p(x);
-        __syncthreads();
-        // dR^T = dN^T T
-        const buffer_t dvs = rows_buffer(pv, in.Hv * in.Dv, min(64, rows_all - 64 * i), in.Dv);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            f32x4 y = zero4();
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (s == 0 && wv >= 2) continue;
-                const bf16x8 ah = frag_t(nh, RS, 32 * s, 16 * c), al = frag_t(nl, RS, 32 * s, 16 * c);
-                y = mfma16(al, x.th[s], y);
-                y = mfma16(ah, x.tl[s], y);
-                y = mfma16(ah, x.th[s], y);
-            }
-            const int at = row * RS + 16 * c + 4 * g4;
-            const u32x2 yh = hi4(y), yl = lo4(y, yh);
-            buf_put16(back, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]});
-            put4(os + at, hi4(y * x.beta));
-            put_split4(sh + at, sl + at, y * (-x.beta * x.eg * x.rk));
-        }
-        wave_sync();
-        buf_put_piece<4 * NC>(dvs, at_o, get_piece<4 * NC>(os + vrow * RS + vcol));
-        const float end = x.end;
-        fetch_t(ahead, x);
-        __syncthreads();
-        // dS0 = e^G_63 dS1 + Q^T (..) + K^T (..)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) st[t][c] *= end;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            bf16x8 bh[NC], bl[NC], ch[NC], cl[NC];
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                bh[c] = frag_t(sh, RS, 32 * s, 16 * c);
-                bl[c] = frag_t(sl, RS, 32 * s, 16 * c);
-                ch[c] = frag_t(oh, RS, 32 * s, 16 * c);
-                cl[c] = frag_t(ol, RS, 32 * s, 16 * c);
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const bf16x8 ka = frag_t(ks, KS, 32 * s, 16 * (NT * wv + t)), qa = frag_t(qs, KS, 32 * s, 16 * (NT * wv + t));
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    st[t][c] = mfma16(ka, bl[c], st[t][c]);
-                    st[t][c] = mfma16(qa, cl[c], st[t][c]);
-                    st[t][c] = mfma16(ka, bh[c], st[t][c]);
-                    st[t][c] = mfma16(qa, ch[c], st[t][c]);
-                }
-            }
-        }
-        pb -= step_b;
-        pv -= step_o;
-        __syncthreads();
-    };
-    BackRows x;
-    if (chunks > 0) {
-        fetch_q(chunks - 1, x);
-        fetch_k(chunks - 1, x);
-        fetch_p(x);
-        fetch_t(chunks - 1, x);
-        for (int i = chunks - 1; i >= 0; --i) chunk(i, x);
-    }
-    if (a.dinitial) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const int k = 16 * (NT * wv + t) + 4 * g4 + v;
-                    if (k < in.Dk && dv0 + 16 * c + l16 < in.Dv) a.dinitial[cell + (int64_t)k * in.Dv + 16 * c] = st[t][c][v];
-                }
-    }
-}
-
 // ---- everything that needs one chunk alone: one workgroup per chunk and key head, its value heads in turn --------------------------------
 // Wave w has rows 16 w ..; N, X and Z go into their products as hi + lo (where keys repeat, a row of X K is a sum that cancels).  Everything is formed transposed (lane: its row, four neighbouring columns), so that a row's factor is one register and its
 // sums stay in four lanes.  dq and dk of the key head are summed over its value heads in registers, in that order.  The columns of the values are taken 64 at
@@ -318,11 +98,11 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 put4(to, u32x2{tn[e][0], tn[e][1]});
                 put4(to + 64 * TS, u32x2{tn[e][2], tn[e][3]});
             }
-            // the state's pieces of four: 16 columns, wave, lane, NS of them
-            constexpr int NS = DK / 64;
+            // the state's pieces: 16 columns, 32 rows, lane, two fours 16 rows apart
             auto place = [&](int e, int half) __attribute__((always_inline)) {
-                const int piece = (tid + 256 * e) * 2 + half, l = piece / NS % 64;
-                return ss + (piece / (NS * 256) * 16 + l % 16) * KS + (piece / (NS * 64) % 4 * NS + piece % NS) * 16 + l / 16 * 4;
+                constexpr int KB = DK / 32;
+                const int piece = tid + 256 * e, l = piece % 64;
+                return ss + (piece / (KB * 64) * 16 + l % 16) * KS + piece / 64 % KB * 32 + half * 16 + l / 16 * 4;
             };
 #pragma unroll
             for (int e = 0; e < DK / 32; ++e) {
@@ -528,14 +308,10 @@ __global__ __launch_bounds__(256) void dsa_delta_param_kernel(DeltaArgs a) {
     if (threadIdx.x == 0) store_any(which ? a.ddt : a.da_log, h, a.in.param_f32, (red[0] + red[1]) + (red[2] + red[3]));
 }
 
-extern "C" int dsa_delta_columns(const DeltaArgs *a);
+extern "C" void dsa_launch_delta_back(const DeltaArgs *a, hipStream_t stream);
 extern "C" hipError_t dsa_launch_delta_bwd(const DeltaArgs *a, hipStream_t stream) {
-    const int nc = dsa_delta_columns(a);
-    const dim3 walks((unsigned)(((int64_t)a->in.N * a->in.Hv + 7) / 8 * 8 * (a->Dvp / (16 * nc)))), grid(a->slots, a->in.Hk);
-    if (a->Dkp == 64 && nc == 1) hipLaunchKernelGGL((dsa_delta_back_kernel<64, 1>), walks, dim3(256), 0, stream, *a);
-    else if (a->Dkp == 64) hipLaunchKernelGGL((dsa_delta_back_kernel<64, 2>), walks, dim3(256), 0, stream, *a);
-    else if (nc == 1) hipLaunchKernelGGL((dsa_delta_back_kernel<128, 1>), walks, dim3(256), 0, stream, *a);
-    else hipLaunchKernelGGL((dsa_delta_back_kernel<128, 2>), walks, dim3(256), 0, stream, *a);
+    const dim3 grid(a->slots, a->in.Hk);
+    dsa_launch_delta_back(a, stream);
     if (a->Dkp == 64 && a->Dvp == 64) hipLaunchKernelGGL((dsa_delta_grad_kernel<64, 64>), grid, dim3(256), 0, stream, *a);
     else if (a->Dkp == 64) hipLaunchKernelGGL((dsa_delta_grad_kernel<64, 128>), grid, dim3(256), 0, stream, *a);
     else if (a->Dvp == 64) hipLaunchKernelGGL((dsa_delta_grad_kernel<128, 64>), grid, dim3(256), 0, stream, *a);

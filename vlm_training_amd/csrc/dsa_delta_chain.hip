@@ -1,0 +1,464 @@
+// Gated delta rule: the walks of the state where there are few of them - a workgroup for 16 or 32 columns, its waves side by side over the rows - so that a chunk's
+// chain of products is short.  (dsa_delta_walk.hip has the walks where there are many, and the rule between them.)
+//
+// Wave w has rows 16 w .. of the chunk and rows Dk/4 w .. of the state, which stay in registers (fp32) from the first chunk to the last.  A chunk is a chain
+// of three products over the same columns - K S0 (and Q S0), T R, K^T N (and P N) - so their results go through LDS to the other waves, a barrier each; they are
+// formed transposed (lane: its row, four neighbouring columns), which makes every factor of a row one register and every access 8 or 16 bytes.
+// Rows of K, Q, T and P are needed by their own wave alone (K by all of them as K^T): T and P come as fragments straight into registers, rows of K, Q and V
+// 16 bytes a lane through the wave's own part of LDS.  The next chunk's loads go out as soon as a register has been read.
+#include "dsa_delta.h"
+
+template <int DK, int NC> struct ChainRows {
+    bf16x8 k[DK / 32], q[DK / 32], th[2], tl[2], ph[2], pl[2];
+    Piece<4 * NC> v;
+    float eg, ec, beta, rk, rq, end;
+};
+template <int DK, int NC, bool SAVE>
+__global__ __launch_bounds__(256, 2) void dsa_delta_chain_kernel(DeltaArgs a) {
+    constexpr int KS = DK + 8, RS = DELTA_RS, NT = DK / 64;
+    __shared__ bf16_t ks[2][64 * KS], sh[16 * NC * KS], sl[16 * NC * KS], rh[64 * RS], rl[64 * RS], pool[4 * 64 * RS];
+    // N and e^(G_63 - G)/|k| N as hi, lo; Q before they are there
+    bf16_t *const nh = pool, *const nl = pool + 64 * RS, *const mh = pool + 128 * RS, *const ml = pool + 192 * RS, *const qt = pool;
+    static_assert(KS <= 4 * RS, "Q lies in N's place");
+    const dsa_delta_args &in = a.in;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g4 = lane >> 4, row = 16 * wv + l16;
+    int64_t unit;
+    int block, slot0, chunks, s0, L;
+    if (!delta_walk_unit(blockIdx.x, a.Dvp / (16 * NC), (int64_t)in.N * in.Hv, unit, block)) return;
+    const int h = (int)(unit % in.Hv), seg = delta_longest(in.cu, in.N, (int)(unit / in.Hv)), hk = h / (in.Hv / in.Hk), dv0 = 16 * NC * block;
+    delta_segment(in.cu, in.N, seg, slot0, chunks, s0, L);
+    chunks = min(chunks, a.slots - slot0);
+    s0 = max(s0, 0);
+    f32x4 st[NT][NC];                                    // S[dk = 16 (NT wv + t) + 4 g4 + v][dv0 + 16 c + l16]
+    const int64_t cell = ((int64_t)seg * in.Hv + h) * in.Dk * in.Dv + dv0 + l16;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const int k = 16 * (NT * wv + t) + 4 * g4 + v;
+                st[t][c][v] = a.initial && k < in.Dk && dv0 + 16 * c + l16 < in.Dv ? a.initial[cell + (int64_t)k * in.Dv + 16 * c] : 0.f;
+            }
+    loads_done();
+    // offsets of this lane, in bytes
+    constexpr int LPR = DK / 8, RPI = 64 / LPR;          // lanes to a row of K or Q, rows to a load
+    const int rrow = 16 * wv + lane / LPR, rcol = lane % LPR * 8, vrow = 16 * wv + lane / 4, vcol = lane % 4 * 4 * NC;
+    const int at_k = rcol < in.Dk ? (rrow * (int)in.k_tok + rcol) * 2 : NOWHERE, at_q = rcol < in.Dk ? (rrow * (int)in.q_tok + rcol) * 2 : NOWHERE;
+    const int at_v = dv0 + vcol < in.Dv ? (vrow * (int)in.v_tok + dv0 + vcol) * 2 : NOWHERE, at_o = dv0 + vcol < in.Dv ? (vrow * in.Hv * in.Dv + dv0 + vcol) * 2 : NOWHERE;
+    const int at_t = wv * 2048 + lane * 16, at_t1 = wv >= 2 ? at_t + 1024 : NOWHERE;       // (rows of T and P end at the diagonal)
+    const int at_s = dv0 * DK * 2 + (NT == 2 ? (wv * 64 + lane) * 16 : (wv / 2 * 64 + lane) * 16 + wv % 2 * 8), at_n = a.Dvp * DK * 2 + (dv0 / 16 * 256 + wv * 64 + lane) * 16;
+    // where the next chunk to be fetched, and the one at hand, lie; a chunk further they are a fixed number of bytes on
+    const int64_t first = (int64_t)slot0 * in.Hv + h;
+    const char *pk = (const char *)in.k + (s0 * in.k_tok + hk * in.k_head) * 2, *pq = (const char *)in.q + (s0 * in.q_tok + hk * in.q_head) * 2;
+    const char *pv = (const char *)in.v + (s0 * in.v_tok + h * in.v_head) * 2, *pm = a.mats + first * a.mats_bytes;
+    char *ps = a.saved + first * a.saved_bytes, *po = (char *)(a.out + ((int64_t)s0 * in.Hv + h) * in.Dv);
+    const int64_t step_m = (int64_t)in.Hv * a.mats_bytes, step_s = (int64_t)in.Hv * a.saved_bytes;
+    const int step_k = (int)in.k_tok * 128, step_q = (int)in.q_tok * 128, step_v = (int)in.v_tok * 128, step_o = in.Hv * in.Dv * 128;
+    const int rows_all = min(L, in.T - s0);              // (one chunk after the other takes its 64 of them)
+    typedef ChainRows<DK, NC> Rows;
+    auto fetch_rows = [&](int i, Rows &w) __attribute__((always_inline)) {
+        const int n = min(64, rows_all - 64 * i);
+        const buffer_t k = rows_buffer(pk, (int)in.k_tok, n, in.Dk), q = rows_buffer(pq, (int)in.q_tok, n, in.Dk), v = rows_buffer(pv, (int)in.v_tok, n, in.Dv);
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) {              
+            w.k[s] = buf16(k, further(at_k, s * RPI * (int)in.k_tok * 2));
+            w.q[s] = buf16(q, further(at_q, s * RPI * (int)in.q_tok * 2));
+        }
+        w.v = buf_piece<4 * NC>(v, at_v);
+        const bool on = i + 1 < chunks;                  // (the last one is fetched again: behind a branch, waits would be for every load in flight)
+        pk += on ? step_k : 0;
+        pq += on ? step_q : 0;
+        pv += on ? step_v : 0;
+    };
+    auto fetch_t = [&](Rows &w) __attribute__((always_inline)) {
+        const buffer_t m = buffer_of(pm, a.mats_bytes);
+        w.th[0] = buf16(m, at_t, DELTA_T);
+        w.tl[0] = buf16(m, at_t, DELTA_T + DELTA_PLANE);
+        w.th[1] = buf16(m, at_t1, DELTA_T);
+        w.tl[1] = buf16(m, at_t1, DELTA_T + DELTA_PLANE);
+    };
+    auto fetch_p = [&](int i, Rows &w) __attribute__((always_inline)) {
+        const buffer_t m = buffer_of(pm, a.mats_bytes);
+        const int p = DELTA_T + a.planes * DELTA_PLANE;
+        w.ph[0] = buf16(m, at_t, p);
+        w.pl[0] = buf16(m, at_t, p + DELTA_PLANE);
+        w.ph[1] = buf16(m, at_t1, p);
+        w.pl[1] = buf16(m, at_t1, p + DELTA_PLANE);
+        w.eg = buf4(m, DELTA_EG * 256 + row * 4);
+        w.ec = buf4(m, DELTA_EC * 256 + row * 4);
+        w.beta = buf4(m, DELTA_BETA * 256 + row * 4);
+        w.rk = buf4(m, DELTA_RK * 256 + row * 4);
+        w.rq = buf4(m, DELTA_RQ * 256 + row * 4);
+        w.end = buf4(m, DELTA_EG * 256 + 252);
+        pm += i + 1 < chunks ? step_m : 0;
+    };
+    auto chunk = [&](int i, Rows &x, bf16_t *kt) __attribute__((always_inline)) {
+        const int ahead = min(i + 1, chunks - 1);
+        // S0 as [dv][dk], K as it is
+        const buffer_t save = buffer_of(ps, a.saved_bytes);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            Piece<4 * NT> all;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int at = (16 * c + l16) * KS + 16 * (NT * wv + t) + 4 * g4;
+                const u32x2 y = hi4(st[t][c]);
+                put4(sh + at, y);
+                put4(sl + at, lo4(st[t][c], y));
+                all.x[2 * t] = y[0];
+                all.x[2 * t + 1] = y[1];
+            }
+            if (SAVE) buf_put_piece<4 * NT>(save, at_s + c * 32 * DK, all);
+        }
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) *reinterpret_cast<bf16x8 *>(kt + (rrow + s * RPI) * KS + rcol) = x.k[s];
+        __syncthreads();
+        // Q and V: the wave's own rows
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) *reinterpret_cast<bf16x8 *>(qt + (rrow + s * RPI) * KS + rcol) = x.q[s];
+        put_piece<4 * NC>(rh + vrow * RS + vcol, x.v);
+        fetch_rows(ahead, x);
+        wave_sync();
+        f32x4 o[NC], r[NC];                              // [dv = 16 c + 4 g4 + v][row]
+#pragma unroll
+        for (int c = 0; c < NC; ++c) o[c] = r[c] = zero4();
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) {
+            const bf16x8 kb = frag_n(kt, KS, 16 * wv, 32 * s), qb = frag_n(qt, KS, 16 * wv, 32 * s);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const bf16x8 ah = frag_n(sh, KS, 16 * c, 32 * s), al = frag_n(sl, KS, 16 * c, 32 * s);
+                r[c] = mfma16(al, kb, r[c]);
+                o[c] = mfma16(al, qb, o[c]);
+                r[c] = mfma16(ah, kb, r[c]);
+                o[c] = mfma16(ah, qb, o[c]);
+            }
+        }
+        const float f = x.eg * x.rk;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int at = row * RS + 16 * c + 4 * g4;
+            put_split4(rh + at, rl + at, (up4(*reinterpret_cast<const u32x2_any *>(rh + at)) - r[c] * f) * x.beta);
+        }
+        __syncthreads();
+        // N^T = R^T T^T
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            f32x4 y = zero4();
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s == 1 && wv < 2) continue;
+                const bf16x8 ah = frag_column(rh, RS, 32 * s, 16 * c), al = frag_column(rl, RS, 32 * s, 16 * c);
+                y = mfma16(al, x.th[s], y);
+                y = mfma16(ah, x.tl[s], y);
+                y = mfma16(ah, x.th[s], y);
+            }
+            const int at = row * RS + 16 * c + 4 * g4;
+            const u32x2 yh = hi4(y), yl = lo4(y, yh);
+            put4(nh + at, yh);
+            put4(nl + at, yl);
+            put_split4(mh + at, ml + at, y * (x.ec * x.rk));
+            if (SAVE) buf_put16(save, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]});
+        }
+        fetch_t(x);
+        __syncthreads();
+        // S1 = e^G_63 S0 + K^T e^(G_63 - G) N
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) st[t][c] *= x.end;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            bf16x8 bh[NC], bl[NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                bh[c] = frag_t(mh, RS, 32 * s, 16 * c);
+                bl[c] = frag_t(ml, RS, 32 * s, 16 * c);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const bf16x8 ka = frag_t(kt, KS, 32 * s, 16 * (NT * wv + t));
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    st[t][c] = mfma16(ka, bl[c], st[t][c]);
+                    st[t][c] = mfma16(ka, bh[c], st[t][c]);
+                }
+            }
+        }
+        // O^T = scale e^G S0^T Q^T + N^T P^T
+        const buffer_t out = rows_buffer(po, in.Hv * in.Dv, min(64, rows_all - 64 * i), in.Dv);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            o[c] *= x.eg * x.rq;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s == 1 && wv < 2) continue;
+                const bf16x8 ah = frag_column(nh, RS, 32 * s, 16 * c), al = frag_column(nl, RS, 32 * s, 16 * c);
+                o[c] = mfma16(al, x.ph[s], o[c]);
+                o[c] = mfma16(ah, x.pl[s], o[c]);
+                o[c] = mfma16(ah, x.ph[s], o[c]);
+            }
+            put4(rh + row * RS + 16 * c + 4 * g4, hi4(o[c]));
+        }
+        wave_sync();
+        buf_put_piece<4 * NC>(out, at_o, get_piece<4 * NC>(rh + vrow * RS + vcol));
+        fetch_p(ahead, x);
+        po += step_o;
+        if (SAVE) ps += step_s;
+    };
+    Rows x;
+    if (chunks > 0) {
+        fetch_rows(0, x);
+        fetch_t(x);
+        fetch_p(0, x);
+        for (int i = 0; i < chunks; ++i) chunk(i, x, ks[i & 1]);
+    }
+    if (a.final) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const int k = 16 * (NT * wv + t) + 4 * g4 + v;
+                    if (k < in.Dk && dv0 + 16 * c + l16 < in.Dv) a.final[cell + (int64_t)k * in.Dv + 16 * c] = st[t][c][v];
+                }
+    }
+}
+
+// Backwards: P and T come transposed.  dR takes the place of dS in LDS once the first product has read that.
+template <int DK, int NC>
+__global__ __launch_bounds__(256, 2) void dsa_delta_chain_back_kernel(DeltaArgs a) {
+    constexpr int KS = DK + 8, RS = DELTA_RS, NT = DK / 64, SS = 16 * NC * KS > 64 * RS ? 16 * NC * KS : 64 * RS;
+    __shared__ bf16_t ks[64 * KS], qs[64 * KS], sh[SS], sl[SS], os[64 * RS], oh[64 * RS], ol[64 * RS], nh[64 * RS], nl[64 * RS];
+    const dsa_delta_args &in = a.in;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g4 = lane >> 4, row = 16 * wv + l16;
+    int64_t unit;
+    int block, slot0, chunks, s0, L;
+    if (!delta_walk_unit(blockIdx.x, a.Dvp / (16 * NC), (int64_t)in.N * in.Hv, unit, block)) return;
+    const int h = (int)(unit % in.Hv), seg = delta_longest(in.cu, in.N, (int)(unit / in.Hv)), hk = h / (in.Hv / in.Hk), dv0 = 16 * NC * block;
+    delta_segment(in.cu, in.N, seg, slot0, chunks, s0, L);
+    chunks = min(chunks, a.slots - slot0);
+    s0 = max(s0, 0);
+    f32x4 st[NT][NC];                                    // dS[dk = 16 (NT wv + t) + 4 g4 + v][dv0 + 16 c + l16]
+    const int64_t cell = ((int64_t)seg * in.Hv + h) * in.Dk * in.Dv + dv0 + l16;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const int k = 16 * (NT * wv + t) + 4 * g4 + v;
+                st[t][c][v] = a.dfinal && k < in.Dk && dv0 + 16 * c + l16 < in.Dv ? a.dfinal[cell + (int64_t)k * in.Dv + 16 * c] : 0.f;
+            }
+    loads_done();
+    // offsets of this lane, in bytes
+    constexpr int LPR = DK / 8, RPI = 64 / LPR;          // lanes to a row of K or Q, rows to a load
+    const int rrow = 16 * wv + lane / LPR, rcol = lane % LPR * 8, vrow = 16 * wv + lane / 4, vcol = lane % 4 * 4 * NC;
+    const int at_k = rcol < in.Dk ? (rrow * (int)in.k_tok + rcol) * 2 : NOWHERE, at_q = rcol < in.Dk ? (rrow * (int)in.q_tok + rcol) * 2 : NOWHERE;
+    const int at_o = dv0 + vcol < in.Dv ? (vrow * in.Hv * in.Dv + dv0 + vcol) * 2 : NOWHERE;
+    const int at_t = wv < 2 ? wv * 2048 + lane * 16 : NOWHERE, at_t1 = wv * 2048 + lane * 16 + 1024;                 // (transposed rows begin at the diagonal)
+    const int at_s = dv0 * DK * 2 + (NT == 2 ? (wv * 64 + lane) * 16 : (wv / 2 * 64 + lane) * 16 + wv % 2 * 8), at_n = a.Dvp * DK * 2 + (dv0 / 16 * 256 + wv * 64 + lane) * 16;
+    struct BackRows {
+        bf16x8 k[DK / 32], q[DK / 32], th[2], tl[2], ph[2], pl[2];
+        Piece<4 * NC> o;
+        float eg, ec, beta, rk, rq, end;
+    };
+    // where the next chunk to be fetched, and the one at hand, lie; a chunk further they are a fixed number of bytes back
+    const int64_t last = (int64_t)(slot0 + chunks - 1) * in.Hv + h, t_last = s0 + 64 * (int64_t)(chunks - 1);
+    const char *pk = (const char *)in.k + (t_last * in.k_tok + hk * in.k_head) * 2, *pq = (const char *)in.q + (t_last * in.q_tok + hk * in.q_head) * 2;
+    const char *po = (const char *)(a.dout + (t_last * in.Hv + h) * in.Dv), *pm = a.mats + last * a.mats_bytes;
+    char *pb = a.back + last * a.back_bytes, *pv = (char *)(a.dv + (t_last * in.Hv + h) * in.Dv);
+    const int64_t step_m = (int64_t)in.Hv * a.mats_bytes, step_b = (int64_t)in.Hv * a.back_bytes;
+    const int step_k = (int)in.k_tok * 128, step_q = (int)in.q_tok * 128, step_o = in.Hv * in.Dv * 128;
+    const int rows_all = min(L, in.T - s0);
+    auto fetch_q = [&](int i, BackRows &w) __attribute__((always_inline)) {
+        const int n = min(64, rows_all - 64 * i);
+        const buffer_t q = rows_buffer(pq, (int)in.q_tok, n, in.Dk), o = rows_buffer(po, in.Hv * in.Dv, n, in.Dv);
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) w.q[s] = buf16(q, further(at_q, s * RPI * (int)in.q_tok * 2));
+        w.o = buf_piece<4 * NC>(o, at_o);
+        pq -= i > 0 ? step_q : 0;                        // (the first one is fetched again: behind a branch, waits would be for every load in flight)
+        po -= i > 0 ? step_o : 0;
+    };
+    auto fetch_k = [&](int i, BackRows &w) __attribute__((always_inline)) {
+        const buffer_t k = rows_buffer(pk, (int)in.k_tok, min(64, rows_all - 64 * i), in.Dk);
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) w.k[s] = buf16(k, further(at_k, s * RPI * (int)in.k_tok * 2));
+        pk -= i > 0 ? step_k : 0;
+    };
+    auto fetch_p = [&](BackRows &w) __attribute__((always_inline)) {
+        const buffer_t m = buffer_of(pm, a.mats_bytes);
+        const int p = DELTA_T + (a.planes + 2) * DELTA_PLANE;
+        w.ph[0] = buf16(m, at_t, p);
+        w.pl[0] = buf16(m, at_t, p + DELTA_PLANE);
+        w.ph[1] = buf16(m, at_t1, p);
+        w.pl[1] = buf16(m, at_t1, p + DELTA_PLANE);
+    };
+    auto fetch_t = [&](int i, BackRows &w) __attribute__((always_inline)) {
+        const buffer_t m = buffer_of(pm, a.mats_bytes);
+        w.th[0] = buf16(m, at_t, DELTA_T + 2 * DELTA_PLANE);
+        w.tl[0] = buf16(m, at_t, DELTA_T + 3 * DELTA_PLANE);
+        w.th[1] = buf16(m, at_t1, DELTA_T + 2 * DELTA_PLANE);
+        w.tl[1] = buf16(m, at_t1, DELTA_T + 3 * DELTA_PLANE);
+        w.eg = buf4(m, DELTA_EG * 256 + row * 4);
+        w.ec = buf4(m, DELTA_EC * 256 + row * 4);
+        w.beta = buf4(m, DELTA_BETA * 256 + row * 4);
+        w.rk = buf4(m, DELTA_RK * 256 + row * 4);
+        w.rq = buf4(m, DELTA_RQ * 256 + row * 4);
+        w.end = buf4(m, DELTA_EG * 256 + 252);
+        pm -= i > 0 ? step_m : 0;
+    };
+    auto chunk = [&](int i, BackRows &x) __attribute__((always_inline)) {
+        const int ahead = max(i - 1, 0);
+        // dS1 as [dv][dk]; K, Q and dO as they are, and scale/|q| e^G dO
+        const buffer_t back = buffer_of(pb, a.back_bytes);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            Piece<4 * NT> all;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int at = (16 * c + l16) * KS + 16 * (NT * wv + t) + 4 * g4;
+                const u32x2 y = hi4(st[t][c]);
+                put4(sh + at, y);
+                put4(sl + at, lo4(st[t][c], y));
+                all.x[2 * t] = y[0];
+                all.x[2 * t + 1] = y[1];
+            }
+            buf_put_piece<4 * NT>(back, at_s + c * 32 * DK, all);
+        }
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) {
+            *reinterpret_cast<bf16x8 *>(ks + (rrow + s * RPI) * KS + rcol) = x.k[s];
+            *reinterpret_cast<bf16x8 *>(qs + (rrow + s * RPI) * KS + rcol) = x.q[s];
+        }
+        put_piece<4 * NC>(os + vrow * RS + vcol, x.o);
+        fetch_q(ahead, x);
+        fetch_k(ahead, x);
+        wave_sync();
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int at = row * RS + 16 * c + 4 * g4;
+            put_split4(oh + at, ol + at, up4(*reinterpret_cast<const u32x2_any *>(os + at)) * (x.eg * x.rq));
+        }
+        __syncthreads();
+        // dN^T = e^(G_63 - G) dS1^T K^T + dO^T P
+        f32x4 r[NC];                                     // [dv = 16 c + 4 g4 + v][row]
+#pragma unroll
+        for (int c = 0; c < NC; ++c) r[c] = zero4();
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) {
+            const bf16x8 kb = frag_n(ks, KS, 16 * wv, 32 * s);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                r[c] = mfma16(frag_n(sl, KS, 16 * c, 32 * s), kb, r[c]);
+                r[c] = mfma16(frag_n(sh, KS, 16 * c, 32 * s), kb, r[c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            r[c] *= x.ec * x.rk;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s == 0 && wv >= 2) continue;
+                const bf16x8 o = frag_column(os, RS, 32 * s, 16 * c);
+                r[c] = mfma16(o, x.pl[s], r[c]);
+                r[c] = mfma16(o, x.ph[s], r[c]);
+            }
+            put_split4(nh + row * RS + 16 * c + 4 * g4, nl + row * RS + 16 * c + 4 * g4, r[c]);
+        }
+        fetch_p(x);
+        __syncthreads();
+        // dR^T = dN^T T
+        const buffer_t dvs = rows_buffer(pv, in.Hv * in.Dv, min(64, rows_all - 64 * i), in.Dv);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            f32x4 y = zero4();
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s == 0 && wv >= 2) continue;
+                const bf16x8 ah = frag_column(nh, RS, 32 * s, 16 * c), al = frag_column(nl, RS, 32 * s, 16 * c);
+                y = mfma16(al, x.th[s], y);
+                y = mfma16(ah, x.tl[s], y);
+                y = mfma16(ah, x.th[s], y);
+            }
+            const int at = row * RS + 16 * c + 4 * g4;
+            const u32x2 yh = hi4(y), yl = lo4(y, yh);
+            buf_put16(back, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]});
+            put4(os + at, hi4(y * x.beta));
+            put_split4(sh + at, sl + at, y * (-x.beta * x.eg * x.rk));
+        }
+        wave_sync();
+        buf_put_piece<4 * NC>(dvs, at_o, get_piece<4 * NC>(os + vrow * RS + vcol));
+        const float end = x.end;
+        fetch_t(ahead, x);
+        __syncthreads();
+        // dS0 = e^G_63 dS1 + Q^T (..) + K^T (..)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) st[t][c] *= end;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            bf16x8 bh[NC], bl[NC], ch[NC], cl[NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                bh[c] = frag_t(sh, RS, 32 * s, 16 * c);
+                bl[c] = frag_t(sl, RS, 32 * s, 16 * c);
+                ch[c] = frag_t(oh, RS, 32 * s, 16 * c);
+                cl[c] = frag_t(ol, RS, 32 * s, 16 * c);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const bf16x8 ka = frag_t(ks, KS, 32 * s, 16 * (NT * wv + t)), qa = frag_t(qs, KS, 32 * s, 16 * (NT * wv + t));
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    st[t][c] = mfma16(ka, bl[c], st[t][c]);
+                    st[t][c] = mfma16(qa, cl[c], st[t][c]);
+                    st[t][c] = mfma16(ka, bh[c], st[t][c]);
+                    st[t][c] = mfma16(qa, ch[c], st[t][c]);
+                }
+            }
+        }
+        pb -= step_b;
+        pv -= step_o;
+        __syncthreads();
+    };
+    BackRows x;
+    if (chunks > 0) {
+        fetch_q(chunks - 1, x);
+        fetch_k(chunks - 1, x);
+        fetch_p(x);
+        fetch_t(chunks - 1, x);
+        for (int i = chunks - 1; i >= 0; --i) chunk(i, x);
+    }
+    if (a.dinitial) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const int k = 16 * (NT * wv + t) + 4 * g4 + v;
+                    if (k < in.Dk && dv0 + 16 * c + l16 < in.Dv) a.dinitial[cell + (int64_t)k * in.Dv + 16 * c] = st[t][c][v];
+                }
+    }
+}
+
+#define CHAIN_BY_SIZE(LAUNCH)                                \
+    if (a->Dkp == 64 && nc == 1) { LAUNCH(64, 1) }           \
+    else if (a->Dkp == 64) { LAUNCH(64, 2) }                 \
+    else if (nc == 1) { LAUNCH(128, 1) }                     \
+    else { LAUNCH(128, 2) }
+static dim3 delta_chains(const DeltaArgs *a, int nc) { return dim3((unsigned)(((int64_t)a->in.N * a->in.Hv + 7) / 8 * 8 * (a->Dvp / (16 * nc)))); }
+extern "C" void dsa_launch_delta_chain(const DeltaArgs *a, int nc, int save, hipStream_t stream) {
+#define DELTA_CHAIN(DK, NC)                                                                                                                \
+    if (save) hipLaunchKernelGGL((dsa_delta_chain_kernel<DK, NC, true>), delta_chains(a, NC), dim3(256), 0, stream, *a);                    \
+    else hipLaunchKernelGGL((dsa_delta_chain_kernel<DK, NC, false>), delta_chains(a, NC), dim3(256), 0, stream, *a);
+    CHAIN_BY_SIZE(DELTA_CHAIN)
+}
+extern "C" void dsa_launch_delta_chain_back(const DeltaArgs *a, int nc, hipStream_t stream) {
+#define DELTA_CHAIN_BACK(DK, NC) hipLaunchKernelGGL((dsa_delta_chain_back_kernel<DK, NC>), delta_chains(a, NC), dim3(256), 0, stream, *a);
+    CHAIN_BY_SIZE(DELTA_CHAIN_BACK)
+}
