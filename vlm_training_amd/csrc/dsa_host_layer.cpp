@@ -368,11 +368,13 @@ variable_list residual_rms_norm(const Tensor &x, const Tensor &y, const Tensor &
         need_gpu(*gate);
         same_device(x, *gate, "gate");
         TORCH_CHECK_VALUE(gate->sizes() == x.sizes() && gate->scalar_type() == at::kBFloat16, "gate must be bf16 and have the shape of x");
-        rows_of_gate = gate->reshape({T, C});
+        rows_of_gate = gate->dim() == 2 ? *gate : gate->reshape({T, C});
     }
     const c10::OptionalDeviceGuard guard(x.device());
-    variable_list out = ResidualNormNode::apply(x.reshape({T, C}), y.reshape({T, C}), weight, post, rows_of_gate, scale, eps, offset);
-    if (x.dim() != 2)
+    // (rows as they are where they are rows: a view is a node of its own, 3 us each way)
+    const bool flat = x.dim() == 2;
+    variable_list out = ResidualNormNode::apply(flat ? x : x.reshape({T, C}), flat ? y : y.reshape({T, C}), weight, post, rows_of_gate, scale, eps, offset);
+    if (!flat)
         for (Tensor &t : out) t = t.view(x.sizes());
     return out;
 }
