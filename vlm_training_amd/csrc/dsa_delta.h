@@ -24,9 +24,11 @@ struct DeltaArgs {
     int slots, Dkp, Dvp;               // chunks at the most; head dims padded to 64 or 128
     // A chunk of a value head ("cell", slots x Hv of them) has a block of each of three arrays.
     // mats: the rows' factors (DELTA_ROWS x 64 floats), then planes of 64 x 64 bf16: T as hi, lo and, where a backward follows, transposed hi, lo; P the same.
-    //       A plane lies in the order of its fragments: wave, half of the columns, lane, eight elements.
+    //       A plane lies in blocks of 16 rows and 32 columns, lane l's eight elements together: row l%16, columns 4 (l/16) + 0..3 and 16 further.  Blocks that are
+    //       all zeros (the upper right quarter, of a transposed one the lower left) are neither written nor read.
     // saved, for the backward: S0 (Dvp x Dkp), N as hi, lo (Dvp x 64 x 2);  back, the backward's own: dS1, dR as hi, lo.  They lie as the walks' lanes
-    //       hold them: 16 columns of the values, wave, lane, its elements (state: Dkp/16 of them, N and dR: four as hi, four as lo).
+    //       have them, 16 columns of the values together: a state 32 rows at a time, lane l's rows 4 (l/16) + 0..3 and 16 further of column l%16; N and dR 16 rows at
+    //       a time, lane l's row l%16, columns 4 (l/16) + 0..3 as hi, then as lo.
     // (A quad of lanes that reads or writes four rows takes four times as long as one that stays in one: with rows of T, P, S and N in row order, K and
     // Q as fragments straight from their rows and 8-byte stores, the walk of 16 384 tokens took 0.62 ms.)
     char *mats, *saved, *back;
@@ -173,7 +175,6 @@ __device__ __forceinline__ buffer_t buffer_of(const void *p, int bytes) {
 __device__ __forceinline__ buffer_t rows_buffer(const char *p, int tok, int rows, int width) { return buffer_of(p, rows > 0 ? ((rows - 1) * tok + width) * 2 : 0); }
 // `at`: a constant that the end is not checked for
 __device__ __forceinline__ bf16x8 buf16(buffer_t b, int off, int at = 0) { return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(b, off, at, 0)); }
-__device__ __forceinline__ u32x2 buf8(buffer_t b, int off) { return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0)); }
 __device__ __forceinline__ float buf4(buffer_t b, int off) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, off, 0, 0)); }
 __device__ __forceinline__ void buf_put8(buffer_t b, int off, u32x2 x) { __builtin_amdgcn_raw_buffer_store_b64(x, b, off, 0, 0); }
 // every load so far has arrived: in front of a loop whose loads are waited for by count (what is in flight there from before would be counted in with them)

@@ -1,4 +1,5 @@
-// Gated delta rule, backward.  With N = T R, R = beta (V - e^G K S0) of a chunk (dsa_delta.h), from its last chunk to its first:
+// Gated delta rule, backward: what the walks (dsa_delta_walk.hip, dsa_delta_chain.hip) leave to do.
+// With N = T R, R = beta (V - e^G K S0) of a chunk (dsa_delta.h), from its last chunk to its first:
 //     dN = P^T dO + e^(G_63 - G) K dS1      dR = T^T dN      dS0 = e^G_63 dS1 + scale Q^T e^G dO - K^T beta e^G dR
 // (the walk, which leaves dS1 and dR of every chunk and dV = beta dR), then all chunks at once
 //     dP = dO N^T   dA = -dR N^T   X = scale E dP   Z = beta E dA (below the diagonal)
@@ -10,9 +11,13 @@
 #include "dsa_delta.h"
 
 // ---- everything that needs one chunk alone: one workgroup per chunk and key head, its value heads in turn --------------------------------
-// Wave w has rows 16 w ..; N, X and Z go into their products as hi + lo (where keys repeat, a row of X K is a sum that cancels).  Everything is formed transposed (lane: its row, four neighbouring columns), so that a row's factor is one register and its
-// sums stay in four lanes.  dq and dk of the key head are summed over its value heads in registers, in that order.  The columns of the values are taken 64 at
-// a time, so that two workgroups share a compute unit's LDS and one's loads pass under the other's products; dO and dR are read by their own rows' wave alone.
+// Wave w has rows 16 w ..; N, X and Z go into their products as hi + lo (where keys repeat, a row of X K is a sum that cancels).  Everything is formed
+// transposed (lane: its row, four neighbouring columns), so that a row's factor is one register and its sums stay in four lanes.  dq and dk of the key head
+// are summed over its value heads in registers, in that order.  The columns of the values are taken 64 at a time, so that two workgroups share a compute
+// unit's LDS and one's loads pass under the other's products; dO and dR are read by their own rows' wave alone.
+// 16 384 rows of 32 heads: 0.42 ms for 1.2 GB.  Neither memory (3 TB/s) nor the matrix units (a fifth) nor LDS (a third) is full: a workgroup waits for its columns'
+// loads twice a head, and registers (203 of 256) have no room for them a step earlier (there they spill: 0.6 ms; in phases that leave room, with dO, dR and N
+// read twice: 0.73 ms where this form takes 0.49).
 template <int DK, int DV>
 __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
     constexpr int KS = DK + 8, TS = DELTA_TS, NT = DK / 16;

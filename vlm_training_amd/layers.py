@@ -5,7 +5,7 @@
 * ``SelfAttention``         - models/qwen3_5/model.py:76-136: the same with ``q_proj`` emitting ``[q | gate]`` per
   head, OffsetRMSNorm (``1 + weight``), a rotary width that may be smaller than head_dim, the output multiplied by
   ``sigmoid(gate)``, and DTensor unwrap / rewrap around the kernels (models/qwen3_5/model.py:124,132).
-* ``GatedDeltaNet``         - models/qwen3_5/model.py:138-228: the linear-attention layers of the same stack: projections -> short convolution with
+* ``GatedDeltaNet``         - models/qwen3_5/model.py:38-44,173-186: the linear-attention layers of the same stack: projections -> short convolution with
   SiLU -> gated delta rule -> gated norm -> ``out_proj``;  ``forward(x, cu_seqlens)``, and ``step(x, state)`` for one token per request.
 * ``DsaIndexer``            - the lightning indexer's projections as module parameters (the reference holds no
   indexer): hidden -> Hi*Di index queries, hidden -> Di index key (one per token), hidden -> Hi head weights.
@@ -263,7 +263,7 @@ class DeltaState:
 
 
 class GatedDeltaNet(nn.Module):
-    """models/qwen3_5/model.py:138-228 (the linear-attention layers of the hybrid stack) with the parameter names of its checkpoints; ``cfg`` holds hidden_size,
+    """models/qwen3_5/model.py:38-44,173-186 (the linear-attention layers of the hybrid stack) with the parameter names of its checkpoints; ``cfg`` holds hidden_size,
     linear_num_key_heads, linear_num_value_heads, linear_key_head_dim, linear_value_head_dim, linear_conv_kernel_dim and
     rms_norm_eps.  Head counts come from the projections' outputs, so a head-sharded layer sees its own."""
 
