@@ -413,6 +413,7 @@ int dsa_round_bf16_x3(const float *a, const float *b, const float *c, int64_t na
  * (Hv) in their inputs' types, all contiguous, dinitial fp32 where it is not null.  `scratch` holds dsa_delta_scratch_bytes(args) bytes.
  * dsa_delta_step: one token for each of T requests; state (T,Hv,Dk,Dv) fp32, requests state_stride elements apart (a multiple of 4, on a 16-byte
  * boundary), is read and written in place.  cu and N are not used.
+ * Outputs, `ws` and `scratch` lie on 16-byte boundaries, here and in the operators below.
  */
 #define DSA_DELTA_MAX_ROW (1 << 23)
 typedef struct {
@@ -433,7 +434,7 @@ int dsa_delta_step(const dsa_delta_args *args, float *state, int64_t state_strid
 /*
  * Short causal convolution over packed sequences (models/qwen3_5/model.py:173-176), depthwise: z_t = bias + sum_{j<W} w[c][W-1-j] x_{t-j} inside
  * a sequence, y = z sigmoid(z) with `silu`, else z.  x (T,C) bf16, rows x_tok elements apart; w (C,W), bias (C, may be null) bf16 or fp32
- * (w_f32, bias_f32); W 2 to 4, C and strides multiples of 8, rows on 16-byte boundaries; y, dx (T,C) bf16 contiguous; rows behind cu[N] give zeros.
+ * (w_f32, bias_f32); W 2 to 4, C and strides multiples of 8, rows on 16-byte boundaries; y, dx (T,C) bf16 contiguous, T up to 2^30; rows behind cu[N] give zeros.
  * initial (N,C,W-1) bf16 holds the inputs before a sequence's first row (null: zeros); final, the same, receives each one's last W-1 inputs.
  * dsa_conv_bwd: dy (T,C) bf16 rows dy_tok apart -> dx, dw, dbias in their inputs' types (dbias null without a bias).  `ws` holds
  * dsa_conv_bwd_workspace_bytes(T, C, W) bytes.  dsa_conv_step: one token for each of B requests, state (B,C,W-1) bf16, requests

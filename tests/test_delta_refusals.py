@@ -78,3 +78,25 @@ def test_norms():
         16, 16, 16, 0, y, gate, 16, 0, post, 0, None, 0, 0.0, 4, 64, 16, ry, 16, 16, dgate, 16, dpost, None, 16, n, None)
     for change, code in ((dict(n=need - 1), -3), (dict(post=16), -1), (dict(post=16, dpost=16), -1), (dict(gate=16), -1), (dict(gate=16, dgate=16, y=None), -1)):
         assert bwd(**change) == code, change
+
+
+def test_outputs_and_workspaces_off_their_boundaries():
+    """What kernels write or read 16 bytes at a time; more rows than a run's 32-bit end can name."""
+    lib = _lib.load()
+    small, large = lib.dsa_delta_workspace_bytes(_args(), 0), lib.dsa_delta_workspace_bytes(_args(), 1)
+    # (buffers too small on top: nothing is launched, whichever is looked at first)
+    assert lib.dsa_delta_fwd(_args(), None, 24, None, 0, 256, small - 1, None) == -1 and b"16-byte" in lib.dsa_last_error()
+    assert lib.dsa_delta_fwd(_args(), None, 16, None, 0, 264, small - 1, None) == -1
+    good = dict(dout=16, ws=256, dq=16, dk=16, dv=16, scratch=256)
+    bwd = lambda dout, ws, dq, dk, dv, scratch: lib.dsa_delta_bwd(_args(), dout, None, ws, large, dq, dk, dv, 16, 16, 16, 16, None, scratch, 0, None)
+    assert bwd(**good) == -3
+    for name, at in good.items():
+        assert bwd(**{**good, name: at + 8}) == -1, name
+        assert b"16-byte" in lib.dsa_last_error()
+    assert lib.dsa_delta_step(_args(), 16, 63, 24, None) == -1
+    conv = lambda T=8, ws=16, dw=16: lib.dsa_conv_bwd(16, 64, 16, 64, 16, 0, None, 0, 1, 16, T, 1, 64, 4, None, 16, dw, None, ws, 0, None)
+    assert conv() == -3 and conv(ws=24) == -1
+    assert conv(T=(1 << 30) + 1) == -2 and b"rows" in lib.dsa_last_error()
+    assert lib.dsa_conv_fwd(16, 64, 16, 0, None, 0, 1, 16, (1 << 30) + 1, 1, 64, 4, None, 16, None, None) == -2
+    assert lib.dsa_gated_norm_bwd(16, 16, 64, 64, 16, 64, 64, 16, 0, 0.0, 4, 1, 64, 16, 16, 16, 16, 24, 0, None) == -1
+    assert lib.dsa_residual_norm_bwd(16, 16, 16, 0, 16, None, 16, 0, None, 0, None, 0, 0.0, 4, 64, 16, None, 16, 16, None, 16, None, None, 24, 0, None) == -1

@@ -1042,6 +1042,7 @@ extern "C" int dsa_round_bf16_x3(const float *a, const float *b, const float *c,
 // ---------------------------------------------------------------------------------------------------
 // gated delta rule
 // ---------------------------------------------------------------------------------------------------
+static bool off16(const void *p) { return ((uintptr_t)p & 15) != 0; }
 static int check_delta(const dsa_delta_args *a, bool packed) {
     if (!a) return fail(DSA_ERR_ARG, "null arguments");
     if (a->T < 0 || a->Hk < 1 || a->Hv < 1 || a->Hv % a->Hk) return fail(DSA_ERR_ARG, "T=%d Hk=%d Hv=%d: value heads must be a multiple of key heads", a->T, a->Hk, a->Hv);
@@ -1095,6 +1096,7 @@ extern "C" size_t dsa_delta_scratch_bytes(const dsa_delta_args *args) {
 extern "C" int dsa_delta_fwd(const dsa_delta_args *args, const float *initial, void *out, float *final, int save, void *ws, size_t ws_bytes, void *stream) {
     if (int rc = check_delta(args, true)) return rc;
     if (args->T > 0 && !out) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if (off16(out) || off16(ws)) return fail(DSA_ERR_ARG, "out and the workspace must lie on 16-byte boundaries");
     DeltaArgs d = {};
     const size_t need = delta_layout(args, save, (char *)ws, &d);
     if (!ws || ws_bytes < need) return fail(DSA_ERR_WORKSPACE, "gated delta rule workspace: have %zu bytes, need %zu", ws_bytes, need);
@@ -1109,7 +1111,8 @@ extern "C" int dsa_delta_bwd(const dsa_delta_args *args, const void *dout, const
                              void *da, void *db, void *da_log, void *ddt_bias, float *dinitial, void *scratch, size_t scratch_bytes, void *stream) {
     if (int rc = check_delta(args, true)) return rc;
     if (!da_log || !ddt_bias || (args->T > 0 && (!dout || !dq || !dk || !dv || !da || !db))) return fail(DSA_ERR_ARG, "null tensor pointer");
-    if ((uintptr_t)dout & 15) return fail(DSA_ERR_ARG, "dout must lie on a 16-byte boundary");
+    if (off16(dout) || off16(ws) || off16(dq) || off16(dk) || off16(dv) || off16(scratch))
+        return fail(DSA_ERR_ARG, "dout, dq, dk, dv, workspace and scratch must lie on 16-byte boundaries");
     DeltaArgs d = {};
     const size_t need = delta_layout(args, 1, (char *)const_cast<void *>(ws), &d), need2 = delta_scratch((char *)scratch, &d);
     if (!ws || ws_bytes < need) return fail(DSA_ERR_WORKSPACE, "gated delta rule workspace: have %zu bytes, need %zu", ws_bytes, need);
@@ -1131,8 +1134,8 @@ extern "C" int dsa_delta_bwd(const dsa_delta_args *args, const void *dout, const
 extern "C" int dsa_delta_step(const dsa_delta_args *args, float *state, int64_t state_stride, void *out, void *stream) {
     if (int rc = check_delta(args, false)) return rc;
     if (args->T == 0) return DSA_OK;
-    if (!state || !out) return fail(DSA_ERR_ARG, "null tensor pointer");
-    if (((uintptr_t)state & 15) || state_stride % 4 || (args->T > 1 && state_stride < (int64_t)args->Hv * args->Dk * args->Dv))
+    if (!state || !out || off16(out)) return fail(DSA_ERR_ARG, "state or out: null or not on a 16-byte boundary");
+    if (off16(state) || state_stride % 4 || (args->T > 1 && state_stride < (int64_t)args->Hv * args->Dk * args->Dv))
         return fail(DSA_ERR_ARG, "state: requests must lie on 16-byte boundaries and apart from each other");
     const hipError_t e = dsa_launch_delta_step(args, state, state_stride, out, (hipStream_t)stream);
     return e == hipSuccess ? DSA_OK : hip_fail(e, "gated delta rule step launch");
@@ -1141,9 +1144,9 @@ extern "C" int dsa_delta_step(const dsa_delta_args *args, float *state, int64_t 
 // ---------------------------------------------------------------------------------------------------
 // short convolution, gated norm, residual norm
 // ---------------------------------------------------------------------------------------------------
-static bool off16(const void *p) { return ((uintptr_t)p & 15) != 0; }
 static int check_conv(const void *x, int64_t x_tok, const void *w, const int32_t *cu, int T, int N, int C, int W) {
     if (T < 0 || N < 1 || !cu) return fail(DSA_ERR_ARG, "T=%d N=%d", T, N);
+    if (T > 1 << 30) return fail(DSA_ERR_UNSUPPORTED, "%d rows: up to 2^30 are supported", T);
     if (W < 2 || W > 4) return fail(DSA_ERR_UNSUPPORTED, "convolution width %d: need 2 to 4", W);
     if (C < 8 || C % 8) return fail(DSA_ERR_UNSUPPORTED, "channels=%d: need a multiple of 8", C);
     if (!w || (T > 0 && !x)) return fail(DSA_ERR_ARG, "null tensor pointer");
@@ -1166,7 +1169,7 @@ extern "C" int dsa_conv_bwd(const void *x, int64_t x_tok, const void *dy, int64_
                             void *stream) {
     if (int rc = check_conv(x, x_tok, w, cu, T, N, C, W)) return rc;
     if (!dw || (bias && !dbias) || (T > 0 && (!dy || !dx))) return fail(DSA_ERR_ARG, "null tensor pointer");
-    if (dy_tok % 8 || off16(dy) || off16(dx)) return fail(DSA_ERR_ARG, "rows must lie on 16-byte boundaries");
+    if (dy_tok % 8 || off16(dy) || off16(dx) || off16(ws)) return fail(DSA_ERR_ARG, "rows and the workspace must lie on 16-byte boundaries");
     const size_t need = dsa_conv_bwd_workspace_bytes(T, C, W);
     if (need && (!ws || ws_bytes < need)) return fail(DSA_ERR_WORKSPACE, "convolution backward workspace: have %zu bytes, need %zu", ws_bytes, need);
     const hipError_t e = dsa_launch_conv_bwd(x, x_tok, dy, dy_tok, w, w_f32, bias, bias_f32, silu, cu, T, N, C, W, initial, dx, dw, bias ? dbias : nullptr, (float *)ws,
@@ -1207,7 +1210,7 @@ extern "C" int dsa_gated_norm_bwd(const void *dy, const void *x, int64_t x_tok, 
                                   float offset, int T, int H, int D, const float *rstd, void *dx, void *dz, void *dw, void *ws, size_t ws_bytes, void *stream) {
     if (int rc = check_gated_norm(x, x_tok, x_head, z, z_tok, z_head, w, T, H, D)) return rc;
     if (!dw || (T > 0 && (!dy || !rstd || !dx || !dz))) return fail(DSA_ERR_ARG, "null tensor pointer");
-    if (off16(dy) || off16(dx) || off16(dz)) return fail(DSA_ERR_ARG, "rows must lie on 16-byte boundaries");
+    if (off16(dy) || off16(dx) || off16(dz) || off16(ws)) return fail(DSA_ERR_ARG, "rows and the workspace must lie on 16-byte boundaries");
     const size_t need = dsa_gated_norm_bwd_workspace_bytes(T, H, D);
     if (need && (!ws || ws_bytes < need)) return fail(DSA_ERR_WORKSPACE, "gated norm backward workspace: have %zu bytes, need %zu", ws_bytes, need);
     const hipError_t e = dsa_launch_gated_norm_bwd(dy, x, x_tok, x_head, z, z_tok, z_head, w, w_f32, offset, T, H, D, rstd, dx, dz, dw, (float *)ws, (hipStream_t)stream);
@@ -1241,8 +1244,8 @@ extern "C" int dsa_residual_norm_bwd(const void *dxn, const void *dh, const void
     if (int rc = check_residual_norm(w, T, C)) return rc;
     if (!dw || (post && !dpost) || (scale && !dscale)) return fail(DSA_ERR_ARG, "null tensor pointer");
     if (T > 0 && (!xn || !rstd || !dx || !dy || (gate && !dgate) || ((post || gate || scale) && !y) || (post && !rstd_y))) return fail(DSA_ERR_ARG, "null tensor pointer");
-    if (off16(dxn) || off16(dh) || off16(xn) || off16(y) || off16(gate) || off16(dx) || off16(dy) || off16(dgate))
-        return fail(DSA_ERR_ARG, "rows must lie on 16-byte boundaries");
+    if (off16(dxn) || off16(dh) || off16(xn) || off16(y) || off16(gate) || off16(dx) || off16(dy) || off16(dgate) || off16(ws))
+        return fail(DSA_ERR_ARG, "rows and the workspace must lie on 16-byte boundaries");
     const size_t need = dsa_residual_norm_bwd_workspace_bytes(T, C);
     if (need && (!ws || ws_bytes < need)) return fail(DSA_ERR_WORKSPACE, "residual norm backward workspace: have %zu bytes, need %zu", ws_bytes, need);
     const hipError_t e = dsa_launch_residual_norm_bwd(dxn, dh, xn, x_f32, y, gate, w, w_f32, post, post_f32, scale, scale_f32, offset, T, C, rstd, rstd_y, dx, dy, dgate, dw,
