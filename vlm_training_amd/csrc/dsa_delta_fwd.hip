@@ -20,6 +20,7 @@ __global__ __launch_bounds__(256, 4) void dsa_delta_prep_kernel(DeltaArgs a) {
     DeltaChunk c;
     if (!delta_locate(in.cu, in.N, in.T, slot, c)) {
         // rows behind the last sequence: zeros
+        if (blockIdx.z) return;
         const int64_t r0 = (int64_t)max(in.cu[in.N], 0) + 64 * (int64_t)c.index;
         for (int r = 0; r < 64 && r0 + r < in.T; ++r)
             for (int i = tid; i < rep * in.Dv; i += 256) a.out[((r0 + r) * in.Hv + hk * rep) * in.Dv + i] = (bf16_t)0.f;
@@ -56,7 +57,7 @@ __global__ __launch_bounds__(256, 4) void dsa_delta_prep_kernel(DeltaArgs a) {
             }
         }
     }
-    for (int u = 0; u < rep; ++u) {
+    for (int u = blockIdx.z; u < rep; u += gridDim.z) {
         const int lane = fresh_lane(), l16 = lane & 15, g4 = lane >> 4, tid = 64 * wv + lane, i = 16 * wv + l16;
         const int h = hk * rep + u;
         const int64_t p = (int64_t)slot * in.Hv + h;
@@ -273,7 +274,10 @@ __global__ __launch_bounds__(256) void dsa_delta_step_kernel(dsa_delta_args in, 
 extern "C" void dsa_launch_delta_walk(const DeltaArgs *a, int save, hipStream_t stream);
 extern "C" hipError_t dsa_launch_delta_fwd(const DeltaArgs *a, int save, hipStream_t stream) {
     if (a->in.T > 0) {
-        const dim3 grid(a->slots, a->in.Hk);
+        // the value heads of a key head one after the other, or a workgroup each where all of these find room at once (16 / 32 heads of 128, us, the first and the
+        // second: 300 rows 17, 12; 1500 rows 20, 17; 3000 rows 26, 28)
+        const int rep = a->in.Hv / a->in.Hk;
+        const dim3 grid(a->slots, a->in.Hk, (int64_t)a->slots * a->in.Hv <= 1024 ? rep : 1);
         if (a->Dkp == 64) hipLaunchKernelGGL((dsa_delta_prep_kernel<64>), grid, dim3(256), 0, stream, *a);
         else hipLaunchKernelGGL((dsa_delta_prep_kernel<128>), grid, dim3(256), 0, stream, *a);
     }
