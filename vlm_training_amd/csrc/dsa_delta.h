@@ -182,11 +182,18 @@ __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70
 // (Never with a scalar offset: the compiler then leaves out the wait state between a 16-byte store and an instruction that overwrites what it stores, and
 // stored values came out wrong here and there.)
 __device__ __forceinline__ void buf_put16(buffer_t b, int off, u32x4 x) { __builtin_amdgcn_raw_buffer_store_b128(x, b, off, 0, 0); }
+// the same, past the caches: what only the chunks' gradients will read (walks of 33 sequences of 16 384 rows together, of 1 of 32 768 and of 4 of 4096, forward / backward:
+// 328 / 369 us -> 326 / 356, 1084 / 1179 -> 1073 / 1139, 372 / 385 -> 366 / 374; outputs so, whose lines come in parts, cost 50 us of the first).
+__device__ __forceinline__ void buf_put16_past(buffer_t b, int off, u32x4 x) { __builtin_amdgcn_raw_buffer_store_b128(x, b, off, 0, 2); }
 // four or eight elements at a time
 template <int N> struct Piece { uint32_t x[N / 2]; };
 template <int N> __device__ __forceinline__ Piece<N> buf_piece(buffer_t b, int off) {
     if constexpr (N == 8) return __builtin_bit_cast(Piece<8>, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
     else return __builtin_bit_cast(Piece<4>, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0));
+}
+template <int N> __device__ __forceinline__ void buf_put_piece_past(buffer_t b, int off, Piece<N> p) {
+    if constexpr (N == 8) buf_put16_past(b, off, __builtin_bit_cast(u32x4, p));
+    else buf_put8(b, off, __builtin_bit_cast(u32x2, p));
 }
 template <int N> __device__ __forceinline__ void buf_put_piece(buffer_t b, int off, Piece<N> p) {
     if constexpr (N == 8) buf_put16(b, off, __builtin_bit_cast(u32x4, p));

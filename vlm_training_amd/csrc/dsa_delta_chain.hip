@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_chain_kernel(DeltaArgs a) {
                 all.x[2 * t] = y[0];
                 all.x[2 * t + 1] = y[1];
             }
-            if (SAVE) buf_put_piece<4 * NT>(save, at_s + c * 32 * DK, all);
+            if (SAVE) buf_put_piece_past<4 * NT>(save, at_s + c * 32 * DK, all);
         }
 #pragma unroll
         for (int s = 0; s < DK / 32; ++s) *reinterpret_cast<bf16x8 *>(kt + (rrow + s * RPI) * KS + rcol) = x.k[s];
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_chain_kernel(DeltaArgs a) {
             put4(nh + at, yh);
             put4(nl + at, yl);
             put_split4(mh + at, ml + at, y * (x.ec * x.rk));
-            if (SAVE) buf_put16(save, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]});
+            if (SAVE) buf_put16_past(save, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]});
         }
         fetch_t(x);
         __syncthreads();
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_chain_back_kernel(DeltaArgs 
                 all.x[2 * t] = y[0];
                 all.x[2 * t + 1] = y[1];
             }
-            buf_put_piece<4 * NT>(back, at_s + c * 32 * DK, all);
+            buf_put_piece_past<4 * NT>(back, at_s + c * 32 * DK, all);
         }
 #pragma unroll
         for (int s = 0; s < DK / 32; ++s) {
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_chain_back_kernel(DeltaArgs 
             }
             const int at = row * RS + 16 * c + 4 * g4;
             const u32x2 yh = hi4(y), yl = lo4(y, yh);
-            buf_put16(back, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]});
+            buf_put16_past(back, at_n + c * 4096, u32x4{yh[0], yh[1], yl[0], yl[1]});
             put4(os + at, hi4(y * x.beta));
             put_split4(sh + at, sl + at, y * (-x.beta * x.eg * x.rk));
         }

@@ -154,8 +154,9 @@ __global__ __launch_bounds__(256, 4) void dsa_delta_prep_kernel(DeltaArgs a) {
         __syncthreads();
         auto plane = [&](bf16_t *to, int at, f32x4 x, f32x4 y) __attribute__((always_inline)) {
             const u32x2 xh = hi4(x), yh = hi4(y), xl = lo4(x, xh), yl = lo4(y, yh);
-            *reinterpret_cast<u32x4_any *>(to + at) = u32x4{xh[0], xh[1], yh[0], yh[1]};
-            *reinterpret_cast<u32x4_any *>(to + 4096 + at) = u32x4{xl[0], xl[1], yl[0], yl[1]};
+            // (past the caches, as everything that a later kernel reads: the walk of 1 sequence of 32 768 rows 1067 -> 1030 us, of 33 sequences 322 -> 308)
+            __builtin_nontemporal_store(u32x4{xh[0], xh[1], yh[0], yh[1]}, reinterpret_cast<u32x4 *>(to + at));
+            __builtin_nontemporal_store(u32x4{xl[0], xl[1], yl[0], yl[1]}, reinterpret_cast<u32x4 *>(to + 4096 + at));
         };
 #pragma unroll
         for (int e = 0; e < 2; ++e) {

@@ -162,7 +162,7 @@ __global__ __launch_bounds__(64 * WALK_W, 2) void dsa_delta_walk_kernel(DeltaArg
         for (int s = 0; s < KB; ++s) {
             bf16x8 sh, sl;
             split8(st[s][0], st[s][1], sh, sl);
-            if (SAVE) buf_put16(save, at_s + s * 1024, __builtin_bit_cast(u32x4, sh));
+            if (SAVE) buf_put16_past(save, at_s + s * 1024, __builtin_bit_cast(u32x4, sh));
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 const bf16x8 kf = frag_rows(t.k, KS, 16 * m, 32 * s), qf = frag_rows(t.q, KS, 16 * m, 32 * s);
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * WALK_W, 2) void dsa_delta_walk_kernel(DeltaArg
             }
             if (SAVE) {
                 const u32x2 yh = hi4(across), yl = lo4(across, yh);
-                buf_put16(save, at_n + m * 1024, u32x4{yh[0], yh[1], yl[0], yl[1]});
+                buf_put16_past(save, at_n + m * 1024, u32x4{yh[0], yh[1], yl[0], yl[1]});
             }
         }
         // S1 = e^G_63 S0 + K^T e^(G_63 - G) N
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * WALK_W, 2) void dsa_delta_back_kernel(DeltaArg
         for (int s = 0; s < KB; ++s) {
             bf16x8 sh, sl;
             split8(st[s][0], st[s][1], sh, sl);
-            buf_put16(back, at_s + s * 1024, __builtin_bit_cast(u32x4, sh));
+            buf_put16_past(back, at_s + s * 1024, __builtin_bit_cast(u32x4, sh));
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 const bf16x8 kf = frag_rows(t.k, KS, 16 * m, 32 * s);
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(64 * WALK_W, 2) void dsa_delta_back_kernel(DeltaArg
             }
             const float beta = t.f[DELTA_BETA * 64 + 16 * m + l16];
             const u32x2 yh = hi4(across), yl = lo4(across, yh);
-            buf_put16(back, at_n + m * 1024, u32x4{yh[0], yh[1], yl[0], yl[1]});
+            buf_put16_past(back, at_n + m * 1024, u32x4{yh[0], yh[1], yl[0], yl[1]});
             put4(t.v + (16 * m + l16) * VS + dv0 + 4 * g4, hi4(across * beta));
         }
         wave_sync();
