@@ -6,9 +6,9 @@
 // formed transposed (lane: its row, four neighbouring columns), which makes every factor of a row one register and every access 8 or 16 bytes.
 // Rows of K, Q, T and P are needed by their own wave alone (K by all of them as K^T): T and P come as fragments straight into registers, rows of K, Q and V
 // 16 bytes a lane through the wave's own part of LDS.  The next chunk's loads go out as soon as a register has been read.
-// One sequence of 32 768 rows, 32 heads of 128: 1.7 us a chunk forwards, 2.1 with what a backward needs, 2.3 backwards: the chain itself is 1.25 us (three phases of LDS reads,
+// One sequence of 32 768 rows, 32 heads of 128: 1.7 us a chunk forwards, 2.0 with what a backward needs, 2.2 backwards: the chain itself is 1.25 us (three phases of LDS reads,
 // products that wait for each other, LDS writes and a barrier), the rest the chunk's 58 KB into the compute unit and the stores.  (Four more waves that
-// only load, through LDS: 1.7, 2.1 and 2.1 us, and a compute unit to each workgroup.)
+// only load, through LDS, were level with that and want a compute unit to each workgroup.)
 #include "dsa_delta.h"
 
 template <int DK, int NC> struct ChainRows {
