@@ -150,6 +150,42 @@ def test_many_sequences(split, n, hv, dk, dv):
     assert off(go[:sum(lens)], o) <= OUT and off(gs, s) <= STATE and not go[sum(lens):].any()
 
 
+@pytest.mark.parametrize("split,n,hv,dk,dv", MANY[1:3])
+def test_many_sequences_captured_and_on_another_stream(split, n, hv, dk, dv):
+    """The same bits eagerly, replayed, on a stream of its own, and without what a backward needs."""
+    _log(f"{split} {n} sequences, captured")
+    lens = [70, 1, 0, 129] + [3] * (n - 4)
+    x = {m: t.to(DEV) for m, t in inputs(sum(lens), hv // 2, hv, dk, dv, seed=31).items()}
+    cu = cu_of(lens)
+    leaves = [x[m].clone().requires_grad_(True) for m in NAMES]
+
+    def step():
+        o, s = V.gated_delta_rule(*leaves, cu, return_final_state=True)
+        return [o.detach(), s.detach(), *torch.autograd.grad(o, leaves, x["dout"])]
+
+    want = [t.clone() for t in step()]
+    with torch.no_grad():
+        o, s = V.gated_delta_rule(*leaves, cu, return_final_state=True)
+    assert torch.equal(o, want[0]) and torch.equal(s, want[1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(other, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for replay in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        other = step()                                   # eager work between the replays
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), f"replay {replay}"
+        assert all(torch.equal(a, b) for a, b in zip(other, want))
+
+
 @pytest.mark.parametrize("kind", ["same_key", "full_decay", "one_reset"])
 @pytest.mark.parametrize("split,n,hv,dk,dv", MANY[1:3])
 def test_corners_in_many_sequences(split, n, hv, dk, dv, kind):

@@ -263,7 +263,7 @@ class DeltaState:
 
 
 class GatedDeltaNet(nn.Module):
-    """models/qwen3_5/model.py:38-44,173-186 (the linear-attention layers of the hybrid stack) with the parameter names of its checkpoints; ``cfg`` holds hidden_size,
+    """models/qwen3_5/model.py:38-44,173-186 (the linear-attention layers of the hybrid stack) with the parameter names of its public checkpoints; ``cfg`` holds hidden_size,
     linear_num_key_heads, linear_num_value_heads, linear_key_head_dim, linear_value_head_dim, linear_conv_kernel_dim and
     rms_norm_eps.  Head counts come from the projections' outputs, so a head-sharded layer sees its own."""
 
