@@ -186,6 +186,31 @@ def test_many_sequences_captured_and_on_another_stream(split, n, hv, dk, dv):
         assert all(torch.equal(a, b) for a, b in zip(other, want))
 
 
+@pytest.mark.parametrize("n,hv", [(3, 4), (64, 8)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_is_not_finite_stays_in_its_sequence(n, hv, bad):
+    """Rows behind the last sequence are not read; a sequence with such rows leaves the others as they are."""
+    lens = [70] + [0] * (n - 3) + [67, 130]
+    T = sum(lens)
+    x = {m: t.to(DEV) for m, t in inputs(T + 40, hv // 2, hv, 128, 128, seed=41).items()}
+    cu = cu_of(lens)
+
+    def run():
+        leaves = [x[m].clone().requires_grad_(True) for m in NAMES]
+        o = V.gated_delta_rule(*leaves, cu)
+        return [o.detach(), *torch.autograd.grad(o, leaves, x["dout"])]
+
+    want = run()
+    for m in ("q", "k", "v", "a", "b", "dout"):
+        x[m][T:] = bad
+    got = run()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for m in ("q", "k", "v", "a", "b", "dout"):
+        x[m][70:137] = bad
+    for a, b in zip(run()[:6], want[:6]):
+        assert torch.equal(a[:70], b[:70]) and torch.equal(a[137:], b[137:])
+
+
 @pytest.mark.parametrize("kind", ["same_key", "full_decay", "one_reset"])
 @pytest.mark.parametrize("split,n,hv,dk,dv", MANY[1:3])
 def test_corners_in_many_sequences(split, n, hv, dk, dv, kind):

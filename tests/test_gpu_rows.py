@@ -93,6 +93,32 @@ def test_gated_rms_norm(T, H, D, dtype, offset):
         close(d[n].grad, c[n].grad, n)
 
 
+@pytest.mark.parametrize("C", [24, 264])
+def test_what_is_not_finite_stays_in_its_sequence(C):
+    lens, T = [13, 5, 0, 60, 1, 40], 119
+    x, dy = torch.randn(T + 30, C, device=DEV).to(BF), torch.randn(T + 30, C, device=DEV).to(BF)
+    w, b, cu = torch.randn(C, 4, device=DEV).to(BF), torch.randn(C, device=DEV).to(BF), cu_of(lens)
+
+    def run():
+        leaf = x.clone().requires_grad_(True)
+        y = V.short_conv(leaf, w, b, cu)
+        return y.detach(), torch.autograd.grad(y, leaf, dy)[0]
+
+    want = run()
+    for lo, hi in ((T, T + 30), (18, 78), (0, 13)):      # rows behind the last sequence, then two whole sequences
+        x[lo:hi] = float("nan")
+        dy[lo:hi] = float("inf")
+        for got, ref in zip(run(), want):
+            keep = torch.ones(T + 30, dtype=torch.bool, device=DEV)
+            keep[18:78] &= hi > T
+            keep[:13] &= lo > 0
+            assert torch.equal(got[keep], ref[keep])
+    z = torch.randn(9, 3, 64, device=DEV).to(BF)
+    z[4, 1] = float("nan")
+    y = V.gated_rms_norm(z, torch.ones_like(z), torch.ones(64, device=DEV))
+    assert torch.isfinite(y).all(-1).logical_not().nonzero().tolist() == [[4, 1]]
+
+
 def test_gated_rms_norm_reads_views_in_place():
     x = torch.randn(20, 3, 2 * 64, device=DEV).to(BF)
     w = torch.ones(64, device=DEV)
