@@ -186,6 +186,37 @@ def test_many_sequences_captured_and_on_another_stream(split, n, hv, dk, dv):
         assert all(torch.equal(a, b) for a, b in zip(other, want))
 
 
+@pytest.mark.parametrize("lens", [[2100] + [0] * 29, [89] * 24, [27] * 80, [1900] + [5] * 299], ids=["one long", "few", "many", "many and one long"])
+def test_how_lengths_choose_the_split(lens):
+    """Batches of 2048 rows and more, whose lengths decide on the device"""
+    hv, T = 2, sum(lens)
+    _log(f"{len(lens)} sequences of up to {max(lens)}")
+    g = torch.Generator().manual_seed(T)
+    x = inputs(T, 1, hv, 72, 72, seed=T)
+    x = {m: t.to(DEV) for m, t in x.items()}
+    start = 0.5 * torch.randn(len(lens), hv, 72, 72, generator=g).to(DEV)
+    cu = cu_of(lens)
+
+    def run(rows, cu, start):
+        leaves = [(x[m][rows] if m in "qkvab" else x[m]).clone().requires_grad_(True) for m in NAMES] + [start.clone().requires_grad_(True)]
+        o, s = V.gated_delta_rule(*leaves[:7], cu, initial_state=leaves[7], return_final_state=True)
+        grads = torch.autograd.grad([o, s], leaves, [x["dout"][rows], start])
+        return [o.detach(), *grads[:5]], [s.detach(), grads[7]]
+
+    got_rows, got_states = run(slice(0, T), cu, start)
+    at = 0
+    for i, L in enumerate(lens):                         # each of a few alone, where there is nothing to choose (the split leaves fp32 sums of other orders: close, not equal)
+        if L and i in (0, 1, 7, len(lens) - 1):
+            rows, states = run(slice(at, at + L), cu_of([L]), start[i:i + 1])
+            for a, b in zip(rows, got_rows):
+                assert off(b[at:at + L], a.cpu()) <= 2.0 ** -7
+            for a, b in zip(states, got_states):
+                assert off(b[i:i + 1], a.cpu()) <= GRAD
+        elif L == 0 and i < 3:
+            assert torch.equal(got_states[0][i], start[i]) and torch.equal(got_states[1][i], start[i])
+        at += L
+
+
 @pytest.mark.parametrize("n,hv", [(3, 4), (64, 8)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_what_is_not_finite_stays_in_its_sequence(n, hv, bad):

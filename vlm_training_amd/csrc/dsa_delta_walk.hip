@@ -125,6 +125,7 @@ __global__ __launch_bounds__(64 * WALK_W, 2) void dsa_delta_walk_kernel(DeltaArg
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
     int64_t unit;
     int block, slot0, chunks, s0, L;
+    if (a.choose && delta_form(a) != DELTA_HEAD) return;
     if (!delta_walk_unit(blockIdx.x, 1, (int64_t)in.N * in.Hv, unit, block)) return;
     const int h = (int)(unit % in.Hv), seg = delta_longest(in.cu, in.N, (int)(unit / in.Hv)), hk = h / (in.Hv / in.Hk), dv0 = 16 * wv;
     delta_segment(in.cu, in.N, seg, slot0, chunks, s0, L);
@@ -269,6 +270,7 @@ __global__ __launch_bounds__(64 * WALK_W, 2) void dsa_delta_back_kernel(DeltaArg
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
     int64_t unit;
     int block, slot0, chunks, s0, L;
+    if (a.choose && delta_form(a) != DELTA_HEAD) return;
     if (!delta_walk_unit(blockIdx.x, 1, (int64_t)in.N * in.Hv, unit, block)) return;
     const int h = (int)(unit % in.Hv), seg = delta_longest(in.cu, in.N, (int)(unit / in.Hv)), hk = h / (in.Hv / in.Hk), dv0 = 16 * wv;
     delta_segment(in.cu, in.N, seg, slot0, chunks, s0, L);
@@ -399,24 +401,38 @@ __global__ __launch_bounds__(64 * WALK_W, 2) void dsa_delta_back_kernel(DeltaArg
         });
 }
 
-// The walks of this file, or dsa_delta_chain.hip's?  Here a workgroup takes a head's whole state, 6 us a chunk alone and 8.5 us with its like on all compute units (bound by
-// memory then); there four or eight take it between them, 2 to 3 us a chunk alone and 5.9 us for two that share a compute unit.  So this file's want several
-// heads to a compute unit, which also evens out sequences of different lengths.  Forward / backward with 32 heads, us, this file's first:
-//     8 sequences of 2048          276 / 309   361 / 379        33 of 65 .. 1669        319 / 349   382 / 409
-//     4 of 4096                    486 / 489   371 / 379        8 of 200 .. 4000        450 / 431   272 / 268
-static bool delta_many(const DeltaArgs *a) { return a->Dkp == 128 && a->Dvp == 128 && (int64_t)a->in.N * a->in.Hv >= 512; }
-// Columns of 16 that a workgroup of dsa_delta_chain.hip's takes: one where two would leave compute units without any.  Forward / backward, us, of one and of two:
-//     1 sequence of 32 768        1088 / 1164   1307 / 1325     2 of 8192      532 / 510   398 / 465
-static int delta_columns(const DeltaArgs *a) { return (int64_t)a->in.N * a->in.Hv * (a->Dvp / 32) < 256 ? 1 : 2; }
-extern "C" void dsa_launch_delta_chain(const DeltaArgs *a, int nc, int save, hipStream_t stream);
-extern "C" void dsa_launch_delta_chain_back(const DeltaArgs *a, int nc, hipStream_t stream);
-extern "C" void dsa_launch_delta_walk(const DeltaArgs *a, int save, hipStream_t stream) {
-    if (!delta_many(a)) return dsa_launch_delta_chain(a, delta_columns(a), save, stream);
-    const dim3 walks((unsigned)(((int64_t)a->in.N * a->in.Hv + 7) / 8 * 8));
-    if (save) hipLaunchKernelGGL(dsa_delta_walk_kernel<true>, walks, dim3(64 * WALK_W), 0, stream, *a);
-    else hipLaunchKernelGGL(dsa_delta_walk_kernel<false>, walks, dim3(64 * WALK_W), 0, stream, *a);
+extern "C" void dsa_launch_delta_chain(const DeltaArgs *a, int form, int save, hipStream_t stream);
+extern "C" void dsa_launch_delta_chain_back(const DeltaArgs *a, int form, hipStream_t stream);
+// The forms that lengths unknown to the host leave: all chunks are those of one longest sequence at the least, of N at the most.  Short batches take one that may not be
+// the best rather than launches for nothing; batches of 512 walks leave DELTA_ONE out, and of 1024 all but DELTA_HEAD (33 sequences: 8 us a launch of 310 for nothing).
+static int delta_forms(DeltaArgs &a, int (&forms)[3]) {
+    const int64_t least = a.in.Hv, most = (int64_t)a.in.N * a.in.Hv;
+    const int low = delta_form_of(a, least, 1), high = delta_form_of(a, most, 1), many = a.Dkp == 128 && a.Dvp == 128 && most >= 512;
+    int n = 0;
+    a.maybe_one = low == DELTA_ONE && (high == DELTA_ONE || most < 512);
+    if ((a.in.T < 2048 || (many && most >= 1024)) && low != high) forms[n++] = many ? DELTA_HEAD : DELTA_TWO;
+    else
+        for (int f = low == DELTA_ONE && !a.maybe_one ? DELTA_TWO : low; f <= high; ++f) forms[n++] = f;
+    a.choose = n > 1;
+    return n;
 }
-extern "C" void dsa_launch_delta_back(const DeltaArgs *a, hipStream_t stream) {
-    if (!delta_many(a)) return dsa_launch_delta_chain_back(a, delta_columns(a), stream);
-    hipLaunchKernelGGL(dsa_delta_back_kernel, dim3((unsigned)(((int64_t)a->in.N * a->in.Hv + 7) / 8 * 8)), dim3(64 * WALK_W), 0, stream, *a);
+extern "C" void dsa_launch_delta_walk(const DeltaArgs *args, int save, hipStream_t stream) {
+    DeltaArgs a = *args;
+    int forms[3];
+    const int n = delta_forms(a, forms);
+    const dim3 walks((unsigned)(((int64_t)a.in.N * a.in.Hv + 7) / 8 * 8));
+    for (int i = 0; i < n; ++i) {
+        if (forms[i] != DELTA_HEAD) dsa_launch_delta_chain(&a, forms[i], save, stream);
+        else if (save) hipLaunchKernelGGL(dsa_delta_walk_kernel<true>, walks, dim3(64 * WALK_W), 0, stream, a);
+        else hipLaunchKernelGGL(dsa_delta_walk_kernel<false>, walks, dim3(64 * WALK_W), 0, stream, a);
+    }
+}
+extern "C" void dsa_launch_delta_back(const DeltaArgs *args, hipStream_t stream) {
+    DeltaArgs a = *args;
+    int forms[3];
+    const int n = delta_forms(a, forms);
+    for (int i = 0; i < n; ++i) {
+        if (forms[i] != DELTA_HEAD) dsa_launch_delta_chain_back(&a, forms[i], stream);
+        else hipLaunchKernelGGL(dsa_delta_back_kernel, dim3((unsigned)(((int64_t)a.in.N * a.in.Hv + 7) / 8 * 8)), dim3(64 * WALK_W), 0, stream, a);
+    }
 }
