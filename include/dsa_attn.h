@@ -467,8 +467,11 @@ int dsa_gated_norm_bwd(const void *dy, const void *x, int64_t x_tok, int64_t x_h
  * with n = norm(y) (post + offset), or y where post is null; gate and scale may be null.  x, xn (T,C) bf16 or fp32 (x_f32), y, gate, h (T,C) bf16, all
  * contiguous on 16-byte boundaries; w, post, scale (C) bf16 or fp32; C a multiple of 8 up to 8192.  rstd, rstd_y (T) fp32 may be null where no backward follows.
  * dsa_residual_norm_bwd: dxn (as xn) and dh, either may be null -> dx (as x), dy, dgate, dw, dpost, dscale (the last three where their inputs are
- * there).  `ws` holds dsa_residual_norm_bwd_workspace_bytes(T, C) bytes.
+ * there).  Its x_f32 also says what `xn` holds: DSA_STREAM_F32 and DSA_STREAM_BF16 x', of a bf16 stream as it was rounded; DSA_STREAM_BF16_BEFORE x, bf16, from
+ * which and y (needed then without post, gate and scale too) x' is formed again: the forward's norm has read it unrounded, and the gradients are taken
+ * there.  `ws` holds dsa_residual_norm_bwd_workspace_bytes(T, C) bytes.
  */
+enum { DSA_STREAM_BF16 = 0, DSA_STREAM_F32 = 1, DSA_STREAM_BF16_BEFORE = 2 };
 size_t dsa_residual_norm_bwd_workspace_bytes(int T, int C);
 int dsa_residual_norm_fwd(const void *x, int x_f32, const void *y, const void *gate, const void *w, int w_f32, const void *post, int post_f32,
                           const void *scale, int scale_f32, float eps, float offset, int T, int C, void *xn, void *h, float *rstd, float *rstd_y,

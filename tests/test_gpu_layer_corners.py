@@ -1,0 +1,68 @@
+"""Short convolution, gated norm and residual norm where their formulas are easily lost: gates at the type's lowest value, large pre-activations, gradients of a
+bf16 residual stream, second derivatives.  Tolerances as in test_gpu_rows.py: a bf16 result's own rounding, 2^-8 of it, and 2^-16 of the largest."""
+import ctypes
+
+import pytest
+import torch
+
+import vlm_training_amd as V
+from oracle import delta_ref as R
+from tests.test_gpu_rows import close, cu_of, leaves
+from vlm_training_amd import _lib
+
+pytestmark = pytest.mark.gpu
+DEV, BF, F32 = "cuda", torch.bfloat16, torch.float32
+
+
+def _log(msg):
+    print(f"[corners] {msg}", flush=True)
+
+
+@pytest.mark.parametrize("post,gate,scale", [(p, g, s) for p in (0, 1) for g in (0, 1) for s in (0, 1)])
+@pytest.mark.parametrize("T,C", [(1, 8), (130, 1000), (700, 264), (5, 2056), (3, 8192)])
+def test_gradients_of_a_bf16_stream_are_those_of_the_unrounded_one(T, C, post, gate, scale):
+    """The forward's norm reads x' before it is rounded, and its gradient is taken there."""
+    _log(f"residual norm {T} {C} {post}{gate}{scale}")
+    g = torch.Generator().manual_seed(T + C + 1)
+    rn = lambda *s: torch.randn(*s, generator=g)
+    x = {"x": (2 * rn(T, C)).to(BF), "y": rn(T, C).to(BF), "w": rn(C), "post": rn(C) if post else None, "gate": rn(T, C).to(BF) if gate else None,
+         "scale": rn(C) if scale else None}
+    grads = rn(T, C).to(BF), rn(T, C).to(BF)
+    c, d = leaves(x, "cpu"), leaves(x, DEV)
+    torch.autograd.backward(R.residual_rms_norm(*c.values(), offset=bool(gate)), [t.double() for t in grads])
+    got = V.residual_rms_norm(d["x"], d["y"], d["w"], post_weight=d["post"], gate=d["gate"], scale=d["scale"], offset=bool(gate))
+    torch.autograd.backward(got, [t.to(DEV) for t in grads])
+    for n in x:
+        if x[n] is not None:
+            close(d[n].grad, c[n].grad, n)
+
+
+def test_gradients_through_the_c_entry_with_a_rounded_stream():
+    """DSA_STREAM_BF16 takes x' as a bf16 stream holds it: its rounding, 2^-8 of a value at the most, is in dw and in one term of dx (2 * 2^-8 of the 2-norm)."""
+    T, C = 130, 264
+    g = torch.Generator().manual_seed(5)
+    rn = lambda *s: torch.randn(*s, generator=g)
+    x, y, w, dxn, dh = (2 * rn(T, C)).to(BF), rn(T, C).to(BF), rn(C), rn(T, C).to(BF), rn(T, C).to(BF)
+    c = {n: t.double().requires_grad_(True) for n, t in (("x", x), ("y", y), ("w", w))}
+    torch.autograd.backward(R.residual_rms_norm(c["x"], c["y"], c["w"]), [dxn.double(), dh.double()])
+    d = [t.to(DEV) for t in (x, y, w, dxn, dh)]
+    xn, h, dx, dy = (torch.empty(T, C, dtype=BF, device=DEV) for _ in range(4))
+    rstd, dw = torch.empty(T, device=DEV), torch.empty(C, device=DEV)
+    lib, p = _lib.load(), lambda t: ctypes.c_void_p(t.data_ptr())
+    n = lib.dsa_residual_norm_bwd_workspace_bytes(T, C)
+    ws = torch.empty(n, dtype=torch.uint8, device=DEV)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.dsa_residual_norm_fwd(p(d[0]), 0, p(d[1]), None, p(d[2]), 1, None, 0, None, 0, 1e-6, 0.0, T, C, p(xn), p(h), p(rstd), None, stream) == 0
+    for kind, wide in ((0, True), (2, False)):
+        assert lib.dsa_residual_norm_bwd(p(d[3]), p(d[4]), p(xn if kind == 0 else d[0]), kind, p(d[1]), None, p(d[2]), 1, None, 0, None, 0, 0.0, T, C, p(rstd), None, p(dx),
+                                         p(dy), None, p(dw), None, None, p(ws), n, stream) == 0
+        torch.cuda.synchronize()
+        for name, got, want in (("dx", dx, c["x"].grad), ("dy", dy, c["y"].grad), ("dw", dw, c["w"].grad)):
+            close(got, want, (kind, name), wide=wide)
+
+
+def test_stream_kinds_that_are_none_are_refused():
+    lib = _lib.load()
+    n = lib.dsa_residual_norm_bwd_workspace_bytes(4, 64)
+    bwd = lambda kind, y: lib.dsa_residual_norm_bwd(16, 16, 16, kind, y, None, 16, 0, None, 0, None, 0, 0.0, 4, 64, 16, None, 16, 16, None, 16, None, None, 16, n - 1, None)
+    assert bwd(3, 16) == -1 and bwd(-1, 16) == -1 and bwd(2, None) == -1 and bwd(2, 16) == -3 and bwd(0, None) == -3

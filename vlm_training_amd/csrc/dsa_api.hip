@@ -1243,7 +1243,9 @@ extern "C" int dsa_residual_norm_bwd(const void *dxn, const void *dh, const void
                                      void *stream) {
     if (int rc = check_residual_norm(w, T, C)) return rc;
     if (!dw || (post && !dpost) || (scale && !dscale)) return fail(DSA_ERR_ARG, "null tensor pointer");
-    if (T > 0 && (!xn || !rstd || !dx || !dy || (gate && !dgate) || ((post || gate || scale) && !y) || (post && !rstd_y))) return fail(DSA_ERR_ARG, "null tensor pointer");
+    if (x_f32 < DSA_STREAM_BF16 || x_f32 > DSA_STREAM_BF16_BEFORE) return fail(DSA_ERR_ARG, "x_f32=%d", x_f32);
+    if (T > 0 && (!xn || !rstd || !dx || !dy || (gate && !dgate) || ((post || gate || scale || (dh && x_f32 == DSA_STREAM_BF16_BEFORE)) && !y) || (post && !rstd_y)))
+        return fail(DSA_ERR_ARG, "null tensor pointer");
     if (off16(dxn) || off16(dh) || off16(xn) || off16(y) || off16(gate) || off16(dx) || off16(dy) || off16(dgate) || off16(ws))
         return fail(DSA_ERR_ARG, "rows and the workspace must lie on 16-byte boundaries");
     const size_t need = dsa_residual_norm_bwd_workspace_bytes(T, C);

@@ -327,8 +327,9 @@ public:
         const Tensor rstd_y = post.defined() ? empty({T}, at::kFloat, x) : Tensor();
         check(dsa_residual_norm_fwd(ptr(x), f32(x), ptr(y), ptr(gate), ptr(w), f32(w), ptr(post), f32(post), ptr(scale), f32(scale), (float)eps, offset ? 1.f : 0.f, (int)T,
                                     (int)C, ptr(xn), ptr(h), fptr(rstd), fptr(rstd_y), stream_of(x)), "dsa_residual_norm_fwd");
-        const bool through = post.defined() || gate.defined() || scale.defined();          // (y is not read otherwise)
-        ctx->save_for_backward({xn, through ? y : Tensor(), gate, w, post, scale, rstd, rstd_y});
+        // (the norm reads x' before it is rounded: of a bf16 stream x and y are kept, from which it is formed again; of an fp32 stream x', and y where it is read)
+        const bool before = !f32(x), through = post.defined() || gate.defined() || scale.defined();
+        ctx->save_for_backward({before ? x : xn, before || through ? y : Tensor(), gate, w, post, scale, rstd, rstd_y});
         ctx->saved_data["o"] = offset;
         ctx->set_materialize_grads(false);
         return {xn, h};
@@ -345,7 +346,7 @@ public:
         const Tensor dx = like(xn), dy = empty({T, C}, at::kBFloat16, xn), dgate = like(gate), dw = like(w), dpost = like(post), dscale = like(scale);
         const size_t bytes = dsa_residual_norm_bwd_workspace_bytes((int)T, (int)C);
         const Tensor ws = empty_bytes(bytes, xn);
-        check(dsa_residual_norm_bwd(ptr(dxn), ptr(dh), ptr(xn), f32(xn), ptr(y), ptr(gate), ptr(w), f32(w), ptr(post), f32(post), ptr(scale), f32(scale),
+        check(dsa_residual_norm_bwd(ptr(dxn), ptr(dh), ptr(xn), f32(xn) ? DSA_STREAM_F32 : DSA_STREAM_BF16_BEFORE, ptr(y), ptr(gate), ptr(w), f32(w), ptr(post), f32(post), ptr(scale), f32(scale),
                                     ctx->saved_data["o"].toBool() ? 1.f : 0.f, (int)T, (int)C, fptr(rstd), fptr(rstd_y), ptr(dx), ptr(dy), ptr(dgate), ptr(dw), ptr(dpost),
                                     ptr(dscale), ptr(ws), bytes, stream_of(xn)), "dsa_residual_norm_bwd");
         return {dx, dy, dw, dpost, dgate, dscale, Tensor(), Tensor()};

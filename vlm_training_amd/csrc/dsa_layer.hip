@@ -5,6 +5,7 @@
 // All are bound by memory: each row is read and written once per pass, sums stay in fp32 registers, parameter gradients are per-workgroup
 // partial sums that a second kernel adds in a fixed order (no atomics).
 #include "dsa_rows.h"
+#include "../../include/dsa_attn.h"
 
 #include <type_traits>
 
@@ -535,8 +536,9 @@ extern "C" hipError_t dsa_launch_gated_norm_bwd(const void *dy, const void *x, i
 // A row of C elements is spread over TPR threads, eight elements each: a wave up to 512, then as many waves as it takes, so that a thread holds one
 // piece of everything (with two pieces per thread the row's values and the three parameters took 256 registers, one wave per SIMD).  The next row's loads go
 // out before this row's sums.  The backward forms both norms' gradients in one pass: d = dx' + norm'(dh) goes to x as it is and on through scale, gate and the
-// first norm to y.  It takes x' as the stream keeps it, of a bf16 stream rounded: that adds to dw's error about what its own rounding to bf16 does (2.4e-3
-// instead of 1.7e-3; x and y read again would be 67 MB more for 8192 rows of 4096).  Those rows: forwards 51 us, 5.2 TB/s, backwards 63 us, 5.3 TB/s.
+// first norm to y.  The forward's norm reads x' before it is rounded: a bf16 stream's is formed again from x and y (STREAM_BEFORE), which a gate, a scale or a first norm
+// read anyway and a plain addition 67 MB more of for 8192 rows of 4096 (x' as it was rounded leaves dx off by 2.5e-3 instead of its own rounding's 1.7e-3, and dw, in
+// fp32 too, by 1.7e-3).  Those rows: forwards 51 us, 5.2 TB/s, backwards 74 us, 5.4 TB/s (of x' as it was rounded 63 us).
 struct ResidualArgs {
     const void *x;                                       // bf16 or fp32 (X32), all (T, C) contiguous
     const bf16_t *y, *gate;
@@ -544,7 +546,7 @@ struct ResidualArgs {
     int w_f32, post_f32, scale_f32, C;
     float eps, offset;
     int64_t rows;
-    void *xn;                                            // x'
+    void *xn;                                            // x';  backward, DSA_STREAM_BF16_BEFORE: x
     bf16_t *h;
     float *rstd, *rstd_y;
     const void *dxn;                                     // gradients of x' and h (null: none)
@@ -653,11 +655,13 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_fwd_k
         }
     }
 }
-template <int TPR, bool X32, bool THROUGH>
+template <int TPR, int STREAM, bool THROUGH>
 __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_bwd_kernel(ResidualArgs a) {
     constexpr int RPB = residual_threads(TPR) / TPR;
+    constexpr bool X32 = STREAM == DSA_STREAM_F32, BEFORE = STREAM == DSA_STREAM_BF16_BEFORE;
     // AHEAD: the next row's loads before this row's sums, the parameters in registers.  1024 threads have 128 registers each, which the sums of three parameters
-    // leave no room for: there every row reads the parameters again.
+    // leave no room for: there every row reads the parameters again, for each of its two sums, and forms the block's output for each (8192 rows of 8192 with norm, gate and
+    // scale, forwards and backwards: 504 us, of an fp32 stream 622; kept through the sum 945 and 728, in registers that spill).
     constexpr bool AHEAD = !(THROUGH && TPR == 1024);
     __shared__ float red[16], sums[RPB > 1 ? 256 : 1][8];
     const int c = threadIdx.x % TPR * 8, ly = threadIdx.x / TPR;
@@ -684,8 +688,8 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_bwd_k
             xr.load(a.xn, at);
             rs_next = a.rstd[clamped];
         }
+        if (THROUGH || (BEFORE && a.dh)) yr.load(a.y, at);
         if (THROUGH) {
-            yr.load(a.y, at);
             if (a.gate) gr.load(a.gate, at);
             if (a.post) ry_next = a.rstd_y[clamped];
         }
@@ -701,18 +705,28 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_bwd_k
             fetch(r);
         }
         const float rs = rs_next, ry = ry_next;
-        f32x8 d = zero8(), xh = zero8(), y = zero8(), g = zero8(), dh = zero8();
+        f32x8 d = zero8(), xh = zero8(), y = zero8(), sg = zero8() + 1.f, dh = zero8();
         if (a.dxn) d = or_zero(dr.get(), live);
         if (a.dh) {
             dh = or_zero(hr.get(), live);
-            xh = or_zero(xr.get(), live) * rs;
+            xh = or_zero(xr.get(), live);
         }
-        if (THROUGH) {
-            y = or_zero(yr.get(), live) * ry;
-            if (a.gate) g = gr.get();
-        }
+        auto block = [&]() {                             // the block's output, normed, and its gate
+            y = or_zero(yr.get(), live);
+            if (THROUGH) {
+                y *= ry;
+                if (a.gate) {
+                    const f32x8 g = gr.get();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sg[i] = sigmoid_f(g[i]);
+                }
+            }
+        };
+        if (AHEAD ? THROUGH || (BEFORE && a.dh) : BEFORE && a.dh) block();
         if (AHEAD) fetch(r + step);
         if (a.dh) {
+            if (BEFORE) xh += THROUGH ? y * post * sg * scale : y;       // (the forward's order)
+            xh *= rs;
             dw += dh * xh;
             dh *= w;
             float dot = 0.f;
@@ -722,13 +736,14 @@ __global__ __launch_bounds__(residual_threads(TPR)) void dsa_residual_norm_bwd_k
         }
         if (live) store8<X32>(a.dx, at, d);
         if (THROUGH) {
-            f32x8 sg = zero8() + 1.f;
-            const f32x8 p = y * post;                    // what gate and scale multiply
-            if (a.gate) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sg[i] = sigmoid_f(g[i]);
-                if (live) store8<false>(a.dgate, at, d * p * scale * sg * (1.f - sg));
+            if (!AHEAD) {
+                int e = cc;
+                asm volatile("" : "+v"(e), "+v"(yr.v[0]), "+v"(gr.v[0]));        // (formed again: not kept through the sum)
+                parameters(e);
+                block();
             }
+            const f32x8 p = y * post;                    // what gate and scale multiply
+            if (a.gate && live) store8<false>(a.dgate, at, d * p * scale * sg * (1.f - sg));
             dscale += or_zero(d * p * sg, live);         // (a row past the last one has its gate's copy)
             d *= scale * sg;
             if (a.post) {
@@ -783,30 +798,30 @@ extern "C" int dsa_residual_norm_blocks(int64_t rows, int C) { return residual_g
         case 512: hipLaunchKernelGGL((K<512, X, P>), dim3(GRID), dim3(512), 0, stream, a); break;                  \
         default: hipLaunchKernelGGL((K<1024, X, P>), dim3(GRID), dim3(1024), 0, stream, a); break;                 \
     }
-#define RNORM_LAUNCH(K, GRID)                                                  \
+#define RNORM_LAUNCH(K, X, GRID)                                               \
     {                                                                          \
-        const bool through = a.post || a.gate || a.scale;                      \
-        if (x_f32 && through) RNORM_SWITCH(K, true, true, GRID)                \
-        else if (x_f32) RNORM_SWITCH(K, true, false, GRID)                     \
-        else if (through) RNORM_SWITCH(K, false, true, GRID)                   \
-        else RNORM_SWITCH(K, false, false, GRID)                               \
+        if (a.post || a.gate || a.scale) RNORM_SWITCH(K, X, true, GRID)        \
+        else RNORM_SWITCH(K, X, false, GRID)                                   \
     }
 extern "C" hipError_t dsa_launch_residual_norm_fwd(const void *x, int x_f32, const void *y, const void *gate, const void *w, int w_f32, const void *post, int post_f32,
                                                    const void *scale, int scale_f32, float eps, float offset, int T, int C, void *xn, void *h, float *rstd, float *rstd_y,
                                                    hipStream_t stream) {
     ResidualArgs a = {x, (const bf16_t *)y, (const bf16_t *)gate, w, post, scale, w_f32, post_f32, scale_f32, C, eps, offset, T, xn, (bf16_t *)h, rstd, rstd_y};
     const int grid = residual_grid(T, C, 1024);
-    if (grid) RNORM_LAUNCH(dsa_residual_norm_fwd_kernel, grid)
+    if (grid && x_f32) RNORM_LAUNCH(dsa_residual_norm_fwd_kernel, true, grid)
+    else if (grid) RNORM_LAUNCH(dsa_residual_norm_fwd_kernel, false, grid)
     return hipGetLastError();
 }
-extern "C" hipError_t dsa_launch_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x_f32, const void *y, const void *gate, const void *w, int w_f32,
+extern "C" hipError_t dsa_launch_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int stream_kind, const void *y, const void *gate, const void *w, int w_f32,
                                                    const void *post, int post_f32, const void *scale, int scale_f32, float offset, int T, int C, const float *rstd,
                                                    const float *rstd_y, void *dx, void *dy, void *dgate, void *dw, void *dpost, void *dscale, float *part,
                                                    hipStream_t stream) {
     ResidualArgs a = {nullptr, (const bf16_t *)y, (const bf16_t *)gate, w, post, scale, w_f32, post_f32, scale_f32, C, 0.f, offset, T, const_cast<void *>(xn), nullptr,
                       const_cast<float *>(rstd), const_cast<float *>(rstd_y), dxn, (const bf16_t *)dh, dx, (bf16_t *)dy, (bf16_t *)dgate, part};
     const int grid = dsa_residual_norm_blocks(T, C);
-    if (grid) RNORM_LAUNCH(dsa_residual_norm_bwd_kernel, grid)
+    if (grid && stream_kind == DSA_STREAM_F32) RNORM_LAUNCH(dsa_residual_norm_bwd_kernel, DSA_STREAM_F32, grid)
+    else if (grid && stream_kind == DSA_STREAM_BF16_BEFORE) RNORM_LAUNCH(dsa_residual_norm_bwd_kernel, DSA_STREAM_BF16_BEFORE, grid)
+    else if (grid) RNORM_LAUNCH(dsa_residual_norm_bwd_kernel, DSA_STREAM_BF16, grid)
     const int at[3] = {0, C, 2 * C}, n[3] = {C, C, C}, f32[3] = {w_f32, post_f32, scale_f32};
     void *const out[3] = {dw, post ? dpost : nullptr, scale ? dscale : nullptr};
     column_sums(part, grid, 3 * (int64_t)C, 3, at, n, out, f32, stream);

@@ -45,7 +45,8 @@ def residual_rms_norm(x, y, weight, *, post_weight=None, gate=None, scale=None, 
 
     ``x' = x + scale * sigmoid(gate) * [rms_norm(y) * post_weight]``, ``h = rms_norm(x') * weight``.  ``post_weight`` (C,) norms the block's output before it
     is added, ``gate`` (..., C) and ``scale`` (a number, or (C,)) weigh it; each may be left out.  x is bf16 or fp32 and so is x'; y, gate
-    and h are bf16; C is a multiple of 8 up to 8192; ``offset=True`` scales by ``1 + weight`` in both norms.  The norm reads x' before it is rounded."""
+    and h are bf16; C is a multiple of 8 up to 8192; ``offset=True`` scales by ``1 + weight`` in both norms.  The norm reads x' before it is rounded, and its
+    gradients are taken there: for them a bf16 stream's x and y are kept, of an fp32 stream x' (and y where one of the three is given)."""
     if isinstance(scale, (int, float)):
         scale = torch.full(x.shape[-1:], float(scale), dtype=torch.float32, device=x.device)
     return tuple(_lib.host().residual_rms_norm(x, y, weight, post_weight, gate, scale, float(eps), bool(offset)))
