@@ -16,7 +16,7 @@
 // are summed over its value heads in registers, in that order.  The columns of the values are taken 64 at a time, so that two workgroups share a compute
 // unit's LDS and one's loads pass under the other's products; dO and dR are read by their own rows' wave alone.
 // 16 384 rows of 32 heads: 0.42 ms for 1.2 GB.  Neither memory (3 TB/s) nor the matrix units (a fifth) nor LDS (a third) is full: a workgroup waits for its columns'
-// loads twice a head, and registers (203 of 256) have no room for them a step earlier (there they spill: 0.6 ms; in phases that leave room, with dO, dR and N
+// loads twice a head, and registers (219 of 256) have no room for them a step earlier (there they spill: 0.6 ms; in phases that leave room, with dO, dR and N
 // read twice: 0.73 ms where this form takes 0.49).
 template <int DK, int DV>
 __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
     f32x4 dq[NT], dk[NT];                                // [16 t + 4 g4 + v][row], times scale/|q| and 1/|k|
 #pragma unroll
     for (int t = 0; t < NT; ++t) dq[t] = dk[t] = zero4();
-    float sum_q = 0.f, sum_k = 0.f;                      // q.dQ and k.dK of the heads so far, this lane's columns
+    float sum_q = 0.f, sum_k = 0.f;                      // q.dQ and k.dK over the heads, this lane's columns
     const bool live = row < c.rows;
     const bf16_t *const krow = ks + row * KS + 4 * g4, *const qrow = qs + row * KS + 4 * g4;
     auto four = [](const bf16_t *p) __attribute__((always_inline)) { return up4(*reinterpret_cast<const u32x2_any *>(p)); };
@@ -70,7 +70,9 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
         const bf16_t *const state = (const bf16_t *)(a.saved + p * a.saved_bytes), *const news = state + DV * DK;
         const bf16_t *const dstate = (const bf16_t *)(a.back + p * a.back_bytes), *const drs = dstate + DV * DK;
         f32x4 x[4], z[4];
-        float dots_ = 0.f, kx = 0.f, dot = 0.f, db = 0.f;
+        // this head's own parts of q.dQ and k.dK: dG is formed of these alone, so that a head neither loses bits to its neighbours nor takes over their NaN.  own_k: what counts
+        // for dG with a plus; dots_, kx: through dS1 and from X^T Q + Z^T K, with a minus
+        float own_q = 0.f, own_k = 0.f, dots_ = 0.f, kx = 0.f, dot = 0.f, db = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) x[t] = z[t] = zero4();
         __syncthreads();                                 // (the previous head's LDS has been read)
@@ -139,6 +141,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 nf[s] = frag_n(ns, TS, 16 * wv, 32 * s, ln);
             }
             // through S0: scale e^G dO S0^T into dQ, -beta e^G dR S0^T into dK
+            float part_q = 0.f, part_k = 0.f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 f32x4 y = zero4(), w = zero4();
@@ -150,8 +153,12 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 }
                 dq[t] += y * fq;
                 dk[t] += w * fk;
+                part_q = dot4(y, four(qrow + 16 * t), part_q);
+                part_k = dot4(w, four(krow + 16 * t), part_k);
                 if (t % 2) __builtin_amdgcn_sched_barrier(0);        // (the products' operands of all t at once are more than the registers hold)
             }
+            own_q += part_q * fq;
+            own_k += part_k * fk;
             __syncthreads();
             // dS1 in the place of S0, their product summed on the way
 #pragma unroll
@@ -199,8 +206,25 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 }
             }
             const int at = row * TS + 16 * t + 4 * g4;
-            put_split4(xs + at, xs + 64 * TS + at, xv);
-            put_split4(zs + at, zs + 64 * TS + at, zv);
+            const u32x2 xh = hi4(xv), zh = hi4(zv), xl = lo4(xv, xh), zl = lo4(zv, zh);
+            put4(xs + at, xh);
+            put4(xs + 64 * TS + at, xl);
+            put4(zs + at, zh);
+            put4(zs + 64 * TS + at, zl);
+            if (t <= wv) {
+                // q.(X K) and k.(Z K) of the row, from X and Z as the products below take them (accumulators of X K and Z K for this head alone have no registers: with
+                // them 23 spill)
+                f32x4 qk = zero4(), kk = zero4();
+#pragma unroll
+                for (int s = 0; s < DK / 32; ++s) {
+                    const bf16x8 kj = frag_n(ks, KS, 16 * t, 32 * s, ln);
+                    qk = mfma16(kj, frag_n(qs, KS, 16 * wv, 32 * s, ln), qk);
+                    kk = mfma16(kj, frag_n(ks, KS, 16 * wv, 32 * s, ln), kk);
+                }
+                own_q = dot4(qk, up4(xh) + up4(xl), own_q);
+                own_k = dot4(kk, up4(zh) + up4(zl), own_k);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) dot += __shfl_xor(dot, m, 64);
@@ -218,7 +242,6 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
                 xt[half][s] = frag_t(xh, TS, 32 * s, 16 * wv, ln);
                 zt[half][s] = frag_t(zh, TS, 32 * s, 16 * wv, ln);
             }
-        float now_q = 0.f, now_k = 0.f;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             f32x4 y = dq[t], w = dk[t], u1 = zero4();
@@ -237,14 +260,11 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             dq[t] = y;
             dk[t] = w + u1;
             kx = dot4(u1, kr, kx);
-            now_q = dot4(y, four(qrow + 16 * t), now_q);
-            now_k = dot4(dk[t], kr, now_k);
             if (t % 2) __builtin_amdgcn_sched_barrier(0);
         }
-        // what the head added to q.dQ and k.dK, less twice the part of k.dK that counts the other way
-        const float sum = over_row((now_q - sum_q) + (now_k - sum_k) - 2.f * (kx + dots_));
-        sum_q = now_q;
-        sum_k = now_k;
+        const float sum = over_row((own_q + own_k) - (kx + dots_));
+        sum_q += own_q;
+        sum_k += own_k + (kx + dots_);
         dots_ = over_row(dots_);
         db = over_row(db);
         if (g4 == 0) {
