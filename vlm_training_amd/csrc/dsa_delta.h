@@ -8,7 +8,8 @@
 //     R = beta (V - e^G K S0)     N = T R     O = scale e^G Q S0 + P N     S1 = e^G_63 S0 + K^T e^(G_63 - G) N
 // T and P depend on no state: all chunks at once; S goes from chunk to chunk, its columns independent of each other.  The factors
 // 1/|q|, 1/|k|, e^G, beta multiply rows of fp32 results, so that q, k and v enter the products as the bf16 they are; T, P, S, R and N go in as two
-// bf16 (hi + lo, 2^-17 of the value is lost), without lo x lo: where keys repeat, rows of P N are sums of 64 terms that cancel to the size of one.
+// bf16 (hi + lo, off by 2^-18 of the value at the most, a product of two, without lo x lo, by three times that): where keys repeat, rows of P N are sums of 64 terms
+// that cancel to the size of one.  One exception: the chunk gradients read S0 and dS1, which the walks keep for them, as one bf16 each (dsa_delta_bwd.hip).
 #pragma once
 #include "dsa_tile.h"
 #include "../../include/dsa_attn.h"
@@ -289,7 +290,7 @@ __device__ __forceinline__ void store_any(void *p, int64_t i, int f32, float x) 
     else reinterpret_cast<bf16_t *>(p)[i] = (bf16_t)x;
 }
 __device__ __forceinline__ float softplus_f(float x) { return x > 20.f ? x : log1pf(expf(x)); }
-// e^x for x <= 0 between rows of a chunk: off by |x| 2^-24 of its value, next to the 2^-17 that E loses in the products
+// e^x for x <= 0 between rows of a chunk: off by |x| 2^-24 of its value, next to the 2^-18 that it loses in the products
 __device__ __forceinline__ float delta_decay(float x) { return __builtin_amdgcn_exp2f(fminf(x, 0.f) * 1.442695041f); }
 // the log decay of a row.  Held above -1e4, where e^g has long been zero: a decay of -inf would make G_i - G_j of later rows NaN.  (A NaN stays one.)
 __device__ __forceinline__ float delta_gate(const dsa_delta_args &in, int64_t t, int h) {

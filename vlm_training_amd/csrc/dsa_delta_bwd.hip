@@ -7,11 +7,13 @@
 //     db = (1 - beta) dR.N                  (dR.N = beta dbeta: both of beta's places, in R and in A, at once)
 //     dG_i = q.(X K + scale e^G S0 dO) + k.(Z K - beta e^G S0 dR) - k.(X^T Q + Z^T K + e^(G_63 - G) dS1 N)
 //     dG_63 also + all k.(e^(G_63 - G) dS1 N) + e^G_63 <dS1, S0>
-// dg is the sum of dG from its row on.  What a pair of rows behind t adds comes in twice with opposite signs, from one X and Z: it leaves 2^-17 of itself.
+// dg is the sum of dG from its row on.  What a pair of rows behind t adds comes in twice with opposite signs, from one X and Z: it leaves 2^-18 of itself.
 #include "dsa_delta.h"
 
 // ---- everything that needs one chunk alone: one workgroup per chunk and key head, its value heads in turn --------------------------------
-// Wave w has rows 16 w ..; N, X and Z go into their products as hi + lo (where keys repeat, a row of X K is a sum that cancels).  Everything is formed
+// Wave w has rows 16 w ..; N, dR, X and Z go into their products as hi + lo (where keys repeat, a row of X K is a sum that cancels).  S0 and dS1 go in as one bf16,
+// off by 2^-9: dq and dk of 16 384 rows of 32 heads are off by 1.97e-3 of their 2-norm, where rounding them to bf16 makes 1.66e-3 (with N and dR, too, as one bf16
+// dk 2.25e-3).  Their low halves would be 64 KB more a chunk and head, 0.57 GB of these rows to write and to read, beside 128 KB that this kernel waits for.  Everything is formed
 // transposed (lane: its row, four neighbouring columns), so that a row's factor is one register and its sums stay in four lanes.  dq and dk of the key head
 // are summed over its value heads in registers, in that order.  The columns of the values are taken 64 at a time, so that two workgroups share a compute
 // unit's LDS and one's loads pass under the other's products; dO and dR are read by their own rows' wave alone.
@@ -135,10 +137,11 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             }
             const float rk = rows[DELTA_RK * 64 + row], eg = rows[DELTA_EG * 64 + row];
             const float fq = eg * rows[DELTA_RQ * 64 + row], fk = -rows[DELTA_BETA * 64 + row] * eg * rk, fs = rows[DELTA_EC * 64 + row] * rk;
-            bf16x8 nf[2];
+            bf16x8 nf[2], nl[2];
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 nf[s] = frag_n(ns, TS, 16 * wv, 32 * s, ln);
+                nl[s] = frag_n(ns + 64 * TS, TS, 16 * wv, 32 * s, ln);
             }
             // through S0: scale e^G dO S0^T into dQ, -beta e^G dR S0^T into dK
             float part_q = 0.f, part_k = 0.f;
@@ -148,6 +151,7 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const bf16x8 m = frag_t(ss, KS, 32 * s, 16 * t, ln);
+                    w = mfma16(m, rl[s], w);
                     y = mfma16(m, of[s], y);
                     w = mfma16(m, rf[s], w);
                 }
@@ -176,7 +180,11 @@ __global__ __launch_bounds__(256, 2) void dsa_delta_grad_kernel(DeltaArgs a) {
             for (int t = 0; t < NT; ++t) {
                 f32x4 y = zero4();
 #pragma unroll
-                for (int s = 0; s < 2; ++s) y = mfma16(frag_t(ss, KS, 32 * s, 16 * t, ln), nf[s], y);
+                for (int s = 0; s < 2; ++s) {
+                    const bf16x8 m = frag_t(ss, KS, 32 * s, 16 * t, ln);
+                    y = mfma16(m, nl[s], y);
+                    y = mfma16(m, nf[s], y);
+                }
                 dk[t] += y * fs;
                 part = dot4(y, four(krow + 16 * t), part);
                 if (t % 2) __builtin_amdgcn_sched_barrier(0);
