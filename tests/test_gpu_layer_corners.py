@@ -18,6 +18,28 @@ def _log(msg):
     print(f"[corners] {msg}", flush=True)
 
 
+def test_gated_norm_with_gates_at_the_lowest_value():
+    """silu of the lowest bf16 is -0 (its sigmoid is 0): so are the row's outputs there, and its gradients."""
+    low = torch.finfo(BF).min
+    g = torch.Generator().manual_seed(1)
+    x = {"x": torch.randn(6, 3, 64, generator=g).to(BF), "z": torch.randn(6, 3, 64, generator=g).to(BF), "w": 1 + torch.rand(64, generator=g)}
+    x["z"][1] = low
+    x["z"][2, :, ::2] = low
+    x["z"][3] = torch.tensor([-1e30, -3e4, -200., -100., -88., -60., 60., 1e4]).repeat(8).to(BF)
+    dy = torch.randn(6, 3, 64, generator=g).to(BF)
+    dy[3] *= 2.0 ** -12                                  # (its largest gate is 1e4: the others' rows set the tolerance)
+    c, d = leaves(x, "cpu"), leaves(x, DEV)
+    want = R.gated_rms_norm(*c.values())
+    want.backward(dy.double())
+    got = V.gated_rms_norm(*d.values())
+    got.backward(dy.to(DEV))
+    assert torch.isfinite(got).all() and not got[1].any()
+    close(got, want, "y")
+    for n in x:
+        assert torch.isfinite(d[n].grad).all(), n
+        close(d[n].grad, c[n].grad, n)
+
+
 @pytest.mark.parametrize("post,gate,scale", [(p, g, s) for p in (0, 1) for g in (0, 1) for s in (0, 1)])
 @pytest.mark.parametrize("T,C", [(1, 8), (130, 1000), (700, 264), (5, 2056), (3, 8192)])
 def test_gradients_of_a_bf16_stream_are_those_of_the_unrounded_one(T, C, post, gate, scale):

@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256) void dsa_gated_norm_kernel(GatedNormArgs a) {
             z = load8<false>(a.z, t * a.z_tok + hh * a.z_head + d0);
             if (BWD) g = load8<false>(a.dy, r * a.D + d0);
         }
-        f32x8 s;
+        f32x8 s;                                         // (z s first: 0 for the lowest z, which times anything else may pass fp32's range)
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[i] = sigmoid_f(z[i]);
         if (!BWD) {
@@ -466,12 +466,12 @@ __global__ __launch_bounds__(256) void dsa_gated_norm_kernel(GatedNormArgs a) {
             for (int m = 1; m < LPR; m <<= 1) ss += __shfl_xor(ss, m, 64);
             const float rs = rsqrtf(ss * (inv / SQUARE_SCALE) + a.eps);
             if (live) {
-                store8<false>(a.y, r * a.D + d0, x * rs * w * z * s);
+                store8<false>(a.y, r * a.D + d0, x * rs * w * (z * s));
                 if (d0 == 0 && a.rstd) a.rstd[r] = rs;
             }
         } else {
             const float rs = live ? a.rstd[r] : 0.f;
-            const f32x8 xh = x * rs, gs = g * z * s, dn = gs * w;
+            const f32x8 xh = x * rs, gs = g * (z * s), dn = gs * w;
             float dot = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) dot += dn[i] * xh[i];
