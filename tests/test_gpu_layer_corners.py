@@ -40,6 +40,29 @@ def test_gated_norm_with_gates_at_the_lowest_value():
         close(d[n].grad, c[n].grad, n)
 
 
+@pytest.mark.parametrize("W", [2, 3, 4])
+def test_convolution_with_large_values(W):
+    """silu'(z) is 1 for every large z and 0 for every low one."""
+    g = torch.Generator().manual_seed(W)
+    T, C = 80, 24
+    size = 2.0 ** torch.linspace(0, 40, T)[:, None]
+    x = (torch.randn(T, C, generator=g).sign() * size * (1 + torch.rand(T, C, generator=g))).to(BF)
+    x[-1] = torch.finfo(BF).min
+    w = torch.zeros(C, W)
+    w[:, W - 1] = 1.0                                    # z = x
+    dy = torch.randn(T, C, generator=g).to(BF)
+    args = {"x": x, "w": w, "b": torch.zeros(C)}
+    c, d = leaves(args, "cpu"), leaves(args, DEV)
+    want, _ = R.short_conv(c["x"], c["w"], c["b"], [T])
+    want.backward(dy.double())
+    got = V.short_conv(d["x"], d["w"], d["b"], cu_of([T]))
+    got.backward(dy.to(DEV))
+    # (below -88.7 e^-z passes fp32's range and z sigmoid(z) becomes 0: off by 89 e^-88.7 = 2.7e-37 at the most)
+    assert ((got.cpu().double() - want.detach()).abs() <= 2.0 ** -8 * want.detach().abs() + 3e-37).all() and not got[-1].any()
+    close(d["x"].grad, c["x"].grad, "dx")
+    close(d["b"].grad, c["b"].grad, "db")
+
+
 @pytest.mark.parametrize("post,gate,scale", [(p, g, s) for p in (0, 1) for g in (0, 1) for s in (0, 1)])
 @pytest.mark.parametrize("T,C", [(1, 8), (130, 1000), (700, 264), (5, 2056), (3, 8192)])
 def test_gradients_of_a_bf16_stream_are_those_of_the_unrounded_one(T, C, post, gate, scale):

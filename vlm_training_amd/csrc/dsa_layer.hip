@@ -230,8 +230,8 @@ __global__ __launch_bounds__(256, BWD ? 3 : 6) void dsa_conv_kernel(ConvArgs a) 
                 if (a.silu) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float s = sigmoid_f(z[i]), zs = z[i] * s;
-                        dz[i] *= s + zs - zs * s;
+                        const float s = sigmoid_f(z[i]);
+                        dz[i] *= s * (1.f + z[i] * (1.f - s));           // (s + z s - z s s would leave nothing of a large z's 1)
                     }
                 }
                 if (INNER || t < t1) {
