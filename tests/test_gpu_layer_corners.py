@@ -111,3 +111,25 @@ def test_stream_kinds_that_are_none_are_refused():
     n = lib.dsa_residual_norm_bwd_workspace_bytes(4, 64)
     bwd = lambda kind, y: lib.dsa_residual_norm_bwd(16, 16, 16, kind, y, None, 16, 0, None, 0, None, 0, 0.0, 4, 64, 16, None, 16, 16, None, 16, None, None, 16, n - 1, None)
     assert bwd(3, 16) == -1 and bwd(-1, 16) == -1 and bwd(2, None) == -1 and bwd(2, 16) == -3 and bwd(0, None) == -3
+
+
+def test_second_derivatives_are_refused():
+    """With create_graph the gradients are the same, and what would need their own derivatives raises - of an input, of a gradient that came in, or of everything at once -
+    rather than leave that share out."""
+    def leaf():
+        return torch.randn(70, 64, device=DEV, generator=torch.Generator(DEV).manual_seed(3)).to(BF).requires_grad_(True)
+
+    w4, n, cu = torch.randn(64, 4, device=DEV), torch.ones(64, device=DEV, requires_grad=True), cu_of([70])
+    a, p = torch.zeros(70, 1, device=DEV), torch.zeros(1, device=DEV)
+    calls = {"gated_delta_rule": lambda x: V.gated_delta_rule(*[x.unsqueeze(1)] * 3, a, a, p, p, cu).squeeze(1), "short_conv": lambda x: V.short_conv(x, w4, None, cu),
+             "gated_rms_norm": lambda x: V.gated_rms_norm(x.unsqueeze(1), x.unsqueeze(1), n).squeeze(1), "residual_rms_norm": lambda x: V.residual_rms_norm(x, x, n)[1]}
+    for name, call in calls.items():
+        x, dy = leaf(), torch.randn(70, 64, device=DEV).to(BF)
+        want, = torch.autograd.grad(call(x), x, dy)
+        dy = dy.clone().requires_grad_(True)
+        first, = torch.autograd.grad(call(x), x, dy, create_graph=True)
+        assert torch.equal(first, want) and first.requires_grad, name
+        penalty = first.float().square().sum() + x.float().square().sum() + dy.float().sum()
+        for ask in (lambda: torch.autograd.grad(penalty, x, retain_graph=True), lambda: torch.autograd.grad(penalty, dy, retain_graph=True), lambda: penalty.backward()):
+            with pytest.raises(NotImplementedError, match=name + ": second"):
+                ask()

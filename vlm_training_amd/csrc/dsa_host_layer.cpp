@@ -2,6 +2,8 @@
 // nodes, as dsa_host.cpp has them for the attention.
 #include "dsa_host.h"
 
+#include <torch/csrc/autograd/functions/utils.h>
+
 namespace {
 
 using at::ScalarType;
@@ -27,6 +29,27 @@ void no_graph(std::initializer_list<const Tensor *> inputs, const char *what) {
     if (!at::GradMode::is_enabled()) return;
     for (const Tensor *t : inputs)
         TORCH_CHECK_VALUE(!t->defined() || !t->requires_grad(), what, " has no backward pass: call it under torch.no_grad() or with detached tensors");
+}
+
+// With create_graph a backward's results carry this node: it leads to all that they depend on - the operator's inputs and the gradients that came in - and stands for
+// second derivatives, which the operators do not have.  Asked for them it raises; first derivatives are what they are without it.
+struct NoSecondDerivative : torch::autograd::Node {
+    const char *what;
+    NoSecondDerivative(const char *what, torch::autograd::edge_list &&next) : Node(std::move(next)), what(what) {}
+    variable_list apply(variable_list &&) override {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": second derivatives are not implemented");
+    }
+};
+variable_list once(variable_list results, const variable_list &grads, const char *what) {
+    if (!at::GradMode::is_enabled()) return results;
+    const auto node = torch::autograd::get_current_node();
+    torch::autograd::edge_list next = node->next_edges();
+    for (const Tensor &g : grads)
+        if (g.defined() && g.requires_grad()) next.push_back(torch::autograd::impl::gradient_edge(g));
+    const auto end = std::make_shared<NoSecondDerivative>(what, std::move(next));
+    for (Tensor &t : results)
+        if (t.defined()) torch::autograd::set_history(t, end);
+    return results;
 }
 
 // ---- gated delta rule ---------------------------------------------------------------------------------------------------
@@ -120,8 +143,8 @@ public:
         const Tensor scratch = empty_bytes(bytes, q);
         check(dsa_delta_bwd(&in.args, ptr(dout), fptr(dfinal), ptr(s[8]), (size_t)s[8].numel(), ptr(dq), ptr(dk), ptr(dv), ptr(da), ptr(db), ptr(dlog), ptr(ddt),
                             fptr(dinitial), ptr(scratch), bytes, stream_of(q)), "dsa_delta_bwd");
-        return {dq, dk, dv, da, db, dlog.to((ScalarType)ctx->saved_data["pa"].toInt()), ddt.to((ScalarType)ctx->saved_data["pd"].toInt()), Tensor(), dinitial,
-                Tensor(), Tensor(), Tensor(), Tensor()};
+        return once({dq, dk, dv, da, db, dlog.to((ScalarType)ctx->saved_data["pa"].toInt()), ddt.to((ScalarType)ctx->saved_data["pd"].toInt()), Tensor(), dinitial,
+                     Tensor(), Tensor(), Tensor(), Tensor()}, grads, "gated_delta_rule");
     }
 };
 
@@ -221,7 +244,7 @@ public:
         check(dsa_conv_bwd(ptr(x), T > 1 ? x.stride(0) : 0, ptr(dy), C, ptr(w), w.scalar_type() == at::kFloat, ptr(bias), bias.defined() && bias.scalar_type() == at::kFloat,
                            ctx->saved_data["s"].toBool(), iptr(cu), (int)T, (int)cu.numel() - 1, (int)C, (int)W, ptr(initial), ptr(dx), ptr(dw), ptr(dbias), ptr(ws), bytes,
                            stream_of(x)), "dsa_conv_bwd");
-        return {dx, dw, dbias, Tensor(), Tensor(), Tensor(), Tensor()};
+        return once({dx, dw, dbias, Tensor(), Tensor(), Tensor(), Tensor()}, grads, "short_conv");
     }
 };
 
@@ -290,7 +313,7 @@ public:
         check(dsa_gated_norm_bwd(ptr(dy), ptr(x), tok_of(x), head_of(x), ptr(z), tok_of(z), head_of(z), ptr(w), w.scalar_type() == at::kFloat,
                                  ctx->saved_data["o"].toBool() ? 1.f : 0.f, (int)T, (int)H, (int)D, fptr(rstd), ptr(dx), ptr(dz), ptr(dw), ptr(ws), bytes, stream_of(x)),
               "dsa_gated_norm_bwd");
-        return {dx, dz, dw, Tensor(), Tensor()};
+        return once({dx, dz, dw, Tensor(), Tensor()}, grads, "gated_rms_norm");
     }
 };
 
@@ -349,7 +372,7 @@ public:
         check(dsa_residual_norm_bwd(ptr(dxn), ptr(dh), ptr(xn), f32(xn) ? DSA_STREAM_F32 : DSA_STREAM_BF16_BEFORE, ptr(y), ptr(gate), ptr(w), f32(w), ptr(post), f32(post), ptr(scale), f32(scale),
                                     ctx->saved_data["o"].toBool() ? 1.f : 0.f, (int)T, (int)C, fptr(rstd), fptr(rstd_y), ptr(dx), ptr(dy), ptr(dgate), ptr(dw), ptr(dpost),
                                     ptr(dscale), ptr(ws), bytes, stream_of(xn)), "dsa_residual_norm_bwd");
-        return {dx, dy, dw, dpost, dgate, dscale, Tensor(), Tensor()};
+        return once({dx, dy, dw, dpost, dgate, dscale, Tensor(), Tensor()}, grads, "residual_rms_norm");
     }
 };
 
