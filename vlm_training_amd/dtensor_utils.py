@@ -41,3 +41,8 @@ def _dtensor_rewrap(tensor, wrap_info):
 def _local(param):
     """The local shard of a parameter, DTensor or plain."""
     return param.to_local() if _is_dtensor(param) else param
+
+
+def _column_sharded(weight) -> bool:
+    """Whether a weight's rows (its output features) lie on several ranks."""
+    return _is_dtensor(weight) and any(p.is_shard(0) and weight.device_mesh.size(i) > 1 for i, p in enumerate(weight.placements))

@@ -27,7 +27,7 @@ import torch.nn as nn
 
 from . import _lib
 from .delta import gated_delta_rule, gated_delta_step, short_conv, short_conv_step
-from .dtensor_utils import _dtensor_rewrap, _dtensor_unwrap, _local
+from .dtensor_utils import _column_sharded, _dtensor_rewrap, _dtensor_unwrap, _local
 from .model_attention import run_varlen_attn
 from .ops import dsa_varlen_attn, indexer_kl_loss
 from .prologue import gated_rms_norm, qk_norm_rope, sigmoid_gate
@@ -265,12 +265,15 @@ class DeltaState:
 class GatedDeltaNet(nn.Module):
     """models/qwen3_5/model.py:38-44,173-186 (the linear-attention layers of the hybrid stack) with the parameter names of its public checkpoints; ``cfg`` holds hidden_size,
     linear_num_key_heads, linear_num_value_heads, linear_key_head_dim, linear_value_head_dim, linear_conv_kernel_dim and
-    rms_norm_eps.  Head counts come from the projections' outputs, so a head-sharded layer sees its own."""
+    rms_norm_eps.  Head counts come from the projections' outputs: a layer whose parameters are those of some of the key heads and their value heads (rows of
+    ``in_proj_qkv`` and channels of ``conv1d`` picked from each of q, k and v, in this order) works on these.  A column shard of ``in_proj_qkv`` is not that - its rows are
+    all q, then all k, then all v - so one is refused, of ``conv1d`` too."""
 
     def __init__(self, cfg):
         super().__init__()
         self.key_dim, self.value_dim = cfg.linear_key_head_dim, cfg.linear_value_head_dim
         hk, hv = cfg.linear_num_key_heads, cfg.linear_num_value_heads
+        self.key_heads = hk
         keys, values = hk * self.key_dim, hv * self.value_dim
         self.in_proj_qkv = nn.Linear(cfg.hidden_size, 2 * keys + values, bias=False)
         self.in_proj_z = nn.Linear(cfg.hidden_size, values, bias=False)
@@ -283,11 +286,20 @@ class GatedDeltaNet(nn.Module):
         self.out_proj = nn.Linear(values, cfg.hidden_size, bias=False)
 
     def _project(self, x):
+        for name in ("in_proj_qkv", "conv1d"):
+            if _column_sharded(getattr(getattr(self, name), "weight", None)):
+                raise ValueError(f"{name}'s rows are [q | k | v]: a column shard of them is not whole heads of each; give the layer the rows of its own heads instead")
         lin = _projections(x, (self.in_proj_qkv, self.in_proj_z, self.in_proj_b, self.in_proj_a), None)
-        if lin is not None:
-            return lin, None
-        h = x.reshape(-1, x.shape[-1])
-        return _dtensor_unwrap(*(_bf16(m(h)) for m in (self.in_proj_qkv, self.in_proj_z, self.in_proj_b, self.in_proj_a)))
+        wrap = None
+        if lin is None:
+            h = x.reshape(-1, x.shape[-1])
+            lin, wrap = _dtensor_unwrap(*(_bf16(m(h)) for m in (self.in_proj_qkv, self.in_proj_z, self.in_proj_b, self.in_proj_a)))
+        channels, values, heads = lin[0].shape[1], lin[1].shape[1], lin[2].shape[1]
+        # (with fewer value heads in in_proj_z than in in_proj_qkv the difference would pass as key heads)
+        if values != heads * self.value_dim or (channels - values) % (2 * self.key_dim) or not 0 < channels - values <= 2 * self.key_heads * self.key_dim:
+            raise ValueError(f"in_proj_qkv gives {channels} channels, in_proj_z {values} and in_proj_b {heads}: not those of the same heads of {self.key_dim} and "
+                             f"{self.value_dim}, up to {self.key_heads} of them key heads")
+        return lin, wrap
 
     def _heads(self, mixed, z):
         """q, k, v and z as (rows, heads, dim) views."""
