@@ -44,3 +44,24 @@ def test_a_value_head_leaves_the_others_of_its_key_head_alone(hv, d, change):
         assert torch.equal(got[n][:, rest], want[n][:, rest]), n
     for n in ("a_log", "dt_bias"):
         assert torch.equal(got[n][rest], want[n][rest]), n
+
+
+@pytest.mark.parametrize("row", [5, 40, 100, 190])
+@pytest.mark.parametrize("lens,hv,d", [([200], 2, 128), ([200] + [3] * 40, 2, 64), ([200] + [0] * 63, 16, 128)], ids=["long", "columns", "heads"])
+def test_what_is_not_finite_leaves_rows_before_its_half_chunk(lens, hv, d, row):
+    """A row's k, v, a or b reaches its own 32-row half of a chunk and what comes behind, its q the row alone."""
+    _log(f"not finite in row {row} of {len(lens)} sequences")
+    x = {n: t.to(DEV) for n, t in inputs(sum(lens), hv // 2, hv, d, d, seed=81).items()}
+    run = lambda: V.gated_delta_rule(*(x[n] for n in NAMES), cu_of(lens))
+    want = run()
+    for n in ("k", "v", "a", "b"):
+        keep = x[n][row].clone()
+        x[n][row] = float("nan")
+        got = run()
+        x[n][row] = keep
+        lo = row // 32 * 32
+        assert torch.equal(got[:lo], want[:lo]) and torch.equal(got[200:], want[200:]), n
+        assert not torch.isfinite(got[row]).any(), n
+    x["q"][row] = float("inf")
+    got = run()
+    assert torch.equal(got[:row], want[:row]) and torch.equal(got[row + 1:], want[row + 1:])
