@@ -17,7 +17,7 @@
 // transposed (lane: its row, four neighbouring columns), so that a row's factor is one register and its sums stay in four lanes.  dq and dk of the key head
 // are summed over its value heads in registers, in that order.  The columns of the values are taken 64 at a time, so that two workgroups share a compute
 // unit's LDS and one's loads pass under the other's products; dO and dR are read by their own rows' wave alone.
-// 16 384 rows of 32 heads: 0.42 ms for 1.2 GB.  Neither memory (3 TB/s) nor the matrix units (a fifth) nor LDS (a third) is full: a workgroup waits for its columns'
+// 16 384 rows of 32 heads: 0.50 ms for 1.2 GB.  Neither memory (2.4 TB/s) nor the matrix units (a fifth) nor LDS (two fifths) is full: a workgroup waits for its columns'
 // loads twice a head, and registers (219 of 256) have no room for them a step earlier (there they spill: 0.6 ms; in phases that leave room, with dO, dR and N
 // read twice: 0.73 ms where this form takes 0.49).
 template <int DK, int DV>

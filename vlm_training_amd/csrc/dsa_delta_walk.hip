@@ -404,7 +404,9 @@ __global__ __launch_bounds__(64 * WALK_W, 2) void dsa_delta_back_kernel(DeltaArg
 extern "C" void dsa_launch_delta_chain(const DeltaArgs *a, int form, int save, hipStream_t stream);
 extern "C" void dsa_launch_delta_chain_back(const DeltaArgs *a, int form, hipStream_t stream);
 // The forms that lengths unknown to the host leave: all chunks are those of one longest sequence at the least, of N at the most.  Short batches take one that may not be
-// the best rather than launches for nothing; batches of 512 walks leave DELTA_ONE out, and of 1024 all but DELTA_HEAD (33 sequences: 8 us a launch of 310 for nothing).
+// the best rather than launches for nothing; batches of 512 walks leave DELTA_ONE out, and of 1024 all but DELTA_HEAD (33 sequences: 8 us a launch of 310 for nothing).  That goes by
+// the numbers alone, and loses where one sequence outlasts the rest: forward and backward, 32 heads, one of 8192 rows beside 32 of 64 takes 1911 us where the long one alone takes
+// 749, one of 2048 among 63 empty ones 469 where it takes 200.
 static int delta_forms(DeltaArgs &a, int (&forms)[3]) {
     const int64_t least = a.in.Hv, most = (int64_t)a.in.N * a.in.Hv;
     const int low = delta_form_of(a, least, 1), high = delta_form_of(a, most, 1), many = a.Dkp == 128 && a.Dvp == 128 && most >= 512;

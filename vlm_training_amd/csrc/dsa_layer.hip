@@ -538,7 +538,7 @@ extern "C" hipError_t dsa_launch_gated_norm_bwd(const void *dy, const void *x, i
 // out before this row's sums.  The backward forms both norms' gradients in one pass: d = dx' + norm'(dh) goes to x as it is and on through scale, gate and the
 // first norm to y.  The forward's norm reads x' before it is rounded: a bf16 stream's is formed again from x and y (STREAM_BEFORE), which a gate, a scale or a first norm
 // read anyway and a plain addition 67 MB more of for 8192 rows of 4096 (x' as it was rounded leaves dx off by 2.5e-3 instead of its own rounding's 1.7e-3, and dw, in
-// fp32 too, by 1.7e-3).  Those rows: forwards 51 us, 5.2 TB/s, backwards 74 us, 5.4 TB/s (of x' as it was rounded 63 us).
+// fp32 too, by 1.7e-3).  Those rows: forwards 51 us, 5.2 TB/s, backwards 73 us, 5.5 TB/s (of x' as it was rounded 63 us).
 struct ResidualArgs {
     const void *x;                                       // bf16 or fp32 (X32), all (T, C) contiguous
     const bf16_t *y, *gate;

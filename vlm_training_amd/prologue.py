@@ -35,7 +35,7 @@ def sigmoid_gate(x, gate):
 @torch.compiler.disable
 def gated_rms_norm(x, gate, weight, eps: float = 1e-6, offset: bool = False):
     """``rms_norm(x) * weight * silu(gate)`` per row of D for x, gate (T, H, D) bf16 views, D a multiple of 8 up to 512; ``offset=True`` scales by
-    ``1 + weight``."""
+    ``1 + weight``.  Second derivatives raise."""
     return _lib.host().gated_rms_norm(x, gate, weight, float(eps), bool(offset))
 
 
@@ -46,7 +46,8 @@ def residual_rms_norm(x, y, weight, *, post_weight=None, gate=None, scale=None, 
     ``x' = x + scale * sigmoid(gate) * [rms_norm(y) * post_weight]``, ``h = rms_norm(x') * weight``.  ``post_weight`` (C,) norms the block's output before it
     is added, ``gate`` (..., C) and ``scale`` (a number, or (C,)) weigh it; each may be left out.  x is bf16 or fp32 and so is x'; y, gate
     and h are bf16; C is a multiple of 8 up to 8192; ``offset=True`` scales by ``1 + weight`` in both norms.  The norm reads x' before it is rounded, and its
-    gradients are taken there: for them a bf16 stream's x and y are kept, of an fp32 stream x' (and y where one of the three is given)."""
+    gradients are taken there: for them a bf16 stream's x and y are kept, of an fp32 stream x' (and y where one of the three is given).  Second
+    derivatives raise."""
     if isinstance(scale, (int, float)):
         scale = torch.full(x.shape[-1:], float(scale), dtype=torch.float32, device=x.device)
     return tuple(_lib.host().residual_rms_norm(x, y, weight, post_weight, gate, scale, float(eps), bool(offset)))
