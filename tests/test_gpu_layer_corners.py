@@ -111,6 +111,8 @@ def test_stream_kinds_that_are_none_are_refused():
     n = lib.dsa_residual_norm_bwd_workspace_bytes(4, 64)
     bwd = lambda kind, y: lib.dsa_residual_norm_bwd(16, 16, 16, kind, y, None, 16, 0, None, 0, None, 0, 0.0, 4, 64, 16, None, 16, 16, None, 16, None, None, 16, n - 1, None)
     assert bwd(3, 16) == -1 and bwd(-1, 16) == -1 and bwd(2, None) == -1 and bwd(2, 16) == -3 and bwd(0, None) == -3
+    fwd = lambda kind, h: lib.dsa_residual_norm_fwd(16, kind, 16, None, 16, 0, None, 0, None, 0, 1e-6, 0.0, 4, 64, 16, h, None, None, None)
+    assert fwd(2, 16) == -1 and b"x_f32" in lib.dsa_last_error() and fwd(1, None) == -1 and b"null" in lib.dsa_last_error()
 
 
 def test_second_derivatives_are_refused():

@@ -1231,6 +1231,7 @@ extern "C" int dsa_residual_norm_fwd(const void *x, int x_f32, const void *y, co
                                      const void *scale, int scale_f32, float eps, float offset, int T, int C, void *xn, void *h, float *rstd, float *rstd_y,
                                      void *stream) {
     if (int rc = check_residual_norm(w, T, C)) return rc;
+    if (x_f32 != DSA_STREAM_BF16 && x_f32 != DSA_STREAM_F32) return fail(DSA_ERR_ARG, "x_f32=%d", x_f32);
     if (T > 0 && (!x || !y || !xn || !h)) return fail(DSA_ERR_ARG, "null tensor pointer");
     if (off16(x) || off16(y) || off16(gate) || off16(xn) || off16(h)) return fail(DSA_ERR_ARG, "rows must lie on 16-byte boundaries");
     const hipError_t e = dsa_launch_residual_norm_fwd(x, x_f32, y, gate, w, w_f32, post, post_f32, scale, scale_f32, eps, offset, T, C, xn, h, rstd, rstd_y,
