@@ -80,3 +80,23 @@ def test_heads_that_do_not_fit_each_other_are_refused():
         setattr(whole, n, getattr(half, n))
     with pytest.raises(RuntimeError, match="GPU only"):
         whole(torch.zeros(1, 5, 64), torch.tensor([0, 5], dtype=torch.int32))
+
+
+def test_every_placement_that_splits_rows_counts():
+    """Strided shards, as they come of two kinds of parallelism at once, are not of the plain ones' class."""
+    from torch.distributed.tensor import Partial, Replicate, Shard
+    from torch.distributed.tensor.placement_types import _StridedShard
+    from vlm_training_amd import dtensor_utils
+
+    class Weight:                                        # (what is looked at of a DTensor)
+        def __init__(self, *placements):
+            self.placements, self.device_mesh = placements, SimpleNamespace(size=lambda i: 1 if i == 2 else 4)
+
+    seen, dtensor_utils.DTensor = dtensor_utils.DTensor, Weight
+    try:
+        split = lambda *p: dtensor_utils._column_sharded(Weight(*p))
+        assert split(Shard(0)) and split(_StridedShard(0, split_factor=2)) and split(Replicate(), Shard(0)) and split(Shard(1), _StridedShard(0, split_factor=4))
+        assert not split(Replicate()) and not split(Shard(1)) and not split(Partial()) and not split(Replicate(), Shard(1), Shard(0)) and not split()
+    finally:
+        dtensor_utils.DTensor = seen
+    assert not dtensor_utils._column_sharded(torch.zeros(4, 4)) and not dtensor_utils._column_sharded(None)

@@ -45,4 +45,4 @@ def _local(param):
 
 def _column_sharded(weight) -> bool:
     """Whether a weight's rows (its output features) lie on several ranks."""
-    return _is_dtensor(weight) and any(p.is_shard(0) and weight.device_mesh.size(i) > 1 for i, p in enumerate(weight.placements))
+    return _is_dtensor(weight) and any(getattr(p, "dim", None) == 0 and weight.device_mesh.size(i) > 1 for i, p in enumerate(weight.placements))
