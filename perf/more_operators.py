@@ -50,7 +50,7 @@ def listed():
         dict(_case("attend", [2048], [16384]), name="attend_chunk_2k"),
         # what a scheduler with chunked prompts sends: a chunk, a short new prompt and forty requests' next tokens, 8-bit cache
         dict(_case("attend", [512, 333] + [1] * 40, [8192, 333] + _spread(40, 200, 4000), kind="e4m3"), name="attend_mixed_8bit"),
-        # odd heads, head_dim, lengths and small pages; a request without new tokens, one without anything
+        # odd heads, head_dim, lengths and small pages; a request without new tokens, one without anything, one whose first new row has no key
         dict(_case("attend", [1, 70, 0, 3, 129, 0, 17], [1, 233, 64, 3, 1000, 0, 16], hq=6, hkv=3, dim=72, page=16), name="attend_odd"),
         # the keys and values of a prompt chunk into a bf16 cache
         dict(_case("write", [8192, 1, 4095, 100], [8192, 500, 10000, 100]), name="write_12k"),
@@ -226,7 +226,7 @@ def _plain_attn(s):
             limit = torch.arange(length - new + lo, length - new + hi, device=DEV).repeat_interleave(group)
             logits.masked_fill_(torch.arange(length, device=DEV) > limit[:, None], -math.inf)
             weight = torch.exp(logits - logits.amax(-1, keepdim=True))
-            o = (weight @ v) / weight.sum(-1, keepdim=True)
+            o = torch.where(limit[:, None] >= 0, (weight @ v) / weight.sum(-1, keepdim=True), 0.0)          # (zeros for a row without a key)
             out[at + lo:at + hi] = o.view(hkv, hi - lo, group, dim).transpose(0, 1).reshape(hi - lo, hq, dim).to(q.dtype)
         at += new
     return out
@@ -308,5 +308,6 @@ def exact(case, seed):
             for h in range(hq):
                 logits = (part[:, h] @ k[h // group].T / math.sqrt(dim)).masked_fill(~seen, -math.inf)
                 o[lo:lo + 256, h] = torch.softmax(logits, -1) @ v[h // group]
+            o[lo:lo + 256][~seen.any(-1)] = 0
         out.append(o)
     return torch.cat(out)
