@@ -481,6 +481,40 @@ int dsa_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x
                           const float *rstd_y, void *dx, void *dy, void *dgate, void *dw, void *dpost, void *dscale, void *ws, size_t ws_bytes,
                           void *stream);
 
+/*
+ * Paged cache of keys and values, for serving (the reference trains only: models/qwen3_vl/model.py:230-278 and models/qwen3_5/model.py:76-136 hold no cache).
+ * k, v: pools of `pages` pages, (pages, Hkv, page, D), a page's rows contiguous, one page k_page / v_page elements behind the other; page 16, 32, 64, 128 or 256,
+ * D a multiple of 8 up to 256.  kind DSA_CACHE_BF16: bf16 rows.  DSA_CACHE_E4M3: D (a multiple of 16) e4m3 values to a row, and a byte b for each row in k_exp, v_exp
+ * (pages, Hkv, page; pages kx_page / vx_page bytes apart): a value stands for itself times 2^(b - 127), b = 255 for NaN.  Written are powers from 2^-100 on, the smallest with which a row's largest
+ * value is at most 448: what the bytes stand for is exact in bf16.  A row with a value that is not finite is NaN as a whole.
+ * table (N, table_pages) int32, rows table_row apart: position p of request n lies on page table[n][p / page], at p % page.
+ * Pools lie on 16-byte boundaries; k_page, v_page are multiples of 8 elements (e4m3: 16), kx_page, vx_page of 16 bytes.
+ * What lies on no page (a page number outside the pool, a position outside the table) is not written and reads as zero.
+ *
+ * dsa_cache_write: request n's new rows cu[n] .. cu[n+1]-1 of k, v (T,Hkv,D) bf16 (token and head strides multiples of 8, rows on 16-byte boundaries) become its last ones,
+ * positions lengths[n] - (cu[n+1] - cu[n]) on.  Two rows that go to one place race.  Rows behind cu[N] go nowhere.
+ * dsa_cache_read: rows cu[n] .. cu[n+1]-1 of k_out, v_out (T,Hkv,D) bf16, contiguous, are request n's positions first[n] on (first null: 0); rows behind cu[N] give zeros.
+ * dsa_paged_attn: q (T,Hq,D) bf16, strided as above; the new rows of request n, its last ones, attend what the cache holds of it up to and with themselves (keys that
+ * lie on no page are zero rows, positions past the table no keys).  out (T,Hq,D) bf16 contiguous, lse (Hq,T) fp32, natural, or null; a row without a key and rows behind cu[N] give zeros and -inf.
+ * max_new, max_length: upper bounds of cu[n+1] - cu[n] and of lengths (0: not known); they choose among kernels, results are right without them.  `ws` holds
+ * dsa_paged_attn_workspace_bytes(...) bytes.  Hq / Hkv up to 16.
+ */
+#define DSA_CACHE_BF16 0
+#define DSA_CACHE_E4M3 1
+typedef struct {
+    void *k, *v, *k_exp, *v_exp;
+    int64_t k_page, v_page, kx_page, vx_page;
+    const int32_t *table;
+    int64_t table_row;
+    int pages, page, table_pages, Hkv, D, kind;
+} dsa_cache_args;
+int dsa_cache_write(const dsa_cache_args *cache, const void *k, int64_t k_tok, int64_t k_head, const void *v, int64_t v_tok, int64_t v_head, const int32_t *cu_seqlens,
+                    const int32_t *lengths, int T, int N, void *stream);
+int dsa_cache_read(const dsa_cache_args *cache, const int32_t *cu_seqlens, const int32_t *first, int T, int N, void *k_out, void *v_out, void *stream);
+size_t dsa_paged_attn_workspace_bytes(const dsa_cache_args *cache, int T, int N, int Hq, int max_new, int max_length);
+int dsa_paged_attn(const dsa_cache_args *cache, const void *q, int64_t q_tok, int64_t q_head, const int32_t *cu_seqlens, const int32_t *lengths, int T, int N, int Hq,
+                   float softmax_scale, int max_new, int max_length, void *out, float *lse, void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

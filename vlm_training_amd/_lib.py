@@ -28,7 +28,18 @@ class DeltaArgs(ctypes.Structure):
                 + [(n, c_int) for n in ("l2_norm", "a_f32", "b_f32", "param_f32")])
 
 
+class CacheArgs(ctypes.Structure):
+    """dsa_cache_args of include/dsa_attn.h."""
+    _fields_ = ([(n, c_void_p) for n in ("k", "v", "k_exp", "v_exp")] + [(n, c_int64) for n in ("k_page", "v_page", "kx_page", "vx_page")]
+                + [("table", c_void_p), ("table_row", c_int64)] + [(n, c_int) for n in ("pages", "page", "table_pages", "Hkv", "D", "kind")])
+
+
 _SIGNATURES = {
+    "dsa_cache_write": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "dsa_cache_read": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "dsa_paged_attn_workspace_bytes": (c_size_t, [c_void_p, c_int, c_int, c_int, c_int, c_int]),
+    "dsa_paged_attn": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p,
+                               c_void_p, c_size_t, c_void_p]),
     "dsa_delta_workspace_bytes": (c_size_t, [c_void_p, c_int]),
     "dsa_delta_scratch_bytes": (c_size_t, [c_void_p]),
     "dsa_delta_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),

@@ -9,6 +9,7 @@
 
 #include "dsa_common.h"
 #include "dsa_delta.h"
+#include "dsa_paged.h"
 #include "../../include/dsa_attn.h"
 
 extern "C" {
@@ -22,6 +23,10 @@ hipError_t dsa_launch_gated_norm_bwd(const void *dy, const void *x, int64_t x_to
 int dsa_residual_norm_blocks(int64_t rows, int C);
 hipError_t dsa_launch_residual_norm_fwd(const void *x, int x_f32, const void *y, const void *gate, const void *w, int w_f32, const void *post, int post_f32, const void *scale, int scale_f32, float eps, float offset, int T, int C, void *xn, void *h, float *rstd, float *rstd_y, hipStream_t stream);
 hipError_t dsa_launch_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x_f32, const void *y, const void *gate, const void *w, int w_f32, const void *post, int post_f32, const void *scale, int scale_f32, float offset, int T, int C, const float *rstd, const float *rstd_y, void *dx, void *dy, void *dgate, void *dw, void *dpost, void *dscale, float *part, hipStream_t stream);
+hipError_t dsa_launch_cache_write(const dsa_cache_args *c, const void *k, int64_t k_tok, int64_t k_head, const void *v, int64_t v_tok, int64_t v_head, const int32_t *cu, const int32_t *lengths, int T, int N, hipStream_t stream);
+hipError_t dsa_launch_cache_read(const dsa_cache_args *c, const int32_t *cu, const int32_t *first, int T, int N, void *k_out, void *v_out, hipStream_t stream);
+hipError_t dsa_launch_paged_step(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream);
+hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PagePlan *plan, int Hq, int blocks, const float *part_o, const float *part_ml, void *out, float *lse, hipStream_t stream);
 hipError_t dsa_launch_delta_fwd(const DeltaArgs *a, int save, hipStream_t stream);
 hipError_t dsa_launch_delta_bwd(const DeltaArgs *a, hipStream_t stream);
 hipError_t dsa_launch_delta_step(const dsa_delta_args *in, float *state, int64_t state_req, void *out, hipStream_t stream);
@@ -1254,4 +1259,98 @@ extern "C" int dsa_residual_norm_bwd(const void *dxn, const void *dh, const void
     const hipError_t e = dsa_launch_residual_norm_bwd(dxn, dh, xn, x_f32, y, gate, w, w_f32, post, post_f32, scale, scale_f32, offset, T, C, rstd, rstd_y, dx, dy, dgate, dw,
                                                       dpost, dscale, (float *)ws, (hipStream_t)stream);
     return e == hipSuccess ? DSA_OK : hip_fail(e, "residual norm backward launch");
+}
+
+// ---- paged cache ---------------------------------------------------------------------------------------------------------
+static int check_cache(const dsa_cache_args *c, const int32_t *cu, int T, int N) {
+    if (!c) return fail(DSA_ERR_ARG, "null cache");
+    if (int rc = check_packed(T, N, cu)) return rc;
+    if (c->kind != DSA_CACHE_BF16 && c->kind != DSA_CACHE_E4M3) return fail(DSA_ERR_ARG, "unknown kind of cache: %d", c->kind);
+    const int e4m3 = c->kind == DSA_CACHE_E4M3, unit = e4m3 ? 16 : 8;
+    if (c->D < unit || c->D > 256 || c->D % unit) return fail(DSA_ERR_UNSUPPORTED, "head_dim %d: need a multiple of %d up to 256", c->D, unit);
+    if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1))) return fail(DSA_ERR_UNSUPPORTED, "pages of %d rows: need 16, 32, 64, 128 or 256", c->page);
+    if (c->pages < 1 || c->Hkv < 1 || c->table_pages < 1) return fail(DSA_ERR_ARG, "pages=%d Hkv=%d table_pages=%d", c->pages, c->Hkv, c->table_pages);
+    if (c->table_pages > INT32_MAX / c->page) return fail(DSA_ERR_UNSUPPORTED, "a table of %d pages of %d rows: positions have 31 bits", c->table_pages, c->page);
+    if (!c->k || !c->v || !c->table || (e4m3 && (!c->k_exp || !c->v_exp))) return fail(DSA_ERR_ARG, "null pool or table pointer");
+    if (N > 1 && c->table_row < c->table_pages) return fail(DSA_ERR_ARG, "table rows %lld apart hold no %d pages", (long long)c->table_row, c->table_pages);
+    if (off16(c->k) || off16(c->v) || c->k_page % unit || c->v_page % unit || (e4m3 && (off16(c->k_exp) || off16(c->v_exp) || (c->kx_page | c->vx_page) % 16)))
+        return fail(DSA_ERR_ARG, "pools and their pages must lie on 16-byte boundaries");
+    const int64_t page = (int64_t)c->Hkv * c->page * c->D, scales = (int64_t)c->Hkv * c->page;
+    if (c->pages > 1 && (c->k_page < page || c->v_page < page || (e4m3 && (c->kx_page < scales || c->vx_page < scales)))) return fail(DSA_ERR_ARG, "pages overlap");
+    return DSA_OK;
+}
+static int check_rows(const void *x, int64_t tok, int64_t head, int T, const char *name) {
+    if (T > 0 && !x) return fail(DSA_ERR_ARG, "%s is null", name);
+    if (off16(x) || (tok | head) % 8) return fail(DSA_ERR_ARG, "rows of %s must lie on 16-byte boundaries", name);
+    return DSA_OK;
+}
+extern "C" int dsa_cache_write(const dsa_cache_args *c, const void *k, int64_t k_tok, int64_t k_head, const void *v, int64_t v_tok, int64_t v_head, const int32_t *cu,
+                               const int32_t *lengths, int T, int N, void *stream) {
+    if (int rc = check_cache(c, cu, T, N)) return rc;
+    if (int rc = check_rows(k, k_tok, k_head, T, "k")) return rc;
+    if (int rc = check_rows(v, v_tok, v_head, T, "v")) return rc;
+    if (!lengths) return fail(DSA_ERR_ARG, "lengths is null");
+    if (T == 0) return DSA_OK;
+    const hipError_t e = dsa_launch_cache_write(c, k, k_tok, k_head, v, v_tok, v_head, cu, lengths, T, N, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "cache write launch");
+}
+extern "C" int dsa_cache_read(const dsa_cache_args *c, const int32_t *cu, const int32_t *first, int T, int N, void *k_out, void *v_out, void *stream) {
+    if (int rc = check_cache(c, cu, T, N)) return rc;
+    if (T == 0) return DSA_OK;
+    if (!k_out || !v_out || off16(k_out) || off16(v_out)) return fail(DSA_ERR_ARG, "k_out or v_out: null or not on a 16-byte boundary");
+    const hipError_t e = dsa_launch_cache_read(c, cu, first, T, N, k_out, v_out, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "cache read launch");
+}
+
+namespace {
+// The plan of a call, from what the host knows
+struct PagedCall {
+    PagePlan plan;
+    int64_t slots;
+    bool join;
+    size_t o_bytes, bytes;
+};
+}  // namespace
+static PagedCall paged_call(const dsa_cache_args *c, const int32_t *cu, const int32_t *lengths, int T, int N, int Hq, int max_new, int max_length) {
+    int gshift = 0;
+    while ((c->Hkv << gshift) < Hq) ++gshift;
+    const int most = max_new > 0 ? std::min(max_new, std::max(T, 1)) : std::max(T, 1), rows = most <= 16 >> gshift ? 16 : 32;
+    const int capacity = c->table_pages * c->page, longest = max_length > 0 ? std::min(max_length, capacity) : capacity;
+    PagedCall p;
+    p.plan = PagePlan{N, T, std::max(1, std::min(most, rows >> gshift)), 0, -1, std::max(1, 1024 / c->Hkv), 8, cu, lengths, capacity};
+    p.join = (longest + 31) / 32 > p.plan.least;
+    if (!p.join) p.plan.least = 1 << 30;                 // (whole walks, whatever the lengths say)
+    p.slots = page_slots(T, N, p.plan.qb, p.plan.target);
+    const size_t records = p.join ? (size_t)p.slots * c->Hkv * (p.plan.qb << gshift) : 0;
+    p.o_bytes = records * c->D * sizeof(float);
+    p.bytes = p.o_bytes + records * 2 * sizeof(float);
+    return p;
+}
+static int check_paged(const dsa_cache_args *c, const int32_t *cu, int T, int N, int Hq, int max_new, int max_length) {
+    if (int rc = check_cache(c, cu, T, N)) return rc;
+    if (Hq < 1 || Hq % c->Hkv) return fail(DSA_ERR_ARG, "Hq=%d must be a multiple of Hkv=%d", Hq, c->Hkv);
+    if (Hq / c->Hkv > 16) return fail(DSA_ERR_UNSUPPORTED, "Hq/Hkv=%d: up to 16", Hq / c->Hkv);
+    if (max_new < 0 || max_length < 0) return fail(DSA_ERR_ARG, "max_new=%d max_length=%d", max_new, max_length);
+    if (paged_call(c, cu, nullptr, T, N, Hq, max_new, max_length).slots * c->Hkv > INT32_MAX) return fail(DSA_ERR_UNSUPPORTED, "too many blocks: T=%d N=%d Hkv=%d", T, N, c->Hkv);
+    return DSA_OK;
+}
+extern "C" size_t dsa_paged_attn_workspace_bytes(const dsa_cache_args *c, int T, int N, int Hq, int max_new, int max_length) {
+    const int32_t any = 0;                               // (no offsets are looked at here)
+    if (check_paged(c, &any, T, N, Hq, max_new, max_length) || T == 0) return 0;
+    return paged_call(c, nullptr, nullptr, T, N, Hq, max_new, max_length).bytes;
+}
+extern "C" int dsa_paged_attn(const dsa_cache_args *c, const void *q, int64_t q_tok, int64_t q_head, const int32_t *cu, const int32_t *lengths, int T, int N, int Hq, float scale,
+                              int max_new, int max_length, void *out, float *lse, void *ws, size_t ws_bytes, void *stream) {
+    if (int rc = check_paged(c, cu, T, N, Hq, max_new, max_length)) return rc;
+    if (int rc = check_rows(q, q_tok, q_head, T, "q")) return rc;
+    if (!lengths) return fail(DSA_ERR_ARG, "lengths is null");
+    if (!(scale > -INFINITY && scale < INFINITY)) return fail(DSA_ERR_ARG, "softmax_scale is not finite");
+    if (T == 0) return DSA_OK;
+    if (!out || off16(out)) return fail(DSA_ERR_ARG, "out: null or not on a 16-byte boundary");
+    const PagedCall p = paged_call(c, cu, lengths, T, N, Hq, max_new, max_length);
+    if (p.bytes && (!ws || off16(ws) || ws_bytes < p.bytes)) return fail(DSA_ERR_WORKSPACE, "workspace: need %zu bytes on a 16-byte boundary, got %zu", p.bytes, ws_bytes);
+    float *const part_o = (float *)ws, *const part_ml = (float *)((char *)ws + p.o_bytes);
+    hipError_t e = dsa_launch_paged_step(c, &p.plan, q, q_tok, q_head, Hq, scale, (int)p.slots, 1, out, lse, part_o, part_ml, (hipStream_t)stream);
+    if (e == hipSuccess && p.join) e = dsa_launch_paged_join(c, &p.plan, Hq, (int)page_blocks(T, N, p.plan.qb), part_o, part_ml, out, lse, (hipStream_t)stream);
+    return e == hipSuccess ? DSA_OK : hip_fail(e, "paged attention launch");
 }

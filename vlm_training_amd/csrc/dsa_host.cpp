@@ -718,6 +718,7 @@ Tensor sigmoid_gate(const Tensor &x, const Tensor &gate) {
 }  // namespace
 
 void bind_layer(py::module_ &m);                      // dsa_host_layer.cpp
+void bind_cache(py::module_ &m);                      // dsa_host_cache.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     const auto nogil = py::call_guard<py::gil_scoped_release>();
@@ -732,4 +733,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("sigmoid_gate", &sigmoid_gate, nogil);
     m.def("project", &project, nogil);
     bind_layer(m);
+    bind_cache(m);
 }

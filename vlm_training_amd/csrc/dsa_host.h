@@ -62,4 +62,17 @@ Tensor checked_cu(const Tensor &cu) {
     return (cu.scalar_type() == at::kInt ? cu : cu.to(at::kInt)).contiguous();
 }
 
+void check_bf16_thd(const Tensor &x, const char *name) {
+    TORCH_CHECK_VALUE(x.dim() == 3 && x.scalar_type() == at::kBFloat16, name, " must be a bf16 (T, H, D) tensor");
+}
+void same_device(const Tensor &a, const Tensor &b, const char *name) {
+    TORCH_CHECK_VALUE(a.device() == b.device(), name, " is on ", b.device().str(), ", the other tensors on ", a.device().str());
+}
+int64_t tok_of(const Tensor &x) { return x.size(0) > 1 ? x.stride(0) : 0; }
+int64_t head_of(const Tensor &x) { return x.size(1) > 1 ? x.stride(1) : 0; }
+void no_graph(std::initializer_list<const Tensor *> inputs, const char *what) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const Tensor *t : inputs)
+        TORCH_CHECK_VALUE(!t->defined() || !t->requires_grad(), what, " has no backward pass: call it under torch.no_grad() or with detached tensors");
+}
 }  // namespace

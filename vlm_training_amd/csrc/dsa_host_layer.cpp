@@ -8,12 +8,6 @@ namespace {
 
 using at::ScalarType;
 
-void check_bf16_thd(const Tensor &x, const char *name) {
-    TORCH_CHECK_VALUE(x.dim() == 3 && x.scalar_type() == at::kBFloat16, name, " must be a bf16 (T, H, D) tensor");
-}
-void same_device(const Tensor &a, const Tensor &b, const char *name) {
-    TORCH_CHECK_VALUE(a.device() == b.device(), name, " is on ", b.device().str(), ", the other tensors on ", a.device().str());
-}
 // The tensor itself where its rows can be read 16 bytes at a time in place, a contiguous copy otherwise
 Tensor rows16(const Tensor &x) {
     const bool ok = x.numel() == 0 || (x.stride(2) == 1 && (x.size(1) == 1 || x.stride(1) % 8 == 0) && (x.size(0) == 1 || (x.stride(0) % 8 == 0 && x.stride(0) <= DSA_DELTA_MAX_ROW)) &&
@@ -22,14 +16,7 @@ Tensor rows16(const Tensor &x) {
     const Tensor c = x.contiguous();
     return aligned16(c) ? c : c.clone();
 }
-int64_t tok_of(const Tensor &x) { return x.size(0) > 1 ? x.stride(0) : 0; }
-int64_t head_of(const Tensor &x) { return x.size(1) > 1 ? x.stride(1) : 0; }
 bool half_or_float(const Tensor &t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
-void no_graph(std::initializer_list<const Tensor *> inputs, const char *what) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor *t : inputs)
-        TORCH_CHECK_VALUE(!t->defined() || !t->requires_grad(), what, " has no backward pass: call it under torch.no_grad() or with detached tensors");
-}
 
 // With create_graph a backward's results carry this node: it leads to all that they depend on - the operator's inputs and the gradients that came in - and stands for
 // second derivatives, which the operators do not have.  Asked for them it raises; first derivatives are what they are without it.
