@@ -83,6 +83,21 @@ def check(out, lse, q, rows, kind, new, lens, scale):
     assert (out[at:] == 0).all() and (lse is None or (lse[:, at:] == -math.inf).all())
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (256, 32)])
+def test_walks_over_many_pages(kind, dim, page):
+    """Several hundred pages to a walk; blocks in pieces; chunks that end in the middle of a block."""
+    print(kind, dim, page, flush=True)
+    new, lens = [75, 1, 40], [6500, 5300, 40]
+    rows, cache, table = make(kind, lens, 1, dim, page, seed=9)
+    q = (torch.randn(sum(new), 4, dim, generator=torch.Generator().manual_seed(1)) * 1.5).to(BF).to(DEV)
+    cu, lengths = _offsets(new).to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    for some in (slice(0, 3), slice(0, 1)):
+        n = sum(new[some])
+        out, lse = V.paged_attn(q[:n], cache, table[some], cu[:len(new[some]) + 1], lengths[some], return_lse=True)
+        check(out, lse, q[:n], rows[some], kind, new[some], lens[some], dim ** -0.5)
+
+
 GEOMETRY = [(4, 4, 64, 16), (8, 2, 128, 64), (6, 3, 72, 32), (16, 1, 128, 128), (5, 1, 80, 16), (4, 2, 256, 64), (3, 1, 96, 256), (2, 1, 8, 16), (12, 2, 144, 64)]
 
 

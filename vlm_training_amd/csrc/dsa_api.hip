@@ -26,6 +26,8 @@ hipError_t dsa_launch_residual_norm_bwd(const void *dxn, const void *dh, const v
 hipError_t dsa_launch_cache_write(const dsa_cache_args *c, const void *k, int64_t k_tok, int64_t k_head, const void *v, int64_t v_tok, int64_t v_head, const int32_t *cu, const int32_t *lengths, int T, int N, hipStream_t stream);
 hipError_t dsa_launch_cache_read(const dsa_cache_args *c, const int32_t *cu, const int32_t *first, int T, int N, void *k_out, void *v_out, hipStream_t stream);
 hipError_t dsa_launch_paged_step(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream);
+hipError_t dsa_launch_paged_walk(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream);
+hipError_t dsa_launch_paged_join_rows(const dsa_cache_args *c, const PagePlan *plan, int Hq, int blocks, const float *part_o, const float *part_ml, void *out, float *lse, hipStream_t stream);
 hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PagePlan *plan, int Hq, int blocks, const float *part_o, const float *part_ml, void *out, float *lse, hipStream_t stream);
 hipError_t dsa_launch_delta_fwd(const DeltaArgs *a, int save, hipStream_t stream);
 hipError_t dsa_launch_delta_bwd(const DeltaArgs *a, hipStream_t stream);
@@ -1303,27 +1305,42 @@ extern "C" int dsa_cache_read(const dsa_cache_args *c, const int32_t *cu, const 
 }
 
 namespace {
-// The plan of a call, from what the host knows
-struct PagedCall {
+// What a call launches, from what the host knows: the kernel for a few rows (dsa_paged_step.hip), the one for many (dsa_paged_walk.hip), or both, each for its requests.
+struct PagedLaunch {
     PagePlan plan;
-    int64_t slots;
+    int64_t blocks, slots;                               // bounds for each kv head; 0: not launched
     bool join;
-    size_t o_bytes, bytes;
+    size_t o_bytes, bytes;                               // of its partial sums
 };
+struct PagedCall { PagedLaunch step, walk; };
 }  // namespace
+static PagedLaunch paged_launch(const dsa_cache_args *c, const int32_t *cu, const int32_t *lengths, int T, int N, int gshift, int qb, int few, int side, int target, int least,
+                                int max_length) {
+    const int capacity = c->table_pages * c->page, longest = max_length > 0 ? std::min(max_length, capacity) : capacity;
+    PagedLaunch p;
+    p.plan = PagePlan{N, T, qb, few, side, std::max(1, target / c->Hkv), least, cu, lengths, capacity};
+    p.join = (longest + 31) / 32 > least;
+    if (!p.join) p.plan.least = 1 << 30;                 // (whole walks, whatever the lengths say)
+    // blocks: of requests of up to `few` rows (one block) as many as there are, of the others one for each qb rows and one more for each request
+    const int64_t requests = std::min<int64_t>(N, side == 1 ? T / (few + 1) : T);
+    p.blocks = side == 0 ? requests : T / qb + requests;
+    p.slots = p.blocks + p.plan.target + 1;              // (with a block's last piece; one more, so that some workgroup is left for the rows behind the last request)
+    const size_t records = p.join ? (size_t)p.slots * c->Hkv * (qb << gshift) : 0;
+    p.o_bytes = records * c->D * sizeof(float);
+    p.bytes = align_up(p.o_bytes + records * 2 * sizeof(float), 256);
+    return p;
+}
 static PagedCall paged_call(const dsa_cache_args *c, const int32_t *cu, const int32_t *lengths, int T, int N, int Hq, int max_new, int max_length) {
     int gshift = 0;
     while ((c->Hkv << gshift) < Hq) ++gshift;
-    const int most = max_new > 0 ? std::min(max_new, std::max(T, 1)) : std::max(T, 1), rows = most <= 16 >> gshift ? 16 : 32;
-    const int capacity = c->table_pages * c->page, longest = max_length > 0 ? std::min(max_length, capacity) : capacity;
-    PagedCall p;
-    p.plan = PagePlan{N, T, std::max(1, std::min(most, rows >> gshift)), 0, -1, std::max(1, 1024 / c->Hkv), 8, cu, lengths, capacity};
-    p.join = (longest + 31) / 32 > p.plan.least;
-    if (!p.join) p.plan.least = 1 << 30;                 // (whole walks, whatever the lengths say)
-    p.slots = page_slots(T, N, p.plan.qb, p.plan.target);
-    const size_t records = p.join ? (size_t)p.slots * c->Hkv * (p.plan.qb << gshift) : 0;
-    p.o_bytes = records * c->D * sizeof(float);
-    p.bytes = p.o_bytes + records * 2 * sizeof(float);
+    const int most = max_new > 0 ? std::min(max_new, std::max(T, 1)) : std::max(T, 1), few = std::max(1, 16 >> gshift);
+    PagedCall p{};
+    if (most <= 32 >> gshift) {
+        p.step = paged_launch(c, cu, lengths, T, N, gshift, most, 0, -1, 1024, 8, max_length);
+    } else {
+        p.walk = paged_launch(c, cu, lengths, T, N, gshift, 128 >> gshift, few, N == 1 ? -1 : 1, c->D > 128 ? 256 : 512, 16, max_length);
+        if (N > 1) p.step = paged_launch(c, cu, lengths, T, N, gshift, few, few, 0, 1024, 8, max_length);
+    }
     return p;
 }
 static int check_paged(const dsa_cache_args *c, const int32_t *cu, int T, int N, int Hq, int max_new, int max_length) {
@@ -1331,13 +1348,15 @@ static int check_paged(const dsa_cache_args *c, const int32_t *cu, int T, int N,
     if (Hq < 1 || Hq % c->Hkv) return fail(DSA_ERR_ARG, "Hq=%d must be a multiple of Hkv=%d", Hq, c->Hkv);
     if (Hq / c->Hkv > 16) return fail(DSA_ERR_UNSUPPORTED, "Hq/Hkv=%d: up to 16", Hq / c->Hkv);
     if (max_new < 0 || max_length < 0) return fail(DSA_ERR_ARG, "max_new=%d max_length=%d", max_new, max_length);
-    if (paged_call(c, cu, nullptr, T, N, Hq, max_new, max_length).slots * c->Hkv > INT32_MAX) return fail(DSA_ERR_UNSUPPORTED, "too many blocks: T=%d N=%d Hkv=%d", T, N, c->Hkv);
+    const PagedCall p = paged_call(c, cu, nullptr, T, N, Hq, max_new, max_length);
+    if (std::max(p.step.slots, p.walk.slots) * c->Hkv > INT32_MAX) return fail(DSA_ERR_UNSUPPORTED, "too many blocks: T=%d N=%d Hkv=%d", T, N, c->Hkv);
     return DSA_OK;
 }
 extern "C" size_t dsa_paged_attn_workspace_bytes(const dsa_cache_args *c, int T, int N, int Hq, int max_new, int max_length) {
     const int32_t any = 0;                               // (no offsets are looked at here)
     if (check_paged(c, &any, T, N, Hq, max_new, max_length) || T == 0) return 0;
-    return paged_call(c, nullptr, nullptr, T, N, Hq, max_new, max_length).bytes;
+    const PagedCall p = paged_call(c, nullptr, nullptr, T, N, Hq, max_new, max_length);
+    return p.step.bytes + p.walk.bytes;
 }
 extern "C" int dsa_paged_attn(const dsa_cache_args *c, const void *q, int64_t q_tok, int64_t q_head, const int32_t *cu, const int32_t *lengths, int T, int N, int Hq, float scale,
                               int max_new, int max_length, void *out, float *lse, void *ws, size_t ws_bytes, void *stream) {
@@ -1348,9 +1367,19 @@ extern "C" int dsa_paged_attn(const dsa_cache_args *c, const void *q, int64_t q_
     if (T == 0) return DSA_OK;
     if (!out || off16(out)) return fail(DSA_ERR_ARG, "out: null or not on a 16-byte boundary");
     const PagedCall p = paged_call(c, cu, lengths, T, N, Hq, max_new, max_length);
-    if (p.bytes && (!ws || off16(ws) || ws_bytes < p.bytes)) return fail(DSA_ERR_WORKSPACE, "workspace: need %zu bytes on a 16-byte boundary, got %zu", p.bytes, ws_bytes);
-    float *const part_o = (float *)ws, *const part_ml = (float *)((char *)ws + p.o_bytes);
-    hipError_t e = dsa_launch_paged_step(c, &p.plan, q, q_tok, q_head, Hq, scale, (int)p.slots, 1, out, lse, part_o, part_ml, (hipStream_t)stream);
-    if (e == hipSuccess && p.join) e = dsa_launch_paged_join(c, &p.plan, Hq, (int)page_blocks(T, N, p.plan.qb), part_o, part_ml, out, lse, (hipStream_t)stream);
+    const size_t need = p.step.bytes + p.walk.bytes;
+    if (need && (!ws || off16(ws) || ws_bytes < need)) return fail(DSA_ERR_WORKSPACE, "workspace: need %zu bytes on a 16-byte boundary, got %zu", need, ws_bytes);
+    hipError_t e = hipSuccess;
+    char *at = (char *)ws;
+    const auto run = [&](const PagedLaunch &l, auto attend, auto join) {
+        if (!l.slots || e != hipSuccess) return;
+        float *const part_o = (float *)at, *const part_ml = (float *)(at + l.o_bytes);
+        // (the kernel for many rows clears those behind the last request where both are launched)
+        e = attend(c, &l.plan, q, q_tok, q_head, Hq, scale, (int)l.slots, &l == &p.walk || !p.walk.slots, out, lse, part_o, part_ml, (hipStream_t)stream);
+        if (e == hipSuccess && l.join) e = join(c, &l.plan, Hq, (int)l.blocks, part_o, part_ml, out, lse, (hipStream_t)stream);
+        at += l.bytes;
+    };
+    run(p.walk, dsa_launch_paged_walk, dsa_launch_paged_join_rows);
+    run(p.step, dsa_launch_paged_step, dsa_launch_paged_join);
     return e == hipSuccess ? DSA_OK : hip_fail(e, "paged attention launch");
 }

@@ -128,6 +128,12 @@ __device__ __forceinline__ bool locate_piece(const PagePlan &p, int slot, PagePi
     spare = taken;
     return false;
 }
-// Slots of a launch for each kv head: pieces and blocks as the plan's bounds have them, and one more, so that some workgroup is left for the rows behind the last request
-static inline int64_t page_blocks(int T, int N, int qb) { return (int64_t)T / qb + (N < T ? N : T); }
-static inline int64_t page_slots(int T, int N, int qb, int target) { return page_blocks(T, N, qb) + target + 1; }
+// Rows behind the last request: zeros, by the workgroups that found no piece (the first of them is 0 of `step`; each its kv head's rows)
+__device__ __forceinline__ void zero_tail(const PagePlan &p, int Hq, int Hkv, int kvh, int at, int step, int d_real, int threads, bf16_t *out, float *lse) {
+    const int from = min(max(p.cu[p.N], 0), p.T), G = Hq / Hkv, tid = threadIdx.x;
+    for (int t = from + at; t < p.T; t += step) {
+        bf16_t *const row = out + ((int64_t)t * Hq + kvh * G) * d_real;
+        for (int i = tid; i < G * d_real / 8; i += threads) *reinterpret_cast<u32x4 *>(row + 8 * i) = u32x4{0u, 0u, 0u, 0u};
+        if (lse && tid < G) lse[(int64_t)(kvh * G + tid) * p.T + t] = -INFINITY;
+    }
+}

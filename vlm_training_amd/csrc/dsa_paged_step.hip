@@ -43,14 +43,7 @@ __global__ __launch_bounds__(NW * 64, 1) void dsa_paged_step_kernel(dsa_cache_ar
     PagePiece pc;
     int spare;
     if (!locate_piece<false>(plan, blockIdx.x / Hkv, pc, spare)) {
-        if (!tail) return;
-        // rows behind the last request: zeros
-        const int from = min(max(plan.cu[plan.N], 0), T), step = slots - spare;
-        for (int t = from + blockIdx.x / Hkv - spare; t < T; t += step) {
-            bf16_t *const row = out + ((int64_t)t * Hq + kvh * G) * d_real;
-            for (int i = tid; i < G * d_real / 8; i += NW * 64) *reinterpret_cast<u32x4 *>(row + 8 * i) = u32x4{0u, 0u, 0u, 0u};
-            if (lse && tid < G) lse[(int64_t)(kvh * G + tid) * T + t] = -INFINITY;
-        }
+        if (tail) zero_tail(plan, Hq, Hkv, kvh, blockIdx.x / Hkv - spare, slots - spare, d_real, NW * 64, out, lse);
         return;
     }
     if (pc.piece >= pc.pieces) return;
@@ -401,6 +394,36 @@ __global__ __launch_bounds__(256) void dsa_paged_join_kernel(dsa_cache_args c, P
     if (lse && tid == 0) lse[hq * plan.T + t] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * LN2_F;
 }
 
+// The same for blocks of many rows, in few pieces: 32 lanes to a row
+__global__ __launch_bounds__(256) void dsa_paged_join_rows_kernel(dsa_cache_args c, PagePlan plan, int Hq, int gshift, const float *__restrict__ part_o, const float *__restrict__ part_ml,
+                                                                  bf16_t *__restrict__ out, float *__restrict__ lse) {
+    const int Hkv = c.Hkv, G = Hq / Hkv, d_real = c.D, rows = plan.qb << gshift, row = blockIdx.y * 8 + threadIdx.x / 32, sub = threadIdx.x % 32;
+    const int kvh = blockIdx.x % Hkv;
+    PagePiece pc;
+    int spare;
+    if (!locate_piece<true>(plan, blockIdx.x / Hkv, pc, spare) || pc.pieces <= 1) return;
+    const int query = pc.first + (row >> gshift), head = row & ((1 << gshift) - 1);
+    if (row >= rows || query >= pc.m || head >= G) return;
+    const int64_t first = ((int64_t)pc.slot * Hkv + kvh) * rows + row, step = (int64_t)Hkv * rows, t = pc.row0 + query, hq = kvh * G + head;
+    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < pc.pieces; ++i) m = fmaxf(m, part_ml[2 * (first + i * step)]);
+    for (int d = 4 * sub; d < d_real; d += 128) {
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        l = 0.f;
+        for (int i = 0; i < pc.pieces; ++i) {
+            const f32x2 ml = *reinterpret_cast<const f32x2 *>(part_ml + 2 * (first + i * step));
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(part_o + (first + i * step) * d_real + d);
+            const float w = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - m);
+            l = fmaf(w, ml[1], l);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, x[e], o[e]);
+        }
+        const float inv = m == -INFINITY ? 0.f : 1.f / l;
+        *reinterpret_cast<u32x2 *>(out + (t * Hq + hq) * d_real + d) = u32x2{pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)};
+    }
+    if (lse && sub == 0) lse[hq * plan.T + t] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * LN2_F;
+}
+
 template <int D, bool E4M3, int RG>
 hipError_t launch_step(const dsa_cache_args &c, const PagePlan &plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, int gshift, int pshift, float scale, int slots,
                        int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream) {
@@ -438,6 +461,13 @@ extern "C" hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PageP
                                             hipStream_t stream) {
     const int gshift = group_shift(Hq, c->Hkv);
     hipLaunchKernelGGL(dsa_paged_join_kernel, dim3((unsigned)blocks * c->Hkv, (unsigned)(plan->qb << gshift)), dim3(256), 0, stream, *c, *plan, Hq, gshift, part_o, part_ml,
+                       (bf16_t *)out, lse);
+    return hipGetLastError();
+}
+extern "C" hipError_t dsa_launch_paged_join_rows(const dsa_cache_args *c, const PagePlan *plan, int Hq, int blocks, const float *part_o, const float *part_ml, void *out, float *lse,
+                                                 hipStream_t stream) {
+    const int gshift = group_shift(Hq, c->Hkv);
+    hipLaunchKernelGGL(dsa_paged_join_rows_kernel, dim3((unsigned)blocks * c->Hkv, (unsigned)((plan->qb << gshift) + 7) / 8), dim3(256), 0, stream, *c, *plan, Hq, gshift, part_o, part_ml,
                        (bf16_t *)out, lse);
     return hipGetLastError();
 }
