@@ -27,7 +27,6 @@ hipError_t dsa_launch_cache_write(const dsa_cache_args *c, const void *k, int64_
 hipError_t dsa_launch_cache_read(const dsa_cache_args *c, const int32_t *cu, const int32_t *first, int T, int N, void *k_out, void *v_out, hipStream_t stream);
 hipError_t dsa_launch_paged_step(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream);
 hipError_t dsa_launch_paged_walk(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream);
-hipError_t dsa_launch_paged_join_rows(const dsa_cache_args *c, const PagePlan *plan, int Hq, int blocks, const float *part_o, const float *part_ml, void *out, float *lse, hipStream_t stream);
 hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PagePlan *plan, int Hq, int blocks, const float *part_o, const float *part_ml, void *out, float *lse, hipStream_t stream);
 hipError_t dsa_launch_delta_fwd(const DeltaArgs *a, int save, hipStream_t stream);
 hipError_t dsa_launch_delta_bwd(const DeltaArgs *a, hipStream_t stream);
@@ -1314,16 +1313,19 @@ struct PagedLaunch {
 };
 struct PagedCall { PagedLaunch step, walk; };
 }  // namespace
-static PagedLaunch paged_launch(const dsa_cache_args *c, const int32_t *cu, const int32_t *lengths, int T, int N, int gshift, int qb, int few, int side, int target, int least,
+static PagedLaunch paged_launch(const dsa_cache_args *c, const int32_t *cu, const int32_t *lengths, int T, int N, int gshift, int qb, int few, int side, bool many, int resident, int least,
                                 int max_length) {
     const int capacity = c->table_pages * c->page, longest = max_length > 0 ? std::min(max_length, capacity) : capacity;
     PagedLaunch p;
-    p.plan = PagePlan{N, T, qb, few, side, std::max(1, target / c->Hkv), least, cu, lengths, capacity};
+    p.plan = PagePlan{N, T, qb, few, side, 0, least, cu, lengths, capacity};
     p.join = (longest + 31) / 32 > least;
     if (!p.join) p.plan.least = 1 << 30;                 // (whole walks, whatever the lengths say)
-    // blocks: of requests of up to `few` rows (one block) as many as there are, of the others one for each qb rows and one more for each request
+    // blocks: of requests of up to `few` rows (one block) as many as there are, of the others the rows' and what the last one of each request lacks
     const int64_t requests = std::min<int64_t>(N, side == 1 ? T / (few + 1) : T);
-    p.blocks = side == 0 ? requests : T / qb + requests;
+    p.blocks = side == 0 ? requests : (T + requests * (qb - 1)) / qb;
+    // Pieces: where blocks are few, so many that all workgroups run at once; else (few rows) two rounds of them, or as many as there are blocks
+    const int64_t at_once = resident / c->Hkv;
+    p.plan.target = (int)std::max<int64_t>(1, 2 * p.blocks <= at_once ? at_once - p.blocks : many ? at_once : std::max(2 * at_once, p.blocks));
     p.slots = p.blocks + p.plan.target + 1;              // (with a block's last piece; one more, so that some workgroup is left for the rows behind the last request)
     const size_t records = p.join ? (size_t)p.slots * c->Hkv * (qb << gshift) : 0;
     p.o_bytes = records * c->D * sizeof(float);
@@ -1334,12 +1336,14 @@ static PagedCall paged_call(const dsa_cache_args *c, const int32_t *cu, const in
     int gshift = 0;
     while ((c->Hkv << gshift) < Hq) ++gshift;
     const int most = max_new > 0 ? std::min(max_new, std::max(T, 1)) : std::max(T, 1), few = std::max(1, 16 >> gshift);
+    // workgroups that run at once, by their LDS
+    const int by_step = 256 * (c->D > 128 || (c->D > 64 && c->kind == DSA_CACHE_BF16) ? 1 : 2), by_walk = c->D > 128 ? 256 : 512;
     PagedCall p{};
     if (most <= 32 >> gshift) {
-        p.step = paged_launch(c, cu, lengths, T, N, gshift, most, 0, -1, 1024, 8, max_length);
+        p.step = paged_launch(c, cu, lengths, T, N, gshift, most, 0, -1, false, by_step, 4, max_length);
     } else {
-        p.walk = paged_launch(c, cu, lengths, T, N, gshift, 128 >> gshift, few, N == 1 ? -1 : 1, c->D > 128 ? 256 : 512, 16, max_length);
-        if (N > 1) p.step = paged_launch(c, cu, lengths, T, N, gshift, few, few, 0, 1024, 8, max_length);
+        p.walk = paged_launch(c, cu, lengths, T, N, gshift, 128 >> gshift, few, N == 1 ? -1 : 1, true, by_walk, 16, max_length);
+        if (N > 1) p.step = paged_launch(c, cu, lengths, T, N, gshift, few, few, 0, false, by_step, 4, max_length);
     }
     return p;
 }
@@ -1371,15 +1375,15 @@ extern "C" int dsa_paged_attn(const dsa_cache_args *c, const void *q, int64_t q_
     if (need && (!ws || off16(ws) || ws_bytes < need)) return fail(DSA_ERR_WORKSPACE, "workspace: need %zu bytes on a 16-byte boundary, got %zu", need, ws_bytes);
     hipError_t e = hipSuccess;
     char *at = (char *)ws;
-    const auto run = [&](const PagedLaunch &l, auto attend, auto join) {
+    const auto run = [&](const PagedLaunch &l, auto attend) {
         if (!l.slots || e != hipSuccess) return;
         float *const part_o = (float *)at, *const part_ml = (float *)(at + l.o_bytes);
         // (the kernel for many rows clears those behind the last request where both are launched)
         e = attend(c, &l.plan, q, q_tok, q_head, Hq, scale, (int)l.slots, &l == &p.walk || !p.walk.slots, out, lse, part_o, part_ml, (hipStream_t)stream);
-        if (e == hipSuccess && l.join) e = join(c, &l.plan, Hq, (int)l.blocks, part_o, part_ml, out, lse, (hipStream_t)stream);
+        if (e == hipSuccess && l.join) e = dsa_launch_paged_join(c, &l.plan, Hq, (int)l.blocks, part_o, part_ml, out, lse, (hipStream_t)stream);
         at += l.bytes;
     };
-    run(p.walk, dsa_launch_paged_walk, dsa_launch_paged_join_rows);
-    run(p.step, dsa_launch_paged_step, dsa_launch_paged_join);
+    run(p.walk, dsa_launch_paged_walk);
+    run(p.step, dsa_launch_paged_step);
     return e == hipSuccess ? DSA_OK : hip_fail(e, "paged attention launch");
 }

@@ -1,6 +1,6 @@
 // The paged cache as kernels see it: where a row lies, e4m3 values as bf16, and how the work of an attention over it is cut.
 #pragma once
-#include "dsa_common.h"
+#include "dsa_tile.h"
 #include "../../include/dsa_attn.h"
 
 // the request whose rows row t lies among: the last n with cu[n] <= t (empty ones are stepped over), by a whole wave.  64 offsets are looked at in one round
@@ -70,37 +70,33 @@ __device__ __forceinline__ PageRequest page_request(const PagePlan &p, int n) {
     r.tiles = (min(r.length, p.capacity) + 31) >> 5;
     return r;
 }
-// tiles to a piece
-__device__ __forceinline__ int piece_tiles(const PagePlan &p) {
-    const int lane = threadIdx.x & 63;
-    float sum = 0.f;
-    for (int n = lane; n < p.N; n += 64) {
-        const PageRequest r = page_request(p, n);
-        sum += (float)r.blocks * (float)r.tiles;
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    // (a little over the sum's own rounding: the slots of a launch are counted for this many pieces)
-    const float per = ceilf(sum * 1.0001f / (float)p.target);
-    return __builtin_amdgcn_readfirstlane(max(p.least, (int)fminf(per, 1e9f)));
+// Sums over the wave by DPP steps (no LDS round trips: a workgroup forms them in front of its first load)
+__device__ __forceinline__ float plan_sum(float x) {
+#define PLAN_STEP(ctrl, rows) x += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), ctrl, rows, 0xf, false))
+    PLAN_STEP(0x111, 0xf); PLAN_STEP(0x112, 0xf); PLAN_STEP(0x114, 0xf); PLAN_STEP(0x118, 0xf); PLAN_STEP(0x142, 0xa); PLAN_STEP(0x143, 0xc);
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), 63));
+#undef PLAN_STEP
 }
-__device__ __forceinline__ int lane_prefix(int x) {                // sums over the lanes up to and with one's own
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int y = __shfl_up(x, off, 64);
-        if ((threadIdx.x & 63) >= off) x += y;
-    }
-    return x;
+// tiles to a piece, from the sum of all blocks' tiles (a little over the sum's own rounding: the slots of a launch are counted for this many pieces)
+__device__ __forceinline__ int piece_tiles(const PagePlan &p, float mine) {
+    return max(p.least, (int)fminf(ceilf(plan_sum(mine) * 1.0001f / (float)p.target), 1e9f));
 }
 // Piece `slot` (BLOCKS: block `slot`) of the launch; false past the last one, with `spare` the number of slots in front that are taken
 template <bool BLOCKS>
 __device__ __forceinline__ bool locate_piece(const PagePlan &p, int slot, PagePiece &out, int &spare) {
-    const int lane = threadIdx.x & 63, per = piece_tiles(p);
+    const int lane = threadIdx.x & 63;
+    PageRequest r = page_request(p, lane);               // (up to 64 requests: looked at once)
+    float sum = (float)r.blocks * (float)r.tiles;
+    for (int n = 64 + lane; n < p.N; n += 64) {
+        const PageRequest x = page_request(p, n);
+        sum += (float)x.blocks * (float)x.tiles;
+    }
+    const int per = piece_tiles(p, sum);
     int slots = 0, taken = 0;                            // of pieces, and of what is counted
     for (int base = 0; base < p.N; base += 64) {
-        const PageRequest r = page_request(p, base + lane);
+        if (base > 0) r = page_request(p, base + lane);
         const int np = max(1, (r.tiles + per - 1) / per), mine = r.blocks * np, count = BLOCKS ? r.blocks : mine;
-        const int upto = lane_prefix(count), slots_upto = BLOCKS ? lane_prefix(mine) : upto;
+        const int upto = wave_prefix_i(count), slots_upto = BLOCKS ? wave_prefix_i(mine) : upto;
         const uint64_t past = __builtin_amdgcn_ballot_w64(taken + upto > slot);
         if (past) {
             const int w = (int)__builtin_ctzll(past);

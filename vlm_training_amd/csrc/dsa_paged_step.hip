@@ -10,7 +10,7 @@
 //
 // P is rounded to bf16 for the second product (each probability by at most 2^-9 of itself, at random); its sum, the statistics and the output's sums are fp32.
 #include "dsa_paged.h"
-#include "dsa_tile.h"
+#include <algorithm>
 
 namespace {
 
@@ -327,101 +327,69 @@ __global__ __launch_bounds__(NW * 64, 1) void dsa_paged_step_kernel(dsa_cache_ar
     }
 }
 
-// The pieces of a block: out = sum of 2^(m_i - m) O_i over sum of 2^(m_i - m) l_i, in the order of the pieces.  One workgroup for each block, kv head and row.
+// The pieces of a block: out = sum of 2^(m_i - m) O_i over sum of 2^(m_i - m) l_i, in a fixed order.  A workgroup takes ITEMS of the block's rows' four columns at a time and
+// has 256 / ITEMS threads for each, which take every so many-th piece: 32 where a few blocks have many pieces (a long request by itself), 256 elsewhere.
+template <int ITEMS>
 __global__ __launch_bounds__(256) void dsa_paged_join_kernel(dsa_cache_args c, PagePlan plan, int Hq, int gshift, const float *__restrict__ part_o, const float *__restrict__ part_ml,
                                                              bf16_t *__restrict__ out, float *__restrict__ lse) {
-    const int Hkv = c.Hkv, G = Hq / Hkv, d_real = c.D, rows = plan.qb << gshift, row = blockIdx.y;
-    const int kvh = blockIdx.x % Hkv;
+    constexpr int GROUPS = 256 / ITEMS;
+    const int Hkv = c.Hkv, G = Hq / Hkv, d_real = c.D, rows = plan.qb << gshift, cols = d_real / 4, kvh = blockIdx.x % Hkv;
     PagePiece pc;
     int spare;
     if (!locate_piece<true>(plan, blockIdx.x / Hkv, pc, spare) || pc.pieces <= 1) return;
-    const int query = pc.first + (row >> gshift), head = row & ((1 << gshift) - 1);
-    if (query >= pc.m || head >= G) return;
-    __shared__ float weight[256], sums[2][256];
-    const int tid = threadIdx.x, cols = d_real / 4;       // four columns a thread, as many groups of threads as there is room for: each takes every so many-th piece
-    const int groups = 256 / cols, group = tid / cols, d = tid % cols * 4;
-    const int64_t first = ((int64_t)pc.slot * Hkv + kvh) * rows + row, step = (int64_t)Hkv * rows;
-    float m = -INFINITY;
-    for (int i = tid; i < pc.pieces; i += 256) m = fmaxf(m, part_ml[2 * (first + i * step)]);
-    sums[0][tid] = m;
-    __syncthreads();
-    for (int off = 128; off > 0; off >>= 1) {
-        if (tid < off) sums[0][tid] = fmaxf(sums[0][tid], sums[0][tid + off]);
-        __syncthreads();
-    }
-    m = sums[0][0];
-    __syncthreads();
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    for (int base = 0; base < pc.pieces; base += 256) {
-        const int i = base + tid;
-        float w = 0.f;
-        if (i < pc.pieces) {
-            const f32x2 ml = *reinterpret_cast<const f32x2 *>(part_ml + 2 * (first + i * step));
-            w = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - m);
-            l = fmaf(w, ml[1], l);
-        }
-        weight[tid] = w;
-        __syncthreads();
-        if (group < groups)
-            for (int k = group; k < 256 && base + k < pc.pieces; k += groups) {
-                const float f = weight[k];
-                if (f != 0.f) {
-                    const f32x4 x = *reinterpret_cast<const f32x4 *>(part_o + (first + (base + k) * step) * d_real + d);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
-                }
-            }
-        __syncthreads();
-    }
-    __shared__ f32x4 parts[256];
-    parts[tid] = o;
-    sums[1][tid] = l;
-    __syncthreads();
-    for (int off = 128; off > 0; off >>= 1) {
-        if (tid < off) sums[1][tid] += sums[1][tid + off];
-        __syncthreads();
-    }
-    l = sums[1][0];
-    const int64_t t = pc.row0 + query, hq = kvh * G + head;
-    if (group == 0) {
-        for (int k = 1; k < groups; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] += parts[k * cols + tid][e];
-        const float inv = m == -INFINITY ? 0.f : 1.f / l;
-        *reinterpret_cast<u32x2 *>(out + (t * Hq + hq) * d_real + d) = u32x2{pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)};
-    }
-    if (lse && tid == 0) lse[hq * plan.T + t] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * LN2_F;
-}
-
-// The same for blocks of many rows, in few pieces: 32 lanes to a row
-__global__ __launch_bounds__(256) void dsa_paged_join_rows_kernel(dsa_cache_args c, PagePlan plan, int Hq, int gshift, const float *__restrict__ part_o, const float *__restrict__ part_ml,
-                                                                  bf16_t *__restrict__ out, float *__restrict__ lse) {
-    const int Hkv = c.Hkv, G = Hq / Hkv, d_real = c.D, rows = plan.qb << gshift, row = blockIdx.y * 8 + threadIdx.x / 32, sub = threadIdx.x % 32;
-    const int kvh = blockIdx.x % Hkv;
-    PagePiece pc;
-    int spare;
-    if (!locate_piece<true>(plan, blockIdx.x / Hkv, pc, spare) || pc.pieces <= 1) return;
-    const int query = pc.first + (row >> gshift), head = row & ((1 << gshift) - 1);
-    if (row >= rows || query >= pc.m || head >= G) return;
-    const int64_t first = ((int64_t)pc.slot * Hkv + kvh) * rows + row, step = (int64_t)Hkv * rows, t = pc.row0 + query, hq = kvh * G + head;
-    float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < pc.pieces; ++i) m = fmaxf(m, part_ml[2 * (first + i * step)]);
-    for (int d = 4 * sub; d < d_real; d += 128) {
+    __shared__ f32x4 sums[GROUPS > 1 ? 256 : 1];
+    __shared__ f32x2 stats[GROUPS > 1 ? 256 : 1];
+    const int tid = threadIdx.x, group = tid / ITEMS, live = min(pc.m - pc.first, plan.qb) << gshift;
+    const int64_t first = (int64_t)pc.slot * Hkv + kvh;
+    for (int base = blockIdx.y * ITEMS; base < live * cols; base += gridDim.y * ITEMS) {
+        const int item = base + tid % ITEMS, row = item / cols, d = item % cols * 4, head = row & ((1 << gshift) - 1);
+        const bool mine = item < live * cols && head < G;
+        float m = -INFINITY, l = 0.f;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        l = 0.f;
-        for (int i = 0; i < pc.pieces; ++i) {
-            const f32x2 ml = *reinterpret_cast<const f32x2 *>(part_ml + 2 * (first + i * step));
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(part_o + (first + i * step) * d_real + d);
-            const float w = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - m);
-            l = fmaf(w, ml[1], l);
+        if (mine) {
+            const int64_t at = first * rows + row, step = (int64_t)Hkv * rows;
+            // the largest first: the loads of sums and weights then wait for nothing
+            for (int i = group; i < pc.pieces; i += GROUPS) m = fmaxf(m, part_ml[2 * (at + i * step)]);
+#pragma unroll 4
+            for (int i = group; i < pc.pieces; i += GROUPS) {
+                const f32x2 ml = *reinterpret_cast<const f32x2 *>(part_ml + 2 * (at + i * step));
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(part_o + (at + i * step) * d_real + d);
+                const float w = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - m);
+                l = fmaf(w, ml[1], l);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, x[e], o[e]);
+                for (int e = 0; e < 4; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, x[e], o[e]);
+            }
         }
-        const float inv = m == -INFINITY ? 0.f : 1.f / l;
-        *reinterpret_cast<u32x2 *>(out + (t * Hq + hq) * d_real + d) = u32x2{pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)};
+        if constexpr (GROUPS > 1) {
+            __syncthreads();
+            sums[tid] = o;
+            stats[tid] = f32x2{m, l};
+            __syncthreads();
+            if (group == 0) {
+                float most = m;
+#pragma unroll
+                for (int k = 1; k < GROUPS; ++k) most = fmaxf(most, stats[k * ITEMS + tid][0]);
+                l = 0.f;
+                o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < GROUPS; ++k) {
+                    const f32x2 ml = stats[k * ITEMS + tid];
+                    const f32x4 x = sums[k * ITEMS + tid];
+                    const float w = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - most);
+                    l = fmaf(w, ml[1], l);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, x[e], o[e]);
+                }
+                m = most;
+            }
+        }
+        if (mine && group == 0) {
+            const int64_t t = pc.row0 + pc.first + (row >> gshift), hq = kvh * G + head;
+            const float inv = m == -INFINITY ? 0.f : 1.f / l;
+            *reinterpret_cast<u32x2 *>(out + (t * Hq + hq) * d_real + d) = u32x2{pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)};
+            if (lse && d == 0) lse[hq * plan.T + t] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * LN2_F;
+        }
     }
-    if (lse && sub == 0) lse[hq * plan.T + t] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * LN2_F;
 }
 
 template <int D, bool E4M3, int RG>
@@ -459,15 +427,11 @@ extern "C" hipError_t dsa_launch_paged_step(const dsa_cache_args *c, const PageP
 }
 extern "C" hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PagePlan *plan, int Hq, int blocks, const float *part_o, const float *part_ml, void *out, float *lse,
                                             hipStream_t stream) {
-    const int gshift = group_shift(Hq, c->Hkv);
-    hipLaunchKernelGGL(dsa_paged_join_kernel, dim3((unsigned)blocks * c->Hkv, (unsigned)(plan->qb << gshift)), dim3(256), 0, stream, *c, *plan, Hq, gshift, part_o, part_ml,
-                       (bf16_t *)out, lse);
-    return hipGetLastError();
-}
-extern "C" hipError_t dsa_launch_paged_join_rows(const dsa_cache_args *c, const PagePlan *plan, int Hq, int blocks, const float *part_o, const float *part_ml, void *out, float *lse,
-                                                 hipStream_t stream) {
-    const int gshift = group_shift(Hq, c->Hkv);
-    hipLaunchKernelGGL(dsa_paged_join_rows_kernel, dim3((unsigned)blocks * c->Hkv, (unsigned)((plan->qb << gshift) + 7) / 8), dim3(256), 0, stream, *c, *plan, Hq, gshift, part_o, part_ml,
-                       (bf16_t *)out, lse);
+    const int gshift = group_shift(Hq, c->Hkv), items = (plan->qb << gshift) * c->D / 4, wg = blocks * c->Hkv;
+    // workgroups enough for the card where the blocks alone are not
+    const bool many = (int64_t)wg * ((items + 255) / 256) < 256;
+    const int y = many ? (items + 31) / 32 : std::max(1, std::min((items + 255) / 256, 2048 / wg));
+    const auto kernel = many ? &dsa_paged_join_kernel<32> : &dsa_paged_join_kernel<256>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)wg, (unsigned)y), dim3(256), 0, stream, *c, *plan, Hq, gshift, part_o, part_ml, (bf16_t *)out, lse);
     return hipGetLastError();
 }

@@ -12,7 +12,6 @@
 // one: values are loaded into registers two steps ahead of the step that writes them to LDS as bf16, K(t+4) and V(t+2) in step t: one conversion for 128 rows, and no rounding, as
 // the scales are powers of two.
 #include "dsa_paged.h"
-#include "dsa_tile.h"
 
 namespace {
 
@@ -20,7 +19,8 @@ constexpr int WALK_WAVES = 4;
 template <int D>
 constexpr int walk_lds_bytes() { return 8 * DirectTile<D>::BYTES + WALK_WAVES * 512 + 16; }
 
-template <int D, bool E4M3>
+// AGPR: the sums in accumulation registers, by name (mfma32_agpr_late)
+template <int D, bool E4M3, bool AGPR>
 __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_walk_kernel(dsa_cache_args c, PagePlan plan, const bf16_t *__restrict__ q, int64_t q_tok, int64_t q_head,
                                                                                            int Hq, int gshift, int pshift, float scale_log2, uint32_t flip, int slots, int tail,
                                                                                            bf16_t *__restrict__ out, float *__restrict__ lse, float *__restrict__ part_o,
@@ -53,9 +53,16 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     float mrun = -INFINITY, lsum = 0.f;
     f32x16 oacc[DT];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) oacc[dt] = zero16();
+    for (int dt = 0; dt < DT; ++dt) {
+        oacc[dt] = zero16();
+        if (AGPR) settle(oacc[dt]);
+    }
     auto finish = [&]() __attribute__((always_inline)) {
         const float l = half_sum_f(lsum);
+        if (AGPR) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) settle(oacc[dt]);
+        }
         if (!row_ok) return;
         if (whole_out) {
             const float inv = mrun == -INFINITY ? 0.f : 1.f / l;
@@ -118,20 +125,18 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     typedef uint32_t codes_t __attribute__((ext_vector_type(CW)));
     codes_t kraw[E4M3 ? 2 : 1][NC], vraw[E4M3 ? 2 : 1][NC];
     uint32_t kex[E4M3 ? 2 : 1][NC], vex[E4M3 ? 2 : 1][NC];
-    const int e_row = lane / PER, e_col = lane % PER * 4 * CW;
+    const int e_row = lane / PER, e_col = lane % PER * 4 * CW, e_off = e_col < d_real ? e_row * d_real + e_col : (int)0x80000000;
+    // (buffers that end with the rows that exist: others read as zero)
     auto fetch = [&](const uint8_t *pool, int64_t stride, const uint8_t *exps, int64_t xstride, int tile, int id_, codes_t (&raw)[NC], uint32_t (&ex)[NC]) __attribute__((always_inline)) {
         const int id = __builtin_amdgcn_readfirstlane(id_), rows = rows_of(tile, id);
         const int64_t place = place_of(tile);
-        const uint8_t *const src = pool + (rows ? id : 0) * stride + place * d_real, *const se = exps + (rows ? id : 0) * xstride + place;
+        const auto values = __builtin_amdgcn_make_buffer_rsrc((void *)(pool + (rows ? id : 0) * stride + place * d_real), 0, rows * d_real, 0x00020000);
+        const auto powers = __builtin_amdgcn_make_buffer_rsrc((void *)(exps + (rows ? id : 0) * xstride + place), 0, rows, 0x00020000);
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const bool there = e_row + 4 * i < rows && e_col < d_real;
-            raw[i] = codes_t{};
-            ex[i] = 127;
-            if (there) {
-                raw[i] = *reinterpret_cast<const codes_t *>(src + (e_row + 4 * i) * d_real + e_col);
-                ex[i] = se[e_row + 4 * i];
-            }
+            if constexpr (CW == 4) raw[i] = __builtin_amdgcn_raw_buffer_load_b128(values, e_off + 4 * i * d_real, 0, 0);
+            else raw[i] = __builtin_amdgcn_raw_buffer_load_b64(values, e_off + 4 * i * d_real, 0, 0);
+            ex[i] = __builtin_amdgcn_raw_buffer_load_b8(powers, e_row + 4 * i, 0, 0);
         }
     };
     auto unpack = [&](const codes_t (&raw)[NC], const uint32_t (&ex)[NC], int slot) __attribute__((always_inline)) {
@@ -227,7 +232,7 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     auto masked = [&](float s, uint32_t word, int vi) __attribute__((always_inline)) {
         return keep_or_neginf(s, bit_mask(word, 8 * (vi >> 2) + (vi & 3)));
     };
-    auto settle = [&](const f32x16 &s, uint32_t word, uint32_t (&p)[8], float &psum) __attribute__((always_inline)) {
+    auto soft = [&](const f32x16 &s, uint32_t word, uint32_t (&p)[8], float &psum) __attribute__((always_inline)) {
         if (__builtin_amdgcn_ballot_w64(row_ok && (mrun == -INFINITY || !(psum <= 256.f)))) {
             asm volatile("" : "+v"(word));              // (nothing of the fast path is kept alive for this one)
             float mloc = -INFINITY;
@@ -237,8 +242,13 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
             if (mloc > mrun) {
                 const float alpha = fast_exp2(mrun - mloc);   // mrun = -inf: 0, and the sums are 0
                 lsum *= alpha;
+                if (AGPR) asm volatile("s_nop 11" : : : "memory");
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
+                for (int dt = 0; dt < DT; ++dt) {
+                    if (AGPR) settle(oacc[dt]);
+                    oacc[dt] *= alpha;
+                    if (AGPR) settle(oacc[dt]);
+                }
                 mrun = mloc;
             }
             const float mneg = (mrun == -INFINITY) ? 0.f : -mrun;
@@ -271,7 +281,7 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
         if (!row_ok) psum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) pE[i] = 0u;
-        settle(sE, live(word_of(0)), pE, psum);
+        soft(sE, live(word_of(0)), pE, psum);
     }
     int id_k = page_at(5), id_v = page_at(3);           // of what the next step requests
     if constexpr (!E4M3) {
@@ -283,7 +293,7 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
         id_v = page_at(4);
         meet_read();
     }
-    constexpr int KA = 4, VA = 4;                       // (divide KS and NP: an operand keeps its register from step to step)
+    constexpr int KA = E4M3 && AGPR ? 2 : 4, VA = E4M3 && D > 64 ? 2 : 4;   // (divide KS and NP: an operand keeps its register from step to step; the values on their way to LDS take registers too)
     static_assert(KS % KA == 0 && NP % VA == 0);
     bf16x8 kr[KA], vr[VA];                              // operands of the next MFMA pairs
     advance(ka_, 2);
@@ -355,7 +365,10 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
         };
 #pragma unroll
         for (int i = 0; i < (NEXT ? NS : NP); ++i) {
-            if (i < NP) oacc[i % DT] = mfma32(vr[i % VA], i < DT ? pB0 : pB1, oacc[i % DT]);
+            if (i < NP) {
+                if (AGPR) mfma32_agpr_late(oacc[i % DT], vr[i % VA], i < DT ? pB0 : pB1, !SM);
+                else oacc[i % DT] = mfma32(vr[i % VA], i < DT ? pB0 : pB1, oacc[i % DT]);
+            }
 #pragma unroll
             for (int r_ = 0; r_ < 2; ++r_)
                 if (REQ && r_ * (NP / 2) / 3 == i) request(r_);
@@ -372,7 +385,7 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
             }
             if (SM) behind(2 * i + 1);
         }
-        if (SM) settle(s, word, pn, psum);
+        if (SM) soft(s, word, pn, psum);
         if (NEXT) sn = snew;
     };
     const std::true_type yes;
@@ -381,7 +394,9 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     const std::integral_constant<int, 1> odd;
     auto meet = [&]() __attribute__((always_inline)) {
         if constexpr (E4M3) {
-            meet_read();
+            // (this step's writes: at least six reads have been issued behind them, and LDS answers in order)
+            asm volatile("s_waitcnt lgkmcnt(6)" : : : "memory");
+            barrier_only();
         } else {
             wait_vmcnt<LPS>();                          // all but what this step requested
             barrier_only();
@@ -419,6 +434,10 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     int *const flag = reinterpret_cast<int *>(dyn_lds + 8 * TL::BYTES + NW * 512);
     {
         float zero = 0.f;
+        if (AGPR) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) settle(oacc[dt]);
+        }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -434,7 +453,10 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     mrun = -INFINITY;
     lsum = 0.f;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) oacc[dt] = zero16();
+    for (int dt = 0; dt < DT; ++dt) {
+        oacc[dt] = zero16();
+        if (AGPR) settle(oacc[dt]);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         ka_[i] = (lds_u8 *)dyn_lds + tl.rowq[i];
@@ -460,7 +482,7 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
         float psum = row_ok ? INFINITY : 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) pE[i] = 0u;
-        settle(sE, live(word_of(tile)), pE, psum);
+        soft(sE, live(word_of(tile)), pE, psum);
         for (int key = 0; key < 32; ++key) {
             const int vi = (key >> 3) * 4 + (key & 3), from = ((key >> 2) & 1) * 32 + j;     // where its probability lies
             uint32_t pair = 0;
@@ -492,7 +514,10 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
         meet_read();
         const u32x4 w0 = {pE[0], pE[1], pE[2], pE[3]}, w1 = {pE[4], pE[5], pE[6], pE[7]};
 #pragma unroll
-        for (int i = 0; i < NP; ++i) oacc[i % DT] = mfma32(read_v(i), __builtin_bit_cast(bf16x8, i < DT ? w0 : w1), oacc[i % DT]);
+        for (int i = 0; i < NP; ++i) {
+            if (AGPR) mfma32_agpr_late(oacc[i % DT], read_v(i), __builtin_bit_cast(bf16x8, i < DT ? w0 : w1), true);
+            else oacc[i % DT] = mfma32(read_v(i), __builtin_bit_cast(bf16x8, i < DT ? w0 : w1), oacc[i % DT]);
+        }
         meet_read();
     }
     finish();
@@ -502,7 +527,7 @@ template <int D, bool E4M3>
 hipError_t launch_walk(const dsa_cache_args &c, const PagePlan &plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, int gshift, int pshift, float scale, int slots, int tail,
                        void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream) {
     constexpr int lds = walk_lds_bytes<D>();
-    const auto kernel = &dsa_paged_walk_kernel<D, E4M3>;
+    const auto kernel = &dsa_paged_walk_kernel<D, E4M3, (D > 128)>;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, dim3((unsigned)slots * c.Hkv), dim3(WALK_WAVES * 64), lds, stream, c, plan, (const bf16_t *)q, q_tok, q_head, Hq, gshift, pshift, fabsf(scale) * LOG2E_F,
@@ -512,18 +537,28 @@ hipError_t launch_walk(const dsa_cache_args &c, const PagePlan &plan, const void
 
 }  // namespace
 
-// plan.qb: 128 rows' queries
-extern "C" hipError_t dsa_launch_paged_walk(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail,
-                                            void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream) {
-    const int gshift = group_shift(Hq, c->Hkv), pshift = __builtin_ctz((unsigned)c->page);
-    if (plan->qb << gshift != 128 || c->D > 256) return hipErrorInvalidValue;
+// plan.qb: 128 rows' queries.  The file is compiled twice, the second time (WALK_256) for head_dim 256, with results of MFMA builtins in vector registers: the sums have the
+// accumulation registers.
+#define WALK_ARGS const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail, void *out, float *lse, \
+    float *part_o, float *part_ml, hipStream_t stream
 #define WALK_CASE(D_, E_) return launch_walk<D_, E_>(*c, *plan, q, q_tok, q_head, Hq, gshift, pshift, logit_scale(scale), slots, tail, out, lse, part_o, part_ml, stream)
-    if (c->kind == DSA_CACHE_E4M3) {
-        if (c->D <= 64) WALK_CASE(64, true);
-        if (c->D <= 128) WALK_CASE(128, true);
-        WALK_CASE(256, true);
-    }
-    if (c->D <= 64) WALK_CASE(64, false);
-    if (c->D <= 128) WALK_CASE(128, false);
+extern "C" hipError_t dsa_launch_paged_walk_256(WALK_ARGS);
+#if WALK_256
+extern "C" hipError_t dsa_launch_paged_walk_256(WALK_ARGS) {
+    const int gshift = group_shift(Hq, c->Hkv), pshift = __builtin_ctz((unsigned)c->page);
+    if (c->kind == DSA_CACHE_E4M3) WALK_CASE(256, true);
     WALK_CASE(256, false);
 }
+#else
+extern "C" hipError_t dsa_launch_paged_walk(WALK_ARGS) {
+    const int gshift = group_shift(Hq, c->Hkv), pshift = __builtin_ctz((unsigned)c->page);
+    if (plan->qb << gshift != 128 || c->D > 256) return hipErrorInvalidValue;
+    if (c->D > 128) return dsa_launch_paged_walk_256(c, plan, q, q_tok, q_head, Hq, scale, slots, tail, out, lse, part_o, part_ml, stream);
+    if (c->kind == DSA_CACHE_E4M3) {
+        if (c->D <= 64) WALK_CASE(64, true);
+        WALK_CASE(128, true);
+    }
+    if (c->D <= 64) WALK_CASE(64, false);
+    WALK_CASE(128, false);
+}
+#endif
