@@ -25,9 +25,9 @@ hipError_t dsa_launch_residual_norm_fwd(const void *x, int x_f32, const void *y,
 hipError_t dsa_launch_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x_f32, const void *y, const void *gate, const void *w, int w_f32, const void *post, int post_f32, const void *scale, int scale_f32, float offset, int T, int C, const float *rstd, const float *rstd_y, void *dx, void *dy, void *dgate, void *dw, void *dpost, void *dscale, float *part, hipStream_t stream);
 hipError_t dsa_launch_cache_write(const dsa_cache_args *c, const void *k, int64_t k_tok, int64_t k_head, const void *v, int64_t v_tok, int64_t v_head, const int32_t *cu, const int32_t *lengths, int T, int N, hipStream_t stream);
 hipError_t dsa_launch_cache_read(const dsa_cache_args *c, const int32_t *cu, const int32_t *first, int T, int N, void *k_out, void *v_out, hipStream_t stream);
-hipError_t dsa_launch_paged_step(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream);
+hipError_t dsa_launch_paged_step(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int waves, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream);
 hipError_t dsa_launch_paged_walk(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream);
-hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PagePlan *plan, int Hq, int blocks, const float *part_o, const float *part_ml, void *out, float *lse, hipStream_t stream);
+hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PagedJoin *many, const PagedJoin *few, int Hq, void *out, float *lse, hipStream_t stream);
 hipError_t dsa_launch_delta_fwd(const DeltaArgs *a, int save, hipStream_t stream);
 hipError_t dsa_launch_delta_bwd(const DeltaArgs *a, hipStream_t stream);
 hipError_t dsa_launch_delta_step(const dsa_delta_args *in, float *state, int64_t state_req, void *out, hipStream_t stream);
@@ -1307,29 +1307,39 @@ namespace {
 // What a call launches, from what the host knows: the kernel for a few rows (dsa_paged_step.hip), the one for many (dsa_paged_walk.hip), or both, each for its requests.
 struct PagedLaunch {
     PagePlan plan;
-    int64_t blocks, slots;                               // bounds for each kv head; 0: not launched
-    bool join;
+    int64_t blocks, slots;                               // bounds for each kv head: of blocks, and of workgroups; 0: not launched
+    int pieces, waves;                                   // of a block at the most; of the kernel for a few rows (dsa_launch_paged_step)
     size_t o_bytes, bytes;                               // of its partial sums
 };
 struct PagedCall { PagedLaunch step, walk; };
 }  // namespace
-static PagedLaunch paged_launch(const dsa_cache_args *c, const int32_t *cu, const int32_t *lengths, int T, int N, int gshift, int qb, int few, int side, bool many, int resident, int least,
+static PagedLaunch paged_launch(const dsa_cache_args *c, const int32_t *cu, const int32_t *lengths, int T, int N, int gshift, int qb, int few, int side, bool many, int resident,
                                 int max_length) {
-    const int capacity = c->table_pages * c->page, longest = max_length > 0 ? std::min(max_length, capacity) : capacity;
-    PagedLaunch p;
-    p.plan = PagePlan{N, T, qb, few, side, 0, least, cu, lengths, capacity};
-    p.join = (longest + 31) / 32 > least;
-    if (!p.join) p.plan.least = 1 << 30;                 // (whole walks, whatever the lengths say)
+    const int capacity = c->table_pages * c->page, longest = max_length > 0 ? std::min(max_length, capacity) : capacity, least = many ? 8 : 4;
+    PagedLaunch p{};
+    p.plan = PagePlan{N, T, qb, few, side, std::max(1, resident / c->Hkv), 0.f, least, (longest + 31) / 32 <= least, 0, cu, lengths, capacity};
     // blocks: of requests of up to `few` rows (one block) as many as there are, of the others the rows' and what the last one of each request lacks
     const int64_t requests = std::min<int64_t>(N, side == 1 ? T / (few + 1) : T);
     p.blocks = side == 0 ? requests : (T + requests * (qb - 1)) / qb;
-    // Pieces: where blocks are few, so many that all workgroups run at once; else (few rows) two rounds of them, or as many as there are blocks
-    const int64_t at_once = resident / c->Hkv;
-    p.plan.target = (int)std::max<int64_t>(1, 2 * p.blocks <= at_once ? at_once - p.blocks : many ? at_once : std::max(2 * at_once, p.blocks));
-    p.slots = p.blocks + p.plan.target + 1;              // (with a block's last piece; one more, so that some workgroup is left for the rows behind the last request)
-    const size_t records = p.join ? (size_t)p.slots * c->Hkv * (qb << gshift) : 0;
-    p.o_bytes = records * c->D * sizeof(float);
-    p.bytes = align_up(p.o_bytes + records * 2 * sizeof(float), 256);
+    int64_t records;
+    if (many) {
+        // Where blocks are few, so many pieces that all workgroups run at once
+        if (2 * p.blocks <= p.plan.target) p.plan.target -= (int)p.blocks;
+        p.slots = p.blocks + p.plan.target + 1;          // (with a block's last piece; one more, so that some workgroup is left for the rows behind the last request)
+        records = p.slots;
+    } else {
+        // Few blocks: their waves side by side on a unit of their own (one token over 1000 keys, 8 kv heads: 9.3 us, two waves to a workgroup 11.8)
+        p.waves = p.blocks * c->Hkv <= 64 ? 4 : 2;
+        if (p.waves == 4 && c->kind == DSA_CACHE_BF16 && c->D > 64) p.plan.target = std::max(1, 256 / c->Hkv);
+        while (p.blocks * ((capacity / 32 >> p.plan.ushift) + 8) >= 1 << 29) ++p.plan.ushift;
+        p.slots = p.plan.target;
+        records = 2 * p.slots;
+    }
+    p.plan.per_target = 1.f / (float)p.plan.target;
+    p.pieces = (int)std::min<int64_t>(p.plan.target, (longest + 31) / 32 / least) + 2;
+    records *= p.plan.whole ? 0 : (int64_t)c->Hkv * (qb << gshift);
+    p.o_bytes = (size_t)records * c->D * sizeof(float);
+    p.bytes = align_up(p.o_bytes + (size_t)records * 2 * sizeof(float), 256);
     return p;
 }
 static PagedCall paged_call(const dsa_cache_args *c, const int32_t *cu, const int32_t *lengths, int T, int N, int Hq, int max_new, int max_length) {
@@ -1337,13 +1347,17 @@ static PagedCall paged_call(const dsa_cache_args *c, const int32_t *cu, const in
     while ((c->Hkv << gshift) < Hq) ++gshift;
     const int most = max_new > 0 ? std::min(max_new, std::max(T, 1)) : std::max(T, 1), few = std::max(1, 16 >> gshift);
     // workgroups that run at once, by their LDS
-    const int by_step = 256 * (c->D > 128 || (c->D > 64 && c->kind == DSA_CACHE_BF16) ? 1 : 2), by_walk = c->D > 128 ? 256 : 512;
+    const int by_step = c->D > 128 ? 256 : 512, by_walk = c->D > 128 ? 256 : 512;
     PagedCall p{};
-    if (most <= 32 >> gshift) {
-        p.step = paged_launch(c, cu, lengths, T, N, gshift, most, 0, -1, false, by_step, 4, max_length);
+    // Few blocks of a few keys each: the kernel for a few rows takes chunks too, 32 rows at a time, its waves a tile each (17 new tokens behind 1000, 32 heads over 8: 13 us, the
+    // kernel for many rows 16; seven requests of up to 129 behind up to 871: 15 against 25 with both kernels; 256 without any behind: 21 against 12)
+    const int longest = max_length > 0 ? std::min(max_length, c->table_pages * c->page) : c->table_pages * c->page, qb = std::max(1, std::min(most, 32 >> gshift));
+    const int64_t blocks = (T + std::min<int64_t>(N, T) * (qb - 1)) / qb * c->Hkv;
+    if (most <= 32 >> gshift || (blocks <= 64 && blocks * ((longest + 31) / 32) <= 2112)) {
+        p.step = paged_launch(c, cu, lengths, T, N, gshift, qb, 0, -1, false, by_step, max_length);
     } else {
-        p.walk = paged_launch(c, cu, lengths, T, N, gshift, 128 >> gshift, few, N == 1 ? -1 : 1, true, by_walk, 16, max_length);
-        if (N > 1) p.step = paged_launch(c, cu, lengths, T, N, gshift, few, few, 0, false, by_step, 4, max_length);
+        p.walk = paged_launch(c, cu, lengths, T, N, gshift, 128 >> gshift, few, N == 1 ? -1 : 1, true, by_walk, max_length);
+        if (N > 1) p.step = paged_launch(c, cu, lengths, T, N, gshift, few, few, 0, false, by_step, max_length);
     }
     return p;
 }
@@ -1375,15 +1389,17 @@ extern "C" int dsa_paged_attn(const dsa_cache_args *c, const void *q, int64_t q_
     if (need && (!ws || off16(ws) || ws_bytes < need)) return fail(DSA_ERR_WORKSPACE, "workspace: need %zu bytes on a 16-byte boundary, got %zu", need, ws_bytes);
     hipError_t e = hipSuccess;
     char *at = (char *)ws;
-    const auto run = [&](const PagedLaunch &l, auto attend) {
-        if (!l.slots || e != hipSuccess) return;
+    PagedJoin joins[2] = {};
+    for (const bool many : {true, false}) {
+        const PagedLaunch &l = many ? p.walk : p.step;
+        if (!l.slots || e != hipSuccess) continue;
         float *const part_o = (float *)at, *const part_ml = (float *)(at + l.o_bytes);
         // (the kernel for many rows clears those behind the last request where both are launched)
-        e = attend(c, &l.plan, q, q_tok, q_head, Hq, scale, (int)l.slots, &l == &p.walk || !p.walk.slots, out, lse, part_o, part_ml, (hipStream_t)stream);
-        if (e == hipSuccess && l.join) e = dsa_launch_paged_join(c, &l.plan, Hq, (int)l.blocks, part_o, part_ml, out, lse, (hipStream_t)stream);
+        e = many ? dsa_launch_paged_walk(c, &l.plan, q, q_tok, q_head, Hq, scale, (int)l.slots, 1, out, lse, part_o, part_ml, (hipStream_t)stream)
+                 : dsa_launch_paged_step(c, &l.plan, q, q_tok, q_head, Hq, scale, l.waves, !p.walk.slots, out, lse, part_o, part_ml, (hipStream_t)stream);
+        if (!l.plan.whole) joins[many ? 0 : 1] = PagedJoin{l.plan, (int)l.blocks, l.pieces, part_o, part_ml};
         at += l.bytes;
-    };
-    run(p.walk, dsa_launch_paged_walk);
-    run(p.step, dsa_launch_paged_step);
+    }
+    if (e == hipSuccess && joins[0].blocks + joins[1].blocks > 0) e = dsa_launch_paged_join(c, &joins[0], &joins[1], Hq, out, lse, (hipStream_t)stream);
     return e == hipSuccess ? DSA_OK : hip_fail(e, "paged attention launch");
 }

@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void dsa_cache_write_kernel(dsa_cache_args c, 
         const bool val = item >= c.Hkv;
         const int head = val ? item - c.Hkv : item;
         const bf16_t *src = val ? (const bf16_t *)in.v + t * in.v_tok + head * in.v_head : (const bf16_t *)in.k + t * in.k_tok + head * in.k_head;
-        return item < items && d < c.D ? *reinterpret_cast<const u32x4 *>(src + d) : u32x4{0u, 0u, 0u, 0u};
+        return item < items && d < c.D ? __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + d)) : u32x4{0u, 0u, 0u, 0u};
     };
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) x[i] = load(i * per + mine);
@@ -108,10 +108,10 @@ __global__ __launch_bounds__(256) void dsa_cache_read_kernel(dsa_cache_args c, c
             if (item < items && d < c.D && id >= 0) {
                 if constexpr (!E4M3) {
                     const bf16_t *src = val ? (const bf16_t *)c.v + id * c.v_page + row * c.D : (const bf16_t *)c.k + id * c.k_page + row * c.D;
-                    x[i] = *reinterpret_cast<const u32x4 *>(src + d);
+                    x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + d));
                 } else {
                     const uint8_t *src = val ? (const uint8_t *)c.v + id * c.v_page + row * c.D : (const uint8_t *)c.k + id * c.k_page + row * c.D;
-                    const u32x2 w = *reinterpret_cast<const u32x2 *>(src + d);
+                    const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(src + d));
                     x[i] = u32x4{w[0], w[1], 0u, 0u};
                     ex[i] = val ? ((const uint8_t *)c.v_exp)[id * c.vx_page + row] : ((const uint8_t *)c.k_exp)[id * c.kx_page + row];
                 }
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256) void dsa_cache_read_kernel(dsa_cache_args c, c
                 x[i] = u32x4{a[0], a[1], b[0], b[1]};
             }
             bf16_t *dst = (val ? v_out : k_out) + ((int64_t)t * c.Hkv + (val ? item - c.Hkv : item)) * c.D;
-            *reinterpret_cast<u32x4 *>(dst + d) = x[i];
+            __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4 *>(dst + d));
         }
     }
 }

@@ -42,12 +42,14 @@ __device__ __forceinline__ u32x2 e4m3_to_bf16(uint32_t w, float scale) {
 __device__ __forceinline__ float exponent_scale(uint32_t b) { return __uint_as_float(b == 255 ? 0x7fc00000u : b << 23); }
 
 // ---- how the work is cut ----
-// A request's new rows go in blocks of `qb` queries, and the keys of each of its blocks in `pieces` of about equal length, as many as make launches of about `target`
-// workgroups for each kv head out of all requests together: a few long requests and a batch of short ones fill the card alike.  Lengths are on the device, so every
-// workgroup forms the plan itself: sums over the requests, one in each lane.
+// A request's new rows go in blocks of `qb` queries.  Lengths are on the device, so every workgroup forms the plan itself: sums over the requests, one in each lane.
 struct PagePlan {
     int N, T, qb, few, side;       // requests of up to `few` new rows are side 0's, others side 1's; side -1: all of them
-    int target, least;             // workgroups aimed at (per kv head); tiles of 32 keys that a piece has at the least
+    int target;                    // workgroups aimed at, or launched, for each kv head
+    float per_target;              // 1 / target
+    int least;                     // tiles of 32 keys that a piece of a block has at the least
+    int whole;                     // no block is cut
+    int ushift;                    // shares are counted in units of 2^ushift tiles
     const int32_t *cu, *lengths;
     int capacity;                  // positions that the table holds
 };
@@ -55,8 +57,15 @@ struct PagePiece {
     int n, row0, m, length;        // request, its first row, its new rows, its length
     int first;                     // first query of the block
     int tile0, tile1;              // the piece's key tiles
-    int piece, pieces;             // pieces of this block that have tiles (1 at the least)
-    int slot;                      // of the block's first piece
+    int piece, pieces;             // which of how many pieces of this block (shares: whether it is the first, and whether there are others)
+    int slot;                      // of the block's first piece's sums (shares: of this one's)
+};
+// what is joined of a launch: its blocks, for each kv head, and their pieces' sums
+struct PagedJoin {
+    PagePlan plan;
+    int blocks;
+    int pieces;                    // of a block, at the most
+    const float *part_o, *part_ml;
 };
 struct PageRequest { int row0, m, length, blocks, tiles; };
 __device__ __forceinline__ PageRequest page_request(const PagePlan &p, int n) {
@@ -79,9 +88,11 @@ __device__ __forceinline__ float plan_sum(float x) {
 }
 // tiles to a piece, from the sum of all blocks' tiles (a little over the sum's own rounding: the slots of a launch are counted for this many pieces)
 __device__ __forceinline__ int piece_tiles(const PagePlan &p, float mine) {
-    return max(p.least, (int)fminf(ceilf(plan_sum(mine) * 1.0001f / (float)p.target), 1e9f));
+    return p.whole ? 1 << 30 : max(p.least, (int)fminf(ceilf(plan_sum(mine) * 1.0001f / (float)p.target), 1e9f));
 }
-// Piece `slot` (BLOCKS: block `slot`) of the launch; false past the last one, with `spare` the number of slots in front that are taken
+// Blocks of many rows: each in pieces of about equal length, as many as make launches of about `target` workgroups for each kv head out of all requests together, but no more
+// than the root of its tiles (a piece more costs the block's sums once more to write and read).  Piece `slot` (BLOCKS: block `slot`) of the launch; false past the last one, with `spare`
+// the number of slots in front that are taken.
 template <bool BLOCKS>
 __device__ __forceinline__ bool locate_piece(const PagePlan &p, int slot, PagePiece &out, int &spare) {
     const int lane = threadIdx.x & 63;
@@ -95,7 +106,7 @@ __device__ __forceinline__ bool locate_piece(const PagePlan &p, int slot, PagePi
     int slots = 0, taken = 0;                            // of pieces, and of what is counted
     for (int base = 0; base < p.N; base += 64) {
         if (base > 0) r = page_request(p, base + lane);
-        const int np = max(1, (r.tiles + per - 1) / per), mine = r.blocks * np, count = BLOCKS ? r.blocks : mine;
+        const int each = max(per, (int)sqrtf((float)r.tiles)), np = max(1, (r.tiles + each - 1) / each), mine = r.blocks * np, count = BLOCKS ? r.blocks : mine;
         const int upto = wave_prefix_i(count), slots_upto = BLOCKS ? wave_prefix_i(mine) : upto;
         const uint64_t past = __builtin_amdgcn_ballot_w64(taken + upto > slot);
         if (past) {
@@ -122,6 +133,127 @@ __device__ __forceinline__ bool locate_piece(const PagePlan &p, int slot, PagePi
         slots += __builtin_amdgcn_readlane(slots_upto, 63);
     }
     spare = taken;
+    return false;
+}
+// Blocks of a few rows: all blocks' tiles one behind the other, each block's behind a few that stand for what going to it costs (BLOCK_COST), cut into equal shares, one for each of `target`
+// workgroups of a kv head: however the lengths are mixed, all of them end together.  A cut that falls within a 16th of a share from a block's end is moved there.  A workgroup goes from block to block through its share; a block that is
+// cut has a piece for each share that it lies in.  Sums of piece 0 lie in slot 2 k - 1, of piece i > 0 in 2 (k + i - 1), k the first cut inside the block, counted from the launch's
+// start: no two pieces share one, and there are 2 `target` of them.
+// (a block's rows, the look-up of its first pages and the joining of its waves take 4 to 5 us one after the other, a tile of a workgroup 1 to 1.5)
+#define BLOCK_COST 4
+struct PageShares {
+    int share, near, cost;         // units of a share, how far a cut is moved at the most, and units in front of a block's tiles
+    __device__ __forceinline__ int first_cut(int u0) const { return (u0 + cost + near + share - 1) / share; }
+    __device__ __forceinline__ int cuts(int u0, int u1) const { return max(0, max(u1 - near, 0) / share - first_cut(u0) + 1); }
+    __device__ __forceinline__ int moved(int x, int u0, int u1) const { return x - u0 < cost + near ? u0 : u1 - x < near ? u1 : x; }
+};
+__device__ __forceinline__ int units_of(const PagePlan &p, int tiles) { return max(1, (BLOCK_COST + tiles + (1 << p.ushift) - 1) >> p.ushift); }
+__device__ __forceinline__ PageShares page_shares(const PagePlan &p, const PageRequest &r) {
+    const int lane = threadIdx.x & 63;
+    int sum = r.blocks * units_of(p, r.tiles);           // (the host chose the unit for the sum to have less than 30 bits)
+    for (int n = 64 + lane; n < p.N; n += 64) {
+        const PageRequest x = page_request(p, n);
+        sum += x.blocks * units_of(p, x.tiles);
+    }
+    sum = wave_sum_i(sum);
+    PageShares s;
+    // (a float's product, rounded up and one more, is enough: divisions of whole numbers take a wave 300 clocks each, in front of its first load)
+    s.share = __builtin_amdgcn_readfirstlane(max(max(p.least >> p.ushift, 1), (int)((float)sum * p.per_target * 1.000001f) + 1));
+    s.cost = BLOCK_COST >> p.ushift;
+    s.near = p.whole ? 1 << 29 : max(1, s.share >> 4);
+    return s;
+}
+// the block of request `n` (lane w of r) that is the order-th of its blocks (the last one, which has the most keys, first) and takes units u0 .. u1 - 1
+__device__ __forceinline__ void share_block(const PagePlan &p, const PageShares &s, const PageRequest &r, int w, int n, int order, int u0, int u1, PagePiece &out) {
+    out.n = n;
+    out.row0 = __builtin_amdgcn_readlane(r.row0, w);
+    out.m = __builtin_amdgcn_readlane(r.m, w);
+    out.length = __builtin_amdgcn_readlane(r.length, w);
+    out.first = (__builtin_amdgcn_readlane(r.blocks, w) - 1 - order) * p.qb;
+}
+struct ShareWalk {
+    PageShares s;
+    PageRequest r;
+    int base, w, order, u0, mine, x0, x1;                // batch of 64 requests, the block's lane in it and its number, its first unit; the share and its ends
+    bool more;
+    __device__ __forceinline__ void start(const PagePlan &p, int share) {
+        r = page_request(p, threadIdx.x & 63);           // (up to 64 requests: looked at once)
+        s = page_shares(p, r);
+        mine = share;
+        x0 = share * s.share;
+        x1 = x0 + s.share;
+        more = false;
+        int before = 0;
+        for (base = 0; base < p.N; base += 64) {
+            if (base > 0) r = page_request(p, base + (threadIdx.x & 63));
+            const int units = units_of(p, r.tiles), count = r.blocks * units, upto = wave_prefix_i(count);
+            const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > x0);
+            if (past) {
+                w = (int)__builtin_ctzll(past);
+                const int at = before + __builtin_amdgcn_readlane(upto, w) - __builtin_amdgcn_readlane(count, w), per = __builtin_amdgcn_readlane(units, w);
+                order = __builtin_amdgcn_readlane(r.blocks, w) > 1 ? (x0 - at) / per : 0;
+                u0 = at + order * per;
+                more = true;
+                return;
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+        }
+    }
+    // the share's next piece
+    __device__ __forceinline__ bool next(const PagePlan &p, PagePiece &out) {
+        while (more && x1 > u0) {
+            const int u1 = u0 + units_of(p, __builtin_amdgcn_readlane(r.tiles, w));
+            const int lo = x0 <= u0 ? u0 : s.moved(x0, u0, u1), hi = x1 >= u1 ? u1 : s.moved(x1, u0, u1);
+            if (lo < hi) {
+                share_block(p, s, r, w, base + w, order, u0, u1, out);
+                const int last = out.length - out.m + min(out.first + p.qb, out.m) - 1;      // position of the block's last row
+                const int tiles = last < 0 ? 0 : (min(last, p.capacity - 1) >> 5) + 1;
+                // (a first piece ends with the first cut inside the block, the next share's start; another begins with its share)
+                out.piece = lo != u0;
+                out.pieces = 1 + (lo != u0 || hi != u1);
+                out.slot = 2 * mine + (lo == u0);
+                out.tile0 = lo == u0 ? 0 : min((lo - u0 - s.cost) << p.ushift, tiles);
+                out.tile1 = hi == u1 ? tiles : min((hi - u0 - s.cost) << p.ushift, tiles);
+            }
+            // on to the next block
+            u0 = u1;
+            if (++order >= __builtin_amdgcn_readlane(r.blocks, w)) {
+                order = 0;
+                uint64_t rest = __builtin_amdgcn_ballot_w64(r.blocks > 0) & (w < 63 ? ~0ull << (w + 1) : 0ull);
+                while (!rest && base + 64 < p.N) {
+                    base += 64;
+                    r = page_request(p, base + (threadIdx.x & 63));
+                    rest = __builtin_amdgcn_ballot_w64(r.blocks > 0);
+                }
+                more = rest != 0;
+                w = more ? (int)__builtin_ctzll(rest) : 0;
+            }
+            if (lo < hi) return true;
+        }
+        return false;
+    }
+};
+// Block `slot` of such a launch
+__device__ __forceinline__ bool locate_share_block(const PagePlan &p, int slot, PagePiece &out) {
+    PageRequest r = page_request(p, threadIdx.x & 63);
+    const PageShares s = page_shares(p, r);
+    int taken = 0, before = 0;
+    for (int base = 0; base < p.N; base += 64) {
+        if (base > 0) r = page_request(p, base + (threadIdx.x & 63));
+        const int units = units_of(p, r.tiles), upto = wave_prefix_i(r.blocks), uupto = wave_prefix_i(r.blocks * units);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(taken + upto > slot);
+        if (past) {
+            const int w = (int)__builtin_ctzll(past), blocks = __builtin_amdgcn_readlane(r.blocks, w), per = __builtin_amdgcn_readlane(units, w);
+            const int order = slot - taken - (__builtin_amdgcn_readlane(upto, w) - blocks);
+            const int u0 = before + __builtin_amdgcn_readlane(uupto, w) - (blocks - order) * per;
+            share_block(p, s, r, w, base + w, order, u0, u0 + per, out);
+            out.pieces = s.cuts(u0, u0 + per) + 1;
+            out.slot = 2 * s.first_cut(u0) - 1;
+            return true;
+        }
+        taken += __builtin_amdgcn_readlane(upto, 63);
+        before += __builtin_amdgcn_readlane(uupto, 63);
+    }
     return false;
 }
 // Rows behind the last request: zeros, by the workgroups that found no piece (the first of them is 0 of `step`; each its kv head's rows)

@@ -31,7 +31,7 @@ constexpr int step_wave_bytes() {
 
 template <int D, bool E4M3, int RG, int NW>
 __global__ __launch_bounds__(NW * 64, 1) void dsa_paged_step_kernel(dsa_cache_args c, PagePlan plan, const bf16_t *__restrict__ q, int64_t q_tok, int64_t q_head, int Hq,
-                                                                    int gshift, int pshift, float scale_log2, int slots, int tail, bf16_t *__restrict__ out,
+                                                                    int gshift, int pshift, float scale_log2, int tail, bf16_t *__restrict__ out,
                                                                     float *__restrict__ lse, float *__restrict__ part_o, float *__restrict__ part_ml) {
     typedef DirectTile<D> TL;
     constexpr int KS = D / 32, DT = D / 16, ROWS = 16 * RG, PITCH = D + 4;
@@ -40,13 +40,11 @@ __global__ __launch_bounds__(NW * 64, 1) void dsa_paged_step_kernel(dsa_cache_ar
     const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int Hkv = c.Hkv, G = Hq / Hkv, kvh = blockIdx.x % Hkv, T = plan.T, d_real = c.D;
+    const int share = blockIdx.x / Hkv;
+    ShareWalk walk;
+    walk.start(plan, share);
     PagePiece pc;
-    int spare;
-    if (!locate_piece<false>(plan, blockIdx.x / Hkv, pc, spare)) {
-        if (tail) zero_tail(plan, Hq, Hkv, kvh, blockIdx.x / Hkv - spare, slots - spare, d_real, NW * 64, out, lse);
-        return;
-    }
-    if (pc.piece >= pc.pieces) return;
+    while (walk.next(plan, pc)) {
     const int keys = min(pc.length, plan.capacity);      // positions that exist
     const int chunks = d_real / 8;
 
@@ -289,7 +287,7 @@ __global__ __launch_bounds__(NW * 64, 1) void dsa_paged_step_kernel(dsa_cache_ar
     __syncthreads();
     const int rows = plan.qb << gshift;
     const bool whole = pc.pieces == 1;
-    const int64_t record = (int64_t)(pc.slot + pc.piece) * Hkv + kvh;
+    const int64_t record = (int64_t)pc.slot * Hkv + kvh;
     for (int i = tid; i < rows * chunks; i += NW * 64) {
         const int row = i / chunks, d = i % chunks * 8;
         if (!live(row)) continue;
@@ -325,18 +323,26 @@ __global__ __launch_bounds__(NW * 64, 1) void dsa_paged_step_kernel(dsa_cache_ar
             if (d == 0) *reinterpret_cast<f32x2 *>(part_ml + (record * rows + row) * 2) = f32x2{m, l};
         }
     }
+    __syncthreads();                                     // the sums are read: the next piece's tiles may come
+    }
+    if (tail) zero_tail(plan, Hq, Hkv, kvh, share, plan.target, d_real, NW * 64, out, lse);
 }
 
 // The pieces of a block: out = sum of 2^(m_i - m) O_i over sum of 2^(m_i - m) l_i, in a fixed order.  A workgroup takes ITEMS of the block's rows' four columns at a time and
-// has 256 / ITEMS threads for each, which take every so many-th piece: 32 where a few blocks have many pieces (a long request by itself), 256 elsewhere.
+// has 256 / ITEMS threads for each, which take every so many-th piece: 8 or 32 where a few blocks have many pieces (a long request by itself), 256 elsewhere.
 template <int ITEMS>
-__global__ __launch_bounds__(256) void dsa_paged_join_kernel(dsa_cache_args c, PagePlan plan, int Hq, int gshift, const float *__restrict__ part_o, const float *__restrict__ part_ml,
+__global__ __launch_bounds__(256) void dsa_paged_join_kernel(dsa_cache_args c, PagedJoin many, PagedJoin few, int Hq, int gshift,
                                                              bf16_t *__restrict__ out, float *__restrict__ lse) {
     constexpr int GROUPS = 256 / ITEMS;
-    const int Hkv = c.Hkv, G = Hq / Hkv, d_real = c.D, rows = plan.qb << gshift, cols = d_real / 4, kvh = blockIdx.x % Hkv;
+    const int Hkv = c.Hkv, G = Hq / Hkv, d_real = c.D, kvh = blockIdx.x % Hkv, at_ = blockIdx.x / Hkv;
+    const bool shares = at_ >= many.blocks;
+    const PagePlan plan = shares ? few.plan : many.plan;
+    const float *const part_o = shares ? few.part_o : many.part_o, *const part_ml = shares ? few.part_ml : many.part_ml;
+    const int rows = plan.qb << gshift, cols = d_real / 4;
     PagePiece pc;
     int spare;
-    if (!locate_piece<true>(plan, blockIdx.x / Hkv, pc, spare) || pc.pieces <= 1) return;
+    if (!(shares ? locate_share_block(plan, at_ - many.blocks, pc) : locate_piece<true>(plan, at_, pc, spare)) || pc.pieces <= 1) return;
+    auto slot_of = [&](int i) { return (int64_t)(shares && i ? 2 * i - 1 : i); };            // of piece i, from the first one's
     __shared__ f32x4 sums[GROUPS > 1 ? 256 : 1];
     __shared__ f32x2 stats[GROUPS > 1 ? 256 : 1];
     const int tid = threadIdx.x, group = tid / ITEMS, live = min(pc.m - pc.first, plan.qb) << gshift;
@@ -348,16 +354,19 @@ __global__ __launch_bounds__(256) void dsa_paged_join_kernel(dsa_cache_args c, P
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         if (mine) {
             const int64_t at = first * rows + row, step = (int64_t)Hkv * rows;
-            // the largest first: the loads of sums and weights then wait for nothing
-            for (int i = group; i < pc.pieces; i += GROUPS) m = fmaxf(m, part_ml[2 * (at + i * step)]);
 #pragma unroll 4
             for (int i = group; i < pc.pieces; i += GROUPS) {
-                const f32x2 ml = *reinterpret_cast<const f32x2 *>(part_ml + 2 * (at + i * step));
-                const f32x4 x = *reinterpret_cast<const f32x4 *>(part_o + (at + i * step) * d_real + d);
-                const float w = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - m);
-                l = fmaf(w, ml[1], l);
+                const f32x2 ml = *reinterpret_cast<const f32x2 *>(part_ml + 2 * (at + slot_of(i) * step));
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(part_o + (at + slot_of(i) * step) * d_real + d);
+                // (sums against the largest so far: no load waits for another piece's)
+                const float most = fmaxf(m, ml[0]), old = m == -INFINITY ? 0.f : fast_exp2(m - most), w = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - most);
+                l = fmaf(w, ml[1], old == 0.f ? 0.f : l * old);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, x[e], o[e]);
+                for (int e = 0; e < 4; ++e) {
+                    o[e] = old == 0.f ? 0.f : o[e] * old;
+                    o[e] = w == 0.f ? o[e] : fmaf(w, x[e], o[e]);
+                }
+                m = most;
             }
         }
         if constexpr (GROUPS > 1) {
@@ -392,46 +401,48 @@ __global__ __launch_bounds__(256) void dsa_paged_join_kernel(dsa_cache_args c, P
     }
 }
 
-template <int D, bool E4M3, int RG>
-hipError_t launch_step(const dsa_cache_args &c, const PagePlan &plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, int gshift, int pshift, float scale, int slots,
-                       int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream) {
-    constexpr int NW = D == 256 && !E4M3 ? 2 : 4, lds = NW * step_wave_bytes<D, E4M3, RG>();
+template <int D, bool E4M3, int RG, int NW>
+hipError_t launch_step(const dsa_cache_args &c, const PagePlan &plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, int gshift, int pshift, float scale, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream) {
+    constexpr int lds = NW * step_wave_bytes<D, E4M3, RG>();
     const auto kernel = &dsa_paged_step_kernel<D, E4M3, RG, NW>;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)slots * c.Hkv), dim3(NW * 64), lds, stream, c, plan, (const bf16_t *)q, q_tok, q_head, Hq, gshift, pshift, scale * LOG2E_F, slots,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)plan.target * c.Hkv), dim3(NW * 64), lds, stream, c, plan, (const bf16_t *)q, q_tok, q_head, Hq, gshift, pshift, scale * LOG2E_F,
                        tail, (bf16_t *)out, lse, part_o, part_ml);
     return hipGetLastError();
 }
 
 }  // namespace
 
-// rows: 16 or 32, what a block of plan.qb queries takes at the most
-extern "C" hipError_t dsa_launch_paged_step(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail,
+// waves: 4 at head_dim 65 to 128 in a bf16 cache (else 2 there): a workgroup to a compute unit, for launches in which single pieces count
+extern "C" hipError_t dsa_launch_paged_step(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int waves, int tail,
                                             void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream) {
     const int gshift = group_shift(Hq, c->Hkv), pshift = __builtin_ctz((unsigned)c->page), rows = plan->qb << gshift;
     const bool e = c->kind == DSA_CACHE_E4M3;
-#define STEP_CASE(D_, E_) return rows <= 16 ? launch_step<D_, E_, 1>(*c, *plan, q, q_tok, q_head, Hq, gshift, pshift, scale, slots, tail, out, lse, part_o, part_ml, stream) \
-                                            : launch_step<D_, E_, 2>(*c, *plan, q, q_tok, q_head, Hq, gshift, pshift, scale, slots, tail, out, lse, part_o, part_ml, stream)
+    // waves: two workgroups to a compute unit (head_dim 256: one of 132 KB)
+#define STEP_ROWS(D_, E_, NW_) return rows <= 16 ? launch_step<D_, E_, 1, NW_>(*c, *plan, q, q_tok, q_head, Hq, gshift, pshift, scale, tail, out, lse, part_o, part_ml, stream) \
+                                                 : launch_step<D_, E_, 2, NW_>(*c, *plan, q, q_tok, q_head, Hq, gshift, pshift, scale, tail, out, lse, part_o, part_ml, stream)
     if (rows > 32 || c->D > 256) return hipErrorInvalidValue;
     if (c->D <= 64) {
-        if (e) STEP_CASE(64, true);
-        STEP_CASE(64, false);
+        if (e) STEP_ROWS(64, true, 4);
+        STEP_ROWS(64, false, 4);
     }
     if (c->D <= 128) {
-        if (e) STEP_CASE(128, true);
-        STEP_CASE(128, false);
+        if (e) STEP_ROWS(128, true, 4);
+        if (waves == 4) STEP_ROWS(128, false, 4);
+        STEP_ROWS(128, false, 2);
     }
-    if (e) STEP_CASE(256, true);
-    STEP_CASE(256, false);
+    if (e) STEP_ROWS(256, true, 4);
+    STEP_ROWS(256, false, 2);
 }
-extern "C" hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PagePlan *plan, int Hq, int blocks, const float *part_o, const float *part_ml, void *out, float *lse,
-                                            hipStream_t stream) {
-    const int gshift = group_shift(Hq, c->Hkv), items = (plan->qb << gshift) * c->D / 4, wg = blocks * c->Hkv;
+// many: of the walk of many rows (blocks 0: none), few: of this file's
+extern "C" hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PagedJoin *many, const PagedJoin *few, int Hq, void *out, float *lse, hipStream_t stream) {
+    const int gshift = group_shift(Hq, c->Hkv), rows = std::max(many->blocks ? many->plan.qb : 0, few->blocks ? few->plan.qb : 0) << gshift, items = rows * c->D / 4;
+    const int wg = (many->blocks + few->blocks) * c->Hkv;
     // workgroups enough for the card where the blocks alone are not
-    const bool many = (int64_t)wg * ((items + 255) / 256) < 256;
-    const int y = many ? (items + 31) / 32 : std::max(1, std::min((items + 255) / 256, 2048 / wg));
-    const auto kernel = many ? &dsa_paged_join_kernel<32> : &dsa_paged_join_kernel<256>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)wg, (unsigned)y), dim3(256), 0, stream, *c, *plan, Hq, gshift, part_o, part_ml, (bf16_t *)out, lse);
+    const bool very = std::max(many->blocks ? many->pieces : 0, few->blocks ? few->pieces : 0) > 16 && (int64_t)wg * ((items + 31) / 32) < 256, some = (int64_t)wg * ((items + 255) / 256) < 256;
+    const int y = very ? (items + 7) / 8 : some ? (items + 31) / 32 : std::max(1, std::min((items + 255) / 256, 8192 / wg));
+    const auto kernel = very ? &dsa_paged_join_kernel<8> : some ? &dsa_paged_join_kernel<32> : &dsa_paged_join_kernel<256>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)wg, (unsigned)y), dim3(256), 0, stream, *c, *many, *few, Hq, gshift, (bf16_t *)out, lse);
     return hipGetLastError();
 }
