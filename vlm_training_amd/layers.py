@@ -10,6 +10,9 @@
 * ``DsaIndexer``            - the lightning indexer's projections as module parameters (the reference holds no
   indexer): hidden -> Hi*Di index queries, hidden -> Di index key (one per token), hidden -> Hi head weights.
 
+Both attention layers have a serving form too, ``extend(x, cos, sin, cache, page_table, cu_seqlens, lengths)``: new tokens of requests whose keys and values lie in a paged
+``KvCache``.  The reference trains only and has none.
+
 The projections stay torch GEMMs (plain ones share one autograd node: ``_projections``).  Norm + RoPE + layout is one
 kernel (``qk_norm_rope``), the attention is
 ``dsa_varlen_attn`` (dense causal without an indexer: the reference's behaviour), the gate is one kernel.
@@ -26,6 +29,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .cache import KvCache, kv_cache_write, paged_attn
 from .delta import gated_delta_rule, gated_delta_step, short_conv, short_conv_step
 from .dtensor_utils import _column_sharded, _dtensor_rewrap, _dtensor_unwrap, _local
 from .model_attention import run_varlen_attn
@@ -140,6 +144,19 @@ def attention_core(module, q_lin, k_lin, v_lin, cos, sin, cu_seqlens, max_seqlen
     return out
 
 
+def cached_attention_core(module, q_lin, k_lin, v_lin, cos, sin, cache: KvCache, page_table, cu_seqlens, lengths, max_new=None, max_length=None, gate=None, offset=False):
+    """``attention_core`` for new tokens whose requests lie in ``cache``: their keys and values go there, then they attend what it holds."""
+    if getattr(module, "indexer", None) is not None:
+        raise NotImplementedError("a DSA layer has no cached form: the indexer selects among the keys of a packed row")
+    eps = getattr(module.q_norm, "eps", None)
+    if eps is None:
+        eps = getattr(module.q_norm, "variance_epsilon", 1e-6)
+    q, k = qk_norm_rope(_bf16(q_lin), _bf16(k_lin), _local(module.q_norm.weight), _local(module.k_norm.weight), cos, sin, eps=eps, offset=offset)
+    kv_cache_write(cache, k, _bf16(v_lin), page_table, cu_seqlens, lengths)
+    out = paged_attn(q, cache, page_table, cu_seqlens, lengths, max_new=max_new, max_length=max_length)
+    return out if gate is None else sigmoid_gate(out, _bf16(gate))
+
+
 def indexer_losses(model: nn.Module):
     """Sum of the indexer losses the DSA layers of ``model`` left behind in their last forward (None if there is none)."""
     total = None
@@ -212,6 +229,18 @@ class Qwen3VLTextAttention(nn.Module):
         return self.o_proj(out.reshape(1, total, -1).to(x.dtype))
 
 
+    @torch.no_grad()
+    def extend(self, x, cos, sin, cache: KvCache, page_table, cu_seqlens, lengths, *, max_new=None, max_length=None):
+        """New tokens of N requests, a whole prompt, a chunk of one or one token, x (T, hidden) or (1, T, hidden) -> the same: they join their requests in ``cache`` and attend them.
+
+        ``cos``, ``sin`` are the tables at the new tokens' positions, ``lengths`` the requests' lengths with them; the rest is as in ``paged_attn``.  A head-sharded layer's cache
+        holds its own kv heads."""
+        h = x.reshape(-1, x.shape[-1])
+        (q, k, v), wrap = _dtensor_unwrap(*(m(h).unflatten(-1, (-1, self.head_dim)) for m in (self.q_proj, self.k_proj, self.v_proj)))
+        out = cached_attention_core(self, q, k, v, cos, sin, cache, page_table, cu_seqlens, lengths, max_new, max_length)
+        return self.o_proj(_dtensor_rewrap(out, wrap).flatten(1).to(x.dtype)).reshape(x.shape)
+
+
 class SelfAttention(nn.Module):
     """models/qwen3_5/model.py:76-136 (the full-attention layers of the hybrid stack): gated, OffsetRMSNorm, the
     rotary width is whatever the cos / sin tables have."""
@@ -252,6 +281,18 @@ class SelfAttention(nn.Module):
         out = attention_core(self, qg[..., :D], k, v, cos, sin, cu_seqlens, max_seqlen, x=x, gate=qg[..., D:], offset=True)
         out = _dtensor_rewrap(out, wrap)
         return self.o_proj(out.reshape(1, total, -1).to(x.dtype))
+
+
+    @torch.no_grad()
+    def extend(self, x, cos, sin, cache: KvCache, page_table, cu_seqlens, lengths, *, max_new=None, max_length=None):
+        """New tokens of N requests, a whole prompt, a chunk of one or one token, x (T, hidden) or (1, T, hidden) -> the same: they join their requests in ``cache`` and attend them.
+
+        ``cos``, ``sin`` are the tables at the new tokens' positions, ``lengths`` the requests' lengths with them; the rest is as in ``paged_attn``.  A head-sharded layer's cache
+        holds its own kv heads."""
+        D, h = self.head_dim, x.reshape(-1, x.shape[-1])
+        (qg, k, v), wrap = _dtensor_unwrap(self.q_proj(h).unflatten(-1, (-1, 2 * D)), self.k_proj(h).unflatten(-1, (-1, D)), self.v_proj(h).unflatten(-1, (-1, D)))
+        out = cached_attention_core(self, qg[..., :D], k, v, cos, sin, cache, page_table, cu_seqlens, lengths, max_new, max_length, gate=qg[..., D:], offset=True)
+        return self.o_proj(_dtensor_rewrap(out, wrap).flatten(1).to(x.dtype)).reshape(x.shape)
 
 
 @dataclass
