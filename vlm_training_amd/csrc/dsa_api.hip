@@ -1277,6 +1277,7 @@ static int check_cache(const dsa_cache_args *c, const int32_t *cu, int T, int N)
     if (off16(c->k) || off16(c->v) || c->k_page % unit || c->v_page % unit || (e4m3 && (off16(c->k_exp) || off16(c->v_exp) || (c->kx_page | c->vx_page) % 16)))
         return fail(DSA_ERR_ARG, "pools and their pages must lie on 16-byte boundaries");
     const int64_t page = (int64_t)c->Hkv * c->page * c->D, scales = (int64_t)c->Hkv * c->page;
+    if (std::max(std::max(c->k_page, c->v_page) * (e4m3 ? 1 : 2), std::max(c->kx_page, c->vx_page)) > UINT32_MAX) return fail(DSA_ERR_UNSUPPORTED, "pages 4 GiB apart and more");
     if (c->pages > 1 && (c->k_page < page || c->v_page < page || (e4m3 && (c->kx_page < scales || c->vx_page < scales)))) return fail(DSA_ERR_ARG, "pages overlap");
     return DSA_OK;
 }
@@ -1317,7 +1318,7 @@ static PagedLaunch paged_launch(const dsa_cache_args *c, const int32_t *cu, cons
                                 int max_length) {
     const int capacity = c->table_pages * c->page, longest = max_length > 0 ? std::min(max_length, capacity) : capacity, least = many ? 8 : 4;
     PagedLaunch p{};
-    p.plan = PagePlan{N, T, qb, few, side, std::max(1, resident / c->Hkv), 0.f, least, (longest + 31) / 32 <= least, 0, cu, lengths, capacity};
+    p.plan = PagePlan{N, T, qb, few, side, std::max(1, resident / c->Hkv), 0.f, least, (longest + 31) / 32 <= least, resident > 256 ? 256 / c->Hkv : 0, 0, cu, lengths, capacity};
     // blocks: of requests of up to `few` rows (one block) as many as there are, of the others the rows' and what the last one of each request lacks
     const int64_t requests = std::min<int64_t>(N, side == 1 ? T / (few + 1) : T);
     p.blocks = side == 0 ? requests : (T + requests * (qb - 1)) / qb;
@@ -1325,6 +1326,7 @@ static PagedLaunch paged_launch(const dsa_cache_args *c, const int32_t *cu, cons
     if (many) {
         // Where blocks are few, so many pieces that all workgroups run at once
         if (2 * p.blocks <= p.plan.target) p.plan.target -= (int)p.blocks;
+        if (N == 1 && p.blocks >= p.plan.target) p.plan.whole = 1;       // (no block is longer than a piece then)
         p.slots = p.blocks + p.plan.target + 1;          // (with a block's last piece; one more, so that some workgroup is left for the rows behind the last request)
         records = p.slots;
     } else {

@@ -49,6 +49,7 @@ struct PagePlan {
     float per_target;              // 1 / target
     int least;                     // tiles of 32 keys that a piece of a block has at the least
     int whole;                     // no block is cut
+    int pair;                      // workgroups of a kv head that run at once, one to a compute unit (0: no second one to a unit)
     int ushift;                    // shares are counted in units of 2^ushift tiles
     const int32_t *cu, *lengths;
     int capacity;                  // positions that the table holds
@@ -108,6 +109,11 @@ __device__ __forceinline__ bool locate_piece(const PagePlan &p, int slot, PagePi
         if (base > 0) r = page_request(p, base + lane);
         const int each = max(per, (int)sqrtf((float)r.tiles)), np = max(1, (r.tiles + each - 1) / each), mine = r.blocks * np, count = BLOCKS ? r.blocks : mine;
         const int upto = wave_prefix_i(count), slots_upto = BLOCKS ? wave_prefix_i(mine) : upto;
+        if (!BLOCKS && p.N <= 64) {
+            // a launch of one round, the units' second workgroups: from the end, so that a unit with a long walk has a short one beside it
+            const int total = __builtin_amdgcn_readlane(upto, 63);
+            if (slot >= p.pair && slot < total && total <= 2 * p.pair) slot = total - 1 - (slot - p.pair);
+        }
         const uint64_t past = __builtin_amdgcn_ballot_w64(taken + upto > slot);
         if (past) {
             const int w = (int)__builtin_ctzll(past);

@@ -441,7 +441,7 @@ extern "C" hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const Paged
     const int wg = (many->blocks + few->blocks) * c->Hkv;
     // workgroups enough for the card where the blocks alone are not
     const bool very = std::max(many->blocks ? many->pieces : 0, few->blocks ? few->pieces : 0) > 16 && (int64_t)wg * ((items + 31) / 32) < 256, some = (int64_t)wg * ((items + 255) / 256) < 256;
-    const int y = very ? (items + 7) / 8 : some ? (items + 31) / 32 : std::max(1, std::min((items + 255) / 256, 8192 / wg));
+    const int y = very ? (items + 7) / 8 : some ? (items + 31) / 32 : std::max(1, std::min((items + 255) / 256, 4096 / wg));
     const auto kernel = very ? &dsa_paged_join_kernel<8> : some ? &dsa_paged_join_kernel<32> : &dsa_paged_join_kernel<256>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)wg, (unsigned)y), dim3(256), 0, stream, *c, *many, *few, Hq, gshift, (bf16_t *)out, lse);
     return hipGetLastError();

@@ -95,15 +95,25 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
         const int from = batch * 64, there = max(min(c.table_pages - from, 64), 0);
         buffer_load_lds4(make_buffer_rsrc(table + min(from, c.table_pages), there * 4), lane * 4, ids0 + (batch & 1) * 256);
     };
-    auto page_at = [&](int tile) __attribute__((always_inline)) {        // of the wave's rows of a tile: looked up one step ahead of its use
-        return mine[((base + tile) * 32 + 8 * wv) >> pshift & 127];
+    // Where the wave's rows of a tile lie.  All of it is scalar and short: scalar instructions too are issued in between the MFMAs (64-bit products of element strides, formed
+    // for each operand and tile, were 130 a step)
+    const int row0 = __builtin_amdgcn_readfirstlane(base * 32 + 8 * wv), end = __builtin_amdgcn_readfirstlane(min(keys, (base + ntiles) * 32)), pmask = c.page - 1;
+    const uint32_t row_b = d_real * (E4M3 ? 1 : 2), k_stride = (uint32_t)c.k_page * (E4M3 ? 1u : 2u), v_stride = (uint32_t)c.v_page * (E4M3 ? 1u : 2u);
+    const unsigned char *const k_pool = (const unsigned char *)c.k + (int64_t)kvh * c.page * row_b, *const v_pool = (const unsigned char *)c.v + (int64_t)kvh * c.page * row_b;
+    auto page_at = [&](int tile) __attribute__((always_inline)) {        // number of their page: looked up one step ahead of its use
+        return mine[(row0 + tile * 32) >> pshift & 127];
     };
-    auto rows_of = [&](int tile, int id) __attribute__((always_inline)) {  // how many of them there are
-        const int p = (base + tile) * 32 + 8 * wv;
-        return (uint32_t)id < (uint32_t)c.pages && tile < ntiles ? min(max(keys - p, 0), 8) : 0;
+    struct Where { uint32_t id, rows, place; };             // page, rows that exist, the first one's place among the page's
+    auto where = [&](int tile, int id_) __attribute__((always_inline)) {
+        const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(id_), p = row0 + tile * 32;
+        const int left = max(end - (int)p, 0);
+        int rows = left;
+        asm("s_min_i32 %0, %0, 8" : "+s"(rows) : : "scc");  // (a clamp would go through the vector pipe and come back)
+        const bool there = id < (uint32_t)c.pages;
+        return Where{there ? id : 0u, there ? (uint32_t)rows : 0u, p & pmask};
     };
-    auto place_of = [&](int tile) __attribute__((always_inline)) {         // of the first of them in the page's rows of this head
-        return (int64_t)kvh * c.page + (((base + tile) * 32 + 8 * wv) & (c.page - 1));
+    auto address = [&](const unsigned char *pool, uint32_t stride, const Where &w, uint32_t bytes) __attribute__((always_inline)) {
+        return pool + (uint64_t)w.id * stride + w.place * bytes;
     };
 
     // ---- requests: bf16 ----
@@ -111,14 +121,14 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     int voff[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) voff[i] = TL::source(i, lane, d_real * 2, chunks);
-    auto load_tile = [&](const bf16_t *pool, int64_t stride, int tile, int id_, int slot) __attribute__((always_inline)) {
-        const int id = __builtin_amdgcn_readfirstlane(id_), rows = rows_of(tile, id);
+    auto load_tile = [&](const unsigned char *pool, uint32_t stride, int tile, int id, int slot) __attribute__((always_inline)) {
+        const Where w = where(tile, id);
         int off[LPW];
 #pragma unroll
         for (int i = 0; i < LPW; ++i) off[i] = voff[i % NV] + i / NV * NV * TL::LOAD_ROWS * d_real * 2;
         constexpr int P1 = LPW > 1 ? 1 : 0, P2 = LPW > 2 ? 2 : P1, P3 = LPW > 2 ? 3 : P2;
         buffer_load_lds16_n<LPW, TL::load_lds(P1), TL::load_lds(P2) - TL::load_lds(P1), TL::load_lds(P3) - TL::load_lds(P2)>(
-            scalar_buffer_rsrc(pool + (rows ? id : 0) * stride + place_of(tile) * d_real, (uint32_t)(rows * d_real * 2)), off, lds0 + slot * TL::BYTES + TL::load_lds(wv * LPW));
+            scalar_buffer_rsrc(address(pool, stride, w, row_b), w.rows * row_b), off, lds0 + slot * TL::BYTES + TL::load_lds(wv * LPW));
     };
     // ---- requests: 8-bit.  A lane has D / 8 values of the wave's eight rows: 8 of row lane / 8 (head_dim 64), 16 of it, or 16 of rows lane / 16 and 4 more (256) ----
     constexpr int NC = D == 256 ? 2 : 1, CW = D == 64 ? 2 : 4, PER = D == 256 ? 16 : 8;
@@ -127,11 +137,12 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     uint32_t kex[E4M3 ? 2 : 1][NC], vex[E4M3 ? 2 : 1][NC];
     const int e_row = lane / PER, e_col = lane % PER * 4 * CW, e_off = e_col < d_real ? e_row * d_real + e_col : (int)0x80000000;
     // (buffers that end with the rows that exist: others read as zero)
-    auto fetch = [&](const uint8_t *pool, int64_t stride, const uint8_t *exps, int64_t xstride, int tile, int id_, codes_t (&raw)[NC], uint32_t (&ex)[NC]) __attribute__((always_inline)) {
-        const int id = __builtin_amdgcn_readfirstlane(id_), rows = rows_of(tile, id);
-        const int64_t place = place_of(tile);
-        const auto values = __builtin_amdgcn_make_buffer_rsrc((void *)(pool + (rows ? id : 0) * stride + place * d_real), 0, rows * d_real, 0x00020000);
-        const auto powers = __builtin_amdgcn_make_buffer_rsrc((void *)(exps + (rows ? id : 0) * xstride + place), 0, rows, 0x00020000);
+    const uint32_t kx_stride = (uint32_t)c.kx_page, vx_stride = (uint32_t)c.vx_page;
+    const unsigned char *const kx_pool = (const unsigned char *)c.k_exp + (int64_t)kvh * c.page, *const vx_pool = (const unsigned char *)c.v_exp + (int64_t)kvh * c.page;
+    auto fetch = [&](const unsigned char *pool, uint32_t stride, const unsigned char *exps, uint32_t xstride, int tile, int id, codes_t (&raw)[NC], uint32_t (&ex)[NC]) __attribute__((always_inline)) {
+        const Where w = where(tile, id);
+        const auto values = __builtin_amdgcn_make_buffer_rsrc((void *)address(pool, stride, w, row_b), 0, w.rows * row_b, 0x00020000);
+        const auto powers = __builtin_amdgcn_make_buffer_rsrc((void *)address(exps, xstride, w, 1u), 0, w.rows, 0x00020000);
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             if constexpr (CW == 4) raw[i] = __builtin_amdgcn_raw_buffer_load_b128(values, e_off + 4 * i * d_real, 0, 0);
@@ -153,13 +164,13 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
         }
     };
     auto fetch_k = [&](int tile, int id, codes_t (&raw)[NC], uint32_t (&ex)[NC]) __attribute__((always_inline)) {
-        fetch((const uint8_t *)c.k, c.k_page, (const uint8_t *)c.k_exp, c.kx_page, tile, id, raw, ex);
+        fetch(k_pool, k_stride, kx_pool, kx_stride, tile, id, raw, ex);
     };
     auto fetch_v = [&](int tile, int id, codes_t (&raw)[NC], uint32_t (&ex)[NC]) __attribute__((always_inline)) {
-        fetch((const uint8_t *)c.v, c.v_page, (const uint8_t *)c.v_exp, c.vx_page, tile, id, raw, ex);
+        fetch(v_pool, v_stride, vx_pool, vx_stride, tile, id, raw, ex);
     };
-    auto load_k = [&](int tile, int id) __attribute__((always_inline)) { load_tile((const bf16_t *)c.k, c.k_page, tile, id, tile & 3); };
-    auto load_v = [&](int tile, int id) __attribute__((always_inline)) { load_tile((const bf16_t *)c.v, c.v_page, tile, id, 4 + (tile & 3)); };
+    auto load_k = [&](int tile, int id) __attribute__((always_inline)) { load_tile(k_pool, k_stride, tile, id, tile & 3); };
+    auto load_v = [&](int tile, int id) __attribute__((always_inline)) { load_tile(v_pool, v_stride, tile, id, 4 + (tile & 3)); };
 
     // page numbers of the first tiles, q in the meantime
     const int batch0 = base * 32 >> pshift >> 6;
@@ -468,8 +479,8 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     for (int tile = 0; tile < ntiles; ++tile) {
         const int id = page_of(c, pc.n, pshift, (base + tile) * 32 + 8 * wv);
         if constexpr (!E4M3) {
-            load_tile((const bf16_t *)c.k, c.k_page, tile, id, 0);
-            load_tile((const bf16_t *)c.v, c.v_page, tile, id, 4);
+            load_tile(k_pool, k_stride, tile, id, 0);
+            load_tile(v_pool, v_stride, tile, id, 4);
             wait_vmcnt<0>();
         } else {
             fetch_k(tile, id, kraw[0], kex[0]);
