@@ -488,7 +488,7 @@ int dsa_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x
  * (pages, Hkv, page; pages kx_page / vx_page bytes apart): a value stands for itself times 2^(b - 127), b = 255 for NaN.  Written are powers from 2^-100 on, the smallest with which a row's largest
  * value is at most 448: what the bytes stand for is exact in bf16.  A row with a value that is not finite is NaN as a whole.
  * table (N, table_pages) int32, rows table_row apart: position p of request n lies on page table[n][p / page], at p % page.
- * Pools lie on 16-byte boundaries; k_page, v_page are multiples of 8 elements (e4m3: 16), kx_page, vx_page of 16 bytes.
+ * Pools lie on 16-byte boundaries; k_page, v_page are multiples of 8 elements (e4m3: 16), kx_page, vx_page of 16 bytes, each under 4 GiB; a table holds up to 2^30 positions.
  * What lies on no page (a page number outside the pool, a position outside the table) is not written and reads as zero.
  *
  * dsa_cache_write: request n's new rows cu[n] .. cu[n+1]-1 of k, v (T,Hkv,D) bf16 (token and head strides multiples of 8, rows on 16-byte boundaries) become its last ones,

@@ -36,13 +36,13 @@ def attend(q, k, v, scale, limits):
     """q (m, Hq, D), k, v (L, Hkv, D) -> (out, lse): row i attends keys 0 .. limits[i]; zeros and -inf where that is none.  What a row does not attend is not looked at."""
     m, hq, d = q.shape
     group = hq // k.shape[1]
+    k, v = (x.double().repeat_interleave(group, 1).transpose(0, 1) for x in (k, v))          # (Hq, L, D)
     out, lse = torch.zeros(m, hq, d, dtype=torch.float64), torch.full((hq, m), -math.inf, dtype=torch.float64)
     for i, limit in enumerate(limits):
-        n = min(limit + 1, k.shape[0])
+        n = min(limit + 1, k.shape[1])
         if n <= 0:
             continue
-        for h in range(hq):
-            s = scale * (k[:n, h // group].double() @ q[i, h].double())
-            lse[h, i] = torch.logsumexp(s, 0)
-            out[i, h] = torch.softmax(s, 0) @ v[:n, h // group].double()
+        s = scale * (k[:, :n] @ q[i].double()[..., None])[..., 0]                             # (Hq, n)
+        lse[:, i] = torch.logsumexp(s, -1)
+        out[i] = (torch.softmax(s, -1)[:, None] @ v[:, :n])[:, 0]
     return out, lse

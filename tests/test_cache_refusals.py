@@ -17,7 +17,7 @@ def _args(**change):
 
 REFUSED = [(dict(kind=2), -1, b"kind"), (dict(D=12), -2, b"head_dim"), (dict(D=264), -2, b"head_dim"), (dict(D=0), -2, b"head_dim"), (dict(D=72, kind=1), -2, b"multiple of 16"),
            (dict(page=8), -2, b"pages of 8"), (dict(page=48), -2, b"pages of 48"), (dict(page=512), -2, b"pages of 512"), (dict(pages=0), -1, b"pages=0"), (dict(Hkv=0), -1, b"Hkv=0"),
-           (dict(table_pages=0), -1, b"table_pages=0"), (dict(table_pages=1 << 26, table_row=1 << 26), -2, b"31 bits"), (dict(k=None), -1, b"null"), (dict(table=None), -1, b"null"),
+           (dict(table_pages=0), -1, b"table_pages=0"), (dict(table_pages=(1 << 24) + 1, table_row=1 << 26), -2, b"2^30"), (dict(k_page=1 << 31), -2, b"4 GiB"), (dict(vx_page=1 << 32, kind=1), -2, b"4 GiB"), (dict(k=None), -1, b"null"), (dict(table=None), -1, b"null"),
            (dict(k_exp=None, kind=1), -1, b"null"), (dict(table_row=7), -1, b"table rows"), (dict(v=8), -1, b"16-byte"), (dict(k_page=2 * 64 * 128 + 4), -1, b"16-byte"),
            (dict(kx_page=136, kind=1), -1, b"16-byte"), (dict(v_page=2 * 64 * 128 - 8), -1, b"overlap"), (dict(vx_page=112, kind=1), -1, b"overlap")]
 
@@ -51,6 +51,10 @@ def test_operands():
                          (dict(out=8), -1), (dict(ws=None), -3), (dict(ws=8), -3), (dict(n=need - 1), -3)):
         assert attn(**change) == code, change
     assert attn(T=0) == 0
+    for T, N, Hkv, new in ((1 << 30, 1 << 30, 2, 1), (1 << 26, 1 << 26, 2, 1), ((1 << 31) - 1, 1, 64, 0)):            # more blocks than a launch has room for
+        many = _args(Hkv=Hkv, k_page=Hkv * 64 * 128, v_page=Hkv * 64 * 128)
+        assert lib.dsa_paged_attn(many, 16, 512, 128, 16, 16, T, N, 2 * Hkv, 1.0, new, 0, 16, None, 16, 1 << 40, None) == -2 and b"too many" in lib.dsa_last_error()
+        assert lib.dsa_paged_attn_workspace_bytes(many, T, N, 2 * Hkv, new, 0) == 0
 
 
 def test_python_entries():

@@ -156,3 +156,35 @@ def test_a_request_of_300000_tokens():
         q = _rand((m, 1, dim), 5, std=3.0)
         out, lse = V.paged_attn(q, cache, table, _offsets([m]).to(DEV), torch.tensor([length], device=DEV), return_lse=True)
         check(out, lse, q, [[x[:length] for x in kv[0]]], "bf16", [m], [length], dim ** -0.5)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [[1, 1, 1], [2, 5, 1], [60, 20, 1]])
+def test_powers_behind_the_last_row_may_be_anything(dim, new):
+    """Pages that were another request's before: NaN's power behind the last row, values that are NaN too."""
+    lens = [70, 33, 1]
+    rows, cache, table = make("e4m3", lens, 2, dim, 64, seed=2)
+    for i, n in enumerate(lens):
+        for p in range(n, (n + 63) // 64 * 64):
+            for pool, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+                scale.view(torch.uint8)[int(table[i, p // 64]), :, p % 64] = 255
+                pool.view(torch.uint8)[int(table[i, p // 64]), :, p % 64, ::3] = 0x7f
+    q = _rand((sum(new), 4, dim), 4)
+    for kw in (dict(), dict(max_new=max(new), max_length=100)):
+        out, lse = V.paged_attn(q, cache, table, _offsets(new).to(DEV), torch.tensor(lens, device=DEV), return_lse=True, **kw)
+        check(out, lse, q, rows, "e4m3", new, lens, dim ** -0.5)
+
+
+@pytest.mark.parametrize("hq,hkv", [(16, 1), (4, 2)])
+def test_later_tokens_that_are_not_finite_with_a_bound_that_does_not_hold(hq, hkv):
+    """One query to a block although there are three: a value behind it in its tile, infinite or NaN, stays out."""
+    rows, cache, table = make("bf16", [40, 3], hkv, 64, 16)
+    for i, n in ((0, 40), (1, 3)):
+        page, place = int(table[i, (n - 1) // 16]), (n - 1) % 16
+        cache.v[page, :, place] = float("nan")
+        cache.v[page, 0, place, 0] = float("inf")
+    q = _rand((6, hq, 64), 1)
+    out, lse = V.paged_attn(q, cache, table, _offsets([3, 3]).to(DEV), torch.tensor([40, 3], device=DEV), max_new=1, return_lse=True)
+    for at, i, n in ((0, 0, 40), (3, 1, 3)):
+        check(out[at:at + 2], lse[:, at:at + 2], q[at:at + 2], [[x[:n - 1] for x in rows[i]]], "bf16", [2], [n - 1], 64 ** -0.5)
+        assert not torch.isfinite(out[at + 2]).any()

@@ -1271,7 +1271,7 @@ static int check_cache(const dsa_cache_args *c, const int32_t *cu, int T, int N)
     if (c->D < unit || c->D > 256 || c->D % unit) return fail(DSA_ERR_UNSUPPORTED, "head_dim %d: need a multiple of %d up to 256", c->D, unit);
     if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1))) return fail(DSA_ERR_UNSUPPORTED, "pages of %d rows: need 16, 32, 64, 128 or 256", c->page);
     if (c->pages < 1 || c->Hkv < 1 || c->table_pages < 1) return fail(DSA_ERR_ARG, "pages=%d Hkv=%d table_pages=%d", c->pages, c->Hkv, c->table_pages);
-    if (c->table_pages > INT32_MAX / c->page) return fail(DSA_ERR_UNSUPPORTED, "a table of %d pages of %d rows: positions have 31 bits", c->table_pages, c->page);
+    if (c->table_pages > (1 << 30) / c->page) return fail(DSA_ERR_UNSUPPORTED, "a table of %d pages of %d rows: positions go up to 2^30", c->table_pages, c->page);
     if (!c->k || !c->v || !c->table || (e4m3 && (!c->k_exp || !c->v_exp))) return fail(DSA_ERR_ARG, "null pool or table pointer");
     if (N > 1 && c->table_row < c->table_pages) return fail(DSA_ERR_ARG, "table rows %lld apart hold no %d pages", (long long)c->table_row, c->table_pages);
     if (off16(c->k) || off16(c->v) || c->k_page % unit || c->v_page % unit || (e4m3 && (off16(c->k_exp) || off16(c->v_exp) || (c->kx_page | c->vx_page) % 16)))
@@ -1328,12 +1328,12 @@ static PagedLaunch paged_launch(const dsa_cache_args *c, const int32_t *cu, cons
         if (2 * p.blocks <= p.plan.target) p.plan.target -= (int)p.blocks;
         if (N == 1 && p.blocks >= p.plan.target) p.plan.whole = 1;       // (no block is longer than a piece then)
         p.slots = p.blocks + p.plan.target + 1;          // (with a block's last piece; one more, so that some workgroup is left for the rows behind the last request)
-        records = p.slots;
+        records = 2 * p.plan.target;                     // (of blocks that are cut: n pieces of more than n - 1 times the length that makes `target` of them)
     } else {
         // Few blocks: their waves side by side on a unit of their own (one token over 1000 keys, 8 kv heads: 9.3 us, two waves to a workgroup 11.8)
         p.waves = p.blocks * c->Hkv <= 64 ? 4 : 2;
         if (p.waves == 4 && c->kind == DSA_CACHE_BF16 && c->D > 64) p.plan.target = std::max(1, 256 / c->Hkv);
-        while (p.blocks * ((capacity / 32 >> p.plan.ushift) + 8) >= 1 << 29) ++p.plan.ushift;
+        while (p.blocks < 1 << 25 && p.blocks * ((capacity / 32 >> p.plan.ushift) + 8) >= 1 << 29) ++p.plan.ushift;
         p.slots = p.plan.target;
         records = 2 * p.slots;
     }
@@ -1369,7 +1369,7 @@ static int check_paged(const dsa_cache_args *c, const int32_t *cu, int T, int N,
     if (Hq / c->Hkv > 16) return fail(DSA_ERR_UNSUPPORTED, "Hq/Hkv=%d: up to 16", Hq / c->Hkv);
     if (max_new < 0 || max_length < 0) return fail(DSA_ERR_ARG, "max_new=%d max_length=%d", max_new, max_length);
     const PagedCall p = paged_call(c, cu, nullptr, T, N, Hq, max_new, max_length);
-    if (std::max(p.step.slots, p.walk.slots) * c->Hkv > INT32_MAX) return fail(DSA_ERR_UNSUPPORTED, "too many blocks: T=%d N=%d Hkv=%d", T, N, c->Hkv);
+    if (std::max(std::max(p.step.blocks, p.step.slots), p.walk.slots + p.step.blocks) * c->Hkv > INT32_MAX || p.step.blocks >= 1 << 25) return fail(DSA_ERR_UNSUPPORTED, "too many blocks: T=%d N=%d Hkv=%d", T, N, c->Hkv);
     return DSA_OK;
 }
 extern "C" size_t dsa_paged_attn_workspace_bytes(const dsa_cache_args *c, int T, int N, int Hq, int max_new, int max_length) {

@@ -104,11 +104,11 @@ __device__ __forceinline__ bool locate_piece(const PagePlan &p, int slot, PagePi
         sum += (float)x.blocks * (float)x.tiles;
     }
     const int per = piece_tiles(p, sum);
-    int slots = 0, taken = 0;                            // of pieces, and of what is counted
+    int slots = 0, taken = 0;                            // of sums, and of what is counted
     for (int base = 0; base < p.N; base += 64) {
         if (base > 0) r = page_request(p, base + lane);
         const int each = max(per, (int)sqrtf((float)r.tiles)), np = max(1, (r.tiles + each - 1) / each), mine = r.blocks * np, count = BLOCKS ? r.blocks : mine;
-        const int upto = wave_prefix_i(count), slots_upto = BLOCKS ? wave_prefix_i(mine) : upto;
+        const int upto = wave_prefix_i(count), sums = np > 1 ? mine : 0, sums_upto = wave_prefix_i(sums);      // (blocks that are not cut have no sums to keep)
         if (!BLOCKS && p.N <= 64) {
             // a launch of one round, the units' second workgroups: from the end, so that a unit with a long walk has a short one beside it
             const int total = __builtin_amdgcn_readlane(upto, 63);
@@ -126,7 +126,7 @@ __device__ __forceinline__ bool locate_piece(const PagePlan &p, int slot, PagePi
             out.m = __builtin_amdgcn_readlane(r.m, w);
             out.length = __builtin_amdgcn_readlane(r.length, w);
             out.first = (blocks - 1 - order) * p.qb;
-            out.slot = slots + __builtin_amdgcn_readlane(slots_upto, w) - __builtin_amdgcn_readlane(mine, w) + order * np_w;
+            out.slot = slots + __builtin_amdgcn_readlane(sums_upto, w) - __builtin_amdgcn_readlane(sums, w) + order * np_w;
             const int last = out.length - out.m + min(out.first + p.qb, out.m) - 1;      // position of the block's last row
             const int tiles = last < 0 ? 0 : (min(last, p.capacity - 1) >> 5) + 1, len = (tiles + np_w - 1) / np_w;
             out.pieces = len > 0 ? (tiles + len - 1) / len : 1;
@@ -136,7 +136,7 @@ __device__ __forceinline__ bool locate_piece(const PagePlan &p, int slot, PagePi
             return true;
         }
         taken += __builtin_amdgcn_readlane(upto, 63);
-        slots += __builtin_amdgcn_readlane(slots_upto, 63);
+        slots += __builtin_amdgcn_readlane(sums_upto, 63);
     }
     spare = taken;
     return false;

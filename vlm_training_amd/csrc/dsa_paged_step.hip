@@ -63,7 +63,7 @@ __global__ __launch_bounds__(NW * 64, 1) void dsa_paged_step_kernel(dsa_cache_ar
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qB[rg][ks] = ok && 4 * ks + g < chunks ? load_bf16x8(src + 32 * ks + 8 * g) : zero_bf16x8();
     }
-    const bool one_limit = plan.qb == 1 || pc.m == 1;    // every row attends the same keys
+    const bool one_limit = pc.m == 1;                    // every row attends all keys that there are
 
     // ---- tiles ----
     unsigned char *const ring = dyn_lds + wv * WAVE_B;   // K | V, or K | V | K | V
@@ -128,9 +128,9 @@ __global__ __launch_bounds__(NW * 64, 1) void dsa_paged_step_kernel(dsa_cache_ar
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const int r = e_row + i;
-                const float s = exponent_scale((ex[op][i >> 2] >> (8 * (i & 3))) & 0xff);
-                codes_t w = raw[op][i];
-                if (!all && tile * 32 + r >= keys) w = codes_t{0u, 0u, 0u, 0u};
+                const bool gone = !all && tile * 32 + r >= keys;        // (what lies behind the last key, values and powers, may be anything)
+                const float s = exponent_scale(gone ? 127u : (ex[op][i >> 2] >> (8 * (i & 3))) & 0xff);
+                const codes_t w = gone ? codes_t{0u, 0u, 0u, 0u} : raw[op][i];
                 const u32x2 a = e4m3_to_bf16(w[0], s), b = e4m3_to_bf16(w[1], s), x = e4m3_to_bf16(w[2], s), y = e4m3_to_bf16(w[3], s);
                 unsigned char *const to = ring + op * TL::BYTES + r / TL::GROUP * TL::GROUP_B + r % TL::GROUP * TL::ROW_B;
                 *reinterpret_cast<u32x4 *>(to + (((2 * e_chunk) ^ TL::xor_of(r)) << 4)) = u32x4{a[0], a[1], b[0], b[1]};
