@@ -9,7 +9,7 @@
 //
 // Every wave brings eight rows of each tile, which lie on one page whatever its size; their page's number comes from a ring in LDS (two batches of 64 numbers a
 // wave, the next one requested as soon as the one before the last is done with).  A bf16 cache: rows go from memory straight into LDS, K five tiles ahead, V three.  An 8-bit
-// one: values are loaded into registers two steps ahead of the step that writes them to LDS as bf16, K(t+4) and V(t+2) in step t: one conversion for 128 rows, and no rounding, as
+// one: values are loaded into registers a step ahead of the one that writes them to LDS as bf16, K(t+4) and V(t+2) in step t: one conversion for 128 rows, and no rounding, as
 // the scales are powers of two.
 #include "dsa_paged.h"
 
@@ -133,8 +133,8 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     // ---- requests: 8-bit.  A lane has D / 8 values of the wave's eight rows: 8 of row lane / 8 (head_dim 64), 16 of it, or 16 of rows lane / 16 and 4 more (256) ----
     constexpr int NC = D == 256 ? 2 : 1, CW = D == 64 ? 2 : 4, PER = D == 256 ? 16 : 8;
     typedef uint32_t codes_t __attribute__((ext_vector_type(CW)));
-    codes_t kraw[E4M3 ? 2 : 1][NC], vraw[E4M3 ? 2 : 1][NC];
-    uint32_t kex[E4M3 ? 2 : 1][NC], vex[E4M3 ? 2 : 1][NC];
+    codes_t kraw[NC], vraw[NC];
+    uint32_t kex[NC], vex[NC];
     const int e_row = lane / PER, e_col = lane % PER * 4 * CW, e_off = e_col < d_real ? e_row * d_real + e_col : (int)0x80000000;
     // (buffers that end with the rows that exist: others read as zero)
     const uint32_t kx_stride = (uint32_t)c.kx_page, vx_stride = (uint32_t)c.vx_page;
@@ -205,10 +205,8 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
         for (int i = 0; i < 4; ++i) fetch_k(i, page_at(i), r[i], x[i]);
         fetch_v(0, page_at(0), r[4], x[4]);
         fetch_v(1, page_at(1), r[5], x[5]);
-        fetch_k(4, page_at(4), kraw[0], kex[0]);
-        fetch_v(2, page_at(2), vraw[0], vex[0]);
-        fetch_k(5, page_at(5), kraw[E4M3 ? 1 : 0], kex[E4M3 ? 1 : 0]);
-        fetch_v(3, page_at(3), vraw[E4M3 ? 1 : 0], vex[E4M3 ? 1 : 0]);
+        fetch_k(4, page_at(4), kraw, kex);
+        fetch_v(2, page_at(2), vraw, vex);
 #pragma unroll
         for (int i = 0; i < 6; ++i) unpack(r[i], x[i], i);              // (slots 0 .. 3 are K's, 4 and 5 V's first)
     }
@@ -300,11 +298,9 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
         meet_read();                                    // every wave is done with K(0) and K(1): their slots may be filled again
         load_k(4, page_at(4));
     } else {
-        id_k = page_at(6);
-        id_v = page_at(4);
         meet_read();
     }
-    constexpr int KA = E4M3 && AGPR ? 2 : 4, VA = E4M3 && D > 64 ? 2 : 4;   // (divide KS and NP: an operand keeps its register from step to step; the values on their way to LDS take registers too)
+    constexpr int KA = 4, VA = 4;                       // (divide KS and NP: an operand keeps its register from step to step)
     static_assert(KS % KA == 0 && NP % VA == 0);
     bf16x8 kr[KA], vr[VA];                              // operands of the next MFMA pairs
     advance(ka_, 2);
@@ -314,11 +310,10 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     for (int i = 0; i < VA; ++i) vr[i] = read_v(i);
     uint32_t word_next = word_of(1);                    // (one-tile pieces never use it)
 
-    // Step t: O += P(t) V(t) with `p`; softmax of tile t+1 from `s` into `pn` (SM); S(t+2) into `sn` (NEXT); requests (REQ); `par`: t & 1
-    auto step = [&](auto masked_, auto sm_, auto next_, auto req_, auto par_, int t_, const uint32_t (&p)[8], const f32x16 &s, uint32_t (&pn)[8],
+    // Step t: O += P(t) V(t) with `p`; softmax of tile t+1 from `s` into `pn` (SM); S(t+2) into `sn` (NEXT); requests (REQ)
+    auto step = [&](auto masked_, auto sm_, auto next_, auto req_, int t_, const uint32_t (&p)[8], const f32x16 &s, uint32_t (&pn)[8],
                     f32x16 &sn) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked_)::value, SM = decltype(sm_)::value, NEXT = decltype(next_)::value, REQ = decltype(req_)::value;
-        constexpr int PAR = E4M3 ? decltype(par_)::value : 0;
         const u32x4 w0 = {p[0], p[1], p[2], p[3]}, w1 = {p[4], p[5], p[6], p[7]};
         const bf16x8 pB0 = __builtin_bit_cast(bf16x8, w0), pB1 = __builtin_bit_cast(bf16x8, w1);
         const uint32_t word = MASKED ? live(word_next) : 0xffffffffu;
@@ -352,26 +347,26 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
             asm volatile("" : "+v"(psum) : : "memory");
             __builtin_amdgcn_sched_barrier(0);
         };
-        // this step's requests: K(t+5) and V(t+3) into LDS; or K(t+4) and V(t+2) from registers into LDS and the loads of K(t+6) and V(t+4)
+        // this step's requests: K(t+5) and V(t+3) into LDS; or K(t+4) and V(t+2) from registers into LDS, and the loads of K(t+5) and V(t+3)
         auto request = [&](int what) __attribute__((always_inline)) {
             if constexpr (!E4M3) {
                 if (what == 0) load_k(t_ + 5, id_k);
                 else load_v(t_ + 3, id_v);
             } else {
                 if (what == 0) {
-                    unpack(kraw[PAR], kex[PAR], t_ & 3);
-                    fetch_k(t_ + 6, id_k, kraw[PAR], kex[PAR]);
+                    unpack(kraw, kex, t_ & 3);
+                    fetch_k(t_ + 5, id_k, kraw, kex);
                 } else {
-                    unpack(vraw[PAR], vex[PAR], 4 + ((t_ + 2) & 3));
-                    fetch_v(t_ + 4, id_v, vraw[PAR], vex[PAR]);
+                    unpack(vraw, vex, 4 + ((t_ + 2) & 3));
+                    fetch_v(t_ + 3, id_v, vraw, vex);
                 }
             }
             if (what == 1) {
                 // numbers for the next step, and the next batch of them once V has come to a batch's first page
-                const int ahead = E4M3 ? 1 : 0, page0 = (base + t_ + 3 + ahead) * 32 >> pshift;
+                const int page0 = (base + t_ + 3) * 32 >> pshift;
                 if (!(page0 & 63)) load_ids((page0 >> 6) + 1);
-                id_k = page_at(t_ + 6 + ahead);
-                id_v = page_at(t_ + 4 + ahead);
+                id_k = page_at(t_ + 6);
+                id_v = page_at(t_ + 4);
             }
         };
 #pragma unroll
@@ -401,8 +396,6 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
     };
     const std::true_type yes;
     const std::false_type no;
-    const std::integral_constant<int, 0> even;
-    const std::integral_constant<int, 1> odd;
     auto meet = [&]() __attribute__((always_inline)) {
         if constexpr (E4M3) {
             // (this step's writes: at least six reads have been issued behind them, and LDS answers in order)
@@ -413,8 +406,8 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
             barrier_only();
         }
     };
-    auto full_step = [&](auto masked_, auto par_, int t_, const uint32_t (&p)[8], const f32x16 &s, uint32_t (&pn)[8], f32x16 &sn) __attribute__((always_inline)) {
-        step(masked_, yes, yes, yes, par_, t_, p, s, pn, sn);
+    auto full_step = [&](auto masked_, int t_, const uint32_t (&p)[8], const f32x16 &s, uint32_t (&pn)[8], f32x16 &sn) __attribute__((always_inline)) {
+        step(masked_, yes, yes, yes, t_, p, s, pn, sn);
         meet();
     };
     int tt = 0;
@@ -422,21 +415,21 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
         // tiles every row of the block attends whole: the softmax without mask arithmetic
         const int whole = (min(past + pc.first, keys - 1) + 1) / 32 - base;
         for (; tt + 3 < ntiles && tt + 2 < whole; tt += 2) {
-            full_step(no, even, tt, pE, sO, pO, sE);
-            full_step(no, odd, tt + 1, pO, sE, pE, sO);
+            full_step(no, tt, pE, sO, pO, sE);
+            full_step(no, tt + 1, pO, sE, pE, sO);
         }
         word_next = word_of(tt + 1);
     }
     for (; tt + 2 < ntiles; tt += 2) {
         // (S of up to two tiles past the end is formed for nothing)
-        full_step(yes, even, tt, pE, sO, pO, sE);
-        full_step(yes, odd, tt + 1, pO, sE, pE, sO);
+        full_step(yes, tt, pE, sO, pO, sE);
+        full_step(yes, tt + 1, pO, sE, pE, sO);
     }
     if (tt + 1 < ntiles) {
-        full_step(yes, even, tt, pE, sO, pO, sE);
-        step(yes, no, no, no, odd, tt + 1, pO, sE, pE, sO);
+        full_step(yes, tt, pE, sO, pO, sE);
+        step(yes, no, no, no, tt + 1, pO, sE, pE, sO);
     } else {
-        step(yes, no, no, no, even, tt, pE, sO, pO, sE);
+        step(yes, no, no, no, tt, pE, sO, pO, sE);
     }
     wait_vmcnt<0>();                                    // no load is left on its way into LDS when the workgroup ends
 
@@ -483,10 +476,10 @@ __global__ __launch_bounds__(WALK_WAVES * 64, D <= 128 ? 2 : 1) void dsa_paged_w
             load_tile(v_pool, v_stride, tile, id, 4);
             wait_vmcnt<0>();
         } else {
-            fetch_k(tile, id, kraw[0], kex[0]);
-            fetch_v(tile, id, vraw[0], vex[0]);
-            unpack(kraw[0], kex[0], 0);
-            unpack(vraw[0], vex[0], 4);
+            fetch_k(tile, id, kraw, kex);
+            fetch_v(tile, id, vraw, vex);
+            unpack(kraw, kex, 0);
+            unpack(vraw, vex, 4);
         }
         meet_read();
         gemm_s(sE);
