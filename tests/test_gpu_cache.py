@@ -39,8 +39,17 @@ def make(kind, lens, hkv, dim, page, seed=0, spare=2, std=1.0, width=None):
         at += need[i]
         k, v = ((torch.randn(n, hkv, dim, generator=g) * std).to(BF) for _ in range(2))
         rows.append([k, v])
-        for p in range(n):
-            put(cache, table, i, p, k[p], v[p])
+        for pool, scale, x in ((cache.k, cache.k_scale, k), (cache.v, cache.v_scale, v)):
+            if n and kind == "e4m3":
+                y, e = R.quantise(x)
+                codes, powers = y.float().to(E4).view(torch.uint8), (e + 127).to(torch.uint8)
+            for b in range(need[i]):
+                id, part = int(table[i, b]), slice(b * page, min(n, (b + 1) * page))
+                if kind == "bf16":
+                    pool[id, :, :part.stop - part.start] = x[part].transpose(0, 1)
+                else:
+                    pool.view(torch.uint8)[id, :, :part.stop - part.start] = codes[part].transpose(0, 1)
+                    scale.view(torch.uint8)[id, :, :part.stop - part.start] = powers[part].transpose(0, 1)
     return rows, V.KvCache(*(t if t is None else t.to(DEV) for t in cache._parts())), table.to(DEV)
 
 

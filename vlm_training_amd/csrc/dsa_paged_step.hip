@@ -8,7 +8,14 @@
 // Every wave has its own tiles in LDS, two of them, filled straight from memory (bf16), or one, into which it writes the values that it has loaded as e4m3 in front
 // of the last tile's products: no barrier until the waves' sums are joined.  Pieces of a block are joined by dsa_paged_join_kernel, in order.
 //
-// P is rounded to bf16 for the second product (each probability by at most 2^-9 of itself, at random); its sum, the statistics and the output's sums are fp32.
+// P is rounded to bf16 for the second product (each probability by at most 2^-8 of itself, at random); its sum, the statistics and the output's sums are fp32.
+//
+// What bounds it: memory.  256 requests over an 8-bit cache of 2.3 GB 434 us (5.4 TB/s with the join), 64 requests of 64 to 8192 bf16 keys 90 us (5.0), one of 131 072 with two heads of
+// 256 64 us (4.2); short batches by the chain of a piece's first loads: offsets and lengths, page numbers, rows, 2 to 3 us, and 1 for the waves' join (one token over 1000 keys:
+// 6.5 us, the join 3.8).  16-row MFMAs: a decoded token's heads are 1 to 16 rows, and two tiles' products of 32-row MFMAs would take as long again.  Sums in vector registers (the
+// compiler's flag for it): with 64 to 128 accumulation registers and their copies one long request took 54 us instead of 48.
+// Two or four workgroups of fewer waves to a unit, waves' tiles two ahead instead of one in an 8-bit cache: within 2 %.  Equal shares instead of equal pieces of each
+// request: 64 requests 99 -> 90, drafts of 24 36 -> 28, two requests of 131 072 and 77 level.
 #include "dsa_paged.h"
 #include <algorithm>
 

@@ -11,6 +11,11 @@
 // wave, the next one requested as soon as the one before the last is done with).  A bf16 cache: rows go from memory straight into LDS, K five tiles ahead, V three.  An 8-bit
 // one: values are loaded into registers a step ahead of the one that writes them to LDS as bf16, K(t+4) and V(t+2) in step t: one conversion for 128 rows, and no rounding, as
 // the scales are powers of two.
+//
+// What bounds it: as the packed forward, power and the instructions beside the MFMAs.  2048 new tokens behind 14 336 (32 heads over 8 of 128) 478 us = 1.08 PFLOP/s, MFMA busy 0.6 of the
+// units' time; page addresses formed in 64 bits for each operand cost 8 % of it, two long walks on one unit (the second half of a launch of one round goes in reverse) 3 %.
+// An 8-bit cache: 1024 behind 60 000 1369 us; the loads two steps ahead instead of one left no registers for operands four MFMAs ahead (1498), and converting in
+// the loads' own step spilled.  A chunk of 512 behind 7680 and a prompt of 333: 93 us, of them 8 for the first loads and 8 for the pieces' sums (33 MB).
 #include "dsa_paged.h"
 
 namespace {
