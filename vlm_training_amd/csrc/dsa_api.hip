@@ -27,7 +27,8 @@ hipError_t dsa_launch_cache_write(const dsa_cache_args *c, const void *k, int64_
 hipError_t dsa_launch_cache_read(const dsa_cache_args *c, const int32_t *cu, const int32_t *first, int T, int N, void *k_out, void *v_out, hipStream_t stream);
 hipError_t dsa_launch_paged_step(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int waves, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream);
 hipError_t dsa_launch_paged_walk(const dsa_cache_args *c, const PagePlan *plan, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, int tail, void *out, float *lse, float *part_o, float *part_ml, hipStream_t stream);
-hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PagedJoin *many, const PagedJoin *few, int Hq, void *out, float *lse, hipStream_t stream);
+hipError_t dsa_launch_paged_both(const dsa_cache_args *c, const PagedPart *many, const PagedPart *few, const void *q, int64_t q_tok, int64_t q_head, int Hq, float scale, int slots, void *out, float *lse, hipStream_t stream);
+hipError_t dsa_launch_paged_join(const dsa_cache_args *c, const PagedPart *many, const PagedPart *few, int Hq, void *out, float *lse, hipStream_t stream);
 hipError_t dsa_launch_delta_fwd(const DeltaArgs *a, int save, hipStream_t stream);
 hipError_t dsa_launch_delta_bwd(const DeltaArgs *a, hipStream_t stream);
 hipError_t dsa_launch_delta_step(const dsa_delta_args *in, float *state, int64_t state_req, void *out, hipStream_t stream);
@@ -1359,7 +1360,8 @@ static PagedCall paged_call(const dsa_cache_args *c, const int32_t *cu, const in
         p.step = paged_launch(c, cu, lengths, T, N, gshift, qb, 0, -1, false, by_step, max_length);
     } else {
         p.walk = paged_launch(c, cu, lengths, T, N, gshift, 128 >> gshift, few, N == 1 ? -1 : 1, true, by_walk, max_length);
-        if (N > 1) p.step = paged_launch(c, cu, lengths, T, N, gshift, few, few, 0, false, by_step, max_length);
+        // (up to head_dim 128 both in one launch, a share to each compute unit: dsa_paged_both.hip)
+        if (N > 1) p.step = paged_launch(c, cu, lengths, T, N, gshift, few, few, 0, false, 256, max_length);
     }
     return p;
 }
@@ -1369,7 +1371,7 @@ static int check_paged(const dsa_cache_args *c, const int32_t *cu, int T, int N,
     if (Hq / c->Hkv > 16) return fail(DSA_ERR_UNSUPPORTED, "Hq/Hkv=%d: up to 16", Hq / c->Hkv);
     if (max_new < 0 || max_length < 0) return fail(DSA_ERR_ARG, "max_new=%d max_length=%d", max_new, max_length);
     const PagedCall p = paged_call(c, cu, nullptr, T, N, Hq, max_new, max_length);
-    if (std::max(std::max(p.step.blocks, p.step.slots), p.walk.slots + p.step.blocks) * c->Hkv > INT32_MAX || p.step.blocks >= 1 << 25) return fail(DSA_ERR_UNSUPPORTED, "too many blocks: T=%d N=%d Hkv=%d", T, N, c->Hkv);
+    if (std::max(std::max(p.step.blocks, p.step.slots), p.walk.slots + p.walk.blocks + p.step.blocks + p.step.slots) * c->Hkv > INT32_MAX || p.step.blocks >= 1 << 25) return fail(DSA_ERR_UNSUPPORTED, "too many blocks: T=%d N=%d Hkv=%d", T, N, c->Hkv);
     return DSA_OK;
 }
 extern "C" size_t dsa_paged_attn_workspace_bytes(const dsa_cache_args *c, int T, int N, int Hq, int max_new, int max_length) {
@@ -1391,17 +1393,22 @@ extern "C" int dsa_paged_attn(const dsa_cache_args *c, const void *q, int64_t q_
     if (need && (!ws || off16(ws) || ws_bytes < need)) return fail(DSA_ERR_WORKSPACE, "workspace: need %zu bytes on a 16-byte boundary, got %zu", need, ws_bytes);
     hipError_t e = hipSuccess;
     char *at = (char *)ws;
-    PagedJoin joins[2] = {};
-    for (const bool many : {true, false}) {
-        const PagedLaunch &l = many ? p.walk : p.step;
-        if (!l.slots || e != hipSuccess) continue;
+    const auto part = [&](const PagedLaunch &l) {
         float *const part_o = (float *)at, *const part_ml = (float *)(at + l.o_bytes);
-        // (the kernel for many rows clears those behind the last request where both are launched)
-        e = many ? dsa_launch_paged_walk(c, &l.plan, q, q_tok, q_head, Hq, scale, (int)l.slots, 1, out, lse, part_o, part_ml, (hipStream_t)stream)
-                 : dsa_launch_paged_step(c, &l.plan, q, q_tok, q_head, Hq, scale, l.waves, !p.walk.slots, out, lse, part_o, part_ml, (hipStream_t)stream);
-        if (!l.plan.whole) joins[many ? 0 : 1] = PagedJoin{l.plan, (int)l.blocks, l.pieces, part_o, part_ml};
         at += l.bytes;
+        return PagedPart{l.plan, (int)l.blocks, l.pieces, part_o, part_ml};
+    };
+    PagedPart many = part(p.walk), few = part(p.step);
+    if (p.walk.slots && p.step.slots && c->D <= 128) {
+        e = dsa_launch_paged_both(c, &many, &few, q, q_tok, q_head, Hq, scale, (int)p.walk.slots, out, lse, (hipStream_t)stream);
+    } else {
+        // (the kernel for many rows clears those behind the last request where both are launched)
+        if (p.walk.slots) e = dsa_launch_paged_walk(c, &many.plan, q, q_tok, q_head, Hq, scale, (int)p.walk.slots, 1, out, lse, many.part_o, many.part_ml, (hipStream_t)stream);
+        if (p.step.slots && e == hipSuccess)
+            e = dsa_launch_paged_step(c, &few.plan, q, q_tok, q_head, Hq, scale, p.step.waves, !p.walk.slots, out, lse, few.part_o, few.part_ml, (hipStream_t)stream);
     }
-    if (e == hipSuccess && joins[0].blocks + joins[1].blocks > 0) e = dsa_launch_paged_join(c, &joins[0], &joins[1], Hq, out, lse, (hipStream_t)stream);
+    for (PagedPart *x : {&many, &few})
+        if (x->plan.whole) x->blocks = 0;                // (nothing to join)
+    if (e == hipSuccess && many.blocks + few.blocks > 0) e = dsa_launch_paged_join(c, &many, &few, Hq, out, lse, (hipStream_t)stream);
     return e == hipSuccess ? DSA_OK : hip_fail(e, "paged attention launch");
 }

@@ -61,12 +61,11 @@ struct PagePiece {
     int piece, pieces;             // which of how many pieces of this block (shares: whether it is the first, and whether there are others)
     int slot;                      // of the block's first piece's sums (shares: of this one's)
 };
-// what is joined of a launch: its blocks, for each kv head, and their pieces' sums
-struct PagedJoin {
+// A kernel's part of a call: its plan, its blocks for each kv head (0: none to join), the pieces of a block at the most, and the pieces' sums
+struct PagedPart {
     PagePlan plan;
-    int blocks;
-    int pieces;                    // of a block, at the most
-    const float *part_o, *part_ml;
+    int blocks, pieces;
+    float *part_o, *part_ml;
 };
 struct PageRequest { int row0, m, length, blocks, tiles; };
 __device__ __forceinline__ PageRequest page_request(const PagePlan &p, int n) {
