@@ -1360,8 +1360,8 @@ static PagedCall paged_call(const dsa_cache_args *c, const int32_t *cu, const in
         p.step = paged_launch(c, cu, lengths, T, N, gshift, qb, 0, -1, false, by_step, max_length);
     } else {
         p.walk = paged_launch(c, cu, lengths, T, N, gshift, 128 >> gshift, few, N == 1 ? -1 : 1, true, by_walk, max_length);
-        // (up to head_dim 128 both in one launch, a share to each compute unit: dsa_paged_both.hip)
-        if (N > 1) p.step = paged_launch(c, cu, lengths, T, N, gshift, few, few, 0, false, 256, max_length);
+        // (up to head_dim 128 both in one launch: dsa_paged_both.hip)
+        if (N > 1) p.step = paged_launch(c, cu, lengths, T, N, gshift, few, few, 0, false, c->kind == DSA_CACHE_E4M3 ? by_step : 256, max_length);
     }
     return p;
 }

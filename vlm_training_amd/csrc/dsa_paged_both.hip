@@ -1,7 +1,10 @@
 // A batch of chunks and of single tokens over a paged cache in one launch: the walks of many rows (dsa_paged_walk.h) beside the shares of a few (dsa_paged_step.h).
 //
-// A walk is bound by its instructions and what they wait for, a share by memory, so a compute unit has one workgroup of each where it can: the first 256 workgroups are
-// walks, the next 256 all shares, the others the rest of the walks.  MEASURED
+// The shares come first: they are bound by memory, end first, and a compute unit whose first one has ended takes a walk beside the other, which is bound by its instructions and what they
+// wait for.  8-bit caches: as many shares as run at once (512 workgroups); bf16: one to a unit, whose waves' tiles of 16 KB keep its memory busy.  us, a launch each -> both in one: a
+// chunk of 512 behind 7680, a prompt of 333 and 40 tokens over 200 to 4000 keys, 8-bit 128 -> 117, bf16 143 -> 117; a chunk of 64 and 200 tokens over 4000 keys, 8-bit 337 -> 317 (with 256
+// shares 460); a prompt of 2000 and 8 tokens over 3000, 8-bit 86 -> 87; two chunks and 64 tokens over 500 71 -> 60; 1000 behind 29 000 and 60 tokens over 8000 731 -> 703.  256 walks in
+// front of the shares: from 3 % less to 19 % more.
 #include "dsa_paged_step.h"
 #include "dsa_paged_walk.h"
 
@@ -18,11 +21,12 @@ template <int D, bool E4M3>
 __global__ __launch_bounds__(WALK_WAVES * 64, 2) void dsa_paged_both_kernel(dsa_cache_args c, PagedPart many, PagedPart few, const bf16_t *__restrict__ q, int64_t q_tok, int64_t q_head,
                                                                             int Hq, int gshift, int pshift, float walk_scale, uint32_t flip, float step_scale, int slots,
                                                                             bf16_t *__restrict__ out, float *__restrict__ lse) {
-    const int at = blockIdx.x / c.Hkv, kvh = blockIdx.x % c.Hkv, first = many.plan.pair, shares = few.plan.target;
-    if (at >= first && at < first + shares)
-        paged_step<D, E4M3, 1, WALK_WAVES, STEP_RING>(c, few.plan, q, q_tok, q_head, Hq, gshift, pshift, step_scale, 0, out, lse, few.part_o, few.part_ml, at - first, kvh);
+    const int at = blockIdx.x / c.Hkv, kvh = blockIdx.x % c.Hkv, shares = few.plan.target;
+    if (at < shares)
+        paged_step<D, E4M3, 1, WALK_WAVES, STEP_RING>(c, few.plan, q, q_tok, q_head, Hq, gshift, pshift, step_scale, 0, out, lse, few.part_o, few.part_ml, at, kvh);
     else
-        paged_walk<D, E4M3, false>(c, many.plan, q, q_tok, q_head, Hq, gshift, pshift, walk_scale, flip, slots, 1, out, lse, many.part_o, many.part_ml, at < first ? at : at - shares, kvh);
+        // (8-bit at head_dim 128: with four operands of V ahead beside the shares' code the loop read spilled registers, and the mixed batch took 145 us)
+        paged_walk<D, E4M3, false, E4M3 && D == 128 ? 2 : 4>(c, many.plan, q, q_tok, q_head, Hq, gshift, pshift, walk_scale, flip, slots, 1, out, lse, many.part_o, many.part_ml, at - shares, kvh);
 }
 
 template <int D, bool E4M3>

@@ -12,7 +12,7 @@
 // one: values are loaded into registers a step ahead of the one that writes them to LDS as bf16, K(t+4) and V(t+2) in step t: one conversion for 128 rows, and no rounding, as
 // the scales are powers of two.
 //
-// What bounds it: as the packed forward, power and the instructions beside the MFMAs.  2048 new tokens behind 14 336 (32 heads over 8 of 128) 478 us = 1.08 PFLOP/s, MFMA busy 0.6 of the
+// What bounds it: as the packed forward, power and the instructions beside the MFMAs.  2048 new tokens behind 14 336 (32 heads over 8 of 128) 470 us = 1.10 PFLOP/s, MFMA busy 0.6 of the
 // units' time; page addresses formed in 64 bits for each operand cost 8 % of it, two long walks on one unit (the second half of a launch of one round goes in reverse) 3 %.
 // An 8-bit cache: 1024 behind 60 000 1369 us; the loads two steps ahead instead of one left no registers for operands four MFMAs ahead (1498), and converting in
 // the loads' own step spilled.  A chunk of 512 behind 7680 and a prompt of 333: 93 us, of them 8 for the first loads and 8 for the pieces' sums (33 MB).
@@ -23,8 +23,8 @@ constexpr int WALK_WAVES = 4;
 template <int D>
 constexpr int walk_lds_bytes() { return 8 * DirectTile<D>::BYTES + WALK_WAVES * 512 + 16; }
 
-// AGPR: the sums in accumulation registers, by name (mfma32_agpr_late)
-template <int D, bool E4M3, bool AGPR>
+// AGPR: the sums in accumulation registers, by name (mfma32_agpr_late); VA: operands of V read ahead (divides NP)
+template <int D, bool E4M3, bool AGPR, int VA = 4>
 __device__ __forceinline__ void paged_walk(const dsa_cache_args &c, const PagePlan &plan, const bf16_t *__restrict__ q, int64_t q_tok, int64_t q_head, int Hq, int gshift, int pshift,
                                            float scale_log2, uint32_t flip, int slots, int tail, bf16_t *__restrict__ out, float *__restrict__ lse, float *__restrict__ part_o,
                                            float *__restrict__ part_ml, int slot, int kvh) {
@@ -303,7 +303,7 @@ __device__ __forceinline__ void paged_walk(const dsa_cache_args &c, const PagePl
     } else {
         meet_read();
     }
-    constexpr int KA = 4, VA = 4;                       // (divide KS and NP: an operand keeps its register from step to step)
+    constexpr int KA = 4;                               // (divides KS: an operand keeps its register from step to step)
     static_assert(KS % KA == 0 && NP % VA == 0);
     bf16x8 kr[KA], vr[VA];                              // operands of the next MFMA pairs
     advance(ka_, 2);
