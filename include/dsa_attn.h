@@ -486,7 +486,7 @@ int dsa_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x
  * k, v: pools of `pages` pages, (pages, Hkv, page, D), a page's rows contiguous, one page k_page / v_page elements behind the other; page 16, 32, 64, 128 or 256,
  * D a multiple of 8 up to 256.  kind DSA_CACHE_BF16: bf16 rows.  DSA_CACHE_E4M3: D (a multiple of 16) e4m3 values to a row, and a byte b for each row in k_exp, v_exp
  * (pages, Hkv, page; pages kx_page / vx_page bytes apart): a value stands for itself times 2^(b - 127), b = 255 for NaN.  Written are powers from 2^-100 on, the smallest with which a row's largest
- * value is at most 448: what the bytes stand for is exact in bf16.  A row with a value that is not finite is NaN as a whole.
+ * value is at most 448: what the bytes stand for is exact in bf16 (at 2^120 values go up to 240: more is no bf16).  A row with a value that is not finite is NaN as a whole.
  * table (N, table_pages) int32, rows table_row apart: position p of request n lies on page table[n][p / page], at p % page.
  * Pools lie on 16-byte boundaries; k_page, v_page are multiples of 8 elements (e4m3: 16), kx_page, vx_page of 16 bytes, each under 4 GiB; a table holds up to 2^30 positions.
  * What lies on no page (a page number outside the pool, a position outside the table) is not written and reads as zero.

@@ -7,7 +7,7 @@ import torch
 
 
 def quantise(x):
-    """Rows (..., D) -> (e4m3 values, exponents): the smallest e >= -100 with max|x| <= 448 * 2^e, x * 2^-e to the nearest of e4m3, ties to even.
+    """Rows (..., D) -> (e4m3 values, exponents): the smallest e >= -100 with max|x| <= 448 * 2^e, x * 2^-e to the nearest of e4m3, ties to even (at e = 120 of those up to 240).
 
     The values come as 64-bit numbers; a row that is not finite is NaN."""
     x = x.double()
@@ -20,6 +20,7 @@ def quantise(x):
     for k in range(-6, 9):
         step = torch.where(y.abs() >= 2.0 ** k, 2.0 ** (k - 3), step)
     y = torch.round(y / step) * step                       # (torch.round: ties to even; the quotient is below 16, so even numbers are even mantissas)
+    y = torch.where((e >= 120)[..., None], y.clamp(-240, 240), y)                              # (256 * 2^120 is no bf16 any more)
     y[~torch.isfinite(x).all(-1)] = math.nan
     return y, e
 

@@ -73,3 +73,9 @@ def test_python_entries():
     for call in (lambda: V.kv_cache_write(cache, grad, x, table, cu, lengths), lambda: V.paged_attn(grad, cache, table, cu, lengths)):
         with pytest.raises(ValueError, match="no backward"):
             call()
+
+
+@pytest.mark.parametrize("page", [0, 8, 48, 512])
+def test_empty_caches_of_other_pages(page):
+    with pytest.raises(ValueError, match="page"):
+        V.KvCache.empty(2, 1, 64, page=page, device="cpu")

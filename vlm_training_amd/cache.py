@@ -30,7 +30,7 @@ class KvCache:
 
     An 8-bit cache has ``k_scale``, ``v_scale`` (pages, kv heads, page) float8_e8m0fnu: a value stands for itself times its row's power of two, the smallest one (from 2^-100 on) with
     which the row's largest value is at most 448.  That rounds a value by at most 2^-4 of itself, or 2^-10 of the power for values under 2^-6 of it, and what is stored is exact in
-    bf16.  A row with a value that is not finite is NaN as a whole."""
+    bf16 (next to bf16's largest value it is 240 * 2^120 at the most, not 2^128).  A row with a value that is not finite is NaN as a whole."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: Optional[torch.Tensor] = None
@@ -39,6 +39,8 @@ class KvCache:
     @classmethod
     def empty(cls, pages: int, heads: int, head_dim: int, *, page: int = 64, dtype=torch.bfloat16, device="cuda"):
         """A cache of zeros; ``dtype`` torch.bfloat16 or torch.float8_e4m3fn."""
+        if page not in (16, 32, 64, 128, 256):
+            raise ValueError(f"a page holds 16, 32, 64, 128 or 256 rows, not {page}")
         if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
             raise ValueError(f"a cache holds torch.bfloat16 or torch.float8_e4m3fn, not {dtype}")
         k, v = (torch.zeros(pages, heads, page, head_dim, dtype=torch.uint8 if dtype.itemsize == 1 else dtype, device=device).view(dtype) for _ in range(2))
@@ -72,7 +74,8 @@ def paged_attn(q, cache: KvCache, page_table, cu_seqlens, lengths, *, max_new=No
     """q (T, q heads, head_dim) bf16 view -> (T, q heads, head_dim): causal attention of each request's new rows over its cached keys and values, their own (already
     written) ones among them; q head h reads kv head ``h // (q heads // kv heads)``, up to 16 to one.
 
-    A row without any key - its request is shorter than its new rows - gives zeros; a key or value that a row does not attend never reaches it, not finite ones either.
+    A row without any key - its request is shorter than its new rows - gives zeros; a key or value that a row does not attend never reaches it, not finite ones either; a
+    NaN logit that it does attend makes it NaN.
     ``max_new`` and ``max_length``, where known, are upper bounds of the requests' new rows and lengths: with them fewer kernels are launched; results do not depend on them but for
     the order of sums.  ``softmax_scale`` defaults to ``head_dim ** -0.5``.  ``return_lse`` adds (q heads, T) fp32: the logarithm of each row's sum of exponentials, -inf
     for rows without a key.  Probabilities are rounded to bf16 for their product with the values; statistics and sums are fp32.  No backward pass."""

@@ -10,9 +10,10 @@ Tensor rows_in_place(const Tensor &x) {
     const Tensor c = x.contiguous();
     return aligned16(c) ? c : c.clone();
 }
+// int64 numbers that no int32 holds as the nearest that one does: nowhere, beyond every table
 Tensor as_int(const Tensor &x, const char *name) {
     TORCH_CHECK_VALUE(x.scalar_type() == at::kInt || x.scalar_type() == at::kLong, name, " must be int32 or int64, not ", x.scalar_type());
-    return x.scalar_type() == at::kInt ? x : x.to(at::kInt);
+    return x.scalar_type() == at::kInt ? x : x.clamp(INT32_MIN, INT32_MAX).to(at::kInt);
 }
 
 struct Cache {

@@ -41,6 +41,11 @@ __device__ __forceinline__ u32x2 e4m3_to_bf16(uint32_t w, float scale) {
 }
 __device__ __forceinline__ float exponent_scale(uint32_t b) { return __uint_as_float(b == 255 ? 0x7fc00000u : b << 23); }
 
+// ---- a row's statistics, once its sums are formed ----
+// The largest logit of a row, for its joining with other pieces' sums: a maximum passes NaN over, so that a piece in which every logit is NaN would pass for one without a key,
+// and one with some of them might weigh 0 beside a far larger logit.  A sum that is NaN counts as infinitely large: the row is NaN as a whole.
+__device__ __forceinline__ float row_maximum(float m, float l) { return l == l ? m : INFINITY; }
+
 // ---- how the work is cut ----
 // A request's new rows go in blocks of `qb` queries.  Lengths are on the device, so every workgroup forms the plan itself: sums over the requests, one in each lane.
 struct PagePlan {

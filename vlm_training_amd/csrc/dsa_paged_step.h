@@ -285,7 +285,7 @@ __device__ __forceinline__ void paged_step(const dsa_cache_args &c, const PagePl
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(sums + (rg * 16 + j) * PITCH + 16 * dt + 4 * g) = oacc[rg][dt];
         if (g == 0) {
-            stats[2 * (rg * 16 + j)] = mrun[rg];
+            stats[2 * (rg * 16 + j)] = row_maximum(mrun[rg], l);
             stats[2 * (rg * 16 + j) + 1] = l;
         }
     }
@@ -305,7 +305,7 @@ __device__ __forceinline__ void paged_step(const dsa_cache_args &c, const PagePl
             const float *const ws = reinterpret_cast<const float *>(at + w * WAVE_B);
             const float mw = ws[ROWS * PITCH + 2 * row], f = mw == -INFINITY ? 0.f : fast_exp2(mw - m);
             l = fmaf(f, ws[ROWS * PITCH + 2 * row + 1], l);
-            if (f != 0.f) {
+            if (mw != -INFINITY) {
                 const f32x4 a = *reinterpret_cast<const f32x4 *>(ws + row * PITCH + d), b = *reinterpret_cast<const f32x4 *>(ws + row * PITCH + d + 4);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {

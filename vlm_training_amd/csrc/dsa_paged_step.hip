@@ -36,11 +36,11 @@ __global__ __launch_bounds__(256) void dsa_paged_join_kernel(dsa_cache_args c, P
                 const f32x4 x = *reinterpret_cast<const f32x4 *>(part_o + (at + slot_of(i) * step) * d_real + d);
                 // (sums against the largest so far: no load waits for another piece's)
                 const float most = fmaxf(m, ml[0]), old = m == -INFINITY ? 0.f : fast_exp2(m - most), w = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - most);
-                l = fmaf(w, ml[1], old == 0.f ? 0.f : l * old);
+                l = fmaf(w, ml[1], l * old);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    o[e] = old == 0.f ? 0.f : o[e] * old;
-                    o[e] = w == 0.f ? o[e] : fmaf(w, x[e], o[e]);
+                    o[e] *= old;
+                    o[e] = ml[0] == -INFINITY ? o[e] : fmaf(w, x[e], o[e]);
                 }
                 m = most;
             }
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void dsa_paged_join_kernel(dsa_cache_args c, P
                     const float w = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - most);
                     l = fmaf(w, ml[1], l);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, x[e], o[e]);
+                    for (int e = 0; e < 4; ++e) o[e] = ml[0] == -INFINITY ? o[e] : fmaf(w, x[e], o[e]);
                 }
                 m = most;
             }

@@ -62,6 +62,7 @@ __device__ __forceinline__ void paged_walk(const dsa_cache_args &c, const PagePl
     }
     auto finish = [&]() __attribute__((always_inline)) {
         const float l = half_sum_f(lsum);
+        mrun = row_maximum(mrun, l);
         if (AGPR) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) settle(oacc[dt]);
