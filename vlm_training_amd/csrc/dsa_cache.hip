@@ -65,15 +65,18 @@ __global__ __launch_bounds__(256) void dsa_cache_write_kernel(dsa_cache_args c, 
                 const int e = scale_exponent(most);
                 const bool finite = most < 0x7f80u;
                 const float mul = __uint_as_float((uint32_t)(127 - e) << 23);
-                // Next to bf16's largest value (a power of 2^120) the nearest code may stand for 2^128: 240 of the power is the last that is finite, and off by 2^-4 at most
-                const float top = e >= 120 ? 240.f : 448.f;
+                // Next to bf16's largest value (a power of 2^120) the nearest code may stand for 2^128: 240 of the power is the last that is finite, and off by 2^-4 at most (0x7f70 is it)
+                if (most > 0x7f70u) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        x[i][j] = (x[i][j] & 0x80008000u) | min(x[i][j] & 0x7fffu, 0x7f70u) | min(x[i][j] & 0x7fff0000u, 0x7f700000u);
+                }
                 u32x2 codes;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t a = x[i][2 * j], b = x[i][2 * j + 1];
-                    auto value = [&](uint32_t bits) { return __builtin_amdgcn_fmed3f(__uint_as_float(bits) * mul, -top, top); };
-                    int w = __builtin_amdgcn_cvt_pk_fp8_f32(value(a << 16), value(a & 0xffff0000u), 0, false);
-                    w = __builtin_amdgcn_cvt_pk_fp8_f32(value(b << 16), value(b & 0xffff0000u), w, true);
+                    int w = __builtin_amdgcn_cvt_pk_fp8_f32(__uint_as_float(a << 16) * mul, __uint_as_float(a & 0xffff0000u) * mul, 0, false);
+                    w = __builtin_amdgcn_cvt_pk_fp8_f32(__uint_as_float(b << 16) * mul, __uint_as_float(b & 0xffff0000u) * mul, w, true);
                     codes[j] = finite ? (uint32_t)w : 0x7f7f7f7fu;
                 }
                 uint8_t *dst = val ? (uint8_t *)c.v + id * c.v_page + row * c.D : (uint8_t *)c.k + id * c.k_page + row * c.D;
