@@ -8,7 +8,7 @@
 // Step t issues the MFMAs of O += P(t) V(t) and of S(t+2) in pairs, with the softmax of tile t+1 between them.
 //
 // Every wave brings eight rows of each tile, which lie on one page whatever its size; their page's number comes from a ring in LDS (two batches of 64 numbers a
-// wave, the next one requested as soon as the one before the last is done with).  A bf16 cache: rows go from memory straight into LDS, K five tiles ahead, V three.  An 8-bit
+// wave, the next one requested as soon as the one before the last is done with: dsa_paged_ring.h).  A bf16 cache: rows go from memory straight into LDS, K five tiles ahead, V three.  An 8-bit
 // one: values are loaded into registers a step ahead of the one that writes them to LDS as bf16, K(t+4) and V(t+2) in step t: one conversion for 128 rows, and no rounding, as
 // the scales are powers of two.
 //
@@ -18,6 +18,7 @@
 // the loads' own step spilled.  A chunk of 512 behind 7680 and a prompt of 333: 93 us, of them 8 for the first loads and 8 for the pieces' sums (33 MB).
 #pragma once
 #include "dsa_paged.h"
+#include "dsa_paged_ring.h"
 
 constexpr int WALK_WAVES = 4;
 template <int D>
@@ -105,7 +106,7 @@ __device__ __forceinline__ void paged_walk(const dsa_cache_args &c, const PagePl
     const uint32_t row_b = d_real * (E4M3 ? 1 : 2), k_stride = (uint32_t)c.k_page * (E4M3 ? 1u : 2u), v_stride = (uint32_t)c.v_page * (E4M3 ? 1u : 2u);
     const unsigned char *const k_pool = (const unsigned char *)c.k + (int64_t)kvh * c.page * row_b, *const v_pool = (const unsigned char *)c.v + (int64_t)kvh * c.page * row_b;
     auto page_at = [&](int tile) __attribute__((always_inline)) {        // number of their page: looked up one step ahead of its use
-        return mine[(row0 + tile * 32) >> pshift & 127];
+        return mine[PageRing::place((row0 + tile * 32) >> pshift)];
     };
     struct Where { uint32_t id, rows, place; };             // page, rows that exist, the first one's place among the page's
     auto where = [&](int tile, int id_) __attribute__((always_inline)) {
@@ -177,9 +178,9 @@ __device__ __forceinline__ void paged_walk(const dsa_cache_args &c, const PagePl
     auto load_v = [&](int tile, int id) __attribute__((always_inline)) { load_tile(v_pool, v_stride, tile, id, 4 + (tile & 3)); };
 
     // page numbers of the first tiles, q in the meantime
-    const int batch0 = base * 32 >> pshift >> 6;
-    load_ids(batch0);
-    load_ids(batch0 + 1);
+    const PageRing ring{base, pshift};
+    load_ids(ring.batch(0));
+    load_ids(ring.batch(0) + 1);
     bf16x8 qB[KS];
     {
         const bf16_t *const qrow = q + (int64_t)t * q_tok + (int64_t)hq * q_head;
@@ -304,6 +305,7 @@ __device__ __forceinline__ void paged_walk(const dsa_cache_args &c, const PagePl
     } else {
         meet_read();
     }
+    if (ring.due_early()) load_ids(ring.batch(2) + 1);  // (one load more on its way: the waits that count loads wait for more)
     constexpr int KA = 4;                               // (divides KS: an operand keeps its register from step to step)
     static_assert(KS % KA == 0 && NP % VA == 0);
     bf16x8 kr[KA], vr[VA];                              // operands of the next MFMA pairs
@@ -367,8 +369,7 @@ __device__ __forceinline__ void paged_walk(const dsa_cache_args &c, const PagePl
             }
             if (what == 1) {
                 // numbers for the next step, and the next batch of them once V has come to a batch's first page
-                const int page0 = (base + t_ + 3) * 32 >> pshift;
-                if (!(page0 & 63)) load_ids((page0 >> 6) + 1);
+                if (ring.due(t_ + 3)) load_ids(ring.batch(t_ + 3) + 1);
                 id_k = page_at(t_ + 6);
                 id_v = page_at(t_ + 4);
             }
