@@ -1283,7 +1283,8 @@ static int check_cache(const dsa_cache_args *c, const int32_t *cu, int T, int N)
     return DSA_OK;
 }
 static int check_rows(const void *x, int64_t tok, int64_t head, int T, const char *name) {
-    if (T > 0 && !x) return fail(DSA_ERR_ARG, "%s is null", name);
+    if (T == 0) return DSA_OK;                           // (no row lies anywhere)
+    if (!x) return fail(DSA_ERR_ARG, "%s is null", name);
     if (off16(x) || (tok | head) % 8) return fail(DSA_ERR_ARG, "rows of %s must lie on 16-byte boundaries", name);
     return DSA_OK;
 }
