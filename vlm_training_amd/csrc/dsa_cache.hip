@@ -13,6 +13,13 @@ namespace {
 
 struct CacheRows { const void *k, *v; int64_t k_tok, k_head, v_tok, v_head; };
 
+// Four tokens to a workgroup.  A launch has fewer than 2^32 threads along x - more are cut to 32 bits without an error -, so that workgroups go on along y.
+inline dim3 token_grid(int T) {
+    const unsigned blocks = (unsigned)(((int64_t)T + 3) / 4), x = blocks < 1u << 22 ? blocks : 1u << 22;
+    return dim3(x, (blocks + x - 1) / x);
+}
+__device__ __forceinline__ int token_of_wave() { return (int)((blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6)); }
+
 // lanes of a row: the power of two that holds D / 8
 inline int row_lanes_shift(int D) {
     int s = 0;
@@ -23,8 +30,8 @@ inline int row_lanes_shift(int D) {
 template <bool E4M3>
 __global__ __launch_bounds__(256) void dsa_cache_write_kernel(dsa_cache_args c, CacheRows in, const int32_t *__restrict__ cu, const int32_t *__restrict__ lengths, int T, int N,
                                                               int pshift, int lshift) {
-    const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= T) return;
+    const int lane = threadIdx.x & 63, t = token_of_wave();
+    if ((uint32_t)t >= (uint32_t)T) return;
     const int sub = lane & ((1 << lshift) - 1), per = 64 >> lshift, mine = lane >> lshift, d = 8 * sub;
     const int items = 2 * c.Hkv;                         // keys of every head, then values
     constexpr int AHEAD = 4;
@@ -91,8 +98,8 @@ __global__ __launch_bounds__(256) void dsa_cache_write_kernel(dsa_cache_args c, 
 template <bool E4M3>
 __global__ __launch_bounds__(256) void dsa_cache_read_kernel(dsa_cache_args c, const int32_t *__restrict__ cu, const int32_t *__restrict__ first, int T, int N, int pshift,
                                                              int lshift, bf16_t *__restrict__ k_out, bf16_t *__restrict__ v_out) {
-    const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= T) return;
+    const int lane = threadIdx.x & 63, t = token_of_wave();
+    if ((uint32_t)t >= (uint32_t)T) return;
     const int sub = lane & ((1 << lshift) - 1), per = 64 >> lshift, mine = lane >> lshift, d = 8 * sub;
     const int items = 2 * c.Hkv;
     const int n = find_request(cu, N, t);
@@ -148,14 +155,14 @@ inline int log2_of(int x) { return __builtin_ctz((unsigned)x); }
 
 extern "C" hipError_t dsa_launch_cache_write(const dsa_cache_args *c, const void *k, int64_t k_tok, int64_t k_head, const void *v, int64_t v_tok, int64_t v_head, const int32_t *cu,
                                              const int32_t *lengths, int T, int N, hipStream_t stream) {
-    const dim3 grid((unsigned)(((int64_t)T + 3) / 4));
+    const dim3 grid = token_grid(T);
     const CacheRows in{k, v, k_tok, k_head, v_tok, v_head};
     const auto kernel = c->kind == DSA_CACHE_E4M3 ? &dsa_cache_write_kernel<true> : &dsa_cache_write_kernel<false>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, *c, in, cu, lengths, T, N, log2_of(c->page), row_lanes_shift(c->D));
     return hipGetLastError();
 }
 extern "C" hipError_t dsa_launch_cache_read(const dsa_cache_args *c, const int32_t *cu, const int32_t *first, int T, int N, void *k_out, void *v_out, hipStream_t stream) {
-    const dim3 grid((unsigned)(((int64_t)T + 3) / 4));
+    const dim3 grid = token_grid(T);
     const auto kernel = c->kind == DSA_CACHE_E4M3 ? &dsa_cache_read_kernel<true> : &dsa_cache_read_kernel<false>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, *c, cu, first, T, N, log2_of(c->page), row_lanes_shift(c->D), (bf16_t *)k_out, (bf16_t *)v_out);
     return hipGetLastError();
