@@ -1372,7 +1372,9 @@ static int check_paged(const dsa_cache_args *c, const int32_t *cu, int T, int N,
     if (Hq / c->Hkv > 16) return fail(DSA_ERR_UNSUPPORTED, "Hq/Hkv=%d: up to 16", Hq / c->Hkv);
     if (max_new < 0 || max_length < 0) return fail(DSA_ERR_ARG, "max_new=%d max_length=%d", max_new, max_length);
     const PagedCall p = paged_call(c, cu, nullptr, T, N, Hq, max_new, max_length);
-    if (std::max(std::max(p.step.blocks, p.step.slots), p.walk.slots + p.walk.blocks + p.step.blocks + p.step.slots) * c->Hkv > INT32_MAX || p.step.blocks >= 1 << 25) return fail(DSA_ERR_UNSUPPORTED, "too many blocks: T=%d N=%d Hkv=%d", T, N, c->Hkv);
+    // A launch has fewer than 2^32 threads along x (more are cut to 32 bits without an error): of the kernels' workgroups of 256, and of the join's, one to a block
+    const int64_t kernels = p.walk.slots + p.step.slots, joins = (p.walk.plan.whole ? 0 : p.walk.blocks) + (p.step.plan.whole ? 0 : p.step.blocks);
+    if (std::max(kernels, joins) * c->Hkv >= 1 << 24 || p.step.blocks >= 1 << 25) return fail(DSA_ERR_UNSUPPORTED, "too many blocks: T=%d N=%d Hkv=%d", T, N, c->Hkv);
     return DSA_OK;
 }
 extern "C" size_t dsa_paged_attn_workspace_bytes(const dsa_cache_args *c, int T, int N, int Hq, int max_new, int max_length) {
