@@ -173,8 +173,8 @@ __device__ __forceinline__ PageShares page_shares(const PagePlan &p, const PageR
     s.near = p.whole ? 1 << 29 : max(1, s.share >> 4);
     return s;
 }
-// the block of request `n` (lane w of r) that is the order-th of its blocks (the last one, which has the most keys, first) and takes units u0 .. u1 - 1
-__device__ __forceinline__ void share_block(const PagePlan &p, const PageShares &s, const PageRequest &r, int w, int n, int order, int u0, int u1, PagePiece &out) {
+// the block of request `n` (lane w of r) that is the order-th of its blocks (the last one, which has the most keys, first): whose it is, and its first query
+__device__ __forceinline__ void share_block(const PagePlan &p, const PageRequest &r, int w, int n, int order, PagePiece &out) {
     out.n = n;
     out.row0 = __builtin_amdgcn_readlane(r.row0, w);
     out.m = __builtin_amdgcn_readlane(r.m, w);
@@ -215,7 +215,7 @@ struct ShareWalk {
             const int u1 = u0 + units_of(p, __builtin_amdgcn_readlane(r.tiles, w));
             const int lo = x0 <= u0 ? u0 : s.moved(x0, u0, u1), hi = x1 >= u1 ? u1 : s.moved(x1, u0, u1);
             if (lo < hi) {
-                share_block(p, s, r, w, base + w, order, u0, u1, out);
+                share_block(p, r, w, base + w, order, out);
                 const int last = out.length - out.m + min(out.first + p.qb, out.m) - 1;      // position of the block's last row
                 const int tiles = last < 0 ? 0 : (min(last, p.capacity - 1) >> 5) + 1;
                 // (a first piece ends with the first cut inside the block, the next share's start; another begins with its share)
@@ -256,7 +256,7 @@ __device__ __forceinline__ bool locate_share_block(const PagePlan &p, int slot, 
             const int w = (int)__builtin_ctzll(past), blocks = __builtin_amdgcn_readlane(r.blocks, w), per = __builtin_amdgcn_readlane(units, w);
             const int order = slot - taken - (__builtin_amdgcn_readlane(upto, w) - blocks);
             const int u0 = before + __builtin_amdgcn_readlane(uupto, w) - (blocks - order) * per;
-            share_block(p, s, r, w, base + w, order, u0, u0 + per, out);
+            share_block(p, r, w, base + w, order, out);
             out.pieces = s.cuts(u0, u0 + per) + 1;
             out.slot = 2 * s.first_cut(u0) - 1;
             return true;
