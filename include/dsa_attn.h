@@ -492,10 +492,12 @@ int dsa_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x
  * What lies on no page (a page number outside the pool, a position outside the table) is not written and reads as zero.
  *
  * dsa_cache_write: request n's new rows cu[n] .. cu[n+1]-1 of k, v (T,Hkv,D) bf16 (token and head strides multiples of 8, rows on 16-byte boundaries) become its last ones,
- * positions lengths[n] - (cu[n+1] - cu[n]) on.  Two rows that go to one place race.  Rows behind cu[N] go nowhere.
+ * positions lengths[n] - (cu[n+1] - cu[n]) on.  Two rows that go to one place race, and so does a row
+ * read from a place that is written (k, v may lie in the pools' other pages).  Rows behind cu[N] go nowhere.
  * dsa_cache_read: rows cu[n] .. cu[n+1]-1 of k_out, v_out (T,Hkv,D) bf16, contiguous, are request n's positions first[n] on (first null: 0); rows behind cu[N] give zeros.
  * dsa_paged_attn: q (T,Hq,D) bf16, strided as above; the new rows of request n, its last ones, attend what the cache holds of it up to and with themselves (keys that
  * lie on no page are zero rows, positions past the table no keys).  out (T,Hq,D) bf16 contiguous, lse (Hq,T) fp32, natural, or null; a row without a key and rows behind cu[N] give zeros and -inf.
+ * Sums are divided at the end: |v| up to 2^89 never passes fp32's range.
  * max_new, max_length: upper bounds of cu[n+1] - cu[n] and of lengths (0: not known); they choose among kernels, results are right without them.  `ws` holds
  * dsa_paged_attn_workspace_bytes(...) bytes.  Hq / Hkv up to 16.
  */

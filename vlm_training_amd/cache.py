@@ -56,8 +56,9 @@ class KvCache:
 def kv_cache_write(cache: KvCache, k, v, page_table, cu_seqlens, lengths) -> None:
     """k, v (T, kv heads, head_dim) bf16 views: request n's rows ``cu_seqlens[n]`` to ``cu_seqlens[n + 1]`` become its last ones, positions ``lengths[n]`` minus their number on.
 
-    The cache is updated in place.  Two rows for one place (a page in two requests' tables where both write) are written in no order; pages that are only read may be
-    shared.  No backward pass."""
+    The cache is updated in place.  Two rows for one place (a page in two requests' tables where both write, keys and values in the same memory) are written in no order; pages
+    that are only read may be shared.  ``k`` and ``v`` may lie in the pools themselves (a page copied to another), but not where the call writes: what it then reads is one or
+    the other.  No backward pass."""
     _lib.host().kv_cache_write(*cache._parts(), k, v, page_table, cu_seqlens, lengths)
 
 
@@ -78,6 +79,7 @@ def paged_attn(q, cache: KvCache, page_table, cu_seqlens, lengths, *, max_new=No
     NaN logit that it does attend makes it NaN.
     ``max_new`` and ``max_length``, where known, are upper bounds of the requests' new rows and lengths: with them fewer kernels are launched; results do not depend on them but for
     the order of sums.  ``softmax_scale`` defaults to ``head_dim ** -0.5``.  ``return_lse`` adds (q heads, T) fp32: the logarithm of each row's sum of exponentials, -inf
-    for rows without a key.  Probabilities are rounded to bf16 for their product with the values; statistics and sums are fp32.  No backward pass."""
+    for rows without a key.  Probabilities are rounded to bf16 for their product with the values; statistics and sums are fp32.  Sums are
+    divided at the end, with weights of up to 2^8: values up to 2^89 never pass their range.  No backward pass."""
     out = _lib.host().paged_attn(q, *cache._parts(), page_table, cu_seqlens, lengths, max_new, max_length, softmax_scale, bool(return_lse))
     return tuple(out) if return_lse else out[0]
