@@ -499,7 +499,7 @@ int dsa_residual_norm_bwd(const void *dxn, const void *dh, const void *xn, int x
  * lie on no page are zero rows, positions past the table no keys).  out (T,Hq,D) bf16 contiguous, lse (Hq,T) fp32, natural, or null; a row without a key and rows behind cu[N] give zeros and -inf.
  * Sums are divided at the end: |v| up to 2^89 never passes fp32's range.
  * max_new, max_length: upper bounds of cu[n+1] - cu[n] and of lengths (0: not known); they choose among kernels, results are right without them.  `ws` holds
- * dsa_paged_attn_workspace_bytes(...) bytes.  Hq / Hkv up to 16.
+ * dsa_paged_attn_workspace_bytes(...) bytes.  Hq / Hkv up to 16; fewer than 2^24 workgroups (blocks of 16 to 128 rows times Hkv).
  */
 #define DSA_CACHE_BF16 0
 #define DSA_CACHE_E4M3 1

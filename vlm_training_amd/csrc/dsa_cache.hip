@@ -6,7 +6,7 @@
 // x * 2^-e is exact, so that each value is rounded once, to nearest even.
 //
 // What bounds them: memory.  12 388 rows of 8 + 8 heads of 128 into a bf16 cache 20.6 us (4.9 TB/s), into an 8-bit one 19 us and back 12; 32 768 rows out of an 8-bit cache 39 us
-// (5.2 TB/s; 45 with the rows going through the caches).  One token for each of 256 requests: 4.5 us each, those round trips.
+// (5.2 TB/s; 45 with the rows going through the caches), out of a bf16 one 47 (5.7).  One token for each of 256 requests: 4.5 us each, those round trips.
 #include "dsa_paged.h"
 
 namespace {

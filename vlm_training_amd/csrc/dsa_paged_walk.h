@@ -12,9 +12,9 @@
 // one: values are loaded into registers a step ahead of the one that writes them to LDS as bf16, K(t+4) and V(t+2) in step t: one conversion for 128 rows, and no rounding, as
 // the scales are powers of two.
 //
-// What bounds it: as the packed forward, power and the instructions beside the MFMAs.  2048 new tokens behind 14 336 (32 heads over 8 of 128) 470 us = 1.10 PFLOP/s, MFMA busy 0.6 of the
+// What bounds it: as the packed forward, power and the instructions beside the MFMAs.  2048 new tokens behind 14 336 (32 heads over 8 of 128) 472 to 485 us = 1.06 to 1.09 PFLOP/s (16 over 2 of 256: 488, 8-bit 573), MFMA busy 0.6 of the
 // units' time; page addresses formed in 64 bits for each operand cost 8 % of it, two long walks on one unit (the second half of a launch of one round goes in reverse) 3 %.
-// An 8-bit cache: 1024 behind 60 000 1369 us; the loads two steps ahead instead of one left no registers for operands four MFMAs ahead (1498), and converting in
+// An 8-bit cache: 1024 behind 60 000 1370 to 1390 us (bf16 1110); the loads two steps ahead instead of one left no registers for operands four MFMAs ahead (1498), and converting in
 // the loads' own step spilled.  A chunk of 512 behind 7680 and a prompt of 333: 93 us, of them 8 for the first loads and 8 for the pieces' sums (33 MB).
 #pragma once
 #include "dsa_paged.h"
