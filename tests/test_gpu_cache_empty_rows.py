@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import vlm_training_amd as V
-from tests.test_gpu_cache import BF, DEV, E4, _offsets, make
+from tests.test_gpu_cache import BF, DEV, _offsets, make
 
 pytestmark = pytest.mark.gpu
 
